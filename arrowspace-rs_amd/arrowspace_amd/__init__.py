@@ -9,3 +9,4 @@ from .api import (ArrowItem, ArrowSpace, ArrowSpaceBuilder, Context, CsrMatrix, 
                   compute_synthetic_lambda, default_context, knn_cosine, laplacian_from_knn, select_tau,
                   ImplicitProjection, calinski_harabasz, compute_jl_dimension, compute_optimal_k, incremental_clustering,
                   kmeans_lloyd, two_nn_ratios)
+from .table import Table4, cross_entropy, cross_entropy_backward  # noqa: F401

@@ -30,7 +30,12 @@ EXPORTS = [
     "as_shard_range", "as_build_laplacian_sharded", "as_lambda_stats_sharded", "as_search_lambda_aware_sharded",
     "as_device_upload", "as_device_download", "as_device_free",
     "as_compute_taumode_signals", "as_csr_set_order", "as_compute_taumode_signals_sharded",
+    "as_cross_entropy_workspace", "as_cross_entropy", "as_cross_entropy_backward", "as_table4_import", "as_table4_pack",
+    "as_table4_export", "as_table4_destroy", "as_table4_items", "as_table4_dim", "as_table4_group", "as_table4_scale_dtype",
+    "as_table4_workspace", "as_table4_scores",
 ]
+
+AS_F64, AS_F32, AS_BF16, AS_F16 = range(4)   # as_dtype
 
 # transport callbacks of as_comm_create_custom (device buffers; byte counts / offsets are arrays of `world` entries)
 AllGatherV = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64),
@@ -144,6 +149,20 @@ def load():
         "as_device_free": (None, [vp, vp]),
         "as_lambda_stats_sharded": (i32, [vp, vp, vp, u64, C.POINTER(dbl), C.POINTER(dbl), C.POINTER(dbl)]),
         "as_search_lambda_aware_sharded": (i32, [vp, vp, vp, vp, vp, u64, u64, dbl, u64, vp, vp]),
+        "as_cross_entropy_workspace": (u64, [u64, u64, u64, i32, i32]),
+        "as_cross_entropy": (i32, [vp, vp, u64, u64, vp, u64, u64, u64, i32, vp, vp, C.c_int64, dbl, vp, vp, vp, u64]),
+        "as_cross_entropy_backward": (i32, [vp, vp, u64, u64, vp, u64, u64, u64, i32, vp, vp, C.c_int64, dbl, vp, vp, vp, vp, u64,
+                                            vp, u64, vp, vp, u64]),
+        "as_table4_import": (i32, [vp, vp, vp, vp, u64, u64, u64, i32, C.POINTER(vp)]),
+        "as_table4_pack": (i32, [vp, vp, u64, u64, u64, i32, u64, i32, C.POINTER(vp)]),
+        "as_table4_export": (i32, [vp, vp, vp, vp, vp]),
+        "as_table4_destroy": (None, [vp]),
+        "as_table4_items": (u64, [vp]),
+        "as_table4_dim": (u64, [vp]),
+        "as_table4_group": (u64, [vp]),
+        "as_table4_scale_dtype": (i32, [vp]),
+        "as_table4_workspace": (u64, [vp, u64, i32]),
+        "as_table4_scores": (i32, [vp, vp, vp, u64, u64, i32, vp, u64, vp, u64]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

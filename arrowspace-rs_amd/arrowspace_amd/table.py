@@ -1,0 +1,275 @@
+"""Operators over a table of rows (what an index holds), over the C ABI: softmax cross entropy against all its items with the
+gradient, and products with a table held in 4 bits.  They have no counterpart in the reference.
+
+Matrices are torch tensors (on a GPU: used in place, on torch's current stream of that GPU, nothing waited for, capturable into a
+graph) or numpy arrays (staged; results come back as numpy arrays, complete).  Rows may be rows of a wider tensor; the values of a
+row must be adjacent.
+"""
+import ctypes as C
+import threading
+
+import numpy as np
+
+from . import _lib
+from ._lib import ArrowSpaceError, AS_BF16, AS_F16, AS_F32, AS_F64, is_tensor
+from .api import Context, DeviceArray
+
+_DTYPES = {"float64": AS_F64, "float32": AS_F32, "bfloat16": AS_BF16, "float16": AS_F16}
+_NAMES = {AS_F64: "float64", AS_F32: "float32", AS_BF16: "bfloat16", AS_F16: "float16"}
+_local = threading.local()
+
+
+def _thread_context(device):
+    """The calling thread's own context on a device (a context is not re-entrant)."""
+    table = getattr(_local, "contexts", None)
+    if table is None:
+        table = _local.contexts = {}
+    ctx = table.get(device)
+    if ctx is None:
+        ctx = table[device] = Context(device)
+    return ctx
+
+
+class _Call:
+    """Where a call's data live, and its context with the right stream."""
+
+    def __init__(self, first, ctx):
+        if isinstance(first, DeviceArray):
+            raise TypeError("a DeviceArray is not taken here: torch tensors or numpy arrays")
+        self.torch = None
+        self.device = None
+        if is_tensor(first):
+            import torch
+            self.torch = torch
+            self.device = first.device
+        if self.device is not None and self.device.type == "cuda":
+            if ctx is None:
+                before = self.torch.cuda.current_device()
+                ctx = _thread_context(self.device.index)
+                if self.torch.cuda.current_device() != before:   # (the first call here makes the context)
+                    self.torch.cuda.set_device(before)
+            elif ctx.device != self.device.index:
+                raise ArrowSpaceError(_lib.AS_ERR_ARG, "tensors of device %d, a context of device %d" % (self.device.index, ctx.device))
+            st = self.torch.cuda.current_stream(self.device).cuda_stream
+            if getattr(ctx, "_stream", "own") != st:
+                ctx.set_stream(st)
+                ctx._stream = st
+        elif ctx is None:
+            ctx = _thread_context(0)
+        self.ctx = ctx
+
+    def empty(self, shape, dtype):
+        """An output beside the call's inputs; dtype a name."""
+        if self.torch is not None:
+            return self.torch.empty(shape, dtype=getattr(self.torch, dtype), device=self.device)
+        return np.empty(shape, dtype=dtype)
+
+    def workspace(self, size):
+        """(tensor, address, bytes): torch's own allocator on a GPU, so that a captured graph keeps what it uses; else the library's."""
+        if not size or self.device is None or self.device.type != "cuda":
+            return None, None, 0
+        w = self.torch.empty(size, dtype=self.torch.uint8, device=self.device)
+        return w, w.data_ptr(), size
+
+
+def _name(a):
+    return str(a.dtype).replace("torch.", "")
+
+
+def _matrix(a, what):
+    """(array, rows, columns, row stride in elements, address) of a matrix whose rows' values are adjacent."""
+    if not is_tensor(a):
+        a = np.asarray(a)
+        if a.ndim != 2:
+            raise ArrowSpaceError(_lib.AS_ERR_SHAPE, "%s must be a matrix, got %d dimensions" % (what, a.ndim))
+        a = np.ascontiguousarray(a)
+        return a, a.shape[0], a.shape[1], a.shape[1], a.ctypes.data
+    if a.dim() != 2:
+        raise ArrowSpaceError(_lib.AS_ERR_SHAPE, "%s must be a matrix, got %d dimensions" % (what, a.dim()))
+    n, d = a.shape
+    step, inner = a.stride()
+    if d > 1 and inner != 1:
+        raise ArrowSpaceError(_lib.AS_ERR_ARG, "the values of a row of %s must be adjacent" % what)
+    if n <= 1:
+        step = max(step, d)
+    if step < d:
+        raise ArrowSpaceError(_lib.AS_ERR_ARG, "rows of %s overlap" % what)
+    return a, n, d, step, a.data_ptr()
+
+
+def _vector(a, n, dtype, what):
+    """Address of a dense vector of n elements, and the array that has to stay alive."""
+    if a is None:
+        return None, None
+    if not is_tensor(a):
+        a = np.asarray(a)
+        if a.dtype != np.dtype(dtype):
+            raise TypeError("%s must be %s, got %s" % (what, dtype, a.dtype))
+        a = np.ascontiguousarray(a)
+        if a.shape != (n,):
+            raise ArrowSpaceError(_lib.AS_ERR_SHAPE, "%s must have %d elements, has shape %s" % (what, n, a.shape))
+        return a.ctypes.data, a
+    if _name(a) != dtype:
+        raise TypeError("%s must be %s, got %s" % (what, dtype, a.dtype))
+    if tuple(a.shape) != (n,):
+        raise ArrowSpaceError(_lib.AS_ERR_SHAPE, "%s must have %d elements, has shape %s" % (what, n, tuple(a.shape)))
+    a = a.contiguous()   # (an expanded gradient, say)
+    return a.data_ptr(), a
+
+
+def _loss_args(x, table, bias, targets, ctx):
+    first = x
+    x, n, d, xs, xp = _matrix(x, "x")
+    table, v, dw, ts, tp = _matrix(table, "table")
+    if d != dw:
+        raise ArrowSpaceError(_lib.AS_ERR_SHAPE, "rows of %d values against a table of %d" % (d, dw))
+    kind = _DTYPES.get(_name(x))
+    if kind is None or kind == AS_F64 or _name(table) != _name(x):
+        raise TypeError("x and table must both be float32, bfloat16 or float16, got %s and %s" % (x.dtype, table.dtype))
+    bp, bias = _vector(bias, v, "float32", "bias")
+    yp, targets = _vector(targets, n, "int64", "targets")
+    if yp is None:
+        raise ArrowSpaceError(_lib.AS_ERR_ARG, "null argument")
+    call = _Call(first, ctx)
+    return call, (xp, n, xs, tp, v, ts, d, kind, bp, yp), (x, table, bias, targets)
+
+
+def cross_entropy(x, table, targets, bias=None, scale=1.0, ignore_index=-100, ctx=None):
+    """Softmax cross entropy of every row of x (n x d) against all rows of the table (v x d), the n x v logits never kept:
+    (losses, lse), both float32 of n.  logits = scale * x @ table.T + bias; losses are 0 where targets == ignore_index and where the
+    bias (-inf) leaves no item.  The mean over the counted rows is losses.sum() / count."""
+    call, (xp, n, xs, tp, v, ts, d, kind, bp, yp), alive = _loss_args(x, table, bias, targets, ctx)
+    losses, lse = call.empty((n,), "float32"), call.empty((n,), "float32")
+    lib, c = call.ctx.lib, call.ctx
+    ws, wp, wb = call.workspace(lib.as_cross_entropy_workspace(n, v, d, kind, 0))
+    c.check(lib.as_cross_entropy(c.h, xp, n, xs, tp, v, ts, d, kind, bp, yp, int(ignore_index), float(scale), _addr(losses), _addr(lse), wp, wb))
+    return losses, lse
+
+
+def cross_entropy_backward(x, table, targets, lse, grad_losses, bias=None, scale=1.0, ignore_index=-100, grad_lse=None, need_x=True,
+                           need_table=True, need_bias=True, ctx=None):
+    """The gradients of cross_entropy's inputs, (grad_x, grad_table, grad_bias), from the gradients of its two outputs (grad_lse
+    None: zero) and the lse that it returned.  grad_x and grad_table have the inputs' type, grad_bias is float32; None where not needed
+    or where there is no bias."""
+    rows = tuple(x.shape)[0]
+    lp, lse = _vector(lse, rows, "float32", "lse")
+    gp, grad_losses = _vector(grad_losses, rows, "float32", "grad_losses")
+    ep, grad_lse = _vector(grad_lse, rows, "float32", "grad_lse")
+    if lp is None or gp is None:
+        raise ArrowSpaceError(_lib.AS_ERR_ARG, "null argument")
+    call, (xp, n, xs, tp, v, ts, d, kind, bp, yp), alive = _loss_args(x, table, bias, targets, ctx)
+    gx = call.empty((n, d), _NAMES[kind]) if need_x else None
+    gw = call.empty((v, d), _NAMES[kind]) if need_table else None
+    gb = call.empty((v,), "float32") if need_bias and bp is not None else None
+    lib, c = call.ctx.lib, call.ctx
+    ws, wp, wb = call.workspace(lib.as_cross_entropy_workspace(n, v, d, kind, 1))
+    c.check(lib.as_cross_entropy_backward(c.h, xp, n, xs, tp, v, ts, d, kind, bp, yp, int(ignore_index), float(scale), lp, gp, ep, _addr(gx), d,
+                                          _addr(gw), d, _addr(gb), wp, wb))
+    return gx, gw, gb
+
+
+def _addr(a):
+    return None if a is None else a.data_ptr() if is_tensor(a) else a.ctypes.data
+
+
+class Table4:
+    """A table of rows in 4 bits with group scales, laid out for the kernels: W = scale * (code - zero), zero 8 unless given.
+    Make one from rows (pack) or from codes that exist already (from_codes); scores(x) is x @ W.T."""
+
+    def __init__(self, ctx, handle):
+        self.ctx, self.h = ctx, handle
+        lib = ctx.lib
+        self.n_items, self.dim, self.group = int(lib.as_table4_items(handle)), int(lib.as_table4_dim(handle)), int(lib.as_table4_group(handle))
+        self.scale_dtype = _NAMES[lib.as_table4_scale_dtype(handle)]
+
+    @classmethod
+    def pack(cls, rows, group=64, scale_dtype="bfloat16", ctx=None):
+        """Quantises rows (float64, float32, bfloat16 or float16): per group the largest magnitude / 7 becomes the scale."""
+        first = rows
+        rows, n, d, step, p = _matrix(rows, "rows")
+        kind, scale_kind = _DTYPES.get(_name(rows)), _scale_kind(scale_dtype)
+        if kind is None:
+            raise TypeError("rows must be floating-point, got %s" % rows.dtype)
+        _check_group(group)
+        call = _Call(first, ctx)
+        h = C.c_void_p()
+        call.ctx.check(call.ctx.lib.as_table4_pack(call.ctx.h, p, n, step, d, kind, int(group), scale_kind, C.byref(h)))
+        return cls(call.ctx, h)
+
+    @classmethod
+    def from_codes(cls, codes, scales, zeros=None, dim=None, group=64, ctx=None):
+        """codes: uint8, n x ceil(dim / 2), column 2 j in the low half of byte j; scales: n x ceil(dim / group), float32, bfloat16 or
+        float16; zeros: uint8 of the scales' shape, or None."""
+        first = codes
+        _check_group(group)
+        codes, n, half, step, cp = _matrix(codes, "codes")
+        dim = 2 * half if dim is None else int(dim)
+        if _name(codes) != "uint8" or (zeros is not None and _name(zeros) != "uint8"):
+            raise TypeError("codes and zeros must be uint8")
+        if (dim + 1) // 2 != half:
+            raise ArrowSpaceError(_lib.AS_ERR_SHAPE, "%d columns take %d bytes a row, codes have %d" % (dim, (dim + 1) // 2, half))
+        scales, sn, sg, sstep, sp = _matrix(scales, "scales")
+        groups = (dim + int(group) - 1) // int(group)
+        if (sn, sg) != (n, groups):
+            raise ArrowSpaceError(_lib.AS_ERR_SHAPE, "scales must be %d x %d, are %d x %d" % (n, groups, sn, sg))
+        zp = None
+        if zeros is not None:
+            zeros, zn, zg, zstep, zp = _matrix(zeros, "zeros")
+            if (zn, zg) != (n, groups):
+                raise ArrowSpaceError(_lib.AS_ERR_SHAPE, "zeros must be %d x %d, are %d x %d" % (n, groups, zn, zg))
+        if n > 1 and (step != half or sstep != groups or (zeros is not None and zstep != groups)):
+            raise ArrowSpaceError(_lib.AS_ERR_ARG, "codes, scales and zeros must be dense")
+        scale_kind = _scale_kind(_name(scales))
+        call = _Call(first, ctx)
+        h = C.c_void_p()
+        call.ctx.check(call.ctx.lib.as_table4_import(call.ctx.h, cp, sp, zp, n, dim, int(group), scale_kind, C.byref(h)))
+        return cls(call.ctx, h)
+
+    def to_codes(self):
+        """(codes, scales, zeros) as host arrays; bfloat16 scales come back as float32."""
+        groups = (self.dim + self.group - 1) // self.group
+        codes = np.empty((self.n_items, (self.dim + 1) // 2), dtype=np.uint8)
+        zeros = np.empty((self.n_items, groups), dtype=np.uint8)
+        raw = np.empty((self.n_items, groups), dtype=np.uint16 if self.scale_dtype == "bfloat16" else self.scale_dtype)
+        self.ctx.check(self.ctx.lib.as_table4_export(self.ctx.h, self.h, codes.ctypes.data, raw.ctypes.data, zeros.ctypes.data))
+        scales = (raw.astype(np.uint32) << 16).view(np.float32) if self.scale_dtype == "bfloat16" else raw
+        return codes, scales, zeros
+
+    def scores(self, x, ctx=None):
+        """x @ W.T for one row or a few (float32, bfloat16 or float16), in x's type."""
+        first = x
+        single = len(x.shape) == 1
+        if single:
+            x = x.reshape(1, -1)
+        x, m, d, step, p = _matrix(x, "x")
+        if d != self.dim:
+            raise ArrowSpaceError(_lib.AS_ERR_DIM, "rows of %d values against a table of %d" % (d, self.dim))
+        kind = _DTYPES.get(_name(x))
+        if kind is None or kind == AS_F64:
+            raise TypeError("x must be float32, bfloat16 or float16, got %s" % x.dtype)
+        call = _Call(first, ctx)
+        out = call.empty((m, self.n_items), _NAMES[kind])
+        lib, c = call.ctx.lib, call.ctx
+        ws, wp, wb = call.workspace(lib.as_table4_workspace(self.h, m, kind))
+        c.check(lib.as_table4_scores(c.h, self.h, p, m, step, kind, _addr(out), self.n_items, wp, wb))
+        return out[0] if single else out
+
+    def __del__(self):
+        try:
+            if self.h:
+                self.ctx.lib.as_table4_destroy(self.h)
+                self.h = None
+        except Exception:  # noqa: BLE001 -- interpreter shutdown
+            pass
+
+
+def _check_group(group):
+    if int(group) not in (32, 64, 128):
+        raise ArrowSpaceError(_lib.AS_ERR_UNSUPPORTED, "groups of 32, 64 or 128 columns, not %d" % int(group))
+
+
+def _scale_kind(name):
+    kind = _DTYPES.get(str(name).replace("torch.", ""))
+    if kind is None or kind == AS_F64:
+        raise TypeError("scales are float32, bfloat16 or float16, not %s" % name)
+    return kind

@@ -226,6 +226,12 @@ hipError_t handle_free(void *p) {
         for (auto sit = c.streams.lower_bound({key.first, (hipStream_t)0}); ok && sit != c.streams.end() && sit->first == key.first; ++sit) {
           if (sit->second == last) continue;  // (a stream several contexts share)
           last = sit->second;
+          hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+          if (hipStreamIsCapturing(sit->second, &capturing) != hipSuccess || capturing != hipStreamCaptureStatusNone) {
+            (void)hipGetLastError();   // (an event there would become part of the graph)
+            ok = false;
+            break;
+          }
           hipEvent_t ev = nullptr;
           if (!c.event_pool.empty()) {
             ev = c.event_pool.back();
@@ -512,6 +518,11 @@ void as_ctx_destroy(as_ctx *ctx) {
   prof_resolve(ctx);
   handle_cache_stream(ctx->device, ctx->stream, false);
   if (ctx->own_stream) (void)hipStreamDestroy(ctx->stream);
+  for (hipStream_t s : ctx->capture_left) (void)hipStreamSynchronize(s);
+  for (hipStream_t s : ctx->parked_streams) {
+    (void)hipStreamSynchronize(s);
+    (void)hipStreamDestroy(s);
+  }
   if (ctx->pinned) (void)hipHostFree(ctx->pinned);
   join_session_close(ctx);
   if (ctx->join_order) (void)hipFree(ctx->join_order);
@@ -525,7 +536,28 @@ const char *as_last_error(const as_ctx *ctx) { return ctx ? ctx->err.c_str() : "
 
 int as_ctx_set_stream(as_ctx *ctx, void *hip_stream) {
   AS_TRY(check_ctx(ctx));
+  hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing((hipStream_t)hip_stream, &capturing) != hipSuccess) (void)hipGetLastError();
+  if (capturing != hipStreamCaptureStatusNone) {
+    // Nothing may be waited for or destroyed beside a capture.  Calls on a capturing stream bring their own workspace, so none of
+    // the context's scratch passes from the old stream's work to the new one's here; its next owner is on a stream that the switch
+    // back synchronises with.
+    if (ctx->own_stream) ctx->parked_streams.push_back(ctx->stream);
+    else if (std::find(ctx->capture_left.begin(), ctx->capture_left.end(), ctx->stream) == ctx->capture_left.end()) ctx->capture_left.push_back(ctx->stream);
+    ctx->own_stream = false;
+    handle_cache_stream(ctx->device, ctx->stream, false);
+    ctx->stream = (hipStream_t)hip_stream;
+    handle_cache_stream(ctx->device, ctx->stream, true);
+    return AS_OK;
+  }
   (void)hipStreamSynchronize(ctx->stream);
+  for (hipStream_t s : ctx->capture_left) (void)hipStreamSynchronize(s);   // (streams left for a capture, not waited for then)
+  ctx->capture_left.clear();
+  for (hipStream_t s : ctx->parked_streams) {
+    (void)hipStreamSynchronize(s);
+    (void)hipStreamDestroy(s);
+  }
+  ctx->parked_streams.clear();
   prof_resolve(ctx);
   handle_cache_stream(ctx->device, ctx->stream, false);
   if (ctx->own_stream) (void)hipStreamDestroy(ctx->stream);

@@ -74,6 +74,7 @@ struct as_ctx {
   hipEvent_t side_start = nullptr, side_done = nullptr;
   int *side_word = nullptr;               // pinned: what the side stream reads back
   bool own_stream = false;
+  std::vector<hipStream_t> parked_streams, capture_left;  // as_ctx_set_stream beside a capture: the context's own stream until it may be destroyed; streams not yet waited for
   std::string err;
   void *pinned = nullptr;  // staging buffer for host <-> device transfers
   std::multimap<size_t, void *> free_blocks;  // workspace cache (capacity -> block)

@@ -1,0 +1,1007 @@
+// table_loss.hip -- softmax cross entropy of rows against a table of items, without keeping the logits, and its gradient.
+//
+//   l_tv = scale <x_t, w_v> + bias_v      lse_t = log sum_v exp(l_tv)      loss_t = lse_t - l_{t, y_t}
+//   with gl = dL/dloss (0 where the row is ignored), ge = dL/dlse:   g_tv = (gl_t + ge_t) exp(l_tv - lse_t) - gl_t [v = y_t]
+//   dX = scale G W      dW = scale G^T X      dbias_v = sum_t g_tv
+//
+// Forward: one product (nt_product.h, the table on the m side, so that a lane holds many items of ONE row) whose ending keeps a
+// running maximum and sum of exponentials per lane and row; what leaves the chip is one (maximum, sum) per row and stretch of the
+// table.  A second kernel joins them and takes the target's logit from a product of its own in f64.
+// Backward: in pieces of the table.  Per piece the logits are made again, their gradient G leaves in 16 bits, row-major AND
+// transposed, and two more products of the same kind give the piece's rows of dW and its part of dX (f32, added up over the pieces in
+// a buffer, rounded once at the end).  Nothing is added with atomics: results do not change from run to run.
+// Types.  bf16 and f16 go to the matrix pipe as they are.  f32 values go as a sum of two f16 (22 bits, after a power of two that
+// brings the matrix' largest finite value to 2^14 .. 2^15), three products per pair of planes: 2.5 PFLOP/s / 3 against the
+// 0.157 of the f32 instruction, and an error per product of 2^-23 of it, which the f32 sums have anyway.
+// Rounding.  G is rounded to 16 bits (f16: after a power of two from the largest coefficient; f32: two planes, 22 bits): half a
+// step per entry, as the gradients that leave are rounded themselves.  Everything else -- logits, maxima, sums, dX over pieces,
+// dbias -- is f32 or wider.
+#include "nt_product.h"
+
+using namespace asx;
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kChips = 256;  // compute units: how many workgroups of the large tile run at once
+
+struct LossArgs {
+  // operands of the product: A the table side (m), B the rows (n)
+  const char *table, *rows;
+  size_t table_ld, rows_ld;       // bytes
+  uint32_t table_plane, rows_plane;  // steps of 64 to the low plane
+  uint32_t n, v;                  // rows of B and of A
+  uint32_t steps, planes;         // steps of 64 along k per plane; 1, or 2 (three passes)
+  uint32_t per;                   // tiles of A a workgroup walks
+  uint32_t v_tiles, n_tiles, chunks;
+  float scale;
+  const float *bias;
+  const unsigned int *rows_top, *table_top;  // two planes: bits of the largest finite magnitude of each matrix, else null
+};
+
+// the power of two a matrix with this largest magnitude is multiplied by (0 or not a number: 1)
+__device__ __forceinline__ float plane_scale(unsigned int top_bits) {
+  const int e = (int)(top_bits >> 23);
+  if (e == 0 || e >= 255) return 1.f;
+  const int s = min(max(14 - (e - 127), -100), 100);
+  return __uint_as_float((unsigned int)(127 + s) << 23);
+}
+__device__ __forceinline__ float product_scale(const LossArgs &a) {
+  if (a.rows_top == nullptr) return 1.f;
+  return 1.f / plane_scale(*a.rows_top) / plane_scale(*a.table_top);
+}
+
+// Workgroups are dealt to the 8 dies in turn; consecutive pieces of work should share a die's cache, so die d takes the d-th eighth.
+__device__ __forceinline__ uint32_t die_order(uint32_t b, uint32_t total) {
+  const uint32_t die = b & 7, at = b >> 3, each = total >> 3, rest = total & 7;
+  return die * each + nt_min(die, rest) + at;
+}
+
+// quad-wide exchange: the value of lane ^ 1 / lane ^ 2
+__device__ __forceinline__ uint32_t quad_xor1(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true); }
+__device__ __forceinline__ uint32_t quad_xor2(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true); }
+__device__ __forceinline__ float add16(float v) {  // sum over the 16 lanes of a row of lanes, in a fixed order
+  v += __uint_as_float(quad_xor1(__float_as_uint(v)));
+  v += __uint_as_float(quad_xor2(__float_as_uint(v)));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, true));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, true));
+  return v;
+}
+
+template <int FMT>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (FMT == AS_BF16) {
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    const bf2 p = {(__bf16)x, (__bf16)y};
+    return __builtin_bit_cast(uint32_t, p);
+  } else {
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    const half2v p = {(_Float16)x, (_Float16)y};
+    return __builtin_bit_cast(uint32_t, p);
+  }
+}
+__device__ __forceinline__ float low_part(float x) {  // what f16 leaves of x (nothing of an infinity)
+  const float hi = (float)(_Float16)x;
+  return __builtin_isfinite(hi) ? x - hi : 0.f;
+}
+
+// ---- forward --------------------------------------------------------------------------------------------------------------------------
+// GENERAL: with a bias, or a scale that is not positive (the maximum is then taken of the scaled logits); else of the raw products.
+template <int FMT, class TILE_, bool GENERAL>
+__global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2 *part) {
+  using TILE = TILE_;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * TILE::kStage];
+  TILE T;
+  T.init(smem);
+  const uint32_t work = die_order(blockIdx.x, gridDim.x);
+  const uint32_t nt = work % a.n_tiles, chunk = work / a.n_tiles;
+  const uint32_t n0 = nt * TILE::BN, vt_end = nt_min((chunk + 1) * a.per, a.v_tiles);
+  uint32_t vt = chunk * a.per;
+  const float nat = a.scale * product_scale(a), unit = GENERAL ? kLog2e : nat * kLog2e;  // exponentials of (x - maximum) * unit to the base 2
+  const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
+  NtOperand B{a.rows + (size_t)n0 * a.rows_ld, a.rows_ld, nt_min(TILE::BN, a.n - n0) - 1, a.rows_plane};
+  auto side = [&](uint32_t tile) {
+    const uint32_t r0 = tile * TILE::BM;
+    return NtOperand{a.table + (size_t)r0 * a.table_ld, a.table_ld, nt_min(TILE::BM, a.v - r0) - 1, a.table_plane};
+  };
+  const uint32_t all = a.planes == 2 ? 3 * a.steps : a.steps;
+  float top[TILE::TN], sum[TILE::TN];
+#pragma unroll
+  for (int j = 0; j < TILE::TN; ++j) top[j] = -INFINITY, sum[j] = 0.f;
+  f32x4 acc[TILE::TM][TILE::TN];
+  NtOperand A = side(vt);
+  T.fetch(0, A, B, nt_col_a(0, a.steps, a.table_plane), nt_col_b(0, a.steps, a.rows_plane));
+  int buf = 0;
+  for (; vt < vt_end; ++vt) {
+    T.zero(acc);
+    const uint32_t last = A.last;
+    for (uint32_t s = 0; s < all; ++s) {
+      TILE::turn();
+      if (s + 1 < all) {
+        T.fetch(buf ^ 1, A, B, nt_col_a(s + 1, a.steps, a.table_plane), nt_col_b(s + 1, a.steps, a.rows_plane));
+      } else if (vt + 1 < vt_end) {
+        A = side(vt + 1);
+        T.fetch(buf ^ 1, A, B, nt_col_a(0, a.steps, a.table_plane), nt_col_b(0, a.steps, a.rows_plane));
+      }
+      T.contract(buf, acc);
+      buf ^= 1;
+    }
+    // this tile's logits: a lane holds 4 TM items of each of its TN rows
+    const uint32_t row0 = wm * (TILE::TM * 16) + q * 8;
+    if constexpr (GENERAL) {
+#pragma unroll
+      for (int i = 0; i < TILE::TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t r = row0 + (i >> 1) * 32 + (i & 1) * 4 + e;
+          const float b = a.bias && r <= last ? a.bias[(size_t)vt * TILE::BM + r] : 0.f;
+#pragma unroll
+          for (int j = 0; j < TILE::TN; ++j) acc[i][j][e] = r > last ? -INFINITY : fmaf(acc[i][j][e], nat, b);
+        }
+    } else if (last + 1 < TILE::BM) {
+#pragma unroll
+      for (int i = 0; i < TILE::TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t r = row0 + (i >> 1) * 32 + (i & 1) * 4 + e;
+          if (r > last)
+#pragma unroll
+            for (int j = 0; j < TILE::TN; ++j) acc[i][j][e] = -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < TILE::TN; ++j) {
+      float m = top[j];
+#pragma unroll
+      for (int i = 0; i < TILE::TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[i][j][e]);
+      // (with a bias the difference first: a bias of the type's lowest value times log2 e would be infinite)
+      const float base = m == -INFINITY ? 0.f : m, shift = -base * unit;
+      auto power = [&](float x) { return __builtin_amdgcn_exp2f(GENERAL ? (x - base) * unit : fmaf(x, unit, shift)); };
+      float s0 = sum[j] * power(top[j]), s1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < TILE::TM; ++i) {
+        s0 += power(acc[i][j][0]);
+        s1 += power(acc[i][j][1]);
+        s0 += power(acc[i][j][2]);
+        s1 += power(acc[i][j][3]);
+      }
+      top[j] = m;
+      sum[j] = s0 + s1;
+    }
+  }
+  // the four lane groups of a row
+#pragma unroll
+  for (int j = 0; j < TILE::TN; ++j) {
+    float m = GENERAL ? top[j] : top[j] == -INFINITY ? -INFINITY : top[j] * nat, s = sum[j];
+#pragma unroll
+    for (int x = 16; x < 64; x <<= 1) {
+      const float mo = __shfl_xor(m, x), so = __shfl_xor(s, x);
+      const float mm = fmaxf(m, mo), base = mm == -INFINITY ? 0.f : mm;
+      s = s * __builtin_amdgcn_exp2f((m - base) * kLog2e) + so * __builtin_amdgcn_exp2f((mo - base) * kLog2e);
+      m = mm;
+    }
+    const uint32_t t = n0 + wn * (TILE::TN * 16) + (j >> 1) * 32 + (col >> 2) * 8 + (j & 1) * 4 + (col & 3);
+    if (q == 0 && t < a.n) part[(size_t)(chunk * TILE::WM + wm) * a.n + t] = float2{m, s};
+  }
+}
+
+// A wave a row: the stretches' (maximum, sum) joined, the target's logit from the inputs themselves.  f64 behind the sums: the loss is a
+// difference of two near numbers where the model is right.
+template <int DT>
+__global__ __launch_bounds__(256) void loss_join_kernel(const float2 *part, uint32_t parts, const void *x, size_t x_stride, const void *table,
+                                                        size_t table_stride, const float *bias, const int64_t *targets, uint32_t n, uint32_t v,
+                                                        uint32_t d, float scale, int64_t ignore, float *losses, float *lse_out) {
+  const uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (t >= n) return;
+  float m = -INFINITY;
+  double s = 0.0;
+  for (uint32_t p = lane; p < parts; p += 64) {
+    const float2 o = part[(size_t)p * n + t];
+    const float mm = fmaxf(m, o.x), base = mm == -INFINITY ? 0.f : mm;
+    s = s * (double)exp2f((m - base) * kLog2e) + (double)o.y * (double)exp2f((o.x - base) * kLog2e);
+    m = mm;
+  }
+  float top = m;
+  for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+  const float base = top == -INFINITY ? 0.f : top;
+  s *= (double)exp2f((m - base) * kLog2e);
+  for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+  const int64_t y = targets[t];
+  const bool ignored = y == ignore, inside = y >= 0 && y < (int64_t)v;
+  double dot = 0.0;
+  if (!ignored && inside) {
+    const size_t xr = (size_t)t * x_stride, wr = (size_t)y * table_stride;
+    for (uint32_t k = lane; k < d; k += 64) dot += (double)load_as_f32<DT>(x, xr + k) * (double)load_as_f32<DT>(table, wr + k);
+    for (int k = 1; k < 64; k <<= 1) dot += __shfl_xor(dot, k);
+  }
+  if (lane == 0) {
+    // (no item left by the bias: the maximum and every term are -inf, s = 0)
+    const double lse = s == 0.0 ? -INFINITY : (double)base + log(s);
+    const double logit = (double)scale * dot + (inside && bias ? (double)bias[y] : 0.0);
+    lse_out[t] = (float)lse;
+    losses[t] = ignored || s == 0.0 ? 0.f : !inside ? NAN : (float)(lse - logit);
+  }
+}
+
+// ---- what the products are made of ----------------------------------------------------------------------------------------------------
+__global__ void zero_words_kernel(unsigned int *w, uint32_t n) {
+  if (threadIdx.x < n) w[threadIdx.x] = 0u;
+}
+// the largest finite magnitude of an f32 matrix (bits of a positive float compare as integers; a maximum has no order)
+__global__ __launch_bounds__(256) void top_kernel(const float *x, size_t stride, uint32_t n, uint32_t d, unsigned int *top) {
+  float m = 0.f;
+  for (uint32_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += gridDim.x * 4)
+    for (uint32_t k = threadIdx.x & 63; k < d; k += 64) {
+      const float y = fabsf(x[(size_t)r * stride + k]);
+      if (y < INFINITY) m = fmaxf(m, y);
+    }
+  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+  if ((threadIdx.x & 63) == 0) raise_max_u32(top, __float_as_uint(m));
+}
+// rows with their length filled to whole steps of 64 by zeros; f32 as two planes.  DT the source's type, FMT the image's.
+template <int DT, int FMT>
+__global__ __launch_bounds__(256) void image_kernel(const void *src, size_t stride, uint32_t n, uint32_t d, uint32_t pitch, const unsigned int *top,
+                                                    unsigned short *out) {
+  constexpr bool two = DT == AS_F32;
+  const float f = two ? plane_scale(*top) : 1.f;
+  const uint64_t words = (uint64_t)n * (pitch / 2);
+  for (uint64_t w = (uint64_t)blockIdx.x * 256 + threadIdx.x; w < words; w += (uint64_t)gridDim.x * 256) {
+    const uint64_t r = w / (pitch / 2);
+    const uint32_t k = (uint32_t)(w % (pitch / 2)) * 2;
+    const float x = k < d ? load_as_f32<DT>(src, r * stride + k) * f : 0.f, y = k + 1 < d ? load_as_f32<DT>(src, r * stride + k + 1) * f : 0.f;
+    unsigned short *o = out + r * pitch * (two ? 2 : 1) + k;
+    *(uint32_t *)o = pack2<FMT>(x, y);
+    if constexpr (two) *(uint32_t *)(o + pitch) = pack2<FMT>(low_part(x), low_part(y));
+  }
+}
+// the same transposed: out[k][r], rows filled to `pitch` by zeros.  64 x 64 through LDS.
+template <int DT, int FMT>
+__global__ __launch_bounds__(256) void transposed_kernel(const void *src, size_t stride, uint32_t n, uint32_t d, uint32_t pitch, const unsigned int *top,
+                                                         unsigned short *out) {
+  constexpr bool two = DT == AS_F32;
+  __shared__ float tile[64][65];
+  const float f = two ? plane_scale(*top) : 1.f;
+  const uint32_t r0 = blockIdx.x * 64, k0 = blockIdx.y * 64;
+  for (uint32_t e = threadIdx.x; e < 4096; e += 256) {
+    const uint32_t r = r0 + (e >> 6), k = k0 + (e & 63);
+    tile[e >> 6][e & 63] = r < n && k < d ? load_as_f32<DT>(src, (size_t)r * stride + k) * f : 0.f;
+  }
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < 2048; e += 256) {
+    const uint32_t k = k0 + (e >> 5), rr = (e & 31) * 2;
+    if (k >= d) continue;
+    const float x = tile[rr][e >> 5], y = tile[rr + 1][e >> 5];
+    unsigned short *o = out + (size_t)k * pitch * (two ? 2 : 1) + r0 + rr;
+    *(uint32_t *)o = pack2<FMT>(x, y);
+    if constexpr (two) *(uint32_t *)(o + pitch) = pack2<FMT>(low_part(x), low_part(y));
+  }
+}
+
+// f16 gradients of logits: multiplied by 2^14 over the power of two of the largest coefficient (entries down to 2^-28 of it keep
+// all 11 bits).  One workgroup; reads 16 bytes a row.
+__global__ __launch_bounds__(1024) void coef_scale_kernel(const float *gl, const float *ge, const int64_t *targets, int64_t ignore, uint32_t n, float *out) {
+  __shared__ float s[16];
+  float m = 0.f;
+  for (uint32_t t = threadIdx.x; t < n; t += 1024) {
+    const float l = targets[t] == ignore ? 0.f : gl[t], b = fabsf(l + (ge ? ge[t] : 0.f)), o = fabsf(l);
+    if (o < INFINITY) m = fmaxf(m, o);
+    if (b < INFINITY) m = fmaxf(m, b);
+  }
+  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) m = fmaxf(m, s[w]);
+    const int e = (int)(__float_as_uint(m) >> 23);
+    const int k = e == 0 ? 0 : min(max(14 - (e - 126), -100), 100);  // m < 2^(e - 126)
+    out[0] = __uint_as_float((unsigned int)(127 + k) << 23);
+    out[1] = __uint_as_float((unsigned int)(127 - k) << 23);
+  }
+}
+
+// ---- gradient of the logits ---------------------------------------------------------------------------------------------------------------
+struct GradArgs {
+  LossArgs l;
+  uint32_t v_begin, v_all;         // first item of the piece (the operand A starts there); items of the table
+  const float *lse, *gl, *ge;
+  const int64_t *targets;
+  int64_t ignore;
+  const float *coef;               // {factor, 1 / factor} of G, or null: 1
+  unsigned short *G, *GT;          // n x (planes * g_pitch), v_pad x (planes * t_pitch)
+  uint32_t g_pitch, t_pitch;
+  float *bias_part;                // (n_tiles WN) x g_pitch sums over the tile's rows, or null
+};
+
+template <int FMT, class TILE_, bool TWO, bool BIAS>
+__global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
+  using TILE = TILE_;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * TILE::kStage];
+  const LossArgs &a = g.l;
+  TILE T;
+  T.init(smem);
+  const uint32_t work = die_order(blockIdx.x, gridDim.x);
+  const uint32_t nt = work % a.n_tiles, chunk = work / a.n_tiles;
+  const uint32_t n0 = nt * TILE::BN, vt_end = nt_min((chunk + 1) * a.per, a.v_tiles);
+  uint32_t vt = chunk * a.per;
+  const float c = a.scale * product_scale(a), factor = g.coef ? g.coef[0] : 1.f;
+  const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
+  NtOperand B{a.rows + (size_t)n0 * a.rows_ld, a.rows_ld, nt_min(TILE::BN, a.n - n0) - 1, a.rows_plane};
+  auto side = [&](uint32_t tile) {
+    const uint32_t r0 = tile * TILE::BM;
+    return NtOperand{a.table + (size_t)r0 * a.table_ld, a.table_ld, nt_min(TILE::BM, a.v - r0) - 1, a.table_plane};
+  };
+  // this lane's rows
+  uint32_t row[TILE::TN];
+  float lse[TILE::TN], every[TILE::TN], one[TILE::TN];
+  int32_t hit[TILE::TN];  // the target within the piece, or far off
+#pragma unroll
+  for (int j = 0; j < TILE::TN; ++j) {
+    const uint32_t t = n0 + wn * (TILE::TN * 16) + (j >> 1) * 32 + (col >> 2) * 8 + (j & 1) * 4 + (col & 3);
+    row[j] = t;
+    lse[j] = INFINITY;  // (rows behind the last: every probability 0)
+    every[j] = one[j] = 0.f;
+    hit[j] = -1;
+    if (t < a.n) {
+      const int64_t y = g.targets[t];
+      const bool counted = y != g.ignore && y >= 0 && y < (int64_t)g.v_all;
+      const float l = counted ? g.gl[t] : 0.f;
+      lse[j] = g.lse[t];
+      one[j] = l * factor;
+      every[j] = (l + (g.ge ? g.ge[t] : 0.f)) * factor;
+      const int64_t at = y - (int64_t)g.v_begin;
+      if (counted && at >= 0 && at < (int64_t)a.v) hit[j] = (int32_t)at;
+      if (lse[j] == -INFINITY) every[j] = one[j] = 0.f, lse[j] = INFINITY, hit[j] = -1;  // no item left by the bias: no gradient
+    }
+  }
+  const uint32_t all = a.planes == 2 ? 3 * a.steps : a.steps;
+  f32x4 acc[TILE::TM][TILE::TN];
+  NtOperand A = side(vt);
+  T.fetch(0, A, B, nt_col_a(0, a.steps, a.table_plane), nt_col_b(0, a.steps, a.rows_plane));
+  int buf = 0;
+  for (; vt < vt_end; ++vt) {
+    T.zero(acc);
+    const uint32_t last = A.last;
+    for (uint32_t s = 0; s < all; ++s) {
+      TILE::turn();
+      if (s + 1 < all) {
+        T.fetch(buf ^ 1, A, B, nt_col_a(s + 1, a.steps, a.table_plane), nt_col_b(s + 1, a.steps, a.rows_plane));
+      } else if (vt + 1 < vt_end) {
+        A = side(vt + 1);
+        T.fetch(buf ^ 1, A, B, nt_col_a(0, a.steps, a.table_plane), nt_col_b(0, a.steps, a.rows_plane));
+      }
+      T.contract(buf, acc);
+      buf ^= 1;
+    }
+    const uint32_t row0 = wm * (TILE::TM * 16) + q * 8;   // within the tile
+    const uint32_t at0 = vt * TILE::BM;                   // of the tile within the piece
+#pragma unroll
+    for (int i = 0; i < TILE::TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t r = row0 + (i >> 1) * 32 + (i & 1) * 4 + e;
+        float b = 0.f;
+        if constexpr (BIAS) b = r > last ? -INFINITY : a.bias[at0 + r];
+#pragma unroll
+        for (int j = 0; j < TILE::TN; ++j) {
+          const float z = BIAS ? fmaf(acc[i][j][e], c, b) - lse[j] : fmaf(acc[i][j][e], c, -lse[j]);
+          acc[i][j][e] = every[j] * __builtin_amdgcn_exp2f(z * kLog2e);
+        }
+      }
+    if (last + 1 < TILE::BM) {
+#pragma unroll
+      for (int i = 0; i < TILE::TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (row0 + (i >> 1) * 32 + (i & 1) * 4 + e > last)
+#pragma unroll
+            for (int j = 0; j < TILE::TN; ++j) acc[i][j][e] = 0.f;
+    }
+    // the targets: few of the tiles hold one of the wave's rows' (hit < 0 is far above any place of the tile)
+    const uint32_t wave0 = at0 + wm * (TILE::TM * 16);
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < TILE::TN; ++j) any |= (uint32_t)hit[j] - wave0 < (uint32_t)(TILE::TM * 16) && hit[j] >= 0;
+    if (__any(any)) {
+#pragma unroll
+      for (int j = 0; j < TILE::TN; ++j)
+#pragma unroll
+        for (int i = 0; i < TILE::TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (hit[j] == (int32_t)(at0 + row0 + (i >> 1) * 32 + (i & 1) * 4 + e)) acc[i][j][e] -= one[j];
+    }
+    if constexpr (BIAS) {
+      if (g.bias_part) {
+        float *bp = g.bias_part + (size_t)(nt * TILE::WN + wn) * g.g_pitch + at0;
+#pragma unroll
+        for (int i = 0; i < TILE::TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < TILE::TN; ++j) s += row[j] < a.n ? acc[i][j][e] : 0.f;
+            s = add16(s);
+            if (col == 0) bp[row0 + (i >> 1) * 32 + (i & 1) * 4 + e] = s;
+          }
+      }
+    }
+    // two columns of accumulators at a time (what is packed and not yet stored stays in registers)
+    const size_t gp = (size_t)g.g_pitch * (TWO ? 2 : 1), tp = (size_t)g.t_pitch * (TWO ? 2 : 1);
+    const bool odd = col & 1, high = col & 2;
+    const uint32_t s0 = odd ? 0x01000504u : 0x05040100u, s1 = odd ? 0x03020706u : 0x07060302u;
+    const uint32_t item = ((col & 1) << 1) | ((col >> 1) & 1);
+    const uint32_t t0 = n0 + wn * (TILE::TN * 16) + (col >> 2) * 8;
+#pragma unroll
+    for (int jj = 0; jj < TILE::TN; jj += 2)
+#pragma unroll
+      for (int plane = 0; plane < (TWO ? 2 : 1); ++plane) {
+        uint32_t w[TILE::TM][2][2];
+#pragma unroll
+        for (int i = 0; i < TILE::TM; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            f32x4 u = acc[i][jj + h];
+            if (TWO && plane == 1) u = f32x4{low_part(u[0]), low_part(u[1]), low_part(u[2]), low_part(u[3])};
+            w[i][h][0] = pack2<FMT>(u[0], u[1]);
+            w[i][h][1] = pack2<FMT>(u[2], u[3]);
+          }
+        // row-major: eight consecutive items a lane
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (row[jj + h] < a.n) {
+            unsigned short *o = g.G + (size_t)row[jj + h] * gp + plane * g.g_pitch + at0 + row0;
+#pragma unroll
+            for (int i = 0; i < TILE::TM; i += 2) *(u32x4 *)(o + i * 16) = u32x4{w[i][h][0], w[i][h][1], w[i + 1][h][0], w[i + 1][h][1]};
+          }
+        // transposed: the quad's four rows of an item meet in one lane (4 x 4 over the quad, two exchanges), eight consecutive rows a lane
+#pragma unroll
+        for (int i = 0; i < TILE::TM; ++i) {
+          uint32_t y[4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t mine = odd ? w[i][h][1] : w[i][h][0], theirs = quad_xor1(odd ? w[i][h][0] : w[i][h][1]);
+            const uint32_t x0 = __builtin_amdgcn_perm(theirs, mine, s0), x1 = __builtin_amdgcn_perm(theirs, mine, s1);
+            const uint32_t other = quad_xor2(high ? x0 : x1);
+            y[2 * h] = high ? other : x0;
+            y[2 * h + 1] = high ? x1 : other;
+          }
+          *(u32x4 *)(g.GT + (size_t)(at0 + row0 + (i >> 1) * 32 + (i & 1) * 4 + item) * tp + plane * g.t_pitch + t0 + jj * 16) = u32x4{y[0], y[1], y[2], y[3]};
+        }
+      }
+  }
+}
+
+// ---- the two gradients: plain products ------------------------------------------------------------------------------------------------------
+struct ProductArgs {
+  const char *A, *B;
+  size_t a_ld, b_ld;
+  uint32_t a_plane, b_plane;
+  uint32_t m, n, m_tiles, n_tiles;
+  uint32_t steps, planes, splits;   // steps of 64 of the whole contraction; a split takes an even share of them
+  float scale;
+  const float *coef;                // 1 / factor of G at [1], or null
+  const unsigned int *top;          // largest magnitude of the other operand's matrix (two planes), or null
+  void *out;                        // n x m rows of `out_stride` elements
+  size_t out_stride;
+  float *sums;                      // instead: f32 [split][n][sums_pitch], added to unless `first`
+  uint32_t sums_pitch;
+  int first, aligned;
+};
+template <int FMT, class TILE_, int OUT>  // OUT: element type of `out`, or 0 (AS_F64) = into `sums`
+__global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
+  using TILE = TILE_;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * TILE::kStage];
+  TILE T;
+  T.init(smem);
+  const uint32_t work = die_order(blockIdx.x, gridDim.x);
+  const uint32_t mt = work % p.m_tiles, rest = work / p.m_tiles, nt = rest % p.n_tiles, split = rest / p.n_tiles;
+  const uint32_t m0 = mt * TILE::BM, n0 = nt * TILE::BN;
+  const uint32_t k0 = (uint32_t)((uint64_t)p.steps * split / p.splits), k1 = (uint32_t)((uint64_t)p.steps * (split + 1) / p.splits);
+  const uint32_t steps = k1 - k0, all = p.planes == 2 ? 3 * steps : steps;
+  const NtOperand A{p.A + (size_t)m0 * p.a_ld + (size_t)k0 * 128, p.a_ld, nt_min(TILE::BM, p.m - m0) - 1, p.a_plane};
+  const NtOperand B{p.B + (size_t)n0 * p.b_ld + (size_t)k0 * 128, p.b_ld, nt_min(TILE::BN, p.n - n0) - 1, p.b_plane};
+  f32x4 acc[TILE::TM][TILE::TN];
+  T.zero(acc);
+  if (all) T.fetch(0, A, B, 0, nt_col_b(0, steps, p.b_plane));
+  int buf = 0;
+  for (uint32_t s = 0; s < all; ++s) {
+    TILE::turn();
+    if (s + 1 < all) T.fetch(buf ^ 1, A, B, nt_col_a(s + 1, steps, p.a_plane), nt_col_b(s + 1, steps, p.b_plane));
+    T.contract(buf, acc);
+    buf ^= 1;
+  }
+  const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
+  const float f = OUT == 0 ? 1.f : p.scale * (p.coef ? p.coef[1] : 1.f) * (p.top ? 1.f / plane_scale(*p.top) : 1.f);
+#pragma unroll
+  for (int j = 0; j < TILE::TN; ++j) {
+    const uint32_t n = n0 + wn * (TILE::TN * 16) + (j >> 1) * 32 + (col >> 2) * 8 + (j & 1) * 4 + (col & 3);
+    if (n >= p.n) continue;
+#pragma unroll
+    for (int i = 0; i < TILE::TM; i += 2) {
+      const uint32_t m = m0 + wm * (TILE::TM * 16) + i * 16 + q * 8;
+      if (m >= p.m) continue;
+      const f32x4 u = acc[i][j] * f, v = acc[i + 1][j] * f;
+      if constexpr (OUT == 0) {
+        float *o = p.sums + ((size_t)split * p.n + n) * p.sums_pitch + m;
+        f32x4 *o4 = (f32x4 *)o;  // (the pitch is a multiple of 8)
+        if (p.first) o4[0] = u, o4[1] = v;
+        else o4[0] += u, o4[1] += v;
+      } else if (p.aligned && m + 8 <= p.m) {
+        if constexpr (OUT == AS_F32) {
+          f32x4 *o = (f32x4 *)((float *)p.out + (size_t)n * p.out_stride + m);
+          o[0] = u, o[1] = v;
+        } else {
+          *(u32x4 *)((unsigned short *)p.out + (size_t)n * p.out_stride + m) =
+              u32x4{pack2<OUT>(u[0], u[1]), pack2<OUT>(u[2], u[3]), pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (m + e < p.m) store_from_f32<OUT>(p.out, (size_t)n * p.out_stride + m + e, e < 4 ? u[e & 3] : v[e & 3]);
+      }
+    }
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void grad_rows_join_kernel(const float *sums, uint32_t splits, uint32_t pitch, uint32_t n, uint32_t d, float scale,
+                                                             const float *coef, const unsigned int *top, void *out, size_t out_stride) {
+  const float f = scale * (coef ? coef[1] : 1.f) * (top ? 1.f / plane_scale(*top) : 1.f);
+  const uint64_t total = (uint64_t)n * d;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
+    const uint64_t t = i / d, k = i % d;
+    float s = 0.f;
+    for (uint32_t p = 0; p < splits; ++p) s += sums[((size_t)p * n + t) * pitch + k];
+    store_from_f32<DT>(out, t * out_stride + k, s * f);
+  }
+}
+__global__ __launch_bounds__(256) void bias_join_kernel(const float *part, uint32_t parts, uint32_t pitch, uint32_t v, const float *coef, float *out) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= v) return;
+  float s = 0.f;
+  for (uint32_t p = 0; p < parts; ++p) s += part[(size_t)p * pitch + i];
+  out[i] = s * (coef ? coef[1] : 1.f);
+}
+template <int DT>
+__global__ __launch_bounds__(256) void zero_rows_kernel(void *out, size_t stride, uint64_t n, uint32_t d) {
+  const uint64_t total = n * d;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256)
+    store_from_f32<DT>(out, (i / d) * stride + i % d, 0.f);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------------------------
+template <int FMT>
+using Slim = NtTile<FMT, 4, 4, 4, 1>;   // 256 x 64
+template <int FMT>
+using Square = NtTile<FMT, 4, 4, 2, 2>; // 128 x 128
+template <int FMT>
+using Large = NtTile<FMT, 8, 4, 2, 4>;  // 256 x 256
+enum { kSlim = 0, kSquare = 1, kLarge = 2 };
+struct TileShape {
+  uint32_t bm, bn, wm, wn;
+};
+constexpr TileShape kShape[3] = {{256, 64, 4, 1}, {128, 128, 2, 2}, {256, 256, 2, 4}};
+
+uint32_t up(uint64_t a, uint32_t b) { return (uint32_t)((a + b - 1) / b * b); }
+
+// How a matrix reaches the products: as it is, or as an image (whole steps of 64, 16-byte rows; f32 always: two planes).
+struct Source {
+  const void *p;
+  size_t stride;
+  uint32_t rows, d;
+  int dt;
+  bool direct() const { return dt != AS_F32 && d % 64 == 0 && stride % 8 == 0 && ((uintptr_t)p & 15) == 0; }
+  uint32_t pitch() const { return up(d, 64); }
+  uint32_t planes() const { return dt == AS_F32 ? 2 : 1; }
+  uint64_t image_elems() const { return direct() ? 0 : (uint64_t)rows * pitch() * planes(); }
+};
+int image_format(int dt) { return dt == AS_BF16 ? AS_BF16 : AS_F16; }
+
+// tile of the products of the logits
+int logits_tile(uint32_t n, uint32_t v) {
+  if (n <= 64) return kSlim;
+  if (n <= 128) return kSquare;
+  // the large tile where the chip gets two rounds of them; below, four times as many small ones
+  return (uint64_t)cdiv(n, 256) * cdiv(v, 256) >= 2 * kChips ? kLarge : kSquare;
+}
+int grad_tile(uint32_t m, uint32_t n) {
+  if (n <= 64) return kSlim;
+  if (m <= 128 || n <= 128) return kSquare;
+  return (uint64_t)cdiv(m, 256) * cdiv(n, 256) >= kChips ? kLarge : kSquare;
+}
+
+struct Plan {
+  uint32_t n, v, d, planes, steps, pitch;
+  int tile;
+  uint32_t n_tiles, v_tiles, per, chunks;
+  // backward
+  uint32_t piece, pieces, t_pitch, splits;
+  int tile_w, tile_x;
+  bool want_x, want_w, want_b, scaled;
+};
+Plan make_plan(uint32_t n, uint32_t v, uint32_t d, int dt) {
+  Plan p{};
+  p.n = n, p.v = v, p.d = d;
+  p.planes = dt == AS_F32 ? 2 : 1;
+  p.steps = cdiv(d, 64);
+  p.pitch = p.steps * 64;
+  p.tile = logits_tile(n, v);
+  p.n_tiles = cdiv(n, kShape[p.tile].bn);
+  p.v_tiles = cdiv(v, kShape[p.tile].bm);
+  return p;
+}
+// tiles a workgroup walks: at least four rounds of workgroups on the chip, so that the last one costs little
+void plan_walk(Plan &p) {
+  const uint64_t tiles = (uint64_t)p.n_tiles * p.v_tiles, groups = 4ull * kChips;
+  p.per = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(p.v_tiles, tiles / groups));
+  p.chunks = cdiv(p.v_tiles, p.per);
+}
+void plan_backward(Plan &p, bool x, bool w, bool b, bool scaled) {
+  p.want_x = x, p.want_w = w, p.want_b = b, p.scaled = scaled;
+  const uint32_t bm = kShape[p.tile].bm, bn = kShape[p.tile].bn;
+  p.t_pitch = up(p.n, std::max(bn, 64u));
+  // G and its transposed form of a piece: 512 MB together (the two products that read them want thousands of items), whole tiles
+  const uint64_t per_item = (uint64_t)p.t_pitch * 2 * 2 * p.planes;
+  uint64_t piece = std::max<uint64_t>((512ull << 20) / per_item / 1024 * 1024, 1024);
+  piece = std::min<uint64_t>(piece, up(p.v, bm));
+  p.piece = (uint32_t)up(piece, bm);
+  p.pieces = cdiv(p.v, p.piece);
+  p.piece = up(cdiv(p.v, p.pieces), bm);  // even pieces
+  p.pieces = cdiv(p.v, p.piece);
+  p.v_tiles = cdiv(p.piece, bm);
+  plan_walk(p);
+  p.tile_w = grad_tile(p.d, std::min(p.piece, p.v));
+  p.tile_x = p.n <= 64 ? kSlim : p.d <= 128 || p.n <= 128 ? kSquare : kLarge;
+  const uint64_t tiles = (uint64_t)cdiv(p.d, kShape[p.tile_x].bm) * cdiv(p.n, kShape[p.tile_x].bn);
+  // the contraction over the piece is split where the output alone does not fill the chip
+  const uint64_t want = (p.tile_x == kLarge ? 1 : 2) * kChips;
+  p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(want / std::max<uint64_t>(tiles, 1), 64), cdiv(p.piece, 256)));
+}
+
+struct ForwardScratch {
+  float2 *part;
+  unsigned int *tops;
+  unsigned short *x_image, *t_image;
+};
+uint64_t forward_layout(const Plan &p, const Source &x, const Source &t, char *base, ForwardScratch &s) {
+  Layout l{base};
+  s.part = l.take<float2>((uint64_t)p.chunks * kShape[p.tile].wm * p.n);
+  s.tops = l.take<unsigned int>(2);
+  s.x_image = l.take<unsigned short>(x.image_elems());
+  s.t_image = l.take<unsigned short>(t.image_elems());
+  return l.at;
+}
+struct BackwardScratch {
+  unsigned int *tops;
+  float *coef;
+  unsigned short *x_image, *t_image, *xt, *wt, *G, *GT;
+  float *sums, *bias_part;
+};
+uint64_t backward_layout(const Plan &p, const Source &x, const Source &t, char *base, BackwardScratch &s) {
+  Layout l{base};
+  const uint64_t pl = p.planes;
+  s.tops = l.take<unsigned int>(2);
+  s.coef = l.take<float>(2);
+  s.x_image = l.take<unsigned short>(x.image_elems());
+  s.t_image = l.take<unsigned short>(t.image_elems());
+  s.xt = l.take<unsigned short>(p.want_w ? (uint64_t)p.d * p.t_pitch * pl : 0);
+  s.wt = l.take<unsigned short>(p.want_x ? (uint64_t)p.d * p.piece * pl : 0);
+  s.G = l.take<unsigned short>((uint64_t)p.n * p.piece * pl);
+  s.GT = l.take<unsigned short>((uint64_t)p.piece * p.t_pitch * pl);
+  s.sums = l.take<float>(p.want_x ? (uint64_t)p.splits * p.n * up(p.d, 8) : 0);
+  s.bias_part = l.take<float>(p.want_b ? (uint64_t)p.n_tiles * kShape[p.tile].wn * p.piece : 0);
+  return l.at;
+}
+
+template <class F>
+void by_tile(int tile, F &&f) {
+  if (tile == kSlim) f(std::integral_constant<int, kSlim>{});
+  else if (tile == kSquare) f(std::integral_constant<int, kSquare>{});
+  else f(std::integral_constant<int, kLarge>{});
+}
+template <int FMT, int K>
+using TileOf = std::conditional_t<K == kSlim, Slim<FMT>, std::conditional_t<K == kSquare, Square<FMT>, Large<FMT>>>;
+template <class F>
+void by_type(int dt, F &&f) {
+  if (dt == AS_F32) f(std::integral_constant<int, AS_F32>{});
+  else if (dt == AS_BF16) f(std::integral_constant<int, AS_BF16>{});
+  else f(std::integral_constant<int, AS_F16>{});
+}
+unsigned spread(uint64_t items, uint64_t per_block) { return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((items + per_block - 1) / per_block, 16384)); }
+
+int make_tops(as_ctx *ctx, const Source &x, const Source &t, unsigned int *tops) {
+  if (x.dt != AS_F32) return AS_OK;
+  hipLaunchKernelGGL(zero_words_kernel, dim3(1), dim3(64), 0, ctx->stream, tops, 2u);
+  hipLaunchKernelGGL(top_kernel, dim3(std::min(cdiv(x.rows, 4), 1024u)), dim3(256), 0, ctx->stream, (const float *)x.p, x.stride, x.rows, x.d, tops);
+  hipLaunchKernelGGL(top_kernel, dim3(std::min(cdiv(t.rows, 4), 1024u)), dim3(256), 0, ctx->stream, (const float *)t.p, t.stride, t.rows, t.d, tops + 1);
+  AS_HIP(ctx, hipGetLastError());
+  return AS_OK;
+}
+int make_image(as_ctx *ctx, const Source &s, const unsigned int *top, unsigned short *image, const char **p, size_t *ld) {
+  if (s.direct()) {
+    *p = (const char *)s.p;
+    *ld = s.stride * 2;
+    return AS_OK;
+  }
+  by_type(s.dt, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    hipLaunchKernelGGL((image_kernel<DT, DT == AS_BF16 ? AS_BF16 : AS_F16>), dim3(spread((uint64_t)s.rows * s.pitch() / 2, 1024)), dim3(256), 0, ctx->stream,
+                       s.p, s.stride, s.rows, s.d, s.pitch(), top, image);
+  });
+  AS_HIP(ctx, hipGetLastError());
+  *p = (const char *)image;
+  *ld = (size_t)s.pitch() * s.planes() * 2;
+  return AS_OK;
+}
+void make_transposed(as_ctx *ctx, const Source &s, uint32_t row0, uint32_t rows, uint32_t pitch, const unsigned int *top, unsigned short *out) {
+  const char *p = (const char *)s.p + (size_t)row0 * s.stride * dtype_size(s.dt);
+  by_type(s.dt, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    hipLaunchKernelGGL((transposed_kernel<DT, DT == AS_BF16 ? AS_BF16 : AS_F16>), dim3(pitch / 64, cdiv(s.d, 64)), dim3(256), 0, ctx->stream, (const void *)p,
+                       s.stride, rows, s.d, pitch, top, out);
+  });
+}
+void launch_product(as_ctx *ctx, int fmt, int tile, int out_type, const ProductArgs &p) {
+  by_tile(tile, [&](auto k) {
+    constexpr int K = decltype(k)::value;
+    const dim3 grid(p.m_tiles * p.n_tiles * p.splits);
+    auto go = [&](auto f, auto o) {
+      constexpr int FMT = decltype(f)::value, OUT = decltype(o)::value;
+      hipLaunchKernelGGL((product_kernel<FMT, TileOf<FMT, K>, OUT>), grid, dim3(TileOf<FMT, K>::NT), 0, ctx->stream, p);
+    };
+    constexpr std::integral_constant<int, AS_BF16> bf{};
+    constexpr std::integral_constant<int, AS_F16> hf{};
+    constexpr std::integral_constant<int, AS_F32> f32{};
+    constexpr std::integral_constant<int, 0> acc{};
+    if (fmt == AS_BF16) out_type == 0 ? go(bf, acc) : go(bf, bf);
+    else out_type == 0 ? go(hf, acc) : out_type == AS_F32 ? go(hf, f32) : go(hf, hf);
+  });
+}
+
+struct LossCall {
+  uint64_t n, v, d, x_stride, table_stride;
+  int dt;
+  float scale;
+};
+int check_loss(as_ctx *ctx, const LossCall &c) {
+  if (!ctx) return AS_ERR_ARG;
+  if (hipSetDevice(ctx->device) != hipSuccess) return fail(ctx, AS_ERR_HIP, "hipSetDevice failed");
+  if (!dtype_is_training(c.dt)) return fail(ctx, AS_ERR_ARG, "dtype must be AS_F32, AS_BF16 or AS_F16");
+  if (c.v == 0 || c.d == 0) return fail(ctx, AS_ERR_SHAPE, "the table needs at least one row and one column");
+  if (c.n >= (1ull << 31) || c.v >= (1ull << 31) || c.d > 65536) return fail(ctx, AS_ERR_UNSUPPORTED, "at most 2^31 - 1 rows and items and 65536 columns");
+  if (c.x_stride < c.d || c.table_stride < c.d) return fail(ctx, AS_ERR_ARG, "a row stride below the number of columns");
+  if (!std::isfinite(c.scale)) return fail(ctx, AS_ERR_ARG, "scale must be finite");
+  return AS_OK;
+}
+// targets in host memory are looked over here; on the device a target outside the table makes its loss NaN (and its row counts as ignored
+// in the gradients)
+int check_targets(as_ctx *ctx, const int64_t *targets, uint64_t n, uint64_t v, int64_t ignore) {
+  if (n == 0 || pointer_home(ctx, targets) != 0) return AS_OK;
+  for (uint64_t t = 0; t < n; ++t)
+    if (targets[t] != ignore && (targets[t] < 0 || targets[t] >= (int64_t)v))
+      return fail(ctx, AS_ERR_ARG, "target " + std::to_string(targets[t]) + " of row " + std::to_string(t) + " is outside the table");
+  return AS_OK;
+}
+uint64_t span(uint64_t rows, uint64_t stride, uint64_t d, int dt) { return rows ? ((rows - 1) * stride + d) * dtype_size(dt) : 0; }
+
+int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *table, const float *bias, const int64_t *targets, int64_t ignore, float *losses,
+                 float *lse, void *workspace, uint64_t workspace_bytes) {
+  AS_TRY(check_loss(ctx, c));
+  if (c.n == 0) return AS_OK;
+  if (!x || !table || !targets || !losses || !lse) return fail(ctx, AS_ERR_ARG, "null argument");
+  AS_TRY(check_targets(ctx, targets, c.n, c.v, ignore));
+  BytesIn X, W, Bi, Y;
+  BytesOut L, S;
+  AS_TRY(X.bind(ctx, x, span(c.n, c.x_stride, c.d, c.dt)));
+  AS_TRY(W.bind(ctx, table, span(c.v, c.table_stride, c.d, c.dt)));
+  AS_TRY(Bi.bind(ctx, bias, bias ? c.v * 4 : 0));
+  AS_TRY(Y.bind(ctx, targets, c.n * 8));
+  AS_TRY(L.bind(ctx, losses, c.n * 4));
+  AS_TRY(S.bind(ctx, lse, c.n * 4));
+  const Source xs{X.p, (size_t)c.x_stride, (uint32_t)c.n, (uint32_t)c.d, c.dt}, ts{W.p, (size_t)c.table_stride, (uint32_t)c.v, (uint32_t)c.d, c.dt};
+  Plan p = make_plan((uint32_t)c.n, (uint32_t)c.v, (uint32_t)c.d, c.dt);
+  plan_walk(p);
+  ForwardScratch s{};
+  Scratch scratch;
+  AS_TRY(scratch.open(ctx, workspace, workspace_bytes, forward_layout(p, xs, ts, nullptr, s)));
+  forward_layout(p, xs, ts, scratch.base, s);
+  ProfScope prof(ctx, "cross_entropy");
+  LossArgs a{};
+  AS_TRY(make_tops(ctx, xs, ts, s.tops));
+  AS_TRY(make_image(ctx, xs, s.tops, s.x_image, &a.rows, &a.rows_ld));
+  AS_TRY(make_image(ctx, ts, s.tops + 1, s.t_image, &a.table, &a.table_ld));
+  a.table_plane = a.rows_plane = p.steps;
+  a.n = p.n, a.v = p.v, a.steps = p.steps, a.planes = p.planes, a.per = p.per, a.v_tiles = p.v_tiles, a.n_tiles = p.n_tiles, a.chunks = p.chunks;
+  a.scale = c.scale, a.bias = (const float *)Bi.p;
+  if (p.planes == 2) a.rows_top = s.tops, a.table_top = s.tops + 1;
+  const bool general = bias || !(c.scale > 0.f);
+  by_tile(p.tile, [&](auto k) {
+    constexpr int K = decltype(k)::value;
+    auto go = [&](auto f, auto gen) {
+      constexpr int FMT = decltype(f)::value;
+      hipLaunchKernelGGL((loss_sums_kernel<FMT, TileOf<FMT, K>, decltype(gen)::value>), dim3(p.n_tiles * p.chunks), dim3(TileOf<FMT, K>::NT), 0, ctx->stream, a,
+                         s.part);
+    };
+    constexpr std::integral_constant<int, AS_BF16> bf{};
+    constexpr std::integral_constant<int, AS_F16> hf{};
+    if (c.dt == AS_BF16) general ? go(bf, std::true_type{}) : go(bf, std::false_type{});
+    else general ? go(hf, std::true_type{}) : go(hf, std::false_type{});
+  });
+  AS_HIP(ctx, hipGetLastError());
+  by_type(c.dt, [&](auto dt) {
+    hipLaunchKernelGGL((loss_join_kernel<decltype(dt)::value>), dim3(cdiv(c.n, 4)), dim3(256), 0, ctx->stream, (const float2 *)s.part,
+                       p.chunks * kShape[p.tile].wm, X.p, (size_t)c.x_stride, W.p, (size_t)c.table_stride, (const float *)Bi.p, (const int64_t *)Y.p, p.n, p.v, p.d,
+                       c.scale, ignore, (float *)L.p, (float *)S.p);
+  });
+  AS_HIP(ctx, hipGetLastError());
+  AS_TRY(L.finish(ctx));
+  AS_TRY(S.finish(ctx));
+  return finish_call(ctx);
+}
+
+int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *table, const float *bias, const int64_t *targets, int64_t ignore, const float *lse,
+                  const float *gl, const float *ge, void *gx, uint64_t gx_stride, void *gw, uint64_t gw_stride, float *gb, void *workspace,
+                  uint64_t workspace_bytes) {
+  AS_TRY(check_loss(ctx, c));
+  if (gb && !bias) return fail(ctx, AS_ERR_ARG, "a gradient of the bias without a bias");
+  if ((gx && gx_stride < c.d) || (gw && gw_stride < c.d)) return fail(ctx, AS_ERR_ARG, "a row stride below the number of columns");
+  if (!gx && !gw && !gb) return AS_OK;
+  if (c.n && (!x || !table || !targets || !lse || !gl)) return fail(ctx, AS_ERR_ARG, "null argument");
+  AS_TRY(check_targets(ctx, targets, c.n, c.v, ignore));
+  BytesIn X, W, Bi, Y, Ls, Gl, Ge;
+  BytesOut Ox, Ow, Ob;
+  AS_TRY(X.bind(ctx, x, span(c.n, c.x_stride, c.d, c.dt)));
+  AS_TRY(W.bind(ctx, table, span(c.n ? c.v : 0, c.table_stride, c.d, c.dt)));
+  AS_TRY(Bi.bind(ctx, bias, bias ? c.v * 4 : 0));
+  AS_TRY(Y.bind(ctx, targets, c.n * 8));
+  AS_TRY(Ls.bind(ctx, lse, c.n * 4));
+  AS_TRY(Gl.bind(ctx, gl, c.n * 4));
+  AS_TRY(Ge.bind(ctx, ge, ge ? c.n * 4 : 0));
+  if (gx && c.n && pointer_home(ctx, gx) == 0 && gx_stride != c.d) return fail(ctx, AS_ERR_ARG, "gradients in host memory must be dense");
+  if (gw && pointer_home(ctx, gw) == 0 && gw_stride != c.d) return fail(ctx, AS_ERR_ARG, "gradients in host memory must be dense");
+  AS_TRY(Ox.bind(ctx, gx, span(c.n, gx_stride, c.d, c.dt)));
+  AS_TRY(Ow.bind(ctx, gw, span(c.v, gw_stride, c.d, c.dt)));
+  AS_TRY(Ob.bind(ctx, gb, c.v * 4));
+  ProfScope prof(ctx, "cross_entropy_backward");
+  if (c.n == 0) {  // a sum over no rows
+    if (gw)
+      by_type(c.dt, [&](auto dt) {
+        hipLaunchKernelGGL((zero_rows_kernel<decltype(dt)::value>), dim3(spread(c.v * c.d, 1024)), dim3(256), 0, ctx->stream, Ow.p, (size_t)gw_stride, c.v, (uint32_t)c.d);
+      });
+    if (gb) hipLaunchKernelGGL((zero_rows_kernel<AS_F32>), dim3(spread(c.v, 1024)), dim3(256), 0, ctx->stream, Ob.p, (size_t)1, c.v, 1u);
+    AS_HIP(ctx, hipGetLastError());
+    AS_TRY(Ow.finish(ctx));
+    AS_TRY(Ob.finish(ctx));
+    return finish_call(ctx);
+  }
+  const Source xs{X.p, (size_t)c.x_stride, (uint32_t)c.n, (uint32_t)c.d, c.dt}, ts{W.p, (size_t)c.table_stride, (uint32_t)c.v, (uint32_t)c.d, c.dt};
+  Plan p = make_plan((uint32_t)c.n, (uint32_t)c.v, (uint32_t)c.d, c.dt);
+  plan_backward(p, gx != nullptr, gw != nullptr, gb != nullptr, c.dt != AS_BF16);
+  BackwardScratch s{};
+  Scratch scratch;
+  AS_TRY(scratch.open(ctx, workspace, workspace_bytes, backward_layout(p, xs, ts, nullptr, s)));
+  backward_layout(p, xs, ts, scratch.base, s);
+  GradArgs g{};
+  LossArgs &a = g.l;
+  const char *table16 = nullptr;
+  AS_TRY(make_tops(ctx, xs, ts, s.tops));
+  AS_TRY(make_image(ctx, xs, s.tops, s.x_image, &a.rows, &a.rows_ld));
+  AS_TRY(make_image(ctx, ts, s.tops + 1, s.t_image, &table16, &a.table_ld));
+  const unsigned int *x_top = p.planes == 2 ? s.tops : nullptr, *w_top = p.planes == 2 ? s.tops + 1 : nullptr;
+  if (p.want_w) make_transposed(ctx, xs, 0, p.n, p.t_pitch, x_top, s.xt);
+  if (p.scaled) hipLaunchKernelGGL(coef_scale_kernel, dim3(1), dim3(1024), 0, ctx->stream, (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p, ignore, p.n, s.coef);
+  AS_HIP(ctx, hipGetLastError());
+  const float *coef = p.scaled ? s.coef : nullptr;
+  a.table_plane = a.rows_plane = p.steps;
+  a.n = p.n, a.steps = p.steps, a.planes = p.planes, a.n_tiles = p.n_tiles, a.per = p.per;
+  a.scale = c.scale;
+  a.rows_top = x_top, a.table_top = w_top;
+  g.lse = (const float *)Ls.p, g.gl = (const float *)Gl.p, g.ge = (const float *)Ge.p, g.targets = (const int64_t *)Y.p, g.ignore = ignore, g.coef = coef;
+  g.G = s.G, g.GT = s.GT, g.g_pitch = p.piece, g.t_pitch = p.t_pitch;
+  g.v_all = p.v;
+  g.bias_part = p.want_b ? s.bias_part : nullptr;
+  const int fmt = image_format(c.dt);
+  for (uint32_t v0 = 0; v0 < p.v; v0 += p.piece) {
+    const uint32_t items = std::min(p.piece, p.v - v0);
+    a.table = table16 + (size_t)v0 * a.table_ld;
+    a.v = items, a.v_tiles = cdiv(items, kShape[p.tile].bm), a.chunks = cdiv(a.v_tiles, p.per);
+    a.bias = bias ? (const float *)Bi.p + v0 : nullptr;
+    g.v_begin = v0;
+    by_tile(p.tile, [&](auto k) {
+      constexpr int K = decltype(k)::value;
+      auto go = [&](auto f, auto two, auto with_bias) {
+        constexpr int FMT = decltype(f)::value;
+        hipLaunchKernelGGL((loss_grad_kernel<FMT, TileOf<FMT, K>, decltype(two)::value, decltype(with_bias)::value>), dim3(a.n_tiles * a.chunks),
+                           dim3(TileOf<FMT, K>::NT), 0, ctx->stream, g);
+      };
+      constexpr std::integral_constant<int, AS_BF16> bf{};
+      constexpr std::integral_constant<int, AS_F16> hf{};
+      constexpr std::true_type yes{};
+      constexpr std::false_type no{};
+      if (c.dt == AS_BF16) bias ? go(bf, no, yes) : go(bf, no, no);
+      else if (c.dt == AS_F16) bias ? go(hf, no, yes) : go(hf, no, no);
+      else bias ? go(hf, yes, yes) : go(hf, yes, no);
+    });
+    if (p.want_b)
+      hipLaunchKernelGGL(bias_join_kernel, dim3(cdiv(items, 256)), dim3(256), 0, ctx->stream, (const float *)s.bias_part, p.n_tiles * kShape[p.tile].wn, p.piece, items,
+                         coef, (float *)Ob.p + v0);
+    if (p.want_w) {
+      ProductArgs w{};
+      w.A = (const char *)s.xt, w.a_ld = (size_t)p.t_pitch * p.planes * 2, w.a_plane = p.t_pitch / 64;
+      w.B = (const char *)s.GT, w.b_ld = (size_t)p.t_pitch * p.planes * 2, w.b_plane = p.t_pitch / 64;
+      w.m = p.d, w.n = items, w.m_tiles = cdiv(p.d, kShape[p.tile_w].bm), w.n_tiles = cdiv(items, kShape[p.tile_w].bn);
+      w.steps = cdiv(p.n, 64), w.planes = p.planes, w.splits = 1;
+      w.scale = c.scale, w.coef = coef, w.top = x_top;
+      w.out = (char *)Ow.p + (size_t)v0 * gw_stride * dtype_size(c.dt), w.out_stride = gw_stride;
+      w.aligned = gw_stride % 8 == 0 && ((uintptr_t)w.out & 15) == 0;
+      launch_product(ctx, fmt, p.tile_w, c.dt, w);
+    }
+    if (p.want_x) {
+      const uint32_t pitch = up(items, 64);
+      make_transposed(ctx, ts, v0, items, pitch, w_top, s.wt);
+      ProductArgs w{};
+      w.A = (const char *)s.wt, w.a_ld = (size_t)pitch * p.planes * 2, w.a_plane = pitch / 64;
+      w.B = (const char *)s.G, w.b_ld = (size_t)p.piece * p.planes * 2, w.b_plane = p.piece / 64;
+      w.m = p.d, w.n = p.n, w.m_tiles = cdiv(p.d, kShape[p.tile_x].bm), w.n_tiles = cdiv(p.n, kShape[p.tile_x].bn);
+      w.steps = pitch / 64, w.planes = p.planes, w.splits = p.splits;
+      w.sums = s.sums, w.sums_pitch = up(p.d, 8), w.first = v0 == 0;
+      launch_product(ctx, fmt, p.tile_x, 0, w);
+    }
+    AS_HIP(ctx, hipGetLastError());
+  }
+  if (p.want_x) {
+    by_type(c.dt, [&](auto dt) {
+      hipLaunchKernelGGL((grad_rows_join_kernel<decltype(dt)::value>), dim3(spread((uint64_t)p.n * p.d, 512)), dim3(256), 0, ctx->stream, (const float *)s.sums, p.splits,
+                         up(p.d, 8), p.n, p.d, c.scale, coef, w_top, Ox.p, (size_t)gx_stride);
+    });
+    AS_HIP(ctx, hipGetLastError());
+  }
+  AS_TRY(Ox.finish(ctx));
+  AS_TRY(Ow.finish(ctx));
+  AS_TRY(Ob.finish(ctx));
+  return finish_call(ctx);
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t as_cross_entropy_workspace(uint64_t n, uint64_t n_items, uint64_t dim, int dtype, int backward) {
+  if (n == 0 || n_items == 0 || dim == 0 || n >= (1ull << 31) || n_items >= (1ull << 31) || dim > 65536 || !dtype_is_training(dtype)) return 0;
+  // (a stride of dim + 1: room for the images whether or not the matrices can be taken as they are)
+  const Source xs{nullptr, (size_t)dim + 1, (uint32_t)n, (uint32_t)dim, dtype}, ts{nullptr, (size_t)dim + 1, (uint32_t)n_items, (uint32_t)dim, dtype};
+  Plan p = make_plan((uint32_t)n, (uint32_t)n_items, (uint32_t)dim, dtype);
+  if (backward) {
+    plan_backward(p, true, true, true, true);
+    BackwardScratch s{};
+    return backward_layout(p, xs, ts, nullptr, s);
+  }
+  plan_walk(p);
+  ForwardScratch s{};
+  return forward_layout(p, xs, ts, nullptr, s);
+}
+
+int as_cross_entropy(as_ctx *ctx, const void *x, uint64_t n, uint64_t x_stride, const void *table, uint64_t n_items, uint64_t table_stride, uint64_t dim,
+                     int dtype, const float *bias, const int64_t *targets, int64_t ignore_index, double scale, float *losses, float *lse, void *workspace,
+                     uint64_t workspace_bytes) {
+  DeviceScope keep;
+  return guarded(ctx, [&] {
+    return forward_call(ctx, LossCall{n, n_items, dim, x_stride, table_stride, dtype, (float)scale}, x, table, bias, targets, ignore_index, losses, lse, workspace,
+                        workspace_bytes);
+  });
+}
+
+int as_cross_entropy_backward(as_ctx *ctx, const void *x, uint64_t n, uint64_t x_stride, const void *table, uint64_t n_items, uint64_t table_stride,
+                              uint64_t dim, int dtype, const float *bias, const int64_t *targets, int64_t ignore_index, double scale, const float *lse,
+                              const float *grad_losses, const float *grad_lse, void *grad_x, uint64_t grad_x_stride, void *grad_table,
+                              uint64_t grad_table_stride, float *grad_bias, void *workspace, uint64_t workspace_bytes) {
+  DeviceScope keep;
+  return guarded(ctx, [&] {
+    return backward_call(ctx, LossCall{n, n_items, dim, x_stride, table_stride, dtype, (float)scale}, x, table, bias, targets, ignore_index, lse, grad_losses, grad_lse,
+                         grad_x, grad_x_stride, grad_table, grad_table_stride, grad_bias, workspace, workspace_bytes);
+  });
+}
+
+}  // extern "C"

@@ -53,6 +53,10 @@ pub struct AsJl {
 pub struct AsComm {
     _private: [u8; 0],
 }
+#[repr(C)]
+pub struct AsTable4 {
+    _private: [u8; 0],
+}
 
 #[link(name = "arrowspace_hip")]
 extern "C" {
@@ -126,4 +130,17 @@ extern "C" {
     pub fn as_search_lambda_aware(ctx: *mut AsCtx, index: *const AsIndex, queries: *const f64, q_lambdas: *const f64, nq: u64, k: u64, alpha: f64, id_offset: u64, idx_out: *mut u64, score_out: *mut f64) -> c_int;
     pub fn as_search_lambda_aware_hybrid(ctx: *mut AsCtx, index: *const AsIndex, queries: *const f64, q_lambdas: *const f64, nq: u64, k: u64, alpha: f64, id_offset: u64, idx_out: *mut u64, score_out: *mut f64) -> c_int;
     pub fn as_range_search(ctx: *mut AsCtx, index: *const AsIndex, lambda_q: f64, eps: f64, id_offset: u64, idx_out: *mut u64, dist_out: *mut f64, cap: u64, n_found: *mut u64) -> c_int;
+    pub fn as_cross_entropy_workspace(n: u64, n_items: u64, dim: u64, dtype: c_int, backward: c_int) -> u64;
+    pub fn as_cross_entropy(ctx: *mut AsCtx, x: *const c_void, n: u64, x_stride: u64, table: *const c_void, n_items: u64, table_stride: u64, dim: u64, dtype: c_int, bias: *const f32, targets: *const i64, ignore_index: i64, scale: f64, losses: *mut f32, lse: *mut f32, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn as_cross_entropy_backward(ctx: *mut AsCtx, x: *const c_void, n: u64, x_stride: u64, table: *const c_void, n_items: u64, table_stride: u64, dim: u64, dtype: c_int, bias: *const f32, targets: *const i64, ignore_index: i64, scale: f64, lse: *const f32, grad_losses: *const f32, grad_lse: *const f32, grad_x: *mut c_void, grad_x_stride: u64, grad_table: *mut c_void, grad_table_stride: u64, grad_bias: *mut f32, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn as_table4_import(ctx: *mut AsCtx, codes: *const u8, scales: *const c_void, zeros: *const u8, n_items: u64, dim: u64, group: u64, scale_dtype: c_int, out: *mut *mut AsTable4) -> c_int;
+    pub fn as_table4_pack(ctx: *mut AsCtx, rows: *const c_void, n_items: u64, row_stride: u64, dim: u64, dtype: c_int, group: u64, scale_dtype: c_int, out: *mut *mut AsTable4) -> c_int;
+    pub fn as_table4_export(ctx: *mut AsCtx, t: *const AsTable4, codes: *mut u8, scales: *mut c_void, zeros: *mut u8) -> c_int;
+    pub fn as_table4_destroy(t: *mut AsTable4);
+    pub fn as_table4_items(t: *const AsTable4) -> u64;
+    pub fn as_table4_dim(t: *const AsTable4) -> u64;
+    pub fn as_table4_group(t: *const AsTable4) -> u64;
+    pub fn as_table4_scale_dtype(t: *const AsTable4) -> c_int;
+    pub fn as_table4_workspace(t: *const AsTable4, m: u64, dtype: c_int) -> u64;
+    pub fn as_table4_scores(ctx: *mut AsCtx, t: *const AsTable4, x: *const c_void, m: u64, x_stride: u64, dtype: c_int, out: *mut c_void, out_stride: u64, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
 }

@@ -9,7 +9,8 @@
  * plain `extern "C"` block (INTEGRATION.md shows the shim).
  *
  * Conventions
- *   - All matrices are row-major f64; indices are u64 at the boundary (usize in the reference).
+ *   - All matrices are row-major f64 (the operators over a table at the end of this file: f32, bf16 or f16, with a row stride);
+ *     indices are u64 at the boundary (usize in the reference).
  *   - Every data pointer may be a HOST pointer or a DEVICE (HBM) pointer; the library asks
  *     the HIP runtime which it is.  Host buffers are staged over PCIe on the context's stream;
  *     device buffers are used in place (this is how bench.py and the multi-GPU driver keep the
@@ -48,6 +49,9 @@ typedef enum {
   AS_ERR_PEER = 11        /* as_build_laplacian_sharded: another rank failed locally; this rank stopped with it */
 } as_status;
 
+/* element types of the operators over a table (as_cross_entropy, as_table4_*); every other matrix is f64 */
+typedef enum { AS_F64 = 0, AS_F32 = 1, AS_BF16 = 2, AS_F16 = 3 } as_dtype;
+
 /* TauMode, src/taumode.rs:75-82 */
 typedef enum { AS_TAU_FIXED = 0, AS_TAU_MEDIAN = 1, AS_TAU_MEAN = 2, AS_TAU_PERCENTILE = 3 } as_tau_mode;
 
@@ -73,6 +77,7 @@ typedef struct {
 typedef struct as_ctx as_ctx;     /* device, stream, workspace */
 typedef struct as_csr as_csr;     /* CSR Laplacian resident in HBM (sprs::CsMat<f64> counterpart) */
 typedef struct as_index as_index; /* items + lambdas resident in HBM (ArrowSpace.data / .lambdas) */
+typedef struct as_table4 as_table4; /* a table of rows in 4 bits with group scales, resident in HBM */
 typedef struct as_jl as_jl;       /* a seeded Gaussian projection resident in HBM (ImplicitProjection, src/reduction.rs:166-203) */
 
 /* ---- context -------------------------------------------------------------------------- */
@@ -488,6 +493,60 @@ int as_search_lambda_aware_hybrid(as_ctx *ctx, const as_index *index, const doub
  * min(cap, found) hits and the total count to *n_found (host pointer). */
 int as_range_search(as_ctx *ctx, const as_index *index, double lambda_q, double eps, uint64_t id_offset,
                     uint64_t *idx_out, double *dist_out, uint64_t cap, uint64_t *n_found);
+
+/* ---- a table of rows: training it, and serving it in 4 bits ---------------------------------------------------------------
+ * The table is what an index holds: a row of `dim` values per item.  These operators have no counterpart in the reference; they
+ * are the same product rows x table that the search scans, with other endings.
+ *   - Element types: as_dtype.  Rows may lie inside wider matrices: strides are in elements, values of a row are adjacent.
+ *   - `workspace` (aligned to 256 bytes) is device memory of the size the *_workspace function names, or NULL: the context's own
+ *     scratch.  A call on a stream that is being captured into a graph must bring one (AS_ERR_UNSUPPORTED otherwise): the graph
+ *     keeps its address, so two graphs that may run at once need two.  Host memory and as_table4_import / _pack / _export are
+ *     refused during a capture.
+ *   - Every pointer is host memory or memory of the context's device (AS_ERR_ARG for another device's).  The caller's current
+ *     device is left as it was.  Results are the same from run to run: nothing is summed with atomics.
+ *
+ * Softmax cross entropy of n rows against n_items items, without keeping the n x n_items logits:
+ *   l_tv = scale <x_t, w_v> + bias_v     lse_t = log sum_v exp(l_tv)     losses_t = lse_t - l_{t, targets_t}
+ * bias[n_items] f32 or NULL; -inf takes an item out.  losses_t is 0 where targets_t == ignore_index (lse_t is still written) and
+ * where the bias leaves no item (lse_t = -inf).  A target outside the table that is not ignore_index: AS_ERR_ARG when the targets
+ * are host memory, a loss of NaN when they are device memory; its row has no gradient through the loss.  n = 0 is allowed.
+ * Products are summed in 32 bits (f32 inputs: as a sum of two f16 each, 22 bits, products of 2^-23). */
+uint64_t as_cross_entropy_workspace(uint64_t n, uint64_t n_items, uint64_t dim, int dtype, int backward);
+int as_cross_entropy(as_ctx *ctx, const void *x, uint64_t n, uint64_t x_stride, const void *table, uint64_t n_items,
+                     uint64_t table_stride, uint64_t dim, int dtype, const float *bias, const int64_t *targets, int64_t ignore_index,
+                     double scale, float *losses, float *lse, void *workspace, uint64_t workspace_bytes);
+/* Its gradient, from grad_losses[n] = dL/dlosses and grad_lse[n] = dL/dlse (or NULL: 0), with lse as the forward call wrote it:
+ *   g_tv = (grad_losses_t + grad_lse_t) exp(l_tv - lse_t) - grad_losses_t [v = targets_t]   (grad_losses_t as 0 on ignored rows)
+ *   grad_x = scale g table      grad_table = scale g^T x      grad_bias_v = sum_t g_tv
+ * grad_x and grad_table have the inputs' type, grad_bias is f32; each may be NULL (not computed).  The logits are made again in
+ * pieces of the table; g is rounded to 16 bits between the products (f32 inputs: to 22), sums are 32 bits wide. */
+int as_cross_entropy_backward(as_ctx *ctx, const void *x, uint64_t n, uint64_t x_stride, const void *table, uint64_t n_items,
+                              uint64_t table_stride, uint64_t dim, int dtype, const float *bias, const int64_t *targets,
+                              int64_t ignore_index, double scale, const float *lse, const float *grad_losses, const float *grad_lse,
+                              void *grad_x, uint64_t grad_x_stride, void *grad_table, uint64_t grad_table_stride, float *grad_bias,
+                              void *workspace, uint64_t workspace_bytes);
+
+/* A table in 4 bits: W_vk = scale_{v, k / group} (code_vk - zero_{v, k / group}), codes 0 .. 15, group 32, 64 or 128 (the last one of
+ * a row may be short).  Plain form: codes n_items x ceil(dim / 2) bytes, column 2 j in the low half of byte j; scales
+ * n_items x ceil(dim / group) of type scale_dtype (AS_F32, AS_BF16, AS_F16); zeros the same shape, bytes 0 .. 15, or NULL: all 8.
+ * import lays such a table out for the kernels (once; the handle owns its memory, inputs are only read).  pack quantises rows of any
+ * as_dtype: scale = the group's largest magnitude / 7 rounded to scale_dtype, codes rounded to nearest even; values must be finite
+ * (AS_ERR_NONFINITE).  export gives the plain form back (zeros may be NULL).  All three return when their work is done. */
+int as_table4_import(as_ctx *ctx, const uint8_t *codes, const void *scales, const uint8_t *zeros, uint64_t n_items, uint64_t dim,
+                     uint64_t group, int scale_dtype, as_table4 **out);
+int as_table4_pack(as_ctx *ctx, const void *rows, uint64_t n_items, uint64_t row_stride, uint64_t dim, int dtype, uint64_t group,
+                   int scale_dtype, as_table4 **out);
+int as_table4_export(as_ctx *ctx, const as_table4 *t, uint8_t *codes, void *scales, uint8_t *zeros);
+void as_table4_destroy(as_table4 *t);
+uint64_t as_table4_items(const as_table4 *t);
+uint64_t as_table4_dim(const as_table4 *t);
+uint64_t as_table4_group(const as_table4 *t);
+int as_table4_scale_dtype(const as_table4 *t);
+/* out_mv = sum_k x_mk W_vk for m rows (made for a few: 64 are one pass over the codes); out has the rows' type (AS_F32, AS_BF16 or
+ * AS_F16), rounded once.  The handle is only read: any number of contexts may use it at once. */
+uint64_t as_table4_workspace(const as_table4 *t, uint64_t m, int dtype);
+int as_table4_scores(as_ctx *ctx, const as_table4 *t, const void *x, uint64_t m, uint64_t x_stride, int dtype, void *out,
+                     uint64_t out_stride, void *workspace, uint64_t workspace_bytes);
 
 #ifdef __cplusplus
 }

@@ -14,10 +14,12 @@ OUT = os.path.join(ROOT, "arrowspace-rs_amd", "host", "rust", "src", "hip.rs")
 
 TYPES = {
     "int": "c_int", "double": "f64", "float": "f32", "uint64_t": "u64", "uint32_t": "u32", "int64_t": "i64", "int32_t": "i32",
+    "uint8_t": "u8",
     "void": None,
 }
 OPAQUE = {"as_ctx": "AsCtx", "as_csr": "AsCsr", "as_index": "AsIndex", "as_graph_params": "AsGraphParams",
-          "as_jl": "AsJl", "as_comm": "AsComm", "as_comm_ops": "AsCommOps", "as_clustering": "AsClustering"}
+          "as_jl": "AsJl", "as_comm": "AsComm", "as_comm_ops": "AsCommOps", "as_clustering": "AsClustering",
+          "as_table4": "AsTable4"}
 
 
 def rust_type(c):
