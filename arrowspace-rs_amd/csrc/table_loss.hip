@@ -16,13 +16,12 @@
 // Rounding.  G is rounded to 16 bits (f16: after a power of two from the largest coefficient; f32: two planes, 22 bits): half a
 // step per entry, as the gradients that leave are rounded themselves.  Everything else -- logits, maxima, sums, dX over pieces,
 // dbias -- is f32 or wider.
-#include "nt_product.h"
+#include "table_loss_rows.h"
 
 using namespace asx;
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kChips = 256;  // compute units: how many workgroups of the large tile run at once
 
 struct LossArgs {
@@ -39,50 +38,9 @@ struct LossArgs {
   const unsigned int *rows_top, *table_top;  // two planes: bits of the largest finite magnitude of each matrix, else null
 };
 
-// the power of two a matrix with this largest magnitude is multiplied by (0 or not a number: 1)
-__device__ __forceinline__ float plane_scale(unsigned int top_bits) {
-  const int e = (int)(top_bits >> 23);
-  if (e == 0 || e >= 255) return 1.f;
-  const int s = min(max(14 - (e - 127), -100), 100);
-  return __uint_as_float((unsigned int)(127 + s) << 23);
-}
 __device__ __forceinline__ float product_scale(const LossArgs &a) {
   if (a.rows_top == nullptr) return 1.f;
   return 1.f / plane_scale(*a.rows_top) / plane_scale(*a.table_top);
-}
-
-// Workgroups are dealt to the 8 dies in turn; consecutive pieces of work should share a die's cache, so die d takes the d-th eighth.
-__device__ __forceinline__ uint32_t die_order(uint32_t b, uint32_t total) {
-  const uint32_t die = b & 7, at = b >> 3, each = total >> 3, rest = total & 7;
-  return die * each + nt_min(die, rest) + at;
-}
-
-// quad-wide exchange: the value of lane ^ 1 / lane ^ 2
-__device__ __forceinline__ uint32_t quad_xor1(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true); }
-__device__ __forceinline__ uint32_t quad_xor2(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true); }
-__device__ __forceinline__ float add16(float v) {  // sum over the 16 lanes of a row of lanes, in a fixed order
-  v += __uint_as_float(quad_xor1(__float_as_uint(v)));
-  v += __uint_as_float(quad_xor2(__float_as_uint(v)));
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, true));
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, true));
-  return v;
-}
-
-template <int FMT>
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-  if constexpr (FMT == AS_BF16) {
-    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-    const bf2 p = {(__bf16)x, (__bf16)y};
-    return __builtin_bit_cast(uint32_t, p);
-  } else {
-    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-    const half2v p = {(_Float16)x, (_Float16)y};
-    return __builtin_bit_cast(uint32_t, p);
-  }
-}
-__device__ __forceinline__ float low_part(float x) {  // what f16 leaves of x (nothing of an infinity)
-  const float hi = (float)(_Float16)x;
-  return __builtin_isfinite(hi) ? x - hi : 0.f;
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------------
@@ -545,16 +503,30 @@ __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
   }
 }
 
+// dX from its parts, in their order: 64 columns a workgroup, 16 waves a sixteenth of the parts each (a few rows have hundreds of parts)
 template <int DT>
-__global__ __launch_bounds__(256) void grad_rows_join_kernel(const float *sums, uint32_t splits, uint32_t pitch, uint32_t n, uint32_t d, float scale,
-                                                             const float *coef, const unsigned int *top, void *out, size_t out_stride) {
+__global__ __launch_bounds__(1024) void grad_rows_join_kernel(const float *sums, uint32_t splits, uint32_t pitch, uint32_t n, uint32_t d, float scale,
+                                                              const float *coef, const unsigned int *top, void *out, size_t out_stride) {
+  __shared__ float s[16][64];
   const float f = scale * (coef ? coef[1] : 1.f) * (top ? 1.f / plane_scale(*top) : 1.f);
-  const uint64_t total = (uint64_t)n * d;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
-    const uint64_t t = i / d, k = i % d;
-    float s = 0.f;
-    for (uint32_t p = 0; p < splits; ++p) s += sums[((size_t)p * n + t) * pitch + k];
-    store_from_f32<DT>(out, t * out_stride + k, s * f);
+  const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint64_t total = (uint64_t)n * pitch;
+  const uint32_t lo = splits * w / 16, hi = splits * (w + 1) / 16;
+  for (uint64_t i0 = (uint64_t)blockIdx.x * 64; i0 < total; i0 += (uint64_t)gridDim.x * 64) {
+    const uint64_t i = i0 + lane;
+    float x = 0.f;
+    if (i < total) {
+#pragma unroll 8
+      for (uint32_t p = lo; p < hi; ++p) x += sums[p * total + i];
+    }
+    s[w][lane] = x;
+    __syncthreads();
+    if (w == 0 && i < total) {
+      for (int k = 1; k < 16; ++k) x += s[k][lane];
+      const uint64_t t = i / pitch, k = i % pitch;
+      if (k < d) store_from_f32<DT>(out, t * out_stride + k, x * f);
+    }
+    __syncthreads();
   }
 }
 __global__ __launch_bounds__(256) void bias_join_kernel(const float *part, uint32_t parts, uint32_t pitch, uint32_t v, const float *coef, float *out) {
@@ -592,8 +564,9 @@ struct Source {
   size_t stride;
   uint32_t rows, d;
   int dt;
-  bool direct() const { return dt != AS_F32 && d % 64 == 0 && stride % 8 == 0 && ((uintptr_t)p & 15) == 0; }
-  uint32_t pitch() const { return up(d, 64); }
+  uint32_t whole;  // columns of an image
+  bool direct() const { return dt != AS_F32 && d == whole && stride % 8 == 0 && ((uintptr_t)p & 15) == 0; }
+  uint32_t pitch() const { return whole; }
   uint32_t planes() const { return dt == AS_F32 ? 2 : 1; }
   uint64_t image_elems() const { return direct() ? 0 : (uint64_t)rows * pitch() * planes(); }
 };
@@ -619,6 +592,8 @@ struct Plan {
   // backward
   uint32_t piece, pieces, t_pitch, splits;
   int tile_w, tile_x;
+  int fused;                 // steps of 32 columns of the form for short rows (table_loss_rows.h), 0: through G in memory
+  uint32_t x_blocks, w_blocks, n_pad;
   bool want_x, want_w, want_b, scaled;
 };
 Plan make_plan(uint32_t n, uint32_t v, uint32_t d, int dt) {
@@ -638,8 +613,22 @@ void plan_walk(Plan &p) {
   p.per = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(p.v_tiles, tiles / groups));
   p.chunks = cdiv(p.v_tiles, p.per);
 }
+// the form for short rows: its steps of 32 columns, and tiles of 16 rows a wave holds (what 256 registers take)
+int fused_steps(uint32_t d, uint32_t planes) { return d <= 64 ? 2 : d <= 128 ? 4 : d <= 256 && planes == 1 ? 8 : 0; }
+constexpr int fused_rows(int steps, int planes) { return steps == 8 || planes == 2 ? 2 : steps == 4 ? 3 : 4; }
 void plan_backward(Plan &p, bool x, bool w, bool b, bool scaled) {
   p.want_x = x, p.want_w = w, p.want_b = b, p.scaled = scaled;
+  p.fused = fused_steps(p.d, p.planes);
+  if (p.fused) {
+    const uint32_t rows = 64 * fused_rows(p.fused, p.planes), stages = cdiv(p.v, 64);
+    p.pitch = p.fused * 32;
+    p.x_blocks = cdiv(p.n, rows);
+    p.w_blocks = cdiv(p.v, rows);
+    p.n_pad = up(p.n, 64);
+    // the items in parts, so that two workgroups a compute unit are there
+    p.splits = std::max(1u, std::min(2u * kChips / std::min(p.x_blocks, 2u * kChips), stages));
+    return;
+  }
   const uint32_t bm = kShape[p.tile].bm, bn = kShape[p.tile].bn;
   p.t_pitch = up(p.n, std::max(bn, 64u));
   // G and its transposed form of a piece: 512 MB together (the two products that read them want thousands of items), whole tiles
@@ -678,6 +667,8 @@ struct BackwardScratch {
   float *coef;
   unsigned short *x_image, *t_image, *xt, *wt, *G, *GT;
   float *sums, *bias_part;
+  float *lse, *every, *one;
+  int *target;
 };
 uint64_t backward_layout(const Plan &p, const Source &x, const Source &t, char *base, BackwardScratch &s) {
   Layout l{base};
@@ -686,6 +677,14 @@ uint64_t backward_layout(const Plan &p, const Source &x, const Source &t, char *
   s.coef = l.take<float>(2);
   s.x_image = l.take<unsigned short>(x.image_elems());
   s.t_image = l.take<unsigned short>(t.image_elems());
+  if (p.fused) {
+    s.lse = l.take<float>(p.n_pad);
+    s.every = l.take<float>(p.n_pad);
+    s.one = l.take<float>(p.n_pad);
+    s.target = l.take<int>(p.n_pad);
+    s.sums = l.take<float>(p.want_x ? (uint64_t)p.splits * p.n * up(p.d, 8) : 0);
+    return l.at;
+  }
   s.xt = l.take<unsigned short>(p.want_w ? (uint64_t)p.d * p.t_pitch * pl : 0);
   s.wt = l.take<unsigned short>(p.want_x ? (uint64_t)p.d * p.piece * pl : 0);
   s.G = l.take<unsigned short>((uint64_t)p.n * p.piece * pl);
@@ -742,6 +741,28 @@ void make_transposed(as_ctx *ctx, const Source &s, uint32_t row0, uint32_t rows,
     hipLaunchKernelGGL((transposed_kernel<DT, DT == AS_BF16 ? AS_BF16 : AS_F16>), dim3(pitch / 64, cdiv(s.d, 64)), dim3(256), 0, ctx->stream, (const void *)p,
                        s.stride, rows, s.d, pitch, top, out);
   });
+}
+template <int FMT, int P, int KD, bool ITEMS, bool BIAS>
+void launch_rows_grad(as_ctx *ctx, const LossRowsArgs &a) {
+  constexpr int OUT = P == 2 ? AS_F32 : FMT;
+  hipLaunchKernelGGL((loss_rows_grad_kernel<FMT, P, fused_rows(KD, P), KD, ITEMS, BIAS, OUT>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
+}
+template <bool ITEMS>
+void launch_rows_grad(as_ctx *ctx, int dt, int steps, bool bias, const LossRowsArgs &a) {
+  auto go = [&](auto fmt, auto planes, auto kd) {
+    constexpr int FMT = decltype(fmt)::value, P = decltype(planes)::value, KD = decltype(kd)::value;
+    if (bias) launch_rows_grad<FMT, P, KD, ITEMS, true>(ctx, a);
+    else launch_rows_grad<FMT, P, KD, ITEMS, false>(ctx, a);
+  };
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  constexpr std::integral_constant<int, 4> four{};
+  constexpr std::integral_constant<int, 8> eight{};
+  constexpr std::integral_constant<int, AS_BF16> bf{};
+  constexpr std::integral_constant<int, AS_F16> hf{};
+  if (dt == AS_F32) steps == 2 ? go(hf, two, two) : go(hf, two, four);
+  else if (dt == AS_BF16) steps == 2 ? go(bf, one, two) : steps == 4 ? go(bf, one, four) : go(bf, one, eight);
+  else steps == 2 ? go(hf, one, two) : steps == 4 ? go(hf, one, four) : go(hf, one, eight);
 }
 void launch_product(as_ctx *ctx, int fmt, int tile, int out_type, const ProductArgs &p) {
   by_tile(tile, [&](auto k) {
@@ -800,9 +821,9 @@ int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tabl
   AS_TRY(Y.bind(ctx, targets, c.n * 8));
   AS_TRY(L.bind(ctx, losses, c.n * 4));
   AS_TRY(S.bind(ctx, lse, c.n * 4));
-  const Source xs{X.p, (size_t)c.x_stride, (uint32_t)c.n, (uint32_t)c.d, c.dt}, ts{W.p, (size_t)c.table_stride, (uint32_t)c.v, (uint32_t)c.d, c.dt};
   Plan p = make_plan((uint32_t)c.n, (uint32_t)c.v, (uint32_t)c.d, c.dt);
   plan_walk(p);
+  const Source xs{X.p, (size_t)c.x_stride, p.n, p.d, c.dt, p.pitch}, ts{W.p, (size_t)c.table_stride, p.v, p.d, c.dt, p.pitch};
   ForwardScratch s{};
   Scratch scratch;
   AS_TRY(scratch.open(ctx, workspace, workspace_bytes, forward_layout(p, xs, ts, nullptr, s)));
@@ -876,9 +897,9 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
     AS_TRY(Ob.finish(ctx));
     return finish_call(ctx);
   }
-  const Source xs{X.p, (size_t)c.x_stride, (uint32_t)c.n, (uint32_t)c.d, c.dt}, ts{W.p, (size_t)c.table_stride, (uint32_t)c.v, (uint32_t)c.d, c.dt};
   Plan p = make_plan((uint32_t)c.n, (uint32_t)c.v, (uint32_t)c.d, c.dt);
   plan_backward(p, gx != nullptr, gw != nullptr, gb != nullptr, c.dt != AS_BF16);
+  const Source xs{X.p, (size_t)c.x_stride, p.n, p.d, c.dt, p.pitch}, ts{W.p, (size_t)c.table_stride, p.v, p.d, c.dt, p.pitch};
   BackwardScratch s{};
   Scratch scratch;
   AS_TRY(scratch.open(ctx, workspace, workspace_bytes, backward_layout(p, xs, ts, nullptr, s)));
@@ -890,10 +911,34 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   AS_TRY(make_image(ctx, xs, s.tops, s.x_image, &a.rows, &a.rows_ld));
   AS_TRY(make_image(ctx, ts, s.tops + 1, s.t_image, &table16, &a.table_ld));
   const unsigned int *x_top = p.planes == 2 ? s.tops : nullptr, *w_top = p.planes == 2 ? s.tops + 1 : nullptr;
-  if (p.want_w) make_transposed(ctx, xs, 0, p.n, p.t_pitch, x_top, s.xt);
+  if (p.want_w && !p.fused) make_transposed(ctx, xs, 0, p.n, p.t_pitch, x_top, s.xt);
   if (p.scaled) hipLaunchKernelGGL(coef_scale_kernel, dim3(1), dim3(1024), 0, ctx->stream, (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p, ignore, p.n, s.coef);
   AS_HIP(ctx, hipGetLastError());
   const float *coef = p.scaled ? s.coef : nullptr;
+  if (p.fused) {
+    hipLaunchKernelGGL(loss_rows_kernel, dim3(cdiv(p.n_pad, 256)), dim3(256), 0, ctx->stream, (const float *)Ls.p, (const float *)Gl.p, (const float *)Ge.p,
+                       (const int64_t *)Y.p, ignore, p.n, p.n_pad, p.v, coef, s.lse, s.every, s.one, s.target);
+    LossRowsArgs r{};
+    r.d = p.d, r.scale = c.scale, r.bias = (const float *)Bi.p, r.coef = coef;
+    r.lse = s.lse, r.every = s.every, r.one = s.one, r.target = s.target;
+    r.r_plane = r.k_plane = (size_t)p.pitch * 2;
+    if (p.want_w || p.want_b) {
+      r.r = table16, r.r_ld = a.table_ld, r.nr = p.v, r.r_top = w_top;
+      r.k = a.rows, r.k_ld = a.rows_ld, r.nk = p.n, r.k_top = x_top;
+      r.r_blocks = p.w_blocks, r.splits = 1;
+      r.out = Ow.p, r.out_stride = gw_stride, r.aligned = gw_stride % 8 == 0 && ((uintptr_t)Ow.p & 15) == 0;
+      r.grad_bias = (float *)Ob.p;
+      launch_rows_grad<true>(ctx, c.dt, p.fused, bias != nullptr, r);
+    }
+    if (p.want_x) {
+      r.r = a.rows, r.r_ld = a.rows_ld, r.nr = p.n, r.r_top = x_top;
+      r.k = table16, r.k_ld = a.table_ld, r.nk = p.v, r.k_top = w_top;
+      r.r_blocks = p.x_blocks, r.splits = p.splits;
+      r.sums = s.sums, r.sums_pitch = up(p.d, 8);
+      launch_rows_grad<false>(ctx, c.dt, p.fused, bias != nullptr, r);
+    }
+    AS_HIP(ctx, hipGetLastError());
+  }
   a.table_plane = a.rows_plane = p.steps;
   a.n = p.n, a.steps = p.steps, a.planes = p.planes, a.n_tiles = p.n_tiles, a.per = p.per;
   a.scale = c.scale;
@@ -903,7 +948,7 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   g.v_all = p.v;
   g.bias_part = p.want_b ? s.bias_part : nullptr;
   const int fmt = image_format(c.dt);
-  for (uint32_t v0 = 0; v0 < p.v; v0 += p.piece) {
+  for (uint32_t v0 = 0; !p.fused && v0 < p.v; v0 += p.piece) {
     const uint32_t items = std::min(p.piece, p.v - v0);
     a.table = table16 + (size_t)v0 * a.table_ld;
     a.v = items, a.v_tiles = cdiv(items, kShape[p.tile].bm), a.chunks = cdiv(a.v_tiles, p.per);
@@ -953,8 +998,8 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   }
   if (p.want_x) {
     by_type(c.dt, [&](auto dt) {
-      hipLaunchKernelGGL((grad_rows_join_kernel<decltype(dt)::value>), dim3(spread((uint64_t)p.n * p.d, 512)), dim3(256), 0, ctx->stream, (const float *)s.sums, p.splits,
-                         up(p.d, 8), p.n, p.d, c.scale, coef, w_top, Ox.p, (size_t)gx_stride);
+      hipLaunchKernelGGL((grad_rows_join_kernel<decltype(dt)::value>), dim3(spread((uint64_t)p.n * up(p.d, 8), 64)), dim3(1024), 0, ctx->stream, (const float *)s.sums,
+                         p.splits, up(p.d, 8), p.n, p.d, c.scale, coef, w_top, Ox.p, (size_t)gx_stride);
     });
     AS_HIP(ctx, hipGetLastError());
   }
@@ -970,11 +1015,11 @@ extern "C" {
 
 uint64_t as_cross_entropy_workspace(uint64_t n, uint64_t n_items, uint64_t dim, int dtype, int backward) {
   if (n == 0 || n_items == 0 || dim == 0 || n >= (1ull << 31) || n_items >= (1ull << 31) || dim > 65536 || !dtype_is_training(dtype)) return 0;
-  // (a stride of dim + 1: room for the images whether or not the matrices can be taken as they are)
-  const Source xs{nullptr, (size_t)dim + 1, (uint32_t)n, (uint32_t)dim, dtype}, ts{nullptr, (size_t)dim + 1, (uint32_t)n_items, (uint32_t)dim, dtype};
   Plan p = make_plan((uint32_t)n, (uint32_t)n_items, (uint32_t)dim, dtype);
+  if (backward) plan_backward(p, true, true, true, true);
+  // (a stride of dim + 1: room for the images whether or not the matrices can be taken as they are)
+  const Source xs{nullptr, (size_t)dim + 1, p.n, p.d, dtype, p.pitch}, ts{nullptr, (size_t)dim + 1, p.v, p.d, dtype, p.pitch};
   if (backward) {
-    plan_backward(p, true, true, true, true);
     BackwardScratch s{};
     return backward_layout(p, xs, ts, nullptr, s);
   }
