@@ -245,7 +245,6 @@ __global__ __launch_bounds__(64 * kWaves) void scores_kernel(ScoresArgs a) {
       uint32_t tile[kVT];
 #pragma unroll
       for (int t = 0; t < kVT; ++t) tile[t] = unit * kVT + t < a.v_tiles ? unit * kVT + t : a.v_tiles - 1;
-#pragma unroll 2
       for (uint32_t kt = k_lo; kt < k_hi; ++kt) {
         u32x4 w[kVT];
         float s[kVT][PG];

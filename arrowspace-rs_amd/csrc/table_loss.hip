@@ -184,35 +184,83 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2 *part, uint
 }
 
 // ---- what the products are made of ----------------------------------------------------------------------------------------------------
-__global__ void zero_words_kernel(unsigned int *w, uint32_t n) {
-  if (threadIdx.x < n) w[threadIdx.x] = 0u;
+// A matrix and its image: rows with their length filled to whole steps by zeros, f32 as two planes.
+struct ImageJob {
+  const void *src;
+  size_t stride;
+  uint32_t n, d, pitch;
+  int quads;               // four values at a time can be loaded (aligned rows)
+  unsigned short *out;
+};
+struct ImageJobs {
+  ImageJob job[2];
+  unsigned int *tops;      // f32: [2] bits of the largest finite magnitude, for everyone behind
+  float *parts;            // ... [2][kTopParts] of the workgroups that looked for it
+};
+constexpr uint32_t kTopParts = 512;
+// threads of a workgroup along a row of `quads` groups of four: a power of two
+__device__ __forceinline__ uint32_t along_row(uint32_t quads) { return quads >= 256 ? 256 : quads <= 1 ? 1 : 1u << (32 - __clz(quads - 1)); }
+template <int DT>
+__device__ __forceinline__ f32x4 load_quad(const ImageJob &j, size_t row, uint32_t k) {
+  if (j.quads && k + 4 <= j.d) {
+    if constexpr (DT == AS_F32) return *(const f32x4 *)((const float *)j.src + row * j.stride + k);
+    const u32x2 w = *(const u32x2 *)((const unsigned short *)j.src + row * j.stride + k);
+    f32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const unsigned short h = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
+      x[e] = DT == AS_BF16 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+    }
+    return x;
+  }
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (k + e < j.d) x[e] = load_as_f32<DT>(j.src, row * j.stride + k + e);
+  return x;
 }
-// the largest finite magnitude of an f32 matrix (bits of a positive float compare as integers; a maximum has no order)
-__global__ __launch_bounds__(256) void top_kernel(const float *x, size_t stride, uint32_t n, uint32_t d, unsigned int *top) {
+// f32: the largest finite magnitude, a part per workgroup
+__global__ __launch_bounds__(256) void top_kernel(ImageJobs jobs) {
+  const ImageJob &j = jobs.job[blockIdx.y];
+  __shared__ float s[4];
+  const uint32_t quads = (j.d + 3) / 4, along = along_row(quads), rows = 256 / along;
   float m = 0.f;
-  for (uint32_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += gridDim.x * 4)
-    for (uint32_t k = threadIdx.x & 63; k < d; k += 64) {
-      const float y = fabsf(x[(size_t)r * stride + k]);
-      if (y < INFINITY) m = fmaxf(m, y);
+  for (uint64_t r = (uint64_t)blockIdx.x * rows + threadIdx.x / along; r < j.n; r += (uint64_t)gridDim.x * rows)
+    for (uint32_t g = threadIdx.x % along; g < quads; g += along) {
+      const f32x4 x = load_quad<AS_F32>(j, r, g * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (fabsf(x[e]) < INFINITY) m = fmaxf(m, fabsf(x[e]));
     }
   for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
-  if ((threadIdx.x & 63) == 0) raise_max_u32(top, __float_as_uint(m));
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) jobs.parts[blockIdx.y * kTopParts + blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
 }
-// rows with their length filled to whole steps of 64 by zeros; f32 as two planes.  DT the source's type, FMT the image's.
 template <int DT, int FMT>
-__global__ __launch_bounds__(256) void image_kernel(const void *src, size_t stride, uint32_t n, uint32_t d, uint32_t pitch, const unsigned int *top,
-                                                    unsigned short *out) {
+__global__ __launch_bounds__(256) void image_kernel(ImageJobs jobs) {
   constexpr bool two = DT == AS_F32;
-  const float f = two ? plane_scale(*top) : 1.f;
-  const uint64_t words = (uint64_t)n * (pitch / 2);
-  for (uint64_t w = (uint64_t)blockIdx.x * 256 + threadIdx.x; w < words; w += (uint64_t)gridDim.x * 256) {
-    const uint64_t r = w / (pitch / 2);
-    const uint32_t k = (uint32_t)(w % (pitch / 2)) * 2;
-    const float x = k < d ? load_as_f32<DT>(src, r * stride + k) * f : 0.f, y = k + 1 < d ? load_as_f32<DT>(src, r * stride + k + 1) * f : 0.f;
-    unsigned short *o = out + r * pitch * (two ? 2 : 1) + k;
-    *(uint32_t *)o = pack2<FMT>(x, y);
-    if constexpr (two) *(uint32_t *)(o + pitch) = pack2<FMT>(low_part(x), low_part(y));
+  const ImageJob &j = jobs.job[blockIdx.y];
+  float f = 1.f;
+  if constexpr (two) {
+    __shared__ float s[4];
+    const float *p = jobs.parts + blockIdx.y * kTopParts;
+    float m = fmaxf(p[threadIdx.x], p[threadIdx.x + 256]);
+    for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    f = plane_scale(__float_as_uint(m));
+    if (blockIdx.x == 0 && threadIdx.x == 0) jobs.tops[blockIdx.y] = __float_as_uint(m);
   }
+  const uint32_t quads = j.pitch / 4, along = along_row(quads), rows = 256 / along;
+  for (uint64_t r = (uint64_t)blockIdx.x * rows + threadIdx.x / along; r < j.n; r += (uint64_t)gridDim.x * rows)
+    for (uint32_t g = threadIdx.x % along; g < quads; g += along) {
+      const f32x4 x = load_quad<DT>(j, r, g * 4) * f;
+      unsigned short *o = j.out + r * j.pitch * (two ? 2 : 1) + g * 4;
+      *(u32x2 *)o = u32x2{pack2<FMT>(x[0], x[1]), pack2<FMT>(x[2], x[3])};
+      if constexpr (two) *(u32x2 *)(o + j.pitch) = u32x2{pack2<FMT>(low_part(x[0]), low_part(x[1])), pack2<FMT>(low_part(x[2]), low_part(x[3]))};
+    }
 }
 // the same transposed: out[k][r], rows filled to `pitch` by zeros.  64 x 64 through LDS.
 template <int DT, int FMT>
@@ -586,7 +634,8 @@ int grad_tile(uint32_t m, uint32_t n) {
 }
 
 struct Plan {
-  uint32_t n, v, d, planes, steps, pitch;
+  uint32_t n, v, d, planes, steps, pitch, parts;
+  int rows_tiles;  // forward for short rows: tiles of 16 rows a wave, 0: the tiled form
   int tile;
   uint32_t n_tiles, v_tiles, per, chunks;
   // backward
@@ -649,22 +698,40 @@ void plan_backward(Plan &p, bool x, bool w, bool b, bool scaled) {
   p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(want / std::max<uint64_t>(tiles, 1), 64), cdiv(p.piece, 256)));
 }
 
+void plan_forward(Plan &p) {
+  p.fused = fused_steps(p.d, p.planes);
+  if (p.fused) {
+    p.pitch = p.fused * 32;
+    p.rows_tiles = p.n <= 64 ? 1 : p.n <= 128 ? 2 : 4;
+    p.x_blocks = cdiv(p.n, 64 * p.rows_tiles);
+    // few rows: the pass over the table is all there is, four workgroups a compute unit keep it in flight
+    const uint32_t groups = (p.rows_tiles == 1 ? 4 : 2) * kChips;
+    p.splits = std::max(1u, std::min(groups / std::min(p.x_blocks, groups), cdiv(p.v, 64)));
+    p.parts = p.splits;
+    return;
+  }
+  plan_walk(p);
+  p.parts = p.chunks * kShape[p.tile].wm;
+}
+
 struct ForwardScratch {
   float2 *part;
   unsigned int *tops;
+  float *top_parts;
   unsigned short *x_image, *t_image;
 };
 uint64_t forward_layout(const Plan &p, const Source &x, const Source &t, char *base, ForwardScratch &s) {
   Layout l{base};
-  s.part = l.take<float2>((uint64_t)p.chunks * kShape[p.tile].wm * p.n);
+  s.part = l.take<float2>((uint64_t)p.parts * p.n);
   s.tops = l.take<unsigned int>(2);
+  s.top_parts = l.take<float>(p.planes == 2 ? 2 * kTopParts : 0);
   s.x_image = l.take<unsigned short>(x.image_elems());
   s.t_image = l.take<unsigned short>(t.image_elems());
   return l.at;
 }
 struct BackwardScratch {
   unsigned int *tops;
-  float *coef;
+  float *top_parts, *coef;
   unsigned short *x_image, *t_image, *xt, *wt, *G, *GT;
   float *sums, *bias_part;
   float *lse, *every, *one;
@@ -674,6 +741,7 @@ uint64_t backward_layout(const Plan &p, const Source &x, const Source &t, char *
   Layout l{base};
   const uint64_t pl = p.planes;
   s.tops = l.take<unsigned int>(2);
+  s.top_parts = l.take<float>(p.planes == 2 ? 2 * kTopParts : 0);
   s.coef = l.take<float>(2);
   s.x_image = l.take<unsigned short>(x.image_elems());
   s.t_image = l.take<unsigned short>(t.image_elems());
@@ -710,28 +778,37 @@ void by_type(int dt, F &&f) {
 }
 unsigned spread(uint64_t items, uint64_t per_block) { return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((items + per_block - 1) / per_block, 16384)); }
 
-int make_tops(as_ctx *ctx, const Source &x, const Source &t, unsigned int *tops) {
-  if (x.dt != AS_F32) return AS_OK;
-  hipLaunchKernelGGL(zero_words_kernel, dim3(1), dim3(64), 0, ctx->stream, tops, 2u);
-  hipLaunchKernelGGL(top_kernel, dim3(std::min(cdiv(x.rows, 4), 1024u)), dim3(256), 0, ctx->stream, (const float *)x.p, x.stride, x.rows, x.d, tops);
-  hipLaunchKernelGGL(top_kernel, dim3(std::min(cdiv(t.rows, 4), 1024u)), dim3(256), 0, ctx->stream, (const float *)t.p, t.stride, t.rows, t.d, tops + 1);
-  AS_HIP(ctx, hipGetLastError());
-  return AS_OK;
-}
-int make_image(as_ctx *ctx, const Source &s, const unsigned int *top, unsigned short *image, const char **p, size_t *ld) {
-  if (s.direct()) {
-    *p = (const char *)s.p;
-    *ld = s.stride * 2;
-    return AS_OK;
-  }
-  by_type(s.dt, [&](auto dt) {
+// The two matrices as the products read them: each as it is, or its image; f32 with the largest magnitudes first.
+struct Operands {
+  const char *x, *t;
+  size_t x_ld, t_ld;
+};
+int make_operands(as_ctx *ctx, const Source &x, const Source &t, unsigned int *tops, float *parts, unsigned short *x_image, unsigned short *t_image, Operands *out) {
+  ImageJobs jobs{};
+  jobs.tops = tops, jobs.parts = parts;
+  uint32_t count = 0;
+  uint64_t most = 1;
+  auto add = [&](const Source &s, unsigned short *image, const char **p, size_t *ld) {
+    if (s.direct()) {
+      *p = (const char *)s.p;
+      *ld = s.stride * 2;
+      return;
+    }
+    const size_t es = dtype_size(s.dt);
+    jobs.job[count++] = ImageJob{s.p, s.stride, s.rows, s.d, s.pitch(), (s.stride % 4 == 0 && ((uintptr_t)s.p & (4 * es - 1)) == 0) ? 1 : 0, image};
+    most = std::max<uint64_t>(most, (uint64_t)s.rows * s.pitch() / 1024);
+    *p = (const char *)image;
+    *ld = (size_t)s.pitch() * s.planes() * 2;
+  };
+  add(x, x_image, &out->x, &out->x_ld);
+  add(t, t_image, &out->t, &out->t_ld);
+  if (!count) return AS_OK;
+  if (x.dt == AS_F32) hipLaunchKernelGGL(top_kernel, dim3(kTopParts, 2), dim3(256), 0, ctx->stream, jobs);
+  by_type(x.dt, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    hipLaunchKernelGGL((image_kernel<DT, DT == AS_BF16 ? AS_BF16 : AS_F16>), dim3(spread((uint64_t)s.rows * s.pitch() / 2, 1024)), dim3(256), 0, ctx->stream,
-                       s.p, s.stride, s.rows, s.d, s.pitch(), top, image);
+    hipLaunchKernelGGL((image_kernel<DT, DT == AS_BF16 ? AS_BF16 : AS_F16>), dim3((unsigned)std::min<uint64_t>(most, 2048), count), dim3(256), 0, ctx->stream, jobs);
   });
   AS_HIP(ctx, hipGetLastError());
-  *p = (const char *)image;
-  *ld = (size_t)s.pitch() * s.planes() * 2;
   return AS_OK;
 }
 void make_transposed(as_ctx *ctx, const Source &s, uint32_t row0, uint32_t rows, uint32_t pitch, const unsigned int *top, unsigned short *out) {
@@ -753,6 +830,29 @@ void launch_rows_grad(as_ctx *ctx, int dt, int steps, bool bias, const LossRowsA
     constexpr int FMT = decltype(fmt)::value, P = decltype(planes)::value, KD = decltype(kd)::value;
     if (bias) launch_rows_grad<FMT, P, KD, ITEMS, true>(ctx, a);
     else launch_rows_grad<FMT, P, KD, ITEMS, false>(ctx, a);
+  };
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  constexpr std::integral_constant<int, 4> four{};
+  constexpr std::integral_constant<int, 8> eight{};
+  constexpr std::integral_constant<int, AS_BF16> bf{};
+  constexpr std::integral_constant<int, AS_F16> hf{};
+  if (dt == AS_F32) steps == 2 ? go(hf, two, two) : go(hf, two, four);
+  else if (dt == AS_BF16) steps == 2 ? go(bf, one, two) : steps == 4 ? go(bf, one, four) : go(bf, one, eight);
+  else steps == 2 ? go(hf, one, two) : steps == 4 ? go(hf, one, four) : go(hf, one, eight);
+}
+template <int FMT, int P, int KD, int RT>
+void launch_rows_sums(as_ctx *ctx, bool general, const LossSumsArgs &a) {
+  const dim3 grid(a.r_blocks * a.splits);
+  if (general) hipLaunchKernelGGL((loss_rows_sums_kernel<FMT, P, RT, KD, true>), grid, dim3(256), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((loss_rows_sums_kernel<FMT, P, RT, KD, false>), grid, dim3(256), 0, ctx->stream, a);
+}
+void launch_rows_sums(as_ctx *ctx, int dt, int steps, int tiles, bool general, const LossSumsArgs &a) {
+  auto go = [&](auto fmt, auto planes, auto kd) {
+    constexpr int FMT = decltype(fmt)::value, P = decltype(planes)::value, KD = decltype(kd)::value;
+    if (tiles == 1) launch_rows_sums<FMT, P, KD, 1>(ctx, general, a);
+    else if (tiles == 2) launch_rows_sums<FMT, P, KD, 2>(ctx, general, a);
+    else launch_rows_sums<FMT, P, KD, 4>(ctx, general, a);
   };
   constexpr std::integral_constant<int, 1> one{};
   constexpr std::integral_constant<int, 2> two{};
@@ -822,7 +922,7 @@ int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tabl
   AS_TRY(L.bind(ctx, losses, c.n * 4));
   AS_TRY(S.bind(ctx, lse, c.n * 4));
   Plan p = make_plan((uint32_t)c.n, (uint32_t)c.v, (uint32_t)c.d, c.dt);
-  plan_walk(p);
+  plan_forward(p);
   const Source xs{X.p, (size_t)c.x_stride, p.n, p.d, c.dt, p.pitch}, ts{W.p, (size_t)c.table_stride, p.v, p.d, c.dt, p.pitch};
   ForwardScratch s{};
   Scratch scratch;
@@ -830,30 +930,39 @@ int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tabl
   forward_layout(p, xs, ts, scratch.base, s);
   ProfScope prof(ctx, "cross_entropy");
   LossArgs a{};
-  AS_TRY(make_tops(ctx, xs, ts, s.tops));
-  AS_TRY(make_image(ctx, xs, s.tops, s.x_image, &a.rows, &a.rows_ld));
-  AS_TRY(make_image(ctx, ts, s.tops + 1, s.t_image, &a.table, &a.table_ld));
+  Operands o{};
+  AS_TRY(make_operands(ctx, xs, ts, s.tops, s.top_parts, s.x_image, s.t_image, &o));
+  a.rows = o.x, a.rows_ld = o.x_ld, a.table = o.t, a.table_ld = o.t_ld;
   a.table_plane = a.rows_plane = p.steps;
   a.n = p.n, a.v = p.v, a.steps = p.steps, a.planes = p.planes, a.per = p.per, a.v_tiles = p.v_tiles, a.n_tiles = p.n_tiles, a.chunks = p.chunks;
   a.scale = c.scale, a.bias = (const float *)Bi.p;
   if (p.planes == 2) a.rows_top = s.tops, a.table_top = s.tops + 1;
   const bool general = bias || !(c.scale > 0.f);
-  by_tile(p.tile, [&](auto k) {
-    constexpr int K = decltype(k)::value;
-    auto go = [&](auto f, auto gen) {
-      constexpr int FMT = decltype(f)::value;
-      hipLaunchKernelGGL((loss_sums_kernel<FMT, TileOf<FMT, K>, decltype(gen)::value>), dim3(p.n_tiles * p.chunks), dim3(TileOf<FMT, K>::NT), 0, ctx->stream, a,
-                         s.part);
-    };
-    constexpr std::integral_constant<int, AS_BF16> bf{};
-    constexpr std::integral_constant<int, AS_F16> hf{};
-    if (c.dt == AS_BF16) general ? go(bf, std::true_type{}) : go(bf, std::false_type{});
-    else general ? go(hf, std::true_type{}) : go(hf, std::false_type{});
-  });
+  if (p.fused) {
+    LossSumsArgs r{};
+    r.r = a.rows, r.r_ld = a.rows_ld, r.nr = p.n, r.r_top = a.rows_top;
+    r.k = a.table, r.k_ld = a.table_ld, r.nk = p.v, r.k_top = a.table_top;
+    r.r_plane = r.k_plane = (size_t)p.pitch * 2;
+    r.r_blocks = p.x_blocks, r.splits = p.splits, r.scale = c.scale, r.bias = a.bias, r.part = s.part;
+    launch_rows_sums(ctx, c.dt, p.fused, p.rows_tiles, general, r);
+  } else {
+    by_tile(p.tile, [&](auto k) {
+      constexpr int K = decltype(k)::value;
+      auto go = [&](auto f, auto gen) {
+        constexpr int FMT = decltype(f)::value;
+        hipLaunchKernelGGL((loss_sums_kernel<FMT, TileOf<FMT, K>, decltype(gen)::value>), dim3(p.n_tiles * p.chunks), dim3(TileOf<FMT, K>::NT), 0, ctx->stream, a,
+                           s.part);
+      };
+      constexpr std::integral_constant<int, AS_BF16> bf{};
+      constexpr std::integral_constant<int, AS_F16> hf{};
+      if (c.dt == AS_BF16) general ? go(bf, std::true_type{}) : go(bf, std::false_type{});
+      else general ? go(hf, std::true_type{}) : go(hf, std::false_type{});
+    });
+  }
   AS_HIP(ctx, hipGetLastError());
   by_type(c.dt, [&](auto dt) {
     hipLaunchKernelGGL((loss_join_kernel<decltype(dt)::value>), dim3(cdiv(c.n, 4)), dim3(256), 0, ctx->stream, (const float2 *)s.part,
-                       p.chunks * kShape[p.tile].wm, X.p, (size_t)c.x_stride, W.p, (size_t)c.table_stride, (const float *)Bi.p, (const int64_t *)Y.p, p.n, p.v, p.d,
+                       p.parts, X.p, (size_t)c.x_stride, W.p, (size_t)c.table_stride, (const float *)Bi.p, (const int64_t *)Y.p, p.n, p.v, p.d,
                        c.scale, ignore, (float *)L.p, (float *)S.p);
   });
   AS_HIP(ctx, hipGetLastError());
@@ -906,10 +1015,10 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   backward_layout(p, xs, ts, scratch.base, s);
   GradArgs g{};
   LossArgs &a = g.l;
-  const char *table16 = nullptr;
-  AS_TRY(make_tops(ctx, xs, ts, s.tops));
-  AS_TRY(make_image(ctx, xs, s.tops, s.x_image, &a.rows, &a.rows_ld));
-  AS_TRY(make_image(ctx, ts, s.tops + 1, s.t_image, &table16, &a.table_ld));
+  Operands o{};
+  AS_TRY(make_operands(ctx, xs, ts, s.tops, s.top_parts, s.x_image, s.t_image, &o));
+  const char *table16 = o.t;
+  a.rows = o.x, a.rows_ld = o.x_ld, a.table_ld = o.t_ld;
   const unsigned int *x_top = p.planes == 2 ? s.tops : nullptr, *w_top = p.planes == 2 ? s.tops + 1 : nullptr;
   if (p.want_w && !p.fused) make_transposed(ctx, xs, 0, p.n, p.t_pitch, x_top, s.xt);
   if (p.scaled) hipLaunchKernelGGL(coef_scale_kernel, dim3(1), dim3(1024), 0, ctx->stream, (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p, ignore, p.n, s.coef);
@@ -1017,13 +1126,13 @@ uint64_t as_cross_entropy_workspace(uint64_t n, uint64_t n_items, uint64_t dim, 
   if (n == 0 || n_items == 0 || dim == 0 || n >= (1ull << 31) || n_items >= (1ull << 31) || dim > 65536 || !dtype_is_training(dtype)) return 0;
   Plan p = make_plan((uint32_t)n, (uint32_t)n_items, (uint32_t)dim, dtype);
   if (backward) plan_backward(p, true, true, true, true);
+  else plan_forward(p);
   // (a stride of dim + 1: room for the images whether or not the matrices can be taken as they are)
   const Source xs{nullptr, (size_t)dim + 1, p.n, p.d, dtype, p.pitch}, ts{nullptr, (size_t)dim + 1, p.v, p.d, dtype, p.pitch};
   if (backward) {
     BackwardScratch s{};
     return backward_layout(p, xs, ts, nullptr, s);
   }
-  plan_walk(p);
   ForwardScratch s{};
   return forward_layout(p, xs, ts, nullptr, s);
 }

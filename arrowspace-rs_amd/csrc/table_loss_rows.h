@@ -129,6 +129,158 @@ __device__ __forceinline__ void lr_transposed2(u32x4 &x, u32x4 &y, uint32_t a) {
   y = u32x4{y0[0], y0[1], y1[0], y1[1]};
 }
 
+// ---- forward for short rows -----------------------------------------------------------------------------------------------------------------
+// The same walk with only the statistics behind it: rows in registers, items in stages of 64, a running maximum and sum of exponentials
+// per lane and row.  For 128 values the matrix pipe needs 16 cycles for 64 logits and the exponentials' path (maximum, multiply-add,
+// exp, add) some 26, so what is saved counts: the maximum that the exponentials are taken against moves only when it is exceeded
+// by 2^20, once per walk in practice, and the rescaling with it.
+struct LossSumsArgs {
+  const char *r, *k;
+  size_t r_ld, k_ld, r_plane, k_plane;
+  uint32_t nr, nk, r_blocks, splits;
+  float scale;
+  const unsigned int *r_top, *k_top;
+  const float *bias;
+  float2 *part;  // [split][nr] (maximum, sum of exponentials against it)
+};
+template <int FMT, int P, int RT, int KD, bool GENERAL>
+__global__ __launch_bounds__(256, 2) void loss_rows_sums_kernel(LossSumsArgs a) {
+  constexpr uint32_t kRow = KD * 64, kPlane = 64 * kRow, kExtra = GENERAL ? 256 : 0, kStage = P * kPlane + kExtra;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
+  const uint32_t lds = (uint32_t)(size_t)(nt_lds *)smem;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, col = lane & 15;
+  const uint32_t work = die_order(blockIdx.x, gridDim.x);
+  const uint32_t rb = work % a.r_blocks, split = work / a.r_blocks;
+  const uint32_t r0 = (rb * 4 + wave) * (16 * RT);
+  const uint32_t stages = (a.nk + 63) / 64;
+  const uint32_t s_lo = (uint32_t)((uint64_t)stages * split / a.splits), s_hi = (uint32_t)((uint64_t)stages * (split + 1) / a.splits);
+  const float nat = a.scale * (P == 2 ? 1.f / plane_scale(*a.r_top) / plane_scale(*a.k_top) : 1.f);
+  const float unit = GENERAL ? kLog2e : nat * kLog2e, slack = fminf(20.f / unit, 1e30f);
+  auto swz = [](uint32_t row) { const uint32_t key = (row & 3) | ((row >> 1) & 4); return KD >= 4 ? key << 1 : key; };
+  auto fetch = [&](int buf, uint32_t s) {
+    char *dst = smem + buf * kStage;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int t = 0; t < KD; ++t) {
+        const uint32_t idx = t * 256 + threadIdx.x, row = idx / (KD * 4), slot = idx % (KD * 4);
+        const uint32_t k = nt_min(s * 64 + row, a.nk - 1);
+        __builtin_amdgcn_global_load_lds((nt_gbl *)(a.k + (size_t)k * a.k_ld + p * a.k_plane + ((slot ^ swz(row)) << 4)),
+                                         (nt_lds *)(dst + p * kPlane + (t * 256 + wave * 64) * 16), 16, 0, 0);
+      }
+    if constexpr (GENERAL) {
+      if (wave == 0 && a.bias)
+        __builtin_amdgcn_global_load_lds((nt_gbl *)(a.bias + nt_min(s * 64 + lane, a.nk - 1)), (nt_lds *)(dst + P * kPlane), 4, 0, 0);
+    }
+  };
+  if (s_lo < s_hi) fetch(0, s_lo);
+  u32x4 R[P][RT][KD];
+  float ref[RT], base[RT], sum[RT];
+#pragma unroll
+  for (int j = 0; j < RT; ++j) {
+    const uint32_t row = nt_min(r0 + j * 16 + col, a.nr - 1);
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int s = 0; s < KD; ++s) R[p][j][s] = *(const u32x4 *)(a.r + (size_t)row * a.r_ld + p * a.r_plane + s * 64 + q * 16);
+    ref[j] = -INFINITY;
+    base[j] = sum[j] = 0.f;
+  }
+  const uint32_t frow = ((col >> 2) << 3) + (col & 3), fa = frow * kRow + ((q ^ swz(frow)) << 4);
+  const bool here = r0 < a.nr;  // (a wave without rows only brings its part of the stages)
+  int buf = 0;
+  for (uint32_t s = s_lo; s < s_hi; ++s, buf ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (s + 1 < s_hi) fetch(buf ^ 1, s + 1);
+    if (!here) continue;
+#pragma unroll 1
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t k0 = s * 64 + h * 32;
+      f32x4 z[2][RT];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < RT; ++j) z[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const uint32_t at = lds + buf * kStage + h * 32 * kRow + fa;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int s4 = 0; s4 < KD; s4 += 4) {
+            u32x4 A[4];
+            const uint32_t ap = at + p * kPlane;
+            if constexpr (KD == 2) i == 0 ? lr_read2<0>(A[0], A[1], ap, ap ^ 64) : lr_read2<4 * kRow>(A[0], A[1], ap, ap ^ 64);
+            else i == 0 ? lr_read4<0>(A, ap ^ (s4 << 6), ap ^ ((s4 + 1) << 6), ap ^ ((s4 + 2) << 6), ap ^ ((s4 + 3) << 6))
+                        : lr_read4<4 * kRow>(A, ap ^ (s4 << 6), ap ^ ((s4 + 1) << 6), ap ^ ((s4 + 2) << 6), ap ^ ((s4 + 3) << 6));
+#pragma unroll
+            for (int t = 0; t < (KD < 4 ? KD : 4); ++t)
+#pragma unroll
+              for (int j = 0; j < RT; ++j) {
+                z[i][j] = nt_mfma<FMT>(A[t], R[0][j][s4 + t], z[i][j]);
+                if (P == 2 && p == 0) z[i][j] = nt_mfma<FMT>(A[t], R[P - 1][j][s4 + t], z[i][j]);
+              }
+          }
+        if constexpr (GENERAL) {
+          f32x4 kb = {0.f, 0.f, 0.f, 0.f};
+          if (a.bias)
+            asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(kb) : "v"(lds + buf * kStage + P * kPlane + h * 128 + q * 32 + i * 16) : "memory");
+#pragma unroll
+          for (int j = 0; j < RT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[i][j][e] = fmaf(z[i][j][e], nat, kb[e]);
+        }
+        if (k0 + 32 > a.nk) {  // items behind the last
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (k0 + q * 8 + i * 4 + e >= a.nk)
+#pragma unroll
+              for (int j = 0; j < RT; ++j) z[i][j][e] = -INFINITY;
+        }
+      }
+      float top[RT];
+      bool over = false;
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        top[j] = fmaxf(fmaxf(fmaxf(z[0][j][0], z[0][j][1]), fmaxf(z[0][j][2], z[0][j][3])), fmaxf(fmaxf(z[1][j][0], z[1][j][1]), fmaxf(z[1][j][2], z[1][j][3])));
+        over |= top[j] > ref[j] + slack;
+      }
+      if (__any(over)) {
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+          if (top[j] > ref[j]) {
+            const float was = ref[j];
+            ref[j] = top[j];
+            sum[j] *= __builtin_amdgcn_exp2f((was - top[j]) * unit);  // (nothing yet: -inf, 0)
+            base[j] = GENERAL ? top[j] : -top[j] * unit;
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        auto power = [&](float x) { return __builtin_amdgcn_exp2f(GENERAL ? (x - base[j]) * unit : fmaf(x, unit, base[j])); };
+        float s0 = power(z[0][j][0]) + power(z[0][j][1]), s1 = power(z[0][j][2]) + power(z[0][j][3]);
+        s0 += power(z[1][j][0]) + power(z[1][j][1]);
+        s1 += power(z[1][j][2]) + power(z[1][j][3]);
+        sum[j] += s0 + s1;
+      }
+    }
+  }
+  if (!here) return;
+#pragma unroll
+  for (int j = 0; j < RT; ++j) {
+    float m = GENERAL ? ref[j] : ref[j] == -INFINITY ? -INFINITY : ref[j] * nat, s = sum[j];
+#pragma unroll
+    for (int x = 16; x < 64; x <<= 1) {
+      const float mo = __shfl_xor(m, x), so = __shfl_xor(s, x);
+      const float mm = fmaxf(m, mo), b = mm == -INFINITY ? 0.f : mm;
+      s = s * __builtin_amdgcn_exp2f((m - b) * kLog2e) + so * __builtin_amdgcn_exp2f((mo - b) * kLog2e);
+      m = mm;
+    }
+    const uint32_t row = r0 + j * 16 + col;
+    if (q == 0 && row < a.nr) a.part[(size_t)split * a.nr + row] = float2{m, s};
+  }
+}
+
 // FMT the operands' type; P planes; RT tiles of 16 rows r a wave; KD steps of 32 columns; ITEMS: the rows r are items (dW), else the
 // batch (dX); OUT: type of dW
 template <int FMT, int P, int RT, int KD, bool ITEMS, bool BIAS, int OUT>
