@@ -13,7 +13,7 @@
 // Types.  bf16 and f16 go to the matrix pipe as they are.  f32 values go as a sum of two f16 (22 bits, after a power of two that
 // brings the matrix' largest finite value to 2^14 .. 2^15), three products per pair of planes: 2.5 PFLOP/s / 3 against the
 // 0.157 of the f32 instruction, and an error per product of 2^-23 of it, which the f32 sums have anyway.
-// Rounding.  G is rounded to 16 bits (f16: after a power of two from the largest coefficient; f32: two planes, 22 bits): half a
+// Rounding.  G is rounded to 16 bits in units of the largest coefficient (coef_scale_kernel; f32: two planes, 22 bits): half a
 // step per entry, as the gradients that leave are rounded themselves.  Everything else -- logits, maxima, sums, dX over pieces,
 // dbias -- is f32 or wider.
 #include "table_loss_rows.h"
@@ -52,7 +52,8 @@ __global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2
   TILE T;
   T.init(smem);
   const uint32_t work = die_order(blockIdx.x, gridDim.x);
-  const uint32_t nt = work % a.n_tiles, chunk = work / a.n_tiles;
+  uint32_t nt, chunk;
+  grid_order(work, a.n_tiles, a.chunks, &nt, &chunk);
   const uint32_t n0 = nt * TILE::BN, vt_end = nt_min((chunk + 1) * a.per, a.v_tiles);
   uint32_t vt = chunk * a.per;
   const float nat = a.scale * product_scale(a), unit = GENERAL ? kLog2e : nat * kLog2e;  // exponentials of (x - maximum) * unit to the base 2
@@ -153,18 +154,29 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2 *part, uint
                                                         uint32_t d, float scale, int64_t ignore, float *losses, float *lse_out) {
   const uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (t >= n) return;
-  float m = -INFINITY;
+  float top = -INFINITY;
   double s = 0.0;
-  for (uint32_t p = lane; p < parts; p += 64) {
-    const float2 o = part[(size_t)p * n + t];
-    const float mm = fmaxf(m, o.x), base = mm == -INFINITY ? 0.f : mm;
-    s = s * (double)exp2f((m - base) * kLog2e) + (double)o.y * (double)exp2f((o.x - base) * kLog2e);
-    m = mm;
+  for (uint32_t p0 = 0; p0 < parts; p0 += 1024) {
+    float2 o[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const uint32_t p = p0 + k * 64 + lane;
+      o[k] = p < parts ? part[(size_t)p * n + t] : float2{-INFINITY, 0.f};
+    }
+    float m = top;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) m = fmaxf(m, o[k].x);
+    const float base = m == -INFINITY ? 0.f : m;
+    float here = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) here += o[k].y * __builtin_amdgcn_exp2f((o[k].x - base) * kLog2e);
+    s = s * (double)__builtin_amdgcn_exp2f((top - base) * kLog2e) + (double)here;
+    top = m;
   }
-  float top = m;
+  const float m = top;
   for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
   const float base = top == -INFINITY ? 0.f : top;
-  s *= (double)exp2f((m - base) * kLog2e);
+  s *= (double)__builtin_amdgcn_exp2f((m - base) * kLog2e);
   for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
   const int64_t y = targets[t];
   const bool ignored = y == ignore, inside = y >= 0 && y < (int64_t)v;
@@ -285,25 +297,31 @@ __global__ __launch_bounds__(256) void transposed_kernel(const void *src, size_t
   }
 }
 
-// f16 gradients of logits: multiplied by 2^14 over the power of two of the largest coefficient (entries down to 2^-28 of it keep
-// all 11 bits).  One workgroup; reads 16 bytes a row.
-__global__ __launch_bounds__(1024) void coef_scale_kernel(const float *gl, const float *ge, const int64_t *targets, int64_t ignore, uint32_t n, float *out) {
-  __shared__ float s[16];
-  float m = 0.f;
+// The unit the gradient of the logits is rounded in: the largest |grad_losses|, so that the entry of a target, -grad_losses (1 - p), is
+// a whole number of steps where all rows weigh the same (the mean of the losses: without this every such entry is off by the SAME
+// part of 2^-9 in bf16, which no sum averages out).  f16: 2^14 of these units, entries down to 2^-28 of one keep all 11 bits.
+// Where grad_lse outweighs grad_losses the largest of their sum.  One workgroup; 16 bytes a row.
+__global__ __launch_bounds__(1024) void coef_scale_kernel(const float *gl, const float *ge, const int64_t *targets, int64_t ignore, uint32_t n, int power, float *out) {
+  __shared__ float s[2][16];
+  float one = 0.f, both = 0.f;
   for (uint32_t t = threadIdx.x; t < n; t += 1024) {
     const float l = targets[t] == ignore ? 0.f : gl[t], b = fabsf(l + (ge ? ge[t] : 0.f)), o = fabsf(l);
-    if (o < INFINITY) m = fmaxf(m, o);
-    if (b < INFINITY) m = fmaxf(m, b);
+    if (o < INFINITY) one = fmaxf(one, o);
+    if (b < INFINITY) both = fmaxf(both, b);
   }
-  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+  for (int k = 1; k < 64; k <<= 1) {
+    one = fmaxf(one, __shfl_xor(one, k));
+    both = fmaxf(both, __shfl_xor(both, k));
+  }
+  if ((threadIdx.x & 63) == 0) s[0][threadIdx.x >> 6] = one, s[1][threadIdx.x >> 6] = both;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 16; ++w) m = fmaxf(m, s[w]);
-    const int e = (int)(__float_as_uint(m) >> 23);
-    const int k = e == 0 ? 0 : min(max(14 - (e - 126), -100), 100);  // m < 2^(e - 126)
-    out[0] = __uint_as_float((unsigned int)(127 + k) << 23);
-    out[1] = __uint_as_float((unsigned int)(127 - k) << 23);
+    for (int w = 1; w < 16; ++w) one = fmaxf(one, s[0][w]), both = fmaxf(both, s[1][w]);
+    float m = both <= 2.f * one ? one : both;
+    if (!(m >= 1e-36f && m <= 1e36f)) m = 1.f;   // (nothing to scale, or nothing that a factor brings into range)
+    const float unit = m * __uint_as_float((unsigned int)(127 - power) << 23);
+    out[0] = 1.f / unit;
+    out[1] = unit;
   }
 }
 
@@ -314,7 +332,7 @@ struct GradArgs {
   const float *lse, *gl, *ge;
   const int64_t *targets;
   int64_t ignore;
-  const float *coef;               // {factor, 1 / factor} of G, or null: 1
+  const float *coef;               // {factor, 1 / factor} of G
   unsigned short *G, *GT;          // n x (planes * g_pitch), v_pad x (planes * t_pitch)
   uint32_t g_pitch, t_pitch;
   float *bias_part;                // (n_tiles WN) x g_pitch sums over the tile's rows, or null
@@ -328,10 +346,11 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
   TILE T;
   T.init(smem);
   const uint32_t work = die_order(blockIdx.x, gridDim.x);
-  const uint32_t nt = work % a.n_tiles, chunk = work / a.n_tiles;
+  uint32_t nt, chunk;
+  grid_order(work, a.n_tiles, a.chunks, &nt, &chunk);
   const uint32_t n0 = nt * TILE::BN, vt_end = nt_min((chunk + 1) * a.per, a.v_tiles);
   uint32_t vt = chunk * a.per;
-  const float c = a.scale * product_scale(a), factor = g.coef ? g.coef[0] : 1.f;
+  const float c = a.scale * product_scale(a), factor = g.coef[0];
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
   NtOperand B{a.rows + (size_t)n0 * a.rows_ld, a.rows_ld, nt_min(TILE::BN, a.n - n0) - 1, a.rows_plane};
   auto side = [&](uint32_t tile) {
@@ -487,7 +506,7 @@ struct ProductArgs {
   uint32_t m, n, m_tiles, n_tiles;
   uint32_t steps, planes, splits;   // steps of 64 of the whole contraction; a split takes an even share of them
   float scale;
-  const float *coef;                // 1 / factor of G at [1], or null
+  const float *coef;                // 1 / factor of G at [1]
   const unsigned int *top;          // largest magnitude of the other operand's matrix (two planes), or null
   void *out;                        // n x m rows of `out_stride` elements
   size_t out_stride;
@@ -502,7 +521,9 @@ __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
   TILE T;
   T.init(smem);
   const uint32_t work = die_order(blockIdx.x, gridDim.x);
-  const uint32_t mt = work % p.m_tiles, rest = work / p.m_tiles, nt = rest % p.n_tiles, split = rest / p.n_tiles;
+  const uint32_t split = work / (p.m_tiles * p.n_tiles);
+  uint32_t mt, nt;
+  grid_order(work - split * p.m_tiles * p.n_tiles, p.n_tiles, p.m_tiles, &nt, &mt);
   const uint32_t m0 = mt * TILE::BM, n0 = nt * TILE::BN;
   const uint32_t k0 = (uint32_t)((uint64_t)p.steps * split / p.splits), k1 = (uint32_t)((uint64_t)p.steps * (split + 1) / p.splits);
   const uint32_t steps = k1 - k0, all = p.planes == 2 ? 3 * steps : steps;
@@ -519,7 +540,7 @@ __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
     buf ^= 1;
   }
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
-  const float f = OUT == 0 ? 1.f : p.scale * (p.coef ? p.coef[1] : 1.f) * (p.top ? 1.f / plane_scale(*p.top) : 1.f);
+  const float f = OUT == 0 ? 1.f : p.scale * p.coef[1] * (p.top ? 1.f / plane_scale(*p.top) : 1.f);
 #pragma unroll
   for (int j = 0; j < TILE::TN; ++j) {
     const uint32_t n = n0 + wn * (TILE::TN * 16) + (j >> 1) * 32 + (col >> 2) * 8 + (j & 1) * 4 + (col & 3);
@@ -551,30 +572,42 @@ __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
   }
 }
 
-// dX from its parts, in their order: 64 columns a workgroup, 16 waves a sixteenth of the parts each (a few rows have hundreds of parts)
-template <int DT>
-__global__ __launch_bounds__(1024) void grad_rows_join_kernel(const float *sums, uint32_t splits, uint32_t pitch, uint32_t n, uint32_t d, float scale,
-                                                              const float *coef, const unsigned int *top, void *out, size_t out_stride) {
-  __shared__ float s[16][64];
-  const float f = scale * (coef ? coef[1] : 1.f) * (top ? 1.f / plane_scale(*top) : 1.f);
-  const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+// dX from its parts, in their order.  FEW parts: a thread four columns; else 64 columns a workgroup, 16 waves a sixteenth of the parts
+// each (a few rows have hundreds of parts: one thread's chain of them would be the whole time).
+template <int DT, bool FEW>
+__global__ __launch_bounds__(FEW ? 256 : 1024) void grad_rows_join_kernel(const float *sums, uint32_t splits, uint32_t pitch, uint32_t n, uint32_t d, float scale,
+                                                                          const float *coef, const unsigned int *top, void *out, size_t out_stride) {
+  const float f = scale * coef[1] * (top ? 1.f / plane_scale(*top) : 1.f);
   const uint64_t total = (uint64_t)n * pitch;
-  const uint32_t lo = splits * w / 16, hi = splits * (w + 1) / 16;
-  for (uint64_t i0 = (uint64_t)blockIdx.x * 64; i0 < total; i0 += (uint64_t)gridDim.x * 64) {
-    const uint64_t i = i0 + lane;
-    float x = 0.f;
-    if (i < total) {
+  if constexpr (FEW) {
+    for (uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < total; i += (uint64_t)gridDim.x * 1024) {
+      f32x4 x = *(const f32x4 *)(sums + i);
+      for (uint32_t p = 1; p < splits; ++p) x += *(const f32x4 *)(sums + p * total + i);
+      const uint64_t t = i / pitch, k = i - t * pitch;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (k + e < d) store_from_f32<DT>(out, t * out_stride + k + e, x[e] * f);
+    }
+  } else {
+    __shared__ float s[16][64];
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const uint32_t lo = splits * w / 16, hi = splits * (w + 1) / 16;
+    for (uint64_t i0 = (uint64_t)blockIdx.x * 64; i0 < total; i0 += (uint64_t)gridDim.x * 64) {
+      const uint64_t i = i0 + lane;
+      float x = 0.f;
+      if (i < total) {
 #pragma unroll 8
-      for (uint32_t p = lo; p < hi; ++p) x += sums[p * total + i];
+        for (uint32_t p = lo; p < hi; ++p) x += sums[p * total + i];
+      }
+      s[w][lane] = x;
+      __syncthreads();
+      if (w == 0 && i < total) {
+        for (int k = 1; k < 16; ++k) x += s[k][lane];
+        const uint64_t t = i / pitch, k = i % pitch;
+        if (k < d) store_from_f32<DT>(out, t * out_stride + k, x * f);
+      }
+      __syncthreads();
     }
-    s[w][lane] = x;
-    __syncthreads();
-    if (w == 0 && i < total) {
-      for (int k = 1; k < 16; ++k) x += s[k][lane];
-      const uint64_t t = i / pitch, k = i % pitch;
-      if (k < d) store_from_f32<DT>(out, t * out_stride + k, x * f);
-    }
-    __syncthreads();
   }
 }
 __global__ __launch_bounds__(256) void bias_join_kernel(const float *part, uint32_t parts, uint32_t pitch, uint32_t v, const float *coef, float *out) {
@@ -582,7 +615,7 @@ __global__ __launch_bounds__(256) void bias_join_kernel(const float *part, uint3
   if (i >= v) return;
   float s = 0.f;
   for (uint32_t p = 0; p < parts; ++p) s += part[(size_t)p * pitch + i];
-  out[i] = s * (coef ? coef[1] : 1.f);
+  out[i] = s * coef[1];
 }
 template <int DT>
 __global__ __launch_bounds__(256) void zero_rows_kernel(void *out, size_t stride, uint64_t n, uint32_t d) {
@@ -620,18 +653,13 @@ struct Source {
 };
 int image_format(int dt) { return dt == AS_BF16 ? AS_BF16 : AS_F16; }
 
-// tile of the products of the logits
-int logits_tile(uint32_t n, uint32_t v) {
-  if (n <= 64) return kSlim;
-  if (n <= 128) return kSquare;
-  // the large tile where the chip gets two rounds of them; below, four times as many small ones
-  return (uint64_t)cdiv(n, 256) * cdiv(v, 256) >= 2 * kChips ? kLarge : kSquare;
+// Which tile.  Rounds of workgroups times what one takes: the large one has the chip's 256 units to itself, two square ones share a
+// unit, each a quarter of the work at 0.8 of the rate (8192 x 16384 x 1024: 259 and 330 us).
+bool large_pays(uint32_t m, uint32_t n) {
+  const uint64_t large = (uint64_t)cdiv(m, 256) * cdiv(n, 256), square = (uint64_t)cdiv(m, 128) * cdiv(n, 128);
+  return 1.6 * (double)((large + kChips - 1) / kChips) <= (double)((square + 2 * kChips - 1) / (2 * kChips));
 }
-int grad_tile(uint32_t m, uint32_t n) {
-  if (n <= 64) return kSlim;
-  if (m <= 128 || n <= 128) return kSquare;
-  return (uint64_t)cdiv(m, 256) * cdiv(n, 256) >= kChips ? kLarge : kSquare;
-}
+int product_tile(uint32_t m, uint32_t n) { return n <= 64 ? kSlim : n <= 128 || m <= 128 || !large_pays(m, n) ? kSquare : kLarge; }
 
 struct Plan {
   uint32_t n, v, d, planes, steps, pitch, parts;
@@ -643,7 +671,7 @@ struct Plan {
   int tile_w, tile_x;
   int fused;                 // steps of 32 columns of the form for short rows (table_loss_rows.h), 0: through G in memory
   uint32_t x_blocks, w_blocks, n_pad;
-  bool want_x, want_w, want_b, scaled;
+  bool want_x, want_w, want_b;
 };
 Plan make_plan(uint32_t n, uint32_t v, uint32_t d, int dt) {
   Plan p{};
@@ -651,38 +679,70 @@ Plan make_plan(uint32_t n, uint32_t v, uint32_t d, int dt) {
   p.planes = dt == AS_F32 ? 2 : 1;
   p.steps = cdiv(d, 64);
   p.pitch = p.steps * 64;
-  p.tile = logits_tile(n, v);
+  p.tile = product_tile(v, n);
   p.n_tiles = cdiv(n, kShape[p.tile].bn);
   p.v_tiles = cdiv(v, kShape[p.tile].bm);
   return p;
 }
-// tiles a workgroup walks: at least four rounds of workgroups on the chip, so that the last one costs little
+// workgroups of a tile that the chip runs at once
+uint32_t slots_of(int tile) { return tile == kLarge ? kChips : 2 * kChips; }
+// tiles a workgroup walks: so many that whole rounds of workgroups fill the chip (1 024 workgroups of six tiles on 256 units: the fifth
+// round is nearly empty, 18 % of the time)
 void plan_walk(Plan &p) {
-  const uint64_t tiles = (uint64_t)p.n_tiles * p.v_tiles, groups = 4ull * kChips;
-  p.per = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(p.v_tiles, tiles / groups));
+  const uint32_t slots = slots_of(p.tile);
+  uint64_t best = ~0ull;
+  for (uint32_t r = 1; r <= 8; ++r) {
+    const uint32_t chunks = std::max(1u, std::min((uint32_t)((uint64_t)slots * r / p.n_tiles), p.v_tiles)), per = cdiv(p.v_tiles, chunks);
+    const uint64_t blocks = (uint64_t)p.n_tiles * cdiv(p.v_tiles, per);
+    // rounds of tiles, and a twentieth of a tile for each workgroup's start
+    const uint64_t cost = (blocks + slots - 1) / slots * (20ull * per + 1);
+    if (cost < best) {
+      best = cost;
+      p.per = per;
+    }
+  }
   p.chunks = cdiv(p.v_tiles, p.per);
 }
+// parts of a contraction whose output has so many tiles
+uint32_t plan_splits(uint64_t tiles, uint32_t slots, uint32_t most) {
+  uint32_t best = 1;
+  double cost = 1e30;
+  for (uint32_t s = 1; s <= std::min(most, 64u); ++s) {
+    const double c = (double)((tiles * s + slots - 1) / slots) / s * (1 + 0.01 * s);
+    if (c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  return best;
+}
+
 // the form for short rows: its steps of 32 columns, and tiles of 16 rows a wave holds (what 256 registers take)
 int fused_steps(uint32_t d, uint32_t planes) { return d <= 64 ? 2 : d <= 128 ? 4 : d <= 256 && planes == 1 ? 8 : 0; }
-constexpr int fused_rows(int steps, int planes) { return steps == 8 || planes == 2 ? 2 : steps == 4 ? 3 : 4; }
-void plan_backward(Plan &p, bool x, bool w, bool b, bool scaled) {
-  p.want_x = x, p.want_w = w, p.want_b = b, p.scaled = scaled;
+// ... and waves a SIMD.  1 024 rows x 1 M items, bf16, us (dW / dX): 64 values 2 tiles x 4 waves 270 / -, 3 x 3 257 / -, 4 x 2 283 / 264;
+// 128 values 2 x 3 515 / 439, 3 x 2 490 / 480, 4 x 2 728 / 632 (spills); 256 values 1 x 2 1 273 / 1 262, 2 x 2 1 437 / 1 410 (spills)
+constexpr int fused_rows(int steps, int planes, bool items) { return planes == 2 ? 2 : steps == 8 ? 1 : steps == 2 || items ? 3 : 2; }
+constexpr int fused_waves(int steps, int planes, bool items) { return planes == 2 || steps == 8 ? 2 : steps == 2 || !items ? 3 : 2; }
+void plan_backward(Plan &p, bool x, bool w, bool b) {
+  p.want_x = x, p.want_w = w, p.want_b = b;
   p.fused = fused_steps(p.d, p.planes);
   if (p.fused) {
-    const uint32_t rows = 64 * fused_rows(p.fused, p.planes), stages = cdiv(p.v, 64);
+    const uint32_t stages = cdiv(p.v, 64), groups = fused_waves(p.fused, p.planes, false) * kChips;
     p.pitch = p.fused * 32;
-    p.x_blocks = cdiv(p.n, rows);
-    p.w_blocks = cdiv(p.v, rows);
+    p.x_blocks = cdiv(p.n, 64 * fused_rows(p.fused, p.planes, false));
+    p.w_blocks = cdiv(p.v, 64 * fused_rows(p.fused, p.planes, true));
     p.n_pad = up(p.n, 64);
-    // the items in parts, so that two workgroups a compute unit are there
-    p.splits = std::max(1u, std::min(2u * kChips / std::min(p.x_blocks, 2u * kChips), stages));
+    // the items in parts, so that the workgroups are there that a compute unit holds
+    p.splits = std::max(1u, std::min(groups / std::min(p.x_blocks, groups), stages));
     return;
   }
   const uint32_t bm = kShape[p.tile].bm, bn = kShape[p.tile].bn;
   p.t_pitch = up(p.n, std::max(bn, 64u));
-  // G and its transposed form of a piece: 512 MB together (the two products that read them want thousands of items), whole tiles
+  // G and its transposed form of a piece: some 512 MB together, and whole rounds of the large tile for the piece's dW
   const uint64_t per_item = (uint64_t)p.t_pitch * 2 * 2 * p.planes;
-  uint64_t piece = std::max<uint64_t>((512ull << 20) / per_item / 1024 * 1024, 1024);
+  const uint32_t round = std::max(1u, (uint32_t)kChips / cdiv(p.d, 256)) * 256;
+  uint64_t piece = std::max<uint64_t>((640ull << 20) / per_item / round, 1) * round;
+  if (piece * per_item > (1024ull << 20)) piece = std::max<uint64_t>((512ull << 20) / per_item / 1024 * 1024, 1024);
   piece = std::min<uint64_t>(piece, up(p.v, bm));
   p.piece = (uint32_t)up(piece, bm);
   p.pieces = cdiv(p.v, p.piece);
@@ -690,14 +750,15 @@ void plan_backward(Plan &p, bool x, bool w, bool b, bool scaled) {
   p.pieces = cdiv(p.v, p.piece);
   p.v_tiles = cdiv(p.piece, bm);
   plan_walk(p);
-  p.tile_w = grad_tile(p.d, std::min(p.piece, p.v));
+  p.tile_w = product_tile(p.d, std::min(p.piece, p.v));
   p.tile_x = p.n <= 64 ? kSlim : p.d <= 128 || p.n <= 128 ? kSquare : kLarge;
   const uint64_t tiles = (uint64_t)cdiv(p.d, kShape[p.tile_x].bm) * cdiv(p.n, kShape[p.tile_x].bn);
   // the contraction over the piece is split where the output alone does not fill the chip
-  const uint64_t want = (p.tile_x == kLarge ? 1 : 2) * kChips;
-  p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(want / std::max<uint64_t>(tiles, 1), 64), cdiv(p.piece, 256)));
+  p.splits = plan_splits(tiles, slots_of(p.tile_x), cdiv(p.piece, 256));
 }
 
+// waves a SIMD of the forward (1 024 rows x 1 M items of 128: four tiles of rows x 2 waves 293 us, x 3 282, two x 4 316)
+constexpr int sums_waves(int steps, int planes, int tiles) { return steps * planes == 8 || tiles < 4 ? 2 : steps * planes == 4 ? 3 : 4; }
 void plan_forward(Plan &p) {
   p.fused = fused_steps(p.d, p.planes);
   if (p.fused) {
@@ -705,7 +766,7 @@ void plan_forward(Plan &p) {
     p.rows_tiles = p.n <= 64 ? 1 : p.n <= 128 ? 2 : 4;
     p.x_blocks = cdiv(p.n, 64 * p.rows_tiles);
     // few rows: the pass over the table is all there is, four workgroups a compute unit keep it in flight
-    const uint32_t groups = (p.rows_tiles == 1 ? 4 : 2) * kChips;
+    const uint32_t groups = (p.rows_tiles == 1 ? 4 : sums_waves(p.fused, p.planes, p.rows_tiles)) * kChips;
     p.splits = std::max(1u, std::min(groups / std::min(p.x_blocks, groups), cdiv(p.v, 64)));
     p.parts = p.splits;
     return;
@@ -822,7 +883,7 @@ void make_transposed(as_ctx *ctx, const Source &s, uint32_t row0, uint32_t rows,
 template <int FMT, int P, int KD, bool ITEMS, bool BIAS>
 void launch_rows_grad(as_ctx *ctx, const LossRowsArgs &a) {
   constexpr int OUT = P == 2 ? AS_F32 : FMT;
-  hipLaunchKernelGGL((loss_rows_grad_kernel<FMT, P, fused_rows(KD, P), KD, ITEMS, BIAS, OUT>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
+  hipLaunchKernelGGL((loss_rows_grad_kernel<FMT, P, fused_rows(KD, P, ITEMS), KD, ITEMS, BIAS, OUT, fused_waves(KD, P, ITEMS)>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
 }
 template <bool ITEMS>
 void launch_rows_grad(as_ctx *ctx, int dt, int steps, bool bias, const LossRowsArgs &a) {
@@ -844,8 +905,8 @@ void launch_rows_grad(as_ctx *ctx, int dt, int steps, bool bias, const LossRowsA
 template <int FMT, int P, int KD, int RT>
 void launch_rows_sums(as_ctx *ctx, bool general, const LossSumsArgs &a) {
   const dim3 grid(a.r_blocks * a.splits);
-  if (general) hipLaunchKernelGGL((loss_rows_sums_kernel<FMT, P, RT, KD, true>), grid, dim3(256), 0, ctx->stream, a);
-  else hipLaunchKernelGGL((loss_rows_sums_kernel<FMT, P, RT, KD, false>), grid, dim3(256), 0, ctx->stream, a);
+  if (general) hipLaunchKernelGGL((loss_rows_sums_kernel<FMT, P, RT, KD, true, sums_waves(KD, P, RT)>), grid, dim3(256), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((loss_rows_sums_kernel<FMT, P, RT, KD, false, sums_waves(KD, P, RT)>), grid, dim3(256), 0, ctx->stream, a);
 }
 void launch_rows_sums(as_ctx *ctx, int dt, int steps, int tiles, bool general, const LossSumsArgs &a) {
   auto go = [&](auto fmt, auto planes, auto kd) {
@@ -1007,7 +1068,7 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
     return finish_call(ctx);
   }
   Plan p = make_plan((uint32_t)c.n, (uint32_t)c.v, (uint32_t)c.d, c.dt);
-  plan_backward(p, gx != nullptr, gw != nullptr, gb != nullptr, c.dt != AS_BF16);
+  plan_backward(p, gx != nullptr, gw != nullptr, gb != nullptr);
   const Source xs{X.p, (size_t)c.x_stride, p.n, p.d, c.dt, p.pitch}, ts{W.p, (size_t)c.table_stride, p.v, p.d, c.dt, p.pitch};
   BackwardScratch s{};
   Scratch scratch;
@@ -1021,9 +1082,10 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   a.rows = o.x, a.rows_ld = o.x_ld, a.table_ld = o.t_ld;
   const unsigned int *x_top = p.planes == 2 ? s.tops : nullptr, *w_top = p.planes == 2 ? s.tops + 1 : nullptr;
   if (p.want_w && !p.fused) make_transposed(ctx, xs, 0, p.n, p.t_pitch, x_top, s.xt);
-  if (p.scaled) hipLaunchKernelGGL(coef_scale_kernel, dim3(1), dim3(1024), 0, ctx->stream, (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p, ignore, p.n, s.coef);
+  hipLaunchKernelGGL(coef_scale_kernel, dim3(1), dim3(1024), 0, ctx->stream, (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p, ignore, p.n,
+                     c.dt == AS_BF16 ? 0 : 14, s.coef);
   AS_HIP(ctx, hipGetLastError());
-  const float *coef = p.scaled ? s.coef : nullptr;
+  const float *coef = s.coef;
   if (p.fused) {
     hipLaunchKernelGGL(loss_rows_kernel, dim3(cdiv(p.n_pad, 256)), dim3(256), 0, ctx->stream, (const float *)Ls.p, (const float *)Gl.p, (const float *)Ge.p,
                        (const int64_t *)Y.p, ignore, p.n, p.n_pad, p.v, coef, s.lse, s.every, s.one, s.target);
@@ -1107,8 +1169,15 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   }
   if (p.want_x) {
     by_type(c.dt, [&](auto dt) {
-      hipLaunchKernelGGL((grad_rows_join_kernel<decltype(dt)::value>), dim3(spread((uint64_t)p.n * up(p.d, 8), 64)), dim3(1024), 0, ctx->stream, (const float *)s.sums,
-                         p.splits, up(p.d, 8), p.n, p.d, c.scale, coef, w_top, Ox.p, (size_t)gx_stride);
+      constexpr int DT = decltype(dt)::value;
+      const uint32_t pitch = up(p.d, 8);
+      const uint64_t total = (uint64_t)p.n * pitch;
+      if (p.splits <= 16)
+        hipLaunchKernelGGL((grad_rows_join_kernel<DT, true>), dim3(spread(total, 1024)), dim3(256), 0, ctx->stream, (const float *)s.sums, p.splits, pitch, p.n, p.d,
+                           c.scale, coef, w_top, Ox.p, (size_t)gx_stride);
+      else
+        hipLaunchKernelGGL((grad_rows_join_kernel<DT, false>), dim3(spread(total, 64)), dim3(1024), 0, ctx->stream, (const float *)s.sums, p.splits, pitch, p.n, p.d,
+                           c.scale, coef, w_top, Ox.p, (size_t)gx_stride);
     });
     AS_HIP(ctx, hipGetLastError());
   }
@@ -1125,7 +1194,7 @@ extern "C" {
 uint64_t as_cross_entropy_workspace(uint64_t n, uint64_t n_items, uint64_t dim, int dtype, int backward) {
   if (n == 0 || n_items == 0 || dim == 0 || n >= (1ull << 31) || n_items >= (1ull << 31) || dim > 65536 || !dtype_is_training(dtype)) return 0;
   Plan p = make_plan((uint32_t)n, (uint32_t)n_items, (uint32_t)dim, dtype);
-  if (backward) plan_backward(p, true, true, true, true);
+  if (backward) plan_backward(p, true, true, true);
   else plan_forward(p);
   // (a stride of dim + 1: room for the images whether or not the matrices can be taken as they are)
   const Source xs{nullptr, (size_t)dim + 1, p.n, p.d, dtype, p.pitch}, ts{nullptr, (size_t)dim + 1, p.v, p.d, dtype, p.pitch};

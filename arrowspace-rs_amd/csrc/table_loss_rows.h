@@ -29,6 +29,14 @@ __device__ __forceinline__ uint32_t die_order(uint32_t b, uint32_t total) {
   return die * each + nt_min(die, rest) + at;
 }
 
+// A grid of rows x cols pieces of work, walked in groups of four columns: the 32 workgroups a die runs at once are 8 x 4 pieces and
+// read 12 sides, not 33 (8192^3 in bf16: 1 049 TFLOP/s in rows of one column, 1 280 so).
+__device__ __forceinline__ void grid_order(uint32_t work, uint32_t rows, uint32_t cols, uint32_t *row, uint32_t *col) {
+  const uint32_t group = work / (4 * rows), at = work - group * 4 * rows, width = nt_min(4, cols - group * 4);
+  *row = at / width;
+  *col = group * 4 + at % width;
+}
+
 // quad-wide exchange: the value of lane ^ 1 / lane ^ 2
 __device__ __forceinline__ uint32_t quad_xor1(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true); }
 __device__ __forceinline__ uint32_t quad_xor2(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true); }
@@ -70,7 +78,7 @@ struct LossRowsArgs {
   const float *lse, *every, *one;
   const int *target;
   const float *bias;              // by item, or null
-  const float *coef;              // {factor, 1 / factor} of g, or null
+  const float *coef;              // {factor, 1 / factor} of g
   float *sums;                    // r = batch: f32 [split][nr][sums_pitch]
   uint32_t sums_pitch;
   void *out;                      // r = items: rows of out_stride elements
@@ -87,7 +95,7 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(const float *lse, const 
   float s = INFINITY, every = 0.f, one = 0.f;
   int at = -1;
   if (t < n && lse[t] != -INFINITY) {  // (-inf: the bias left no item, no gradient)
-    const float f = coef ? coef[0] : 1.f;
+    const float f = coef[0];
     const int64_t y = targets[t];
     if (y != ignore && y >= 0 && y < (int64_t)v) {
       at = (int)y;
@@ -99,35 +107,44 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(const float *lse, const 
   o_lse[t] = s, o_every[t] = every, o_one[t] = one, o_target[t] = at;
 }
 
-template <int OFF>
-__device__ __forceinline__ void lr_read4(u32x4 (&x)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-  asm volatile(
-      "ds_read_b128 %0, %4 offset:%8\n\tds_read_b128 %1, %5 offset:%8\n\tds_read_b128 %2, %6 offset:%8\n\tds_read_b128 %3, %7 offset:%8\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
-      : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(OFF)
-      : "memory");
+// Stages go through registers into LDS and not by direct loads: behind a direct load in flight hipcc waits for it in front of every
+// LDS read, and reads written by hand, each batch with its own wait, left the two waves of a SIMD waiting half their time (565 us for
+// the dX of 1 024 rows against a million items; this form: see the kernel).
+typedef short short4v __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x4 lr_row(const char *smem, uint32_t at) { return *(const u32x4 *)(smem + at); }
+// rows 0 .. 3 and 4 .. 7 (`half` bytes on) of this lane's column, transposed
+__device__ __forceinline__ u32x4 lr_column(const char *smem, uint32_t at, uint32_t half) {
+  typedef __attribute__((address_space(3))) short4v lds_short4;
+  const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(smem + at)));
+  const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(smem + at + half)));
+  return u32x4{x[0], x[1], y[0], y[1]};
 }
-template <int OFF>
-__device__ __forceinline__ void lr_read2(u32x4 &x, u32x4 &y, uint32_t a0, uint32_t a1) {
-  asm volatile("ds_read_b128 %0, %2 offset:%4\n\tds_read_b128 %1, %3 offset:%4\n\ts_waitcnt lgkmcnt(0)"
-               : "=&v"(x), "=&v"(y)
-               : "v"(a0), "v"(a1), "n"(OFF)
-               : "memory");
-}
-// two tiles (columns 4 h .. of each eight) of 4 + 4 rows, transposed: HALF bytes from rows 0 .. 3 to rows 4 .. 7
-template <int HALF>
-__device__ __forceinline__ void lr_transposed2(u32x4 &x, u32x4 &y, uint32_t a) {
-  u32x2 x0, x1, y0, y1;
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%5\n\tds_read_b64_tr_b16 %2, %4 offset:8\n\tds_read_b64_tr_b16 %3, %4 offset:%6\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(x0), "=&v"(x1), "=&v"(y0), "=&v"(y1)
-      : "v"(a), "n"(HALF), "n"(HALF + 8)
-      : "memory");
-  x = u32x4{x0[0], x0[1], x1[0], x1[1]};
-  y = u32x4{y0[0], y0[1], y1[0], y1[1]};
-}
+// A stage of 64 rows of the k side, P planes of 64 KD bytes a row: 16-byte piece c of row r at place c ^ swizzle(r), so that a fragment
+// read (8 rows) and a transposed read (4 rows) spread over the banks
+template <int P, int KD>
+struct LrStage {
+  static constexpr uint32_t kRow = KD * 64, kPlane = 64 * kRow;
+  u32x4 piece[P][KD];
+  __device__ __forceinline__ static uint32_t swizzle(uint32_t row) {
+    const uint32_t key = (row & 3) | ((row >> 1) & 4);
+    return KD >= 4 ? key << 1 : key;
+  }
+  __device__ __forceinline__ void load(const char *k, size_t ld, size_t plane, uint32_t nk, uint32_t s) {
+#pragma unroll
+    for (int t = 0; t < KD; ++t) {
+      const uint32_t idx = t * 256 + threadIdx.x, row = idx / (KD * 4), slot = idx % (KD * 4);
+      const char *src = k + (size_t)nt_min(s * 64 + row, nk - 1) * ld + ((slot ^ swizzle(row)) << 4);
+#pragma unroll
+      for (int p = 0; p < P; ++p) piece[p][t] = *(const u32x4 *)(src + p * plane);
+    }
+  }
+  __device__ __forceinline__ void store(char *dst) const {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int t = 0; t < KD; ++t) *(u32x4 *)(dst + p * kPlane + (t * 256 + threadIdx.x) * 16) = piece[p][t];
+  }
+};
 
 // ---- forward for short rows -----------------------------------------------------------------------------------------------------------------
 // The same walk with only the statistics behind it: rows in registers, items in stages of 64, a running maximum and sum of exponentials
@@ -143,11 +160,11 @@ struct LossSumsArgs {
   const float *bias;
   float2 *part;  // [split][nr] (maximum, sum of exponentials against it)
 };
-template <int FMT, int P, int RT, int KD, bool GENERAL>
-__global__ __launch_bounds__(256, 2) void loss_rows_sums_kernel(LossSumsArgs a) {
-  constexpr uint32_t kRow = KD * 64, kPlane = 64 * kRow, kExtra = GENERAL ? 256 : 0, kStage = P * kPlane + kExtra;
+template <int FMT, int P, int RT, int KD, bool GENERAL, int WAVES>
+__global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs a) {
+  typedef LrStage<P, KD> Stage;
+  constexpr uint32_t kRow = Stage::kRow, kPlane = Stage::kPlane, kExtra = GENERAL ? 256 : 0, kStage = P * kPlane + kExtra;
   __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
-  const uint32_t lds = (uint32_t)(size_t)(nt_lds *)smem;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, col = lane & 15;
   const uint32_t work = die_order(blockIdx.x, gridDim.x);
   const uint32_t rb = work % a.r_blocks, split = work / a.r_blocks;
@@ -156,24 +173,17 @@ __global__ __launch_bounds__(256, 2) void loss_rows_sums_kernel(LossSumsArgs a) 
   const uint32_t s_lo = (uint32_t)((uint64_t)stages * split / a.splits), s_hi = (uint32_t)((uint64_t)stages * (split + 1) / a.splits);
   const float nat = a.scale * (P == 2 ? 1.f / plane_scale(*a.r_top) / plane_scale(*a.k_top) : 1.f);
   const float unit = GENERAL ? kLog2e : nat * kLog2e, slack = fminf(20.f / unit, 1e30f);
-  auto swz = [](uint32_t row) { const uint32_t key = (row & 3) | ((row >> 1) & 4); return KD >= 4 ? key << 1 : key; };
-  auto fetch = [&](int buf, uint32_t s) {
-    char *dst = smem + buf * kStage;
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int t = 0; t < KD; ++t) {
-        const uint32_t idx = t * 256 + threadIdx.x, row = idx / (KD * 4), slot = idx % (KD * 4);
-        const uint32_t k = nt_min(s * 64 + row, a.nk - 1);
-        __builtin_amdgcn_global_load_lds((nt_gbl *)(a.k + (size_t)k * a.k_ld + p * a.k_plane + ((slot ^ swz(row)) << 4)),
-                                         (nt_lds *)(dst + p * kPlane + (t * 256 + wave * 64) * 16), 16, 0, 0);
-      }
-    if constexpr (GENERAL) {
-      if (wave == 0 && a.bias)
-        __builtin_amdgcn_global_load_lds((nt_gbl *)(a.bias + nt_min(s * 64 + lane, a.nk - 1)), (nt_lds *)(dst + P * kPlane), 4, 0, 0);
-    }
+  Stage stage;
+  float extra = 0.f;
+  auto load = [&](uint32_t s) {
+    stage.load(a.k, a.k_ld, a.k_plane, a.nk, s);
+    if (GENERAL && a.bias && threadIdx.x < 64) extra = a.bias[nt_min(s * 64 + threadIdx.x, a.nk - 1)];
   };
-  if (s_lo < s_hi) fetch(0, s_lo);
+  auto store = [&](int buf) {
+    stage.store(smem + buf * kStage);
+    if (GENERAL && threadIdx.x < 64) *(float *)(smem + buf * kStage + P * kPlane + threadIdx.x * 4) = extra;
+  };
+  if (s_lo < s_hi) load(s_lo);
   u32x4 R[P][RT][KD];
   float ref[RT], base[RT], sum[RT];
 #pragma unroll
@@ -186,45 +196,36 @@ __global__ __launch_bounds__(256, 2) void loss_rows_sums_kernel(LossSumsArgs a) 
     ref[j] = -INFINITY;
     base[j] = sum[j] = 0.f;
   }
-  const uint32_t frow = ((col >> 2) << 3) + (col & 3), fa = frow * kRow + ((q ^ swz(frow)) << 4);
+  const uint32_t frow = ((col >> 2) << 3) + (col & 3), fa = frow * kRow + ((q ^ Stage::swizzle(frow)) << 4);
   const bool here = r0 < a.nr;  // (a wave without rows only brings its part of the stages)
+  if (s_lo < s_hi) store(0);
   int buf = 0;
   for (uint32_t s = s_lo; s < s_hi; ++s, buf ^= 1) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (s + 1 < s_hi) fetch(buf ^ 1, s + 1);
-    if (!here) continue;
+    __syncthreads();
+    if (s + 1 < s_hi) load(s + 1);
+    const char *here_in = smem + buf * kStage;
 #pragma unroll 1
-    for (uint32_t h = 0; h < 2; ++h) {
+    for (uint32_t h = 0; h < 2 && here; ++h) {
       const uint32_t k0 = s * 64 + h * 32;
       f32x4 z[2][RT];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int j = 0; j < RT; ++j) z[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const uint32_t at = lds + buf * kStage + h * 32 * kRow + fa;
+        const uint32_t at = h * 32 * kRow + fa + i * 4 * kRow;
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll
-          for (int s4 = 0; s4 < KD; s4 += 4) {
-            u32x4 A[4];
-            const uint32_t ap = at + p * kPlane;
-            if constexpr (KD == 2) i == 0 ? lr_read2<0>(A[0], A[1], ap, ap ^ 64) : lr_read2<4 * kRow>(A[0], A[1], ap, ap ^ 64);
-            else i == 0 ? lr_read4<0>(A, ap ^ (s4 << 6), ap ^ ((s4 + 1) << 6), ap ^ ((s4 + 2) << 6), ap ^ ((s4 + 3) << 6))
-                        : lr_read4<4 * kRow>(A, ap ^ (s4 << 6), ap ^ ((s4 + 1) << 6), ap ^ ((s4 + 2) << 6), ap ^ ((s4 + 3) << 6));
+          for (int t = 0; t < KD; ++t) {
+            const u32x4 A = lr_row(here_in, p * kPlane + (at ^ (t << 6)));
 #pragma unroll
-            for (int t = 0; t < (KD < 4 ? KD : 4); ++t)
-#pragma unroll
-              for (int j = 0; j < RT; ++j) {
-                z[i][j] = nt_mfma<FMT>(A[t], R[0][j][s4 + t], z[i][j]);
-                if (P == 2 && p == 0) z[i][j] = nt_mfma<FMT>(A[t], R[P - 1][j][s4 + t], z[i][j]);
-              }
+            for (int j = 0; j < RT; ++j) {
+              z[i][j] = nt_mfma<FMT>(A, R[0][j][t], z[i][j]);
+              if (P == 2 && p == 0) z[i][j] = nt_mfma<FMT>(A, R[P - 1][j][t], z[i][j]);
+            }
           }
         if constexpr (GENERAL) {
-          f32x4 kb = {0.f, 0.f, 0.f, 0.f};
-          if (a.bias)
-            asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(kb) : "v"(lds + buf * kStage + P * kPlane + h * 128 + q * 32 + i * 16) : "memory");
+          const f32x4 kb = *(const f32x4 *)(here_in + P * kPlane + h * 128 + q * 32 + i * 16);
 #pragma unroll
           for (int j = 0; j < RT; ++j)
 #pragma unroll
@@ -264,6 +265,7 @@ __global__ __launch_bounds__(256, 2) void loss_rows_sums_kernel(LossSumsArgs a) 
         sum[j] += s0 + s1;
       }
     }
+    if (s + 1 < s_hi) store(buf ^ 1);
   }
   if (!here) return;
 #pragma unroll
@@ -283,12 +285,12 @@ __global__ __launch_bounds__(256, 2) void loss_rows_sums_kernel(LossSumsArgs a) 
 
 // FMT the operands' type; P planes; RT tiles of 16 rows r a wave; KD steps of 32 columns; ITEMS: the rows r are items (dW), else the
 // batch (dX); OUT: type of dW
-template <int FMT, int P, int RT, int KD, bool ITEMS, bool BIAS, int OUT>
-__global__ __launch_bounds__(256, 2) void loss_rows_grad_kernel(LossRowsArgs a) {
-  constexpr uint32_t kRow = KD * 64, kPlane = 64 * kRow, kExtra = 1024, kStage = P * kPlane + kExtra;
+template <int FMT, int P, int RT, int KD, bool ITEMS, bool BIAS, int OUT, int WAVES>
+__global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs a) {
+  typedef LrStage<P, KD> Stage;
+  constexpr uint32_t kRow = Stage::kRow, kPlane = Stage::kPlane, kExtra = 1024, kStage = P * kPlane + kExtra;
   constexpr bool FAST = !BIAS && P == 1;  // 16-bit gradients: the exponent in one multiply-add (its constants are rounded: 2e-6 of the probability)
   __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
-  const uint32_t lds = (uint32_t)(size_t)(nt_lds *)smem;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, col = lane & 15;
   const uint32_t work = die_order(blockIdx.x, gridDim.x);
   const uint32_t rb = work % a.r_blocks, split = work / a.r_blocks;
@@ -297,27 +299,20 @@ __global__ __launch_bounds__(256, 2) void loss_rows_grad_kernel(LossRowsArgs a) 
   const uint32_t s_lo = (uint32_t)((uint64_t)stages * split / a.splits), s_hi = (uint32_t)((uint64_t)stages * (split + 1) / a.splits);
   const float nat = a.scale * (P == 2 ? 1.f / plane_scale(*a.r_top) / plane_scale(*a.k_top) : 1.f);
   const float c = FAST ? nat * kLog2e : nat;
-  auto swz = [](uint32_t row) { const uint32_t key = (row & 3) | ((row >> 1) & 4); return KD >= 4 ? key << 1 : key; };
-  auto fetch = [&](int buf, uint32_t s) {
-    char *dst = smem + buf * kStage;
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int t = 0; t < KD; ++t) {
-        const uint32_t idx = t * 256 + threadIdx.x, row = idx / (KD * 4), slot = idx % (KD * 4);
-        const uint32_t k = nt_min(s * 64 + row, a.nk - 1);
-        __builtin_amdgcn_global_load_lds((nt_gbl *)(a.k + (size_t)k * a.k_ld + p * a.k_plane + ((slot ^ swz(row)) << 4)),
-                                         (nt_lds *)(dst + p * kPlane + (t * 256 + wave * 64) * 16), 16, 0, 0);
-      }
-    if constexpr (ITEMS) {  // by row of the batch: the waves bring one array each
-      const char *src = wave == 0 ? (const char *)a.lse : wave == 1 ? (const char *)a.every : wave == 2 ? (const char *)a.one : (const char *)a.target;
-      __builtin_amdgcn_global_load_lds((nt_gbl *)(src + ((size_t)s * 64 + lane) * 4), (nt_lds *)(dst + P * kPlane + wave * 256), 4, 0, 0);
-    } else if constexpr (BIAS) {
-      if (wave == 0)
-        __builtin_amdgcn_global_load_lds((nt_gbl *)(a.bias + nt_min(s * 64 + lane, a.nk - 1)), (nt_lds *)(dst + P * kPlane), 4, 0, 0);
-    }
+  Stage stage;
+  float extra = 0.f;
+  // by row of the batch: the waves bring one array each; else the items' bias
+  const float *by_k = ITEMS ? (wave == 0 ? a.lse : wave == 1 ? a.every : wave == 2 ? a.one : (const float *)a.target) : a.bias;
+  auto load = [&](uint32_t s) {
+    stage.load(a.k, a.k_ld, a.k_plane, a.nk, s);
+    if (ITEMS) extra = by_k[s * 64 + lane];
+    else if (BIAS && wave == 0) extra = by_k[nt_min(s * 64 + lane, a.nk - 1)];
   };
-  if (s_lo < s_hi) fetch(0, s_lo);
+  auto store = [&](int buf) {
+    stage.store(smem + buf * kStage);
+    if (ITEMS || (BIAS && wave == 0)) *(float *)(smem + buf * kStage + P * kPlane + threadIdx.x * 4) = extra;
+  };
+  if (s_lo < s_hi) load(s_lo);
   // this wave's rows
   u32x4 R[P][RT][KD];
   float lse[RT], every[RT], one[RT], rbias[RT], bsum[RT];
@@ -347,48 +342,45 @@ __global__ __launch_bounds__(256, 2) void loss_rows_grad_kernel(LossRowsArgs a) 
     for (int j = 0; j < RT; ++j) out[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   // addresses within a stage: fragment rows of the logits (k = 8 (row / 4) + 4 i + row % 4), rows of the transposed reads (8 q + ...)
   const uint32_t frow = ((col >> 2) << 3) + (col & 3), trow = (q << 3) + ((lane >> 2) & 3);
-  const uint32_t fa = frow * kRow + ((q ^ swz(frow)) << 4), ta = trow * kRow + (((lane & 3) ^ swz(trow)) << 4);
+  const uint32_t fa = frow * kRow + ((q ^ Stage::swizzle(frow)) << 4), ta = trow * kRow + (((lane & 3) ^ Stage::swizzle(trow)) << 4);
+  if (s_lo < s_hi) store(0);
   int buf = 0;
   for (uint32_t s = s_lo; s < s_hi; ++s, buf ^= 1) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (s + 1 < s_hi) fetch(buf ^ 1, s + 1);
-    const uint32_t base = lds + buf * kStage;
+    __syncthreads();
+    if (s + 1 < s_hi) load(s + 1);
+    const char *here_in = smem + buf * kStage;
 #pragma unroll 1
     for (uint32_t h = 0; h < 2; ++h) {
-      const uint32_t k0 = s * 64 + h * 32, extra = base + P * kPlane + h * 128;
+      const uint32_t k0 = s * 64 + h * 32, by = P * kPlane + h * 128;
       uint32_t G[P][RT][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         f32x4 z[RT];
 #pragma unroll
         for (int j = 0; j < RT; ++j) z[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const uint32_t at = base + h * 32 * kRow + fa;
+        // (the matrix work of one wave goes in front of the others' exponentials: 4 %)
+        __builtin_amdgcn_s_setprio(1);
+        const uint32_t at = h * 32 * kRow + fa + i * 4 * kRow;
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll
-          for (int s4 = 0; s4 < KD; s4 += 4) {
-            u32x4 A[4];
-            const uint32_t ap = at + p * kPlane;
-            if constexpr (KD == 2) i == 0 ? lr_read2<0>(A[0], A[1], ap, ap ^ 64) : lr_read2<4 * kRow>(A[0], A[1], ap, ap ^ 64);
-            else i == 0 ? lr_read4<0>(A, ap ^ (s4 << 6), ap ^ ((s4 + 1) << 6), ap ^ ((s4 + 2) << 6), ap ^ ((s4 + 3) << 6))
-                        : lr_read4<4 * kRow>(A, ap ^ (s4 << 6), ap ^ ((s4 + 1) << 6), ap ^ ((s4 + 2) << 6), ap ^ ((s4 + 3) << 6));
+          for (int t = 0; t < KD; ++t) {
+            const u32x4 A = lr_row(here_in, p * kPlane + (at ^ (t << 6)));
 #pragma unroll
-            for (int t = 0; t < (KD < 4 ? KD : 4); ++t)
-#pragma unroll
-              for (int j = 0; j < RT; ++j) {
-                z[j] = nt_mfma<FMT>(A[t], R[0][j][s4 + t], z[j]);
-                if (P == 2 && p == 0) z[j] = nt_mfma<FMT>(A[t], R[P - 1][j][s4 + t], z[j]);
-              }
+            for (int j = 0; j < RT; ++j) {
+              z[j] = nt_mfma<FMT>(A, R[0][j][t], z[j]);
+              if (P == 2 && p == 0) z[j] = nt_mfma<FMT>(A, R[P - 1][j][t], z[j]);
+            }
           }
+        __builtin_amdgcn_s_setprio(0);
         // the gradients of four logits a row
-        u32x4 kl, ke;
+        u32x4 kl = {}, ke = {};
         f32x4 kb = {0.f, 0.f, 0.f, 0.f};
         if constexpr (ITEMS) {
-          lr_read2<0>(kl, ke, extra + q * 32 + i * 16, extra + 256 + q * 32 + i * 16);
+          kl = lr_row(here_in, by + q * 32 + i * 16);
+          ke = lr_row(here_in, by + 256 + q * 32 + i * 16);
         } else if constexpr (BIAS) {
-          asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(kb) : "v"(extra + q * 32 + i * 16) : "memory");
+          kb = *(const f32x4 *)(here_in + by + q * 32 + i * 16);
         }
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
@@ -413,11 +405,9 @@ __global__ __launch_bounds__(256, 2) void loss_rows_grad_kernel(LossRowsArgs a) 
         }
         // targets: rare
         if constexpr (ITEMS) {
-          int tg;
-          asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(tg) : "v"(extra + 768 + (lane & 31) * 4) : "memory");
-          if (__any((uint32_t)tg - r0 < 16u * RT)) {
-            u32x4 kt, ko;
-            lr_read2<0>(kt, ko, extra + 768 + q * 32 + i * 16, extra + 512 + q * 32 + i * 16);
+          const uint32_t tg = *(const uint32_t *)(here_in + by + 768 + (lane & 31) * 4);
+          if (__any(tg - r0 < 16u * RT)) {
+            const u32x4 kt = lr_row(here_in, by + 768 + q * 32 + i * 16), ko = lr_row(here_in, by + 512 + q * 32 + i * 16);
 #pragma unroll
             for (int j = 0; j < RT; ++j)
 #pragma unroll
@@ -447,13 +437,14 @@ __global__ __launch_bounds__(256, 2) void loss_rows_grad_kernel(LossRowsArgs a) 
           }
         }
       }
-      const uint32_t at = base + h * 32 * kRow + ta;
+      __builtin_amdgcn_s_setprio(1);
+      const uint32_t at = h * 32 * kRow + ta;
 #pragma unroll
       for (int t = 0; t < KD; ++t)
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          u32x4 y0, y1;
-          lr_transposed2<4 * kRow>(y0, y1, (at + p * kPlane) ^ (t << 6));
+          // columns 4 h .. 4 h + 3 of each eight: two tiles
+          const u32x4 y0 = lr_column(here_in, p * kPlane + (at ^ (t << 6)), 4 * kRow), y1 = lr_column(here_in, p * kPlane + (at ^ (t << 6)) + 8, 4 * kRow);
 #pragma unroll
           for (int j = 0; j < RT; ++j) {
             const u32x4 g0 = u32x4{G[0][j][0], G[0][j][1], G[0][j][2], G[0][j][3]};
@@ -467,8 +458,10 @@ __global__ __launch_bounds__(256, 2) void loss_rows_grad_kernel(LossRowsArgs a) 
           }
         }
     }
+    __builtin_amdgcn_s_setprio(0);
+    if (s + 1 < s_hi) store(buf ^ 1);
   }
-  const float f = ITEMS ? a.scale * (a.coef ? a.coef[1] : 1.f) * (P == 2 ? 1.f / plane_scale(*a.k_top) : 1.f) : 1.f;
+  const float f = ITEMS ? a.scale * a.coef[1] * (P == 2 ? 1.f / plane_scale(*a.k_top) : 1.f) : 1.f;
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
     const uint32_t row = r0 + j * 16 + col;
@@ -476,7 +469,7 @@ __global__ __launch_bounds__(256, 2) void loss_rows_grad_kernel(LossRowsArgs a) 
       float b = bsum[j];
       b += __shfl_xor(b, 16);
       b += __shfl_xor(b, 32);
-      if (a.grad_bias && q == 0 && row < a.nr) a.grad_bias[row] = b * (a.coef ? a.coef[1] : 1.f);
+      if (a.grad_bias && q == 0 && row < a.nr) a.grad_bias[row] = b * a.coef[1];
     }
     if (row >= a.nr) continue;
 #pragma unroll
