@@ -328,10 +328,9 @@ __global__ __launch_bounds__(1024) void coef_scale_kernel(const float *gl, const
 // ---- gradient of the logits ---------------------------------------------------------------------------------------------------------------
 struct GradArgs {
   LossArgs l;
-  uint32_t v_begin, v_all;         // first item of the piece (the operand A starts there); items of the table
-  const float *lse, *gl, *ge;
-  const int64_t *targets;
-  int64_t ignore;
+  uint32_t v_begin;                // first item of the piece (the operand A starts there)
+  const float *lse, *every, *entry;  // by row, filled to whole tiles (loss_rows_kernel)
+  const int *target;
   const float *coef;               // {factor, 1 / factor} of G
   unsigned short *G, *GT;          // n x (planes * g_pitch), v_pad x (planes * t_pitch)
   uint32_t g_pitch, t_pitch;
@@ -350,7 +349,7 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
   grid_order(work, a.n_tiles, a.chunks, &nt, &chunk);
   const uint32_t n0 = nt * TILE::BN, vt_end = nt_min((chunk + 1) * a.per, a.v_tiles);
   uint32_t vt = chunk * a.per;
-  const float c = a.scale * product_scale(a), factor = g.coef[0];
+  const float c = a.scale * product_scale(a);
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
   NtOperand B{a.rows + (size_t)n0 * a.rows_ld, a.rows_ld, nt_min(TILE::BN, a.n - n0) - 1, a.rows_plane};
   auto side = [&](uint32_t tile) {
@@ -359,26 +358,17 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
   };
   // this lane's rows
   uint32_t row[TILE::TN];
-  float lse[TILE::TN], every[TILE::TN], one[TILE::TN];
+  float lse[TILE::TN], every[TILE::TN], entry[TILE::TN];
   int32_t hit[TILE::TN];  // the target within the piece, or far off
 #pragma unroll
   for (int j = 0; j < TILE::TN; ++j) {
     const uint32_t t = n0 + wn * (TILE::TN * 16) + (j >> 1) * 32 + (col >> 2) * 8 + (j & 1) * 4 + (col & 3);
     row[j] = t;
-    lse[j] = INFINITY;  // (rows behind the last: every probability 0)
-    every[j] = one[j] = 0.f;
-    hit[j] = -1;
-    if (t < a.n) {
-      const int64_t y = g.targets[t];
-      const bool counted = y != g.ignore && y >= 0 && y < (int64_t)g.v_all;
-      const float l = counted ? g.gl[t] : 0.f;
-      lse[j] = g.lse[t];
-      one[j] = l * factor;
-      every[j] = (l + (g.ge ? g.ge[t] : 0.f)) * factor;
-      const int64_t at = y - (int64_t)g.v_begin;
-      if (counted && at >= 0 && at < (int64_t)a.v) hit[j] = (int32_t)at;
-      if (lse[j] == -INFINITY) every[j] = one[j] = 0.f, lse[j] = INFINITY, hit[j] = -1;  // no item left by the bias: no gradient
-    }
+    lse[j] = g.lse[t];
+    every[j] = g.every[t];
+    entry[j] = g.entry[t];
+    const uint32_t at = (uint32_t)g.target[t] - g.v_begin;
+    hit[j] = at < a.v ? (int32_t)at : -1;
   }
   const uint32_t all = a.planes == 2 ? 3 * a.steps : a.steps;
   f32x4 acc[TILE::TM][TILE::TN];
@@ -435,7 +425,7 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
         for (int i = 0; i < TILE::TM; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (hit[j] == (int32_t)(at0 + row0 + (i >> 1) * 32 + (i & 1) * 4 + e)) acc[i][j][e] -= one[j];
+            if (hit[j] == (int32_t)(at0 + row0 + (i >> 1) * 32 + (i & 1) * 4 + e)) acc[i][j][e] = entry[j];
     }
     if constexpr (BIAS) {
       if (g.bias_part) {
@@ -513,7 +503,65 @@ struct ProductArgs {
   float *sums;                      // instead: f32 [split][n][sums_pitch], added to unless `first`
   uint32_t sums_pitch;
   int first, aligned;
+  // dW of one plane: the rows whose target is one of the output's, by the rest of their entry there (null: left out)
+  const int *target;
+  const float *rest;
+  uint32_t n_rows, n_begin;         // rows of the batch; item of output row 0
+  const char *x;                    // the batch as an operand (whole steps of 64 columns)
+  size_t x_ld;
 };
+// dW's part of a tile from what 16 bits left of the entries at the targets: rows of the batch in order, a list of those that meet the
+// tile per workgroup's width of rows, each added by the lanes that hold its item.  A tile of 256 items meets 16 of 8 192 rows where
+// the table has 131 072; tables of less than half the rows go without (their items are sums of several entries, whose roundings
+// average out).
+template <int FMT, class TILE>
+__device__ __forceinline__ void add_rest(const ProductArgs &p, const TILE &T, char *smem, uint32_t m0, uint32_t n0, f32x4 (&acc)[TILE::TM][TILE::TN]) {
+  u32x2 *list = (u32x2 *)smem;
+  uint32_t *counts = (uint32_t *)(smem + TILE::NT * 8);
+  const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
+  for (uint32_t t0 = 0; t0 < p.n_rows; t0 += TILE::NT) {
+    __syncthreads();
+    const uint32_t t = t0 + threadIdx.x, v = t < p.n_rows ? (uint32_t)p.target[t] - p.n_begin - n0 : ~0u;
+    const bool meets = v < nt_min(TILE::BN, p.n - n0);
+    const uint64_t ballot = __ballot(meets);
+    if (T.lane == 0) counts[T.wave] = (uint32_t)__popcll(ballot);
+    __syncthreads();
+    uint32_t before = 0, total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < TILE::NT / 64; ++w) {
+      if (w < T.wave) before += counts[w];
+      total += counts[w];
+    }
+    if (meets) list[before + (uint32_t)__popcll(ballot & ((1ull << T.lane) - 1))] = u32x2{t, v};
+    __syncthreads();
+    for (uint32_t k = 0; k < total; ++k) {
+      const uint32_t row = __builtin_amdgcn_readfirstlane(list[k][0]), at = __builtin_amdgcn_readfirstlane(list[k][1]);
+      if (at / (TILE::TN * 16) != wn) continue;
+      const uint32_t in = at % (TILE::TN * 16), jj = ((in >> 5) << 1) | ((in >> 2) & 1), c = (((in >> 3) & 3) << 2) | (in & 3);
+      if (col != c) continue;
+      const float r = p.rest[row];
+#pragma unroll
+      for (int i = 0; i < TILE::TM; i += 2) {
+        const uint32_t m = m0 + wm * (TILE::TM * 16) + i * 16 + q * 8;
+        if (m >= p.m) continue;
+        const u32x4 w = *(const u32x4 *)(p.x + (size_t)row * p.x_ld + m * 2);  // (zeros behind the row's values)
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const unsigned short u = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
+          y[e] = FMT == AS_BF16 ? bf16_to_f32(u) : (float)__builtin_bit_cast(_Float16, u);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < TILE::TN; ++j)
+          if (j == jj) {
+            acc[i][j] += f32x4{y[0], y[1], y[2], y[3]} * r;
+            acc[i + 1][j] += f32x4{y[4], y[5], y[6], y[7]} * r;
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+}
 template <int FMT, class TILE_, int OUT>  // OUT: element type of `out`, or 0 (AS_F64) = into `sums`
 __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
   using TILE = TILE_;
@@ -539,6 +587,8 @@ __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
     T.contract(buf, acc);
     buf ^= 1;
   }
+  if constexpr (OUT == FMT)
+    if (p.target) add_rest<FMT>(p, T, smem, m0, n0, acc);
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
   const float f = OUT == 0 ? 1.f : p.scale * p.coef[1] * (p.top ? 1.f / plane_scale(*p.top) : 1.f);
 #pragma unroll
@@ -576,7 +626,13 @@ __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
 // each (a few rows have hundreds of parts: one thread's chain of them would be the whole time).
 template <int DT, bool FEW>
 __global__ __launch_bounds__(FEW ? 256 : 1024) void grad_rows_join_kernel(const float *sums, uint32_t splits, uint32_t pitch, uint32_t n, uint32_t d, float scale,
-                                                                          const float *coef, const unsigned int *top, void *out, size_t out_stride) {
+                                                                          const float *coef, const unsigned int *top, const int *target, const float *rest,
+                                                                          const void *table, size_t table_stride, void *out, size_t out_stride) {
+  // (rest: of the entry at the row's target, times that item)
+  auto more = [&](uint64_t t, uint64_t k) {
+    const int y = target[t];
+    return y < 0 ? 0.f : rest[t] * load_as_f32<DT>(table, (size_t)y * table_stride + k);
+  };
   const float f = scale * coef[1] * (top ? 1.f / plane_scale(*top) : 1.f);
   const uint64_t total = (uint64_t)n * pitch;
   if constexpr (FEW) {
@@ -586,7 +642,7 @@ __global__ __launch_bounds__(FEW ? 256 : 1024) void grad_rows_join_kernel(const 
       const uint64_t t = i / pitch, k = i - t * pitch;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (k + e < d) store_from_f32<DT>(out, t * out_stride + k + e, x[e] * f);
+        if (k + e < d) store_from_f32<DT>(out, t * out_stride + k + e, (rest ? x[e] + more(t, k + e) : x[e]) * f);
     }
   } else {
     __shared__ float s[16][64];
@@ -604,7 +660,7 @@ __global__ __launch_bounds__(FEW ? 256 : 1024) void grad_rows_join_kernel(const 
       if (w == 0 && i < total) {
         for (int k = 1; k < 16; ++k) x += s[k][lane];
         const uint64_t t = i / pitch, k = i % pitch;
-        if (k < d) store_from_f32<DT>(out, t * out_stride + k, x * f);
+        if (k < d) store_from_f32<DT>(out, t * out_stride + k, (rest ? x + more(t, k) : x) * f);
       }
       __syncthreads();
     }
@@ -738,6 +794,7 @@ void plan_backward(Plan &p, bool x, bool w, bool b) {
   }
   const uint32_t bm = kShape[p.tile].bm, bn = kShape[p.tile].bn;
   p.t_pitch = up(p.n, std::max(bn, 64u));
+  p.n_pad = p.t_pitch;
   // G and its transposed form of a piece: some 512 MB together, and whole rounds of the large tile for the piece's dW
   const uint64_t per_item = (uint64_t)p.t_pitch * 2 * 2 * p.planes;
   const uint32_t round = std::max(1u, (uint32_t)kChips / cdiv(p.d, 256)) * 256;
@@ -795,7 +852,7 @@ struct BackwardScratch {
   float *top_parts, *coef;
   unsigned short *x_image, *t_image, *xt, *wt, *G, *GT;
   float *sums, *bias_part;
-  float *lse, *every, *one;
+  float *lse, *every, *entry, *rest;
   int *target;
 };
 uint64_t backward_layout(const Plan &p, const Source &x, const Source &t, char *base, BackwardScratch &s) {
@@ -806,11 +863,12 @@ uint64_t backward_layout(const Plan &p, const Source &x, const Source &t, char *
   s.coef = l.take<float>(2);
   s.x_image = l.take<unsigned short>(x.image_elems());
   s.t_image = l.take<unsigned short>(t.image_elems());
+  s.lse = l.take<float>(p.n_pad);
+  s.every = l.take<float>(p.n_pad);
+  s.entry = l.take<float>(p.n_pad);
+  s.rest = l.take<float>(p.n_pad);
+  s.target = l.take<int>(p.n_pad);
   if (p.fused) {
-    s.lse = l.take<float>(p.n_pad);
-    s.every = l.take<float>(p.n_pad);
-    s.one = l.take<float>(p.n_pad);
-    s.target = l.take<int>(p.n_pad);
     s.sums = l.take<float>(p.want_x ? (uint64_t)p.splits * p.n * up(p.d, 8) : 0);
     return l.at;
   }
@@ -1086,12 +1144,18 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
                      c.dt == AS_BF16 ? 0 : 14, s.coef);
   AS_HIP(ctx, hipGetLastError());
   const float *coef = s.coef;
+  const float *rest = p.planes == 1 ? s.rest : nullptr;
+  by_type(c.dt, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    hipLaunchKernelGGL((loss_rows_kernel<DT, DT == AS_BF16 ? AS_BF16 : AS_F16>), dim3(cdiv(p.n_pad, 4)), dim3(256), 0, ctx->stream, X.p, (size_t)c.x_stride, W.p,
+                       (size_t)c.table_stride, p.d, (const float *)Bi.p, c.scale, (const float *)Ls.p, (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p,
+                       ignore, p.n, p.n_pad, p.v, coef, s.lse, s.every, s.entry, s.target, s.rest);
+  });
+  AS_HIP(ctx, hipGetLastError());
   if (p.fused) {
-    hipLaunchKernelGGL(loss_rows_kernel, dim3(cdiv(p.n_pad, 256)), dim3(256), 0, ctx->stream, (const float *)Ls.p, (const float *)Gl.p, (const float *)Ge.p,
-                       (const int64_t *)Y.p, ignore, p.n, p.n_pad, p.v, coef, s.lse, s.every, s.one, s.target);
     LossRowsArgs r{};
     r.d = p.d, r.scale = c.scale, r.bias = (const float *)Bi.p, r.coef = coef;
-    r.lse = s.lse, r.every = s.every, r.one = s.one, r.target = s.target;
+    r.lse = s.lse, r.every = s.every, r.entry = s.entry, r.rest = s.rest, r.target = s.target;
     r.r_plane = r.k_plane = (size_t)p.pitch * 2;
     if (p.want_w || p.want_b) {
       r.r = table16, r.r_ld = a.table_ld, r.nr = p.v, r.r_top = w_top;
@@ -1114,9 +1178,8 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   a.n = p.n, a.steps = p.steps, a.planes = p.planes, a.n_tiles = p.n_tiles, a.per = p.per;
   a.scale = c.scale;
   a.rows_top = x_top, a.table_top = w_top;
-  g.lse = (const float *)Ls.p, g.gl = (const float *)Gl.p, g.ge = (const float *)Ge.p, g.targets = (const int64_t *)Y.p, g.ignore = ignore, g.coef = coef;
+  g.lse = s.lse, g.every = s.every, g.entry = s.entry, g.target = s.target, g.coef = coef;
   g.G = s.G, g.GT = s.GT, g.g_pitch = p.piece, g.t_pitch = p.t_pitch;
-  g.v_all = p.v;
   g.bias_part = p.want_b ? s.bias_part : nullptr;
   const int fmt = image_format(c.dt);
   for (uint32_t v0 = 0; !p.fused && v0 < p.v; v0 += p.piece) {
@@ -1152,6 +1215,7 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
       w.scale = c.scale, w.coef = coef, w.top = x_top;
       w.out = (char *)Ow.p + (size_t)v0 * gw_stride * dtype_size(c.dt), w.out_stride = gw_stride;
       w.aligned = gw_stride % 8 == 0 && ((uintptr_t)w.out & 15) == 0;
+      if (rest && p.v >= p.n / 2) w.target = s.target, w.rest = rest, w.n_rows = p.n, w.n_begin = v0, w.x = o.x, w.x_ld = o.x_ld;
       launch_product(ctx, fmt, p.tile_w, c.dt, w);
     }
     if (p.want_x) {
@@ -1174,10 +1238,10 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
       const uint64_t total = (uint64_t)p.n * pitch;
       if (p.splits <= 16)
         hipLaunchKernelGGL((grad_rows_join_kernel<DT, true>), dim3(spread(total, 1024)), dim3(256), 0, ctx->stream, (const float *)s.sums, p.splits, pitch, p.n, p.d,
-                           c.scale, coef, w_top, Ox.p, (size_t)gx_stride);
+                           c.scale, coef, w_top, (const int *)s.target, rest, W.p, (size_t)c.table_stride, Ox.p, (size_t)gx_stride);
       else
         hipLaunchKernelGGL((grad_rows_join_kernel<DT, false>), dim3(spread(total, 64)), dim3(1024), 0, ctx->stream, (const float *)s.sums, p.splits, pitch, p.n, p.d,
-                           c.scale, coef, w_top, Ox.p, (size_t)gx_stride);
+                           c.scale, coef, w_top, (const int *)s.target, rest, W.p, (size_t)c.table_stride, Ox.p, (size_t)gx_stride);
     });
     AS_HIP(ctx, hipGetLastError());
   }

@@ -49,6 +49,11 @@ __device__ __forceinline__ float add16(float v) {  // sum over the 16 lanes of a
 }
 
 template <int FMT>
+__device__ __forceinline__ float rounded16(float x) {
+  if constexpr (FMT == AS_BF16) return (float)(__bf16)x;
+  else return (float)(_Float16)x;
+}
+template <int FMT>
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
   if constexpr (FMT == AS_BF16) {
     typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
@@ -75,7 +80,7 @@ struct LossRowsArgs {
   float scale;
   const unsigned int *r_top, *k_top;  // f32: bits of the largest magnitude of the two matrices
   // by row of the batch, filled to whole 64s (probability 0, no target)
-  const float *lse, *every, *one;
+  const float *lse, *every, *entry, *rest;
   const int *target;
   const float *bias;              // by item, or null
   const float *coef;              // {factor, 1 / factor} of g
@@ -87,24 +92,42 @@ struct LossRowsArgs {
   float *grad_bias;               // r = items: sum over k of g, or null
 };
 
-// lanes' coefficients of the gradient by row of the batch
-__global__ __launch_bounds__(256) void loss_rows_kernel(const float *lse, const float *gl, const float *ge, const int64_t *targets, int64_t ignore, uint32_t n,
-                                                        uint32_t padded, uint32_t v, const float *coef, float *o_lse, float *o_every, float *o_one, int *o_target) {
-  const uint32_t t = blockIdx.x * 256 + threadIdx.x;
+// By row of the batch, a wave each: the coefficient of its probabilities, and its entry at its target.  That entry is most of a row's
+// gradient and often all of its item's, so it comes from a product in f64, the kernels put it in place of their own, and what 16 bits
+// leave of it (`rest`, as much as the rounding of the result) is added in f32: to dX where its parts are joined, to dW behind the
+// product.  coef: {factor, 1 / factor} of g.
+template <int DT, int FMT>
+__global__ __launch_bounds__(256) void loss_rows_kernel(const void *x, size_t x_stride, const void *table, size_t table_stride, uint32_t d, const float *bias,
+                                                        float scale, const float *lse, const float *gl, const float *ge, const int64_t *targets, int64_t ignore,
+                                                        uint32_t n, uint32_t padded, uint32_t v, const float *coef, float *o_lse, float *o_every, float *o_entry,
+                                                        int *o_target, float *o_rest) {
+  const uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (t >= padded) return;
-  float s = INFINITY, every = 0.f, one = 0.f;
+  float s = INFINITY, every = 0.f, entry = 0.f;   // (behind the last row: probability 0)
   int at = -1;
   if (t < n && lse[t] != -INFINITY) {  // (-inf: the bias left no item, no gradient)
     const float f = coef[0];
     const int64_t y = targets[t];
+    float one = 0.f;
+    s = lse[t];
     if (y != ignore && y >= 0 && y < (int64_t)v) {
       at = (int)y;
       one = gl[t] * f;
     }
-    s = lse[t];
     every = one + (ge ? ge[t] * f : 0.f);
+    if (at >= 0) {
+      double dot = 0.0;
+      for (uint32_t k = lane; k < d; k += 64)
+        dot += (double)load_as_f32<DT>(x, (size_t)t * x_stride + k) * (double)load_as_f32<DT>(table, (size_t)y * table_stride + k);
+      for (int k = 1; k < 64; k <<= 1) dot += __shfl_xor(dot, k);
+      const double z = (double)scale * dot + (bias ? (double)bias[y] : 0.0) - (double)s;
+      entry = (float)((double)every * exp(z) - (double)one);
+    }
   }
-  o_lse[t] = s, o_every[t] = every, o_one[t] = one, o_target[t] = at;
+  if (lane == 0) {
+    o_lse[t] = s, o_every[t] = every, o_entry[t] = entry, o_target[t] = at;
+    o_rest[t] = DT == AS_F32 || !__builtin_isfinite(entry) ? 0.f : entry - rounded16<FMT>(entry);
+  }
 }
 
 // Stages go through registers into LDS and not by direct loads: behind a direct load in flight hipcc waits for it in front of every
@@ -299,10 +322,13 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
   const uint32_t s_lo = (uint32_t)((uint64_t)stages * split / a.splits), s_hi = (uint32_t)((uint64_t)stages * (split + 1) / a.splits);
   const float nat = a.scale * (P == 2 ? 1.f / plane_scale(*a.r_top) / plane_scale(*a.k_top) : 1.f);
   const float c = FAST ? nat * kLog2e : nat;
+  constexpr uint32_t kList = 64;  // (items that more rows meet than that are sums of many entries, whose roundings average out)
+  __shared__ u32x2 list[ITEMS && P == 1 ? 4 : 1][kList];
+  uint32_t list_len = 0;
   Stage stage;
   float extra = 0.f;
   // by row of the batch: the waves bring one array each; else the items' bias
-  const float *by_k = ITEMS ? (wave == 0 ? a.lse : wave == 1 ? a.every : wave == 2 ? a.one : (const float *)a.target) : a.bias;
+  const float *by_k = ITEMS ? (wave == 0 ? a.lse : wave == 1 ? a.every : wave == 2 ? a.entry : (const float *)a.target) : a.bias;
   auto load = [&](uint32_t s) {
     stage.load(a.k, a.k_ld, a.k_plane, a.nk, s);
     if (ITEMS) extra = by_k[s * 64 + lane];
@@ -315,7 +341,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
   if (s_lo < s_hi) load(s_lo);
   // this wave's rows
   u32x4 R[P][RT][KD];
-  float lse[RT], every[RT], one[RT], rbias[RT], bsum[RT];
+  float lse[RT], every[RT], entry[RT], rbias[RT], bsum[RT];
   int hit[RT];
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
@@ -324,14 +350,14 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
     for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int s = 0; s < KD; ++s) R[p][j][s] = *(const u32x4 *)(a.r + (size_t)row * a.r_ld + p * a.r_plane + s * 64 + q * 16);
-    lse[j] = every[j] = one[j] = rbias[j] = bsum[j] = 0.f;
+    lse[j] = every[j] = entry[j] = rbias[j] = bsum[j] = 0.f;
     hit[j] = -1;
     if constexpr (ITEMS) {
       if (BIAS) rbias[j] = a.bias[row];
     } else {
       lse[j] = FAST ? a.lse[row] * kLog2e : a.lse[row];
       every[j] = a.every[row];
-      one[j] = a.one[row];
+      entry[j] = a.entry[row];
       hit[j] = a.target[row];
     }
   }
@@ -403,28 +429,32 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
 #pragma unroll
               for (int j = 0; j < RT; ++j) z[j][e] = 0.f;
         }
-        // targets: rare
+        // targets: few of the steps hold one
+        bool any = false;
+        const uint32_t tg = ITEMS ? *(const uint32_t *)(here_in + by + 768 + (lane & 31) * 4) - r0 : 0u;
         if constexpr (ITEMS) {
-          const uint32_t tg = *(const uint32_t *)(here_in + by + 768 + (lane & 31) * 4);
-          if (__any(tg - r0 < 16u * RT)) {
-            const u32x4 kt = lr_row(here_in, by + 768 + q * 32 + i * 16), ko = lr_row(here_in, by + 512 + q * 32 + i * 16);
-#pragma unroll
-            for (int j = 0; j < RT; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (kt[e] == r0 + j * 16 + col) z[j][e] -= __uint_as_float(ko[e]);
-          }
+          any = tg < 16u * RT;
         } else {
-          bool any = false;
 #pragma unroll
           for (int j = 0; j < RT; ++j) any |= (uint32_t)hit[j] - k0 < 32u;
-          if (__any(any)) {
-#pragma unroll
-            for (int j = 0; j < RT; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if ((uint32_t)hit[j] == k0 + q * 8 + i * 4 + e) z[j][e] -= one[j];
+        }
+        if (__any(any)) {
+          u32x4 kt = {}, kg = {};
+          if constexpr (ITEMS) {
+            kt = lr_row(here_in, by + 768 + q * 32 + i * 16);
+            kg = lr_row(here_in, by + 512 + q * 32 + i * 16);
+            if (P == 1 && i == 0) {  // the rows that meet this wave's items, in order, for the end
+              const uint32_t met = (uint32_t)__ballot(any && lane < 32);
+              const uint32_t place = list_len + __popc(met & ((1u << (lane & 31)) - 1));
+              if (any && lane < 32 && place < kList) list[wave][place] = u32x2{k0 + lane, tg};
+              list_len += __popc(met);
+            }
           }
+#pragma unroll
+          for (int j = 0; j < RT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (ITEMS ? kt[e] == r0 + j * 16 + col : (uint32_t)hit[j] == k0 + q * 8 + i * 4 + e) z[j][e] = ITEMS ? __uint_as_float(kg[e]) : entry[j];
         }
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
@@ -460,6 +490,31 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
     }
     __builtin_amdgcn_s_setprio(0);
     if (s + 1 < s_hi) store(buf ^ 1);
+  }
+  if constexpr (ITEMS && P == 1) {  // what 16 bits left of the entries at the targets
+    list_len = nt_min(list_len, kList);
+    for (uint32_t n = 0; n < list_len; ++n) {
+      const uint32_t t = __builtin_amdgcn_readfirstlane(list[wave][n][0]), at = __builtin_amdgcn_readfirstlane(list[wave][n][1]);
+      if (col != (at & 15)) continue;
+      const float rest = a.rest[t];
+#pragma unroll
+      for (int s = 0; s < KD; ++s) {
+        const u32x4 w = *(const u32x4 *)(a.k + (size_t)t * a.k_ld + s * 64 + q * 16);
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const unsigned short u = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
+          y[e] = FMT == AS_BF16 ? bf16_to_f32(u) : (float)__builtin_bit_cast(_Float16, u);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < RT; ++j)
+          if (j == at >> 4) {
+            out[2 * s][j] += f32x4{y[0], y[1], y[2], y[3]} * rest;
+            out[2 * s + 1][j] += f32x4{y[4], y[5], y[6], y[7]} * rest;
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
   }
   const float f = ITEMS ? a.scale * a.coef[1] * (P == 2 ? 1.f / plane_scale(*a.k_top) : 1.f) : 1.f;
 #pragma unroll
