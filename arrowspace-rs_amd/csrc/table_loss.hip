@@ -28,7 +28,7 @@ struct LossArgs {
   // operands of the product: A the table side (m), B the rows (n)
   const char *table, *rows;
   size_t table_ld, rows_ld;       // bytes
-  uint32_t table_plane, rows_plane;  // steps of 64 to the low plane
+  size_t table_plane, rows_plane; // bytes to the low plane
   uint32_t n, v;                  // rows of B and of A
   uint32_t steps, planes;         // steps of 64 along k per plane; 1, or 2 (three passes)
   uint32_t per;                   // tiles of A a workgroup walks
@@ -58,10 +58,10 @@ __global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2
   uint32_t vt = chunk * a.per;
   const float nat = a.scale * product_scale(a), unit = GENERAL ? kLog2e : nat * kLog2e;  // exponentials of (x - maximum) * unit to the base 2
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
-  NtOperand B{a.rows + (size_t)n0 * a.rows_ld, a.rows_ld, nt_min(TILE::BN, a.n - n0) - 1, a.rows_plane};
+  NtOperand B{a.rows + (size_t)n0 * a.rows_ld, a.rows_ld, nt_min(TILE::BN, a.n - n0) - 1, 0, a.rows_plane};
   auto side = [&](uint32_t tile) {
     const uint32_t r0 = tile * TILE::BM;
-    return NtOperand{a.table + (size_t)r0 * a.table_ld, a.table_ld, nt_min(TILE::BM, a.v - r0) - 1, a.table_plane};
+    return NtOperand{a.table + (size_t)r0 * a.table_ld, a.table_ld, nt_min(TILE::BM, a.v - r0) - 1, 0, a.table_plane};
   };
   const uint32_t all = a.planes == 2 ? 3 * a.steps : a.steps;
   float top[TILE::TN], sum[TILE::TN];
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2
   for (int j = 0; j < TILE::TN; ++j) top[j] = -INFINITY, sum[j] = 0.f;
   f32x4 acc[TILE::TM][TILE::TN];
   NtOperand A = side(vt);
-  T.fetch(0, A, B, nt_col_a(0, a.steps, a.table_plane), nt_col_b(0, a.steps, a.rows_plane));
+  T.fetch(0, A, B, 0, a.steps);
   int buf = 0;
   for (; vt < vt_end; ++vt) {
     T.zero(acc);
@@ -77,10 +77,10 @@ __global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2
     for (uint32_t s = 0; s < all; ++s) {
       TILE::turn();
       if (s + 1 < all) {
-        T.fetch(buf ^ 1, A, B, nt_col_a(s + 1, a.steps, a.table_plane), nt_col_b(s + 1, a.steps, a.rows_plane));
+        T.fetch(buf ^ 1, A, B, s + 1, a.steps);
       } else if (vt + 1 < vt_end) {
         A = side(vt + 1);
-        T.fetch(buf ^ 1, A, B, nt_col_a(0, a.steps, a.table_plane), nt_col_b(0, a.steps, a.rows_plane));
+        T.fetch(buf ^ 1, A, B, 0, a.steps);
       }
       T.contract(buf, acc);
       buf ^= 1;
@@ -274,29 +274,6 @@ __global__ __launch_bounds__(256) void image_kernel(ImageJobs jobs) {
       if constexpr (two) *(u32x2 *)(o + j.pitch) = u32x2{pack2<FMT>(low_part(x[0]), low_part(x[1])), pack2<FMT>(low_part(x[2]), low_part(x[3]))};
     }
 }
-// the same transposed: out[k][r], rows filled to `pitch` by zeros.  64 x 64 through LDS.
-template <int DT, int FMT>
-__global__ __launch_bounds__(256) void transposed_kernel(const void *src, size_t stride, uint32_t n, uint32_t d, uint32_t pitch, const unsigned int *top,
-                                                         unsigned short *out) {
-  constexpr bool two = DT == AS_F32;
-  __shared__ float tile[64][65];
-  const float f = two ? plane_scale(*top) : 1.f;
-  const uint32_t r0 = blockIdx.x * 64, k0 = blockIdx.y * 64;
-  for (uint32_t e = threadIdx.x; e < 4096; e += 256) {
-    const uint32_t r = r0 + (e >> 6), k = k0 + (e & 63);
-    tile[e >> 6][e & 63] = r < n && k < d ? load_as_f32<DT>(src, (size_t)r * stride + k) * f : 0.f;
-  }
-  __syncthreads();
-  for (uint32_t e = threadIdx.x; e < 2048; e += 256) {
-    const uint32_t k = k0 + (e >> 5), rr = (e & 31) * 2;
-    if (k >= d) continue;
-    const float x = tile[rr][e >> 5], y = tile[rr + 1][e >> 5];
-    unsigned short *o = out + (size_t)k * pitch * (two ? 2 : 1) + r0 + rr;
-    *(uint32_t *)o = pack2<FMT>(x, y);
-    if constexpr (two) *(uint32_t *)(o + pitch) = pack2<FMT>(low_part(x), low_part(y));
-  }
-}
-
 // The unit the gradient of the logits is rounded in: the largest |grad_losses|, so that the entry of a target, -grad_losses (1 - p), is
 // a whole number of steps where all rows weigh the same (the mean of the losses: without this every such entry is off by the SAME
 // part of 2^-9 in bf16, which no sum averages out).  f16: 2^14 of these units, entries down to 2^-28 of one keep all 11 bits.
@@ -332,8 +309,8 @@ struct GradArgs {
   const float *lse, *every, *entry;  // by row, filled to whole tiles (loss_rows_kernel)
   const int *target;
   const float *coef;               // {factor, 1 / factor} of G
-  unsigned short *G, *GT;          // n x (planes * g_pitch), v_pad x (planes * t_pitch)
-  uint32_t g_pitch, t_pitch;
+  unsigned short *G;               // (rows filled to whole tiles) x (planes * g_pitch)
+  uint32_t g_pitch;
   float *bias_part;                // (n_tiles WN) x g_pitch sums over the tile's rows, or null
 };
 
@@ -351,10 +328,10 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
   uint32_t vt = chunk * a.per;
   const float c = a.scale * product_scale(a);
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
-  NtOperand B{a.rows + (size_t)n0 * a.rows_ld, a.rows_ld, nt_min(TILE::BN, a.n - n0) - 1, a.rows_plane};
+  NtOperand B{a.rows + (size_t)n0 * a.rows_ld, a.rows_ld, nt_min(TILE::BN, a.n - n0) - 1, 0, a.rows_plane};
   auto side = [&](uint32_t tile) {
     const uint32_t r0 = tile * TILE::BM;
-    return NtOperand{a.table + (size_t)r0 * a.table_ld, a.table_ld, nt_min(TILE::BM, a.v - r0) - 1, a.table_plane};
+    return NtOperand{a.table + (size_t)r0 * a.table_ld, a.table_ld, nt_min(TILE::BM, a.v - r0) - 1, 0, a.table_plane};
   };
   // this lane's rows
   uint32_t row[TILE::TN];
@@ -373,7 +350,7 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
   const uint32_t all = a.planes == 2 ? 3 * a.steps : a.steps;
   f32x4 acc[TILE::TM][TILE::TN];
   NtOperand A = side(vt);
-  T.fetch(0, A, B, nt_col_a(0, a.steps, a.table_plane), nt_col_b(0, a.steps, a.rows_plane));
+  T.fetch(0, A, B, 0, a.steps);
   int buf = 0;
   for (; vt < vt_end; ++vt) {
     T.zero(acc);
@@ -381,10 +358,10 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
     for (uint32_t s = 0; s < all; ++s) {
       TILE::turn();
       if (s + 1 < all) {
-        T.fetch(buf ^ 1, A, B, nt_col_a(s + 1, a.steps, a.table_plane), nt_col_b(s + 1, a.steps, a.rows_plane));
+        T.fetch(buf ^ 1, A, B, s + 1, a.steps);
       } else if (vt + 1 < vt_end) {
         A = side(vt + 1);
-        T.fetch(buf ^ 1, A, B, nt_col_a(0, a.steps, a.table_plane), nt_col_b(0, a.steps, a.rows_plane));
+        T.fetch(buf ^ 1, A, B, 0, a.steps);
       }
       T.contract(buf, acc);
       buf ^= 1;
@@ -442,57 +419,53 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
           }
       }
     }
-    // two columns of accumulators at a time (what is packed and not yet stored stays in registers)
-    const size_t gp = (size_t)g.g_pitch * (TWO ? 2 : 1), tp = (size_t)g.t_pitch * (TWO ? 2 : 1);
-    const bool odd = col & 1, high = col & 2;
-    const uint32_t s0 = odd ? 0x01000504u : 0x05040100u, s1 = odd ? 0x03020706u : 0x07060302u;
-    const uint32_t item = ((col & 1) << 1) | ((col >> 1) & 1);
-    const uint32_t t0 = n0 + wn * (TILE::TN * 16) + (col >> 2) * 8;
+    // eight consecutive items a lane (rows behind the last: zeros, the product over the batch reads them)
+    const size_t gp = (size_t)g.g_pitch * (TWO ? 2 : 1);
 #pragma unroll
-    for (int jj = 0; jj < TILE::TN; jj += 2)
+    for (int j = 0; j < TILE::TN; ++j) {
+      unsigned short *o = g.G + (size_t)row[j] * gp + at0 + row0;
 #pragma unroll
-      for (int plane = 0; plane < (TWO ? 2 : 1); ++plane) {
-        uint32_t w[TILE::TM][2][2];
-#pragma unroll
-        for (int i = 0; i < TILE::TM; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            f32x4 u = acc[i][jj + h];
-            if (TWO && plane == 1) u = f32x4{low_part(u[0]), low_part(u[1]), low_part(u[2]), low_part(u[3])};
-            w[i][h][0] = pack2<FMT>(u[0], u[1]);
-            w[i][h][1] = pack2<FMT>(u[2], u[3]);
-          }
-        // row-major: eight consecutive items a lane
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (row[jj + h] < a.n) {
-            unsigned short *o = g.G + (size_t)row[jj + h] * gp + plane * g.g_pitch + at0 + row0;
-#pragma unroll
-            for (int i = 0; i < TILE::TM; i += 2) *(u32x4 *)(o + i * 16) = u32x4{w[i][h][0], w[i][h][1], w[i + 1][h][0], w[i + 1][h][1]};
-          }
-        // transposed: the quad's four rows of an item meet in one lane (4 x 4 over the quad, two exchanges), eight consecutive rows a lane
-#pragma unroll
-        for (int i = 0; i < TILE::TM; ++i) {
-          uint32_t y[4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t mine = odd ? w[i][h][1] : w[i][h][0], theirs = quad_xor1(odd ? w[i][h][0] : w[i][h][1]);
-            const uint32_t x0 = __builtin_amdgcn_perm(theirs, mine, s0), x1 = __builtin_amdgcn_perm(theirs, mine, s1);
-            const uint32_t other = quad_xor2(high ? x0 : x1);
-            y[2 * h] = high ? other : x0;
-            y[2 * h + 1] = high ? x1 : other;
-          }
-          *(u32x4 *)(g.GT + (size_t)(at0 + row0 + (i >> 1) * 32 + (i & 1) * 4 + item) * tp + plane * g.t_pitch + t0 + jj * 16) = u32x4{y[0], y[1], y[2], y[3]};
-        }
+      for (int i = 0; i < TILE::TM; i += 2) {
+        const f32x4 u = acc[i][j], v = acc[i + 1][j];
+        *(u32x4 *)(o + i * 16) = u32x4{pack2<FMT>(u[0], u[1]), pack2<FMT>(u[2], u[3]), pack2<FMT>(v[0], v[1]), pack2<FMT>(v[2], v[3])};
+        if constexpr (TWO)
+          *(u32x4 *)(o + g.g_pitch + i * 16) = u32x4{pack2<FMT>(low_part(u[0]), low_part(u[1])), pack2<FMT>(low_part(u[2]), low_part(u[3])),
+                                                     pack2<FMT>(low_part(v[0]), low_part(v[1])), pack2<FMT>(low_part(v[2]), low_part(v[3]))};
       }
+    }
   }
 }
 
+// The rows of the batch that meet each 64 items of the table, in order, a wave each (64 kept: items that more rows meet are sums of
+// many entries, whose roundings average out).
+constexpr uint32_t kMet = 64;
+__global__ __launch_bounds__(256) void met_kernel(const int *target, uint32_t n, uint32_t groups, u32x2 *list, uint32_t *count) {
+  const uint32_t group = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (group >= groups) return;
+  uint32_t len = 0;
+  for (uint32_t t0 = 0; t0 < n && len < kMet; t0 += 512) {
+    uint32_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = t0 + k * 64 + lane < n ? (uint32_t)target[t0 + k * 64 + lane] - group * 64 : ~0u;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint64_t met = __ballot(v[k] < 64);
+      const uint32_t place = len + (uint32_t)__popcll(met & ((1ull << lane) - 1));
+      if (v[k] < 64 && place < kMet) list[(size_t)group * kMet + place] = u32x2{t0 + k * 64 + lane, v[k]};
+      len += (uint32_t)__popcll(met);
+    }
+  }
+  if (lane == 0) count[group] = len < kMet ? len : kMet;
+}
+
 // ---- the two gradients: plain products ------------------------------------------------------------------------------------------------------
+// A (m: columns of x or of the table) is read transposed, a row per k; B (n: g) transposed for dW, along k for dX.
 struct ProductArgs {
   const char *A, *B;
   size_t a_ld, b_ld;
-  uint32_t a_plane, b_plane;
+  size_t a_plane, b_plane;          // bytes
+  uint32_t a_cols, b_cols;          // 16-byte pieces of a row that may be read (transposed)
+  uint32_t k_a, k_b;                // rows that may be read (transposed)
   uint32_t m, n, m_tiles, n_tiles;
   uint32_t steps, planes, splits;   // steps of 64 of the whole contraction; a split takes an even share of them
   float scale;
@@ -503,68 +476,50 @@ struct ProductArgs {
   float *sums;                      // instead: f32 [split][n][sums_pitch], added to unless `first`
   uint32_t sums_pitch;
   int first, aligned;
-  // dW of one plane: the rows whose target is one of the output's, by the rest of their entry there (null: left out)
-  const int *target;
+  // dW of one plane: by 64 items the rows of the batch that meet them, what 16 bits left of those rows' entries (null: none)
+  const u32x2 *met;
+  const uint32_t *met_count;
   const float *rest;
-  uint32_t n_rows, n_begin;         // rows of the batch; item of output row 0
-  const char *x;                    // the batch as an operand (whole steps of 64 columns)
-  size_t x_ld;
 };
-// dW's part of a tile from what 16 bits left of the entries at the targets: rows of the batch in order, a list of those that meet the
-// tile per workgroup's width of rows, each added by the lanes that hold its item.  A tile of 256 items meets 16 of 8 192 rows where
-// the table has 131 072; tables of less than half the rows go without (their items are sums of several entries, whose roundings
-// average out).
 template <int FMT, class TILE>
-__device__ __forceinline__ void add_rest(const ProductArgs &p, const TILE &T, char *smem, uint32_t m0, uint32_t n0, f32x4 (&acc)[TILE::TM][TILE::TN]) {
-  u32x2 *list = (u32x2 *)smem;
-  uint32_t *counts = (uint32_t *)(smem + TILE::NT * 8);
+__device__ __forceinline__ void add_rest(const ProductArgs &p, const TILE &T, uint32_t m0, uint32_t n0, f32x4 (&acc)[TILE::TM][TILE::TN]) {
+  static_assert(TILE::TN == 4, "a wave's columns are one list's items");
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
-  for (uint32_t t0 = 0; t0 < p.n_rows; t0 += TILE::NT) {
-    __syncthreads();
-    const uint32_t t = t0 + threadIdx.x, v = t < p.n_rows ? (uint32_t)p.target[t] - p.n_begin - n0 : ~0u;
-    const bool meets = v < nt_min(TILE::BN, p.n - n0);
-    const uint64_t ballot = __ballot(meets);
-    if (T.lane == 0) counts[T.wave] = (uint32_t)__popcll(ballot);
-    __syncthreads();
-    uint32_t before = 0, total = 0;
+  if (n0 + wn * 64 >= p.n) return;
+  const uint32_t group = (n0 >> 6) + wn, len = p.met_count[group];
+  if (!len) return;
+  const u32x2 mine = p.met[(size_t)group * kMet + (T.lane < len ? T.lane : 0)];
+  const float mine_rest = p.rest[mine[0]];
+  for (uint32_t k = 0; k < len; ++k) {
+    const uint32_t row = __builtin_amdgcn_readlane(mine[0], k), in = __builtin_amdgcn_readlane(mine[1], k);
+    const float r = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine_rest), k));
+    const uint32_t jj = ((in >> 5) << 1) | ((in >> 2) & 1), c = (((in >> 3) & 3) << 2) | (in & 3);
+    if (col != c) continue;
 #pragma unroll
-    for (uint32_t w = 0; w < TILE::NT / 64; ++w) {
-      if (w < T.wave) before += counts[w];
-      total += counts[w];
-    }
-    if (meets) list[before + (uint32_t)__popcll(ballot & ((1ull << T.lane) - 1))] = u32x2{t, v};
-    __syncthreads();
-    for (uint32_t k = 0; k < total; ++k) {
-      const uint32_t row = __builtin_amdgcn_readfirstlane(list[k][0]), at = __builtin_amdgcn_readfirstlane(list[k][1]);
-      if (at / (TILE::TN * 16) != wn) continue;
-      const uint32_t in = at % (TILE::TN * 16), jj = ((in >> 5) << 1) | ((in >> 2) & 1), c = (((in >> 3) & 3) << 2) | (in & 3);
-      if (col != c) continue;
-      const float r = p.rest[row];
+    for (int i = 0; i < TILE::TM; i += 2) {
+      const uint32_t m = m0 + wm * (TILE::TM * 16) + i * 16 + q * 8;
+      if (m >= p.m) continue;
+      const u32x4 w = *(const u32x4 *)(p.A + (size_t)row * p.a_ld + m * 2);  // (zeros behind the row's values)
+      float y[8];
 #pragma unroll
-      for (int i = 0; i < TILE::TM; i += 2) {
-        const uint32_t m = m0 + wm * (TILE::TM * 16) + i * 16 + q * 8;
-        if (m >= p.m) continue;
-        const u32x4 w = *(const u32x4 *)(p.x + (size_t)row * p.x_ld + m * 2);  // (zeros behind the row's values)
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const unsigned short u = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
-          y[e] = FMT == AS_BF16 ? bf16_to_f32(u) : (float)__builtin_bit_cast(_Float16, u);
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < TILE::TN; ++j)
-          if (j == jj) {
-            acc[i][j] += f32x4{y[0], y[1], y[2], y[3]} * r;
-            acc[i + 1][j] += f32x4{y[4], y[5], y[6], y[7]} * r;
-          }
-        __builtin_amdgcn_sched_barrier(0);
+      for (int e = 0; e < 8; ++e) {
+        const unsigned short u = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
+        y[e] = FMT == AS_BF16 ? bf16_to_f32(u) : (float)__builtin_bit_cast(_Float16, u);
       }
+#pragma unroll
+      for (uint32_t j = 0; j < TILE::TN; ++j)
+        if (j == jj) {
+          acc[i][j] += f32x4{y[0], y[1], y[2], y[3]} * r;
+          acc[i + 1][j] += f32x4{y[4], y[5], y[6], y[7]} * r;
+        }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
-template <int FMT, class TILE_, int OUT>  // OUT: element type of `out`, or 0 (AS_F64) = into `sums`
+template <int FMT, class TILE_, int OUT>  // OUT: element type of `out` (dW), or 0 (AS_F64) = into `sums` (dX)
 __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
   using TILE = TILE_;
+  constexpr bool BT = OUT != 0;
   __shared__ __attribute__((aligned(1024))) char smem[2 * TILE::kStage];
   TILE T;
   T.init(smem);
@@ -575,20 +530,21 @@ __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
   const uint32_t m0 = mt * TILE::BM, n0 = nt * TILE::BN;
   const uint32_t k0 = (uint32_t)((uint64_t)p.steps * split / p.splits), k1 = (uint32_t)((uint64_t)p.steps * (split + 1) / p.splits);
   const uint32_t steps = k1 - k0, all = p.planes == 2 ? 3 * steps : steps;
-  const NtOperand A{p.A + (size_t)m0 * p.a_ld + (size_t)k0 * 128, p.a_ld, nt_min(TILE::BM, p.m - m0) - 1, p.a_plane};
-  const NtOperand B{p.B + (size_t)n0 * p.b_ld + (size_t)k0 * 128, p.b_ld, nt_min(TILE::BN, p.n - n0) - 1, p.b_plane};
+  const NtOperand A{p.A + (size_t)k0 * 64 * p.a_ld + m0 * 2, p.a_ld, p.a_cols - 1 - m0 / 8, p.k_a - 1 - k0 * 64, p.a_plane};
+  const NtOperand B = BT ? NtOperand{p.B + (size_t)k0 * 64 * p.b_ld + n0 * 2, p.b_ld, p.b_cols - 1 - n0 / 8, p.k_b - 1 - k0 * 64, p.b_plane}
+                         : NtOperand{p.B + (size_t)n0 * p.b_ld + (size_t)k0 * 128, p.b_ld, nt_min(TILE::BN, p.n - n0) - 1, 0, p.b_plane};
   f32x4 acc[TILE::TM][TILE::TN];
   T.zero(acc);
-  if (all) T.fetch(0, A, B, 0, nt_col_b(0, steps, p.b_plane));
+  if (all) T.fetch(0, A, B, 0, steps);
   int buf = 0;
   for (uint32_t s = 0; s < all; ++s) {
     TILE::turn();
-    if (s + 1 < all) T.fetch(buf ^ 1, A, B, nt_col_a(s + 1, steps, p.a_plane), nt_col_b(s + 1, steps, p.b_plane));
+    if (s + 1 < all) T.fetch(buf ^ 1, A, B, s + 1, steps);
     T.contract(buf, acc);
     buf ^= 1;
   }
   if constexpr (OUT == FMT)
-    if (p.target) add_rest<FMT>(p, T, smem, m0, n0, acc);
+    if (p.met) add_rest<FMT>(p, T, m0, n0, acc);
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
   const float f = OUT == 0 ? 1.f : p.scale * p.coef[1] * (p.top ? 1.f / plane_scale(*p.top) : 1.f);
 #pragma unroll
@@ -670,6 +626,7 @@ __global__ __launch_bounds__(256) void bias_join_kernel(const float *part, uint3
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;
   if (i >= v) return;
   float s = 0.f;
+#pragma unroll 16
   for (uint32_t p = 0; p < parts; ++p) s += part[(size_t)p * pitch + i];
   out[i] = s * coef[1];
 }
@@ -681,12 +638,12 @@ __global__ __launch_bounds__(256) void zero_rows_kernel(void *out, size_t stride
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------------
-template <int FMT>
-using Slim = NtTile<FMT, 4, 4, 4, 1>;   // 256 x 64
-template <int FMT>
-using Square = NtTile<FMT, 4, 4, 2, 2>; // 128 x 128
-template <int FMT>
-using Large = NtTile<FMT, 8, 4, 2, 4>;  // 256 x 256
+template <int FMT, bool AT = false, bool BT = false>
+using Slim = NtTile<FMT, 4, 4, 4, 1, AT, BT>;   // 256 x 64
+template <int FMT, bool AT = false, bool BT = false>
+using Square = NtTile<FMT, 4, 4, 2, 2, AT, BT>; // 128 x 128
+template <int FMT, bool AT = false, bool BT = false>
+using Large = NtTile<FMT, 8, 4, 2, 4, AT, BT>;  // 256 x 256
 enum { kSlim = 0, kSquare = 1, kLarge = 2 };
 struct TileShape {
   uint32_t bm, bn, wm, wn;
@@ -723,7 +680,7 @@ struct Plan {
   int tile;
   uint32_t n_tiles, v_tiles, per, chunks;
   // backward
-  uint32_t piece, pieces, t_pitch, splits;
+  uint32_t piece, pieces, splits;
   int tile_w, tile_x;
   int fused;                 // steps of 32 columns of the form for short rows (table_loss_rows.h), 0: through G in memory
   uint32_t x_blocks, w_blocks, n_pad;
@@ -793,13 +750,12 @@ void plan_backward(Plan &p, bool x, bool w, bool b) {
     return;
   }
   const uint32_t bm = kShape[p.tile].bm, bn = kShape[p.tile].bn;
-  p.t_pitch = up(p.n, std::max(bn, 64u));
-  p.n_pad = p.t_pitch;
-  // G and its transposed form of a piece: some 512 MB together, and whole rounds of the large tile for the piece's dW
-  const uint64_t per_item = (uint64_t)p.t_pitch * 2 * 2 * p.planes;
+  p.n_pad = up(p.n, std::max(bn, 64u));
+  // G of a piece: some 256 MB, what the last cache before memory holds, and whole rounds of the large tile for the piece's dW
+  const uint64_t per_item = (uint64_t)p.n_pad * 2 * p.planes;
   const uint32_t round = std::max(1u, (uint32_t)kChips / cdiv(p.d, 256)) * 256;
-  uint64_t piece = std::max<uint64_t>((640ull << 20) / per_item / round, 1) * round;
-  if (piece * per_item > (1024ull << 20)) piece = std::max<uint64_t>((512ull << 20) / per_item / 1024 * 1024, 1024);
+  uint64_t piece = std::max<uint64_t>((320ull << 20) / per_item / round, 1) * round;
+  if (piece * per_item > (512ull << 20)) piece = std::max<uint64_t>((256ull << 20) / per_item / 1024 * 1024, 1024);
   piece = std::min<uint64_t>(piece, up(p.v, bm));
   p.piece = (uint32_t)up(piece, bm);
   p.pieces = cdiv(p.v, p.piece);
@@ -850,7 +806,9 @@ uint64_t forward_layout(const Plan &p, const Source &x, const Source &t, char *b
 struct BackwardScratch {
   unsigned int *tops;
   float *top_parts, *coef;
-  unsigned short *x_image, *t_image, *xt, *wt, *G, *GT;
+  unsigned short *x_image, *t_image, *G;
+  u32x2 *met;
+  uint32_t *met_count;
   float *sums, *bias_part;
   float *lse, *every, *entry, *rest;
   int *target;
@@ -872,10 +830,10 @@ uint64_t backward_layout(const Plan &p, const Source &x, const Source &t, char *
     s.sums = l.take<float>(p.want_x ? (uint64_t)p.splits * p.n * up(p.d, 8) : 0);
     return l.at;
   }
-  s.xt = l.take<unsigned short>(p.want_w ? (uint64_t)p.d * p.t_pitch * pl : 0);
-  s.wt = l.take<unsigned short>(p.want_x ? (uint64_t)p.d * p.piece * pl : 0);
-  s.G = l.take<unsigned short>((uint64_t)p.n * p.piece * pl);
-  s.GT = l.take<unsigned short>((uint64_t)p.piece * p.t_pitch * pl);
+  s.G = l.take<unsigned short>((uint64_t)p.n_pad * p.piece * pl);
+  const uint64_t groups = p.want_w && p.planes == 1 ? (p.v + 63) / 64 : 0;
+  s.met = l.take<u32x2>(groups * kMet);
+  s.met_count = l.take<uint32_t>(groups);
   s.sums = l.take<float>(p.want_x ? (uint64_t)p.splits * p.n * up(p.d, 8) : 0);
   s.bias_part = l.take<float>(p.want_b ? (uint64_t)p.n_tiles * kShape[p.tile].wn * p.piece : 0);
   return l.at;
@@ -887,8 +845,8 @@ void by_tile(int tile, F &&f) {
   else if (tile == kSquare) f(std::integral_constant<int, kSquare>{});
   else f(std::integral_constant<int, kLarge>{});
 }
-template <int FMT, int K>
-using TileOf = std::conditional_t<K == kSlim, Slim<FMT>, std::conditional_t<K == kSquare, Square<FMT>, Large<FMT>>>;
+template <int FMT, int K, bool AT = false, bool BT = false>
+using TileOf = std::conditional_t<K == kSlim, Slim<FMT, AT, BT>, std::conditional_t<K == kSquare, Square<FMT, AT, BT>, Large<FMT, AT, BT>>>;
 template <class F>
 void by_type(int dt, F &&f) {
   if (dt == AS_F32) f(std::integral_constant<int, AS_F32>{});
@@ -929,14 +887,6 @@ int make_operands(as_ctx *ctx, const Source &x, const Source &t, unsigned int *t
   });
   AS_HIP(ctx, hipGetLastError());
   return AS_OK;
-}
-void make_transposed(as_ctx *ctx, const Source &s, uint32_t row0, uint32_t rows, uint32_t pitch, const unsigned int *top, unsigned short *out) {
-  const char *p = (const char *)s.p + (size_t)row0 * s.stride * dtype_size(s.dt);
-  by_type(s.dt, [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
-    hipLaunchKernelGGL((transposed_kernel<DT, DT == AS_BF16 ? AS_BF16 : AS_F16>), dim3(pitch / 64, cdiv(s.d, 64)), dim3(256), 0, ctx->stream, (const void *)p,
-                       s.stride, rows, s.d, pitch, top, out);
-  });
 }
 template <int FMT, int P, int KD, bool ITEMS, bool BIAS>
 void launch_rows_grad(as_ctx *ctx, const LossRowsArgs &a) {
@@ -989,7 +939,8 @@ void launch_product(as_ctx *ctx, int fmt, int tile, int out_type, const ProductA
     const dim3 grid(p.m_tiles * p.n_tiles * p.splits);
     auto go = [&](auto f, auto o) {
       constexpr int FMT = decltype(f)::value, OUT = decltype(o)::value;
-      hipLaunchKernelGGL((product_kernel<FMT, TileOf<FMT, K>, OUT>), grid, dim3(TileOf<FMT, K>::NT), 0, ctx->stream, p);
+      typedef TileOf<FMT, K, true, OUT != 0> TILE;
+      hipLaunchKernelGGL((product_kernel<FMT, TILE, OUT>), grid, dim3(TILE::NT), 0, ctx->stream, p);
     };
     constexpr std::integral_constant<int, AS_BF16> bf{};
     constexpr std::integral_constant<int, AS_F16> hf{};
@@ -1052,7 +1003,7 @@ int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tabl
   Operands o{};
   AS_TRY(make_operands(ctx, xs, ts, s.tops, s.top_parts, s.x_image, s.t_image, &o));
   a.rows = o.x, a.rows_ld = o.x_ld, a.table = o.t, a.table_ld = o.t_ld;
-  a.table_plane = a.rows_plane = p.steps;
+  a.table_plane = a.rows_plane = (size_t)p.pitch * 2;
   a.n = p.n, a.v = p.v, a.steps = p.steps, a.planes = p.planes, a.per = p.per, a.v_tiles = p.v_tiles, a.n_tiles = p.n_tiles, a.chunks = p.chunks;
   a.scale = c.scale, a.bias = (const float *)Bi.p;
   if (p.planes == 2) a.rows_top = s.tops, a.table_top = s.tops + 1;
@@ -1139,7 +1090,6 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   const char *table16 = o.t;
   a.rows = o.x, a.rows_ld = o.x_ld, a.table_ld = o.t_ld;
   const unsigned int *x_top = p.planes == 2 ? s.tops : nullptr, *w_top = p.planes == 2 ? s.tops + 1 : nullptr;
-  if (p.want_w && !p.fused) make_transposed(ctx, xs, 0, p.n, p.t_pitch, x_top, s.xt);
   hipLaunchKernelGGL(coef_scale_kernel, dim3(1), dim3(1024), 0, ctx->stream, (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p, ignore, p.n,
                      c.dt == AS_BF16 ? 0 : 14, s.coef);
   AS_HIP(ctx, hipGetLastError());
@@ -1174,14 +1124,18 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
     }
     AS_HIP(ctx, hipGetLastError());
   }
-  a.table_plane = a.rows_plane = p.steps;
+  a.table_plane = a.rows_plane = (size_t)p.pitch * 2;
   a.n = p.n, a.steps = p.steps, a.planes = p.planes, a.n_tiles = p.n_tiles, a.per = p.per;
   a.scale = c.scale;
   a.rows_top = x_top, a.table_top = w_top;
   g.lse = s.lse, g.every = s.every, g.entry = s.entry, g.target = s.target, g.coef = coef;
-  g.G = s.G, g.GT = s.GT, g.g_pitch = p.piece, g.t_pitch = p.t_pitch;
+  g.G = s.G, g.g_pitch = p.piece;
   g.bias_part = p.want_b ? s.bias_part : nullptr;
   const int fmt = image_format(c.dt);
+  if (!p.fused && rest && p.want_w) {
+    const uint32_t groups = cdiv(p.v, 64);
+    hipLaunchKernelGGL(met_kernel, dim3(cdiv(groups, 4)), dim3(256), 0, ctx->stream, (const int *)s.target, p.n, groups, s.met, s.met_count);
+  }
   for (uint32_t v0 = 0; !p.fused && v0 < p.v; v0 += p.piece) {
     const uint32_t items = std::min(p.piece, p.v - v0);
     a.table = table16 + (size_t)v0 * a.table_ld;
@@ -1206,26 +1160,24 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
     if (p.want_b)
       hipLaunchKernelGGL(bias_join_kernel, dim3(cdiv(items, 256)), dim3(256), 0, ctx->stream, (const float *)s.bias_part, p.n_tiles * kShape[p.tile].wn, p.piece, items,
                          coef, (float *)Ob.p + v0);
+    ProductArgs w{};
+    w.B = (const char *)s.G, w.b_ld = (size_t)p.piece * p.planes * 2, w.b_plane = (size_t)p.piece * 2, w.b_cols = p.piece / 8, w.k_b = p.n_pad;
+    w.m = p.d, w.a_plane = (size_t)p.pitch * 2, w.a_cols = p.pitch / 8, w.planes = p.planes;
+    w.scale = c.scale, w.coef = coef;
     if (p.want_w) {
-      ProductArgs w{};
-      w.A = (const char *)s.xt, w.a_ld = (size_t)p.t_pitch * p.planes * 2, w.a_plane = p.t_pitch / 64;
-      w.B = (const char *)s.GT, w.b_ld = (size_t)p.t_pitch * p.planes * 2, w.b_plane = p.t_pitch / 64;
-      w.m = p.d, w.n = items, w.m_tiles = cdiv(p.d, kShape[p.tile_w].bm), w.n_tiles = cdiv(items, kShape[p.tile_w].bn);
-      w.steps = cdiv(p.n, 64), w.planes = p.planes, w.splits = 1;
-      w.scale = c.scale, w.coef = coef, w.top = x_top;
+      w.A = a.rows, w.a_ld = a.rows_ld, w.k_a = p.n;
+      w.n = items, w.m_tiles = cdiv(p.d, kShape[p.tile_w].bm), w.n_tiles = cdiv(items, kShape[p.tile_w].bn);
+      w.steps = cdiv(p.n, 64), w.splits = 1, w.top = x_top;
       w.out = (char *)Ow.p + (size_t)v0 * gw_stride * dtype_size(c.dt), w.out_stride = gw_stride;
       w.aligned = gw_stride % 8 == 0 && ((uintptr_t)w.out & 15) == 0;
-      if (rest && p.v >= p.n / 2) w.target = s.target, w.rest = rest, w.n_rows = p.n, w.n_begin = v0, w.x = o.x, w.x_ld = o.x_ld;
+      if (rest) w.met = s.met + (size_t)(v0 / 64) * kMet, w.met_count = s.met_count + v0 / 64, w.rest = rest;
       launch_product(ctx, fmt, p.tile_w, c.dt, w);
     }
     if (p.want_x) {
-      const uint32_t pitch = up(items, 64);
-      make_transposed(ctx, ts, v0, items, pitch, w_top, s.wt);
-      ProductArgs w{};
-      w.A = (const char *)s.wt, w.a_ld = (size_t)pitch * p.planes * 2, w.a_plane = pitch / 64;
-      w.B = (const char *)s.G, w.b_ld = (size_t)p.piece * p.planes * 2, w.b_plane = p.piece / 64;
-      w.m = p.d, w.n = p.n, w.m_tiles = cdiv(p.d, kShape[p.tile_x].bm), w.n_tiles = cdiv(p.n, kShape[p.tile_x].bn);
-      w.steps = pitch / 64, w.planes = p.planes, w.splits = p.splits;
+      w.met = nullptr;
+      w.A = a.table, w.a_ld = a.table_ld, w.k_a = items;
+      w.n = p.n, w.m_tiles = cdiv(p.d, kShape[p.tile_x].bm), w.n_tiles = cdiv(p.n, kShape[p.tile_x].bn);
+      w.steps = cdiv(items, 64), w.splits = p.splits;
       w.sums = s.sums, w.sums_pitch = up(p.d, 8), w.first = v0 == 0;
       launch_product(ctx, fmt, p.tile_x, 0, w);
     }
