@@ -17,6 +17,18 @@ from .api import Context, DeviceArray
 _DTYPES = {"float64": AS_F64, "float32": AS_F32, "bfloat16": AS_BF16, "float16": AS_F16}
 _NAMES = {AS_F64: "float64", AS_F32: "float32", AS_BF16: "bfloat16", AS_F16: "float16"}
 _local = threading.local()
+_torch = None          # the module, once a tensor has been seen
+_raw_stream = None     # device index -> address of torch's current stream there
+_kinds = {}            # torch dtype -> name
+
+
+def _need_torch():
+    global _torch, _raw_stream
+    import torch
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    for name in ("float64", "float32", "bfloat16", "float16", "int64", "uint8"):
+        _kinds[getattr(torch, name)] = name
+    _torch = torch
 
 
 def _thread_context(device):
@@ -26,31 +38,34 @@ def _thread_context(device):
         table = _local.contexts = {}
     ctx = table.get(device)
     if ctx is None:
+        before = _torch.cuda.current_device() if _torch is not None and _torch.cuda.is_available() else None
         ctx = table[device] = Context(device)
+        if before is not None and before != device:
+            _torch.cuda.set_device(before)
     return ctx
 
 
 class _Call:
     """Where a call's data live, and its context with the right stream."""
+    __slots__ = ("device", "cuda", "ctx", "torch")
 
     def __init__(self, first, ctx):
         if isinstance(first, DeviceArray):
             raise TypeError("a DeviceArray is not taken here: torch tensors or numpy arrays")
-        self.torch = None
-        self.device = None
+        self.device, self.cuda, self.torch = None, False, False
         if is_tensor(first):
-            import torch
-            self.torch = torch
+            if _torch is None:
+                _need_torch()
+            self.torch = True
             self.device = first.device
-        if self.device is not None and self.device.type == "cuda":
+            self.cuda = first.is_cuda
+        if self.cuda:
+            index = self.device.index
             if ctx is None:
-                before = self.torch.cuda.current_device()
-                ctx = _thread_context(self.device.index)
-                if self.torch.cuda.current_device() != before:   # (the first call here makes the context)
-                    self.torch.cuda.set_device(before)
-            elif ctx.device != self.device.index:
-                raise ArrowSpaceError(_lib.AS_ERR_ARG, "tensors of device %d, a context of device %d" % (self.device.index, ctx.device))
-            st = self.torch.cuda.current_stream(self.device).cuda_stream
+                ctx = _thread_context(index)
+            elif ctx.device != index:
+                raise ArrowSpaceError(_lib.AS_ERR_ARG, "tensors of device %d, a context of device %d" % (index, ctx.device))
+            st = _raw_stream(index)
             if getattr(ctx, "_stream", "own") != st:
                 ctx.set_stream(st)
                 ctx._stream = st
@@ -59,21 +74,24 @@ class _Call:
         self.ctx = ctx
 
     def empty(self, shape, dtype):
-        """An output beside the call's inputs; dtype a name."""
-        if self.torch is not None:
-            return self.torch.empty(shape, dtype=getattr(self.torch, dtype), device=self.device)
-        return np.empty(shape, dtype=dtype)
+        """(array, address) of an output beside the call's inputs; dtype a name."""
+        if self.torch:
+            a = _torch.empty(shape, dtype=getattr(_torch, dtype), device=self.device)
+            return a, a.data_ptr()
+        a = np.empty(shape, dtype=dtype)
+        return a, a.ctypes.data
 
     def workspace(self, size):
         """(tensor, address, bytes): torch's own allocator on a GPU, so that a captured graph keeps what it uses; else the library's."""
-        if not size or self.device is None or self.device.type != "cuda":
+        if not size or not self.cuda:
             return None, None, 0
-        w = self.torch.empty(size, dtype=self.torch.uint8, device=self.device)
+        w = _torch.empty(size, dtype=_torch.uint8, device=self.device)
         return w, w.data_ptr(), size
 
 
 def _name(a):
-    return str(a.dtype).replace("torch.", "")
+    name = _kinds.get(a.dtype)
+    return name if name is not None else str(a.dtype).replace("torch.", "")
 
 
 def _matrix(a, what):
@@ -139,10 +157,13 @@ def cross_entropy(x, table, targets, bias=None, scale=1.0, ignore_index=-100, ct
     (losses, lse), both float32 of n.  logits = scale * x @ table.T + bias; losses are 0 where targets == ignore_index and where the
     bias (-inf) leaves no item.  The mean over the counted rows is losses.sum() / count."""
     call, (xp, n, xs, tp, v, ts, d, kind, bp, yp), alive = _loss_args(x, table, bias, targets, ctx)
-    losses, lse = call.empty((n,), "float32"), call.empty((n,), "float32")
-    lib, c = call.ctx.lib, call.ctx
+    (losses, op), (lse, lp) = call.empty((n,), "float32"), call.empty((n,), "float32")
+    c = call.ctx
+    lib = c.lib
     ws, wp, wb = call.workspace(lib.as_cross_entropy_workspace(n, v, d, kind, 0))
-    c.check(lib.as_cross_entropy(c.h, xp, n, xs, tp, v, ts, d, kind, bp, yp, int(ignore_index), float(scale), _addr(losses), _addr(lse), wp, wb))
+    rc = lib.as_cross_entropy(c.h, xp, n, xs, tp, v, ts, d, kind, bp, yp, int(ignore_index), float(scale), op, lp, wp, wb)
+    if rc:
+        c.check(rc)
     return losses, lse
 
 
@@ -158,18 +179,18 @@ def cross_entropy_backward(x, table, targets, lse, grad_losses, bias=None, scale
     if lp is None or gp is None:
         raise ArrowSpaceError(_lib.AS_ERR_ARG, "null argument")
     call, (xp, n, xs, tp, v, ts, d, kind, bp, yp), alive = _loss_args(x, table, bias, targets, ctx)
-    gx = call.empty((n, d), _NAMES[kind]) if need_x else None
-    gw = call.empty((v, d), _NAMES[kind]) if need_table else None
-    gb = call.empty((v,), "float32") if need_bias and bp is not None else None
-    lib, c = call.ctx.lib, call.ctx
+    none = (None, None)
+    gx, gxp = call.empty((n, d), _NAMES[kind]) if need_x else none
+    gw, gwp = call.empty((v, d), _NAMES[kind]) if need_table else none
+    gb, gbp = call.empty((v,), "float32") if need_bias and bp is not None else none
+    c = call.ctx
+    lib = c.lib
     ws, wp, wb = call.workspace(lib.as_cross_entropy_workspace(n, v, d, kind, 1))
-    c.check(lib.as_cross_entropy_backward(c.h, xp, n, xs, tp, v, ts, d, kind, bp, yp, int(ignore_index), float(scale), lp, gp, ep, _addr(gx), d,
-                                          _addr(gw), d, _addr(gb), wp, wb))
+    rc = lib.as_cross_entropy_backward(c.h, xp, n, xs, tp, v, ts, d, kind, bp, yp, int(ignore_index), float(scale), lp, gp, ep, gxp, d, gwp, d,
+                                       gbp, wp, wb)
+    if rc:
+        c.check(rc)
     return gx, gw, gb
-
-
-def _addr(a):
-    return None if a is None else a.data_ptr() if is_tensor(a) else a.ctypes.data
 
 
 class Table4:
@@ -248,10 +269,13 @@ class Table4:
         if kind is None or kind == AS_F64:
             raise TypeError("x must be float32, bfloat16 or float16, got %s" % x.dtype)
         call = _Call(first, ctx)
-        out = call.empty((m, self.n_items), _NAMES[kind])
-        lib, c = call.ctx.lib, call.ctx
+        out, op = call.empty((m, self.n_items), _NAMES[kind])
+        c = call.ctx
+        lib = c.lib
         ws, wp, wb = call.workspace(lib.as_table4_workspace(self.h, m, kind))
-        c.check(lib.as_table4_scores(c.h, self.h, p, m, step, kind, _addr(out), self.n_items, wp, wb))
+        rc = lib.as_table4_scores(c.h, self.h, p, m, step, kind, op, self.n_items, wp, wb)
+        if rc:
+            c.check(rc)
         return out[0] if single else out
 
     def __del__(self):

@@ -16,7 +16,7 @@
 // Rounding.  G is rounded to 16 bits in units of the largest coefficient (coef_scale_kernel; f32: two planes, 22 bits): half a
 // step per entry, as the gradients that leave are rounded themselves.  Everything else -- logits, maxima, sums, dX over pieces,
 // dbias -- is f32 or wider.
-#include "table_loss_rows.h"
+#include "table_loss_few.h"
 
 using namespace asx;
 
@@ -209,13 +209,17 @@ struct ImageJobs {
   unsigned int *tops;      // f32: [2] bits of the largest finite magnitude, for everyone behind
   float *parts;            // ... [2][kTopParts] of the workgroups that looked for it
 };
-constexpr uint32_t kTopParts = 512;
 // threads of a workgroup along a row of `quads` groups of four: a power of two
 __device__ __forceinline__ uint32_t along_row(uint32_t quads) { return quads >= 256 ? 256 : quads <= 1 ? 1 : 1u << (32 - __clz(quads - 1)); }
 template <int DT>
 __device__ __forceinline__ f32x4 load_quad(const ImageJob &j, size_t row, uint32_t k) {
-  if (j.quads && k + 4 <= j.d) {
-    if constexpr (DT == AS_F32) return *(const f32x4 *)((const float *)j.src + row * j.stride + k);
+  if constexpr (DT == AS_F32)
+    if (k + 4 <= j.d) {
+      f32x4 x;
+      __builtin_memcpy(&x, (const float *)j.src + row * j.stride + k, 16);  // (16-byte loads need 4-byte alignment)
+      return x;
+    }
+  if (DT != AS_F32 && j.quads && k + 4 <= j.d) {
     const u32x2 w = *(const u32x2 *)((const unsigned short *)j.src + row * j.stride + k);
     f32x4 x;
 #pragma unroll
@@ -232,11 +236,12 @@ __device__ __forceinline__ f32x4 load_quad(const ImageJob &j, size_t row, uint32
   return x;
 }
 // f32: the largest finite magnitude, a part per workgroup
-__global__ __launch_bounds__(256) void top_kernel(ImageJobs jobs) {
+__global__ __launch_bounds__(1024) void top_kernel(ImageJobs jobs) {
   const ImageJob &j = jobs.job[blockIdx.y];
-  __shared__ float s[4];
-  const uint32_t quads = (j.d + 3) / 4, along = along_row(quads), rows = 256 / along;
+  __shared__ float s[16];
+  const uint32_t quads = (j.d + 3) / 4, along = along_row(quads), rows = 1024 / along;
   float m = 0.f;
+#pragma unroll 2
   for (uint64_t r = (uint64_t)blockIdx.x * rows + threadIdx.x / along; r < j.n; r += (uint64_t)gridDim.x * rows)
     for (uint32_t g = threadIdx.x % along; g < quads; g += along) {
       const f32x4 x = load_quad<AS_F32>(j, r, g * 4);
@@ -247,7 +252,10 @@ __global__ __launch_bounds__(256) void top_kernel(ImageJobs jobs) {
   for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x == 0) jobs.parts[blockIdx.y * kTopParts + blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) m = fmaxf(m, s[w]);
+    jobs.parts[blockIdx.y * kTopParts + blockIdx.x] = m;
+  }
 }
 template <int DT, int FMT>
 __global__ __launch_bounds__(256) void image_kernel(ImageJobs jobs) {
@@ -255,15 +263,9 @@ __global__ __launch_bounds__(256) void image_kernel(ImageJobs jobs) {
   const ImageJob &j = jobs.job[blockIdx.y];
   float f = 1.f;
   if constexpr (two) {
-    __shared__ float s[4];
-    const float *p = jobs.parts + blockIdx.y * kTopParts;
-    float m = fmaxf(p[threadIdx.x], p[threadIdx.x + 256]);
-    for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    f = plane_scale(__float_as_uint(m));
-    if (blockIdx.x == 0 && threadIdx.x == 0) jobs.tops[blockIdx.y] = __float_as_uint(m);
+    const unsigned int top = top_of_parts(jobs.parts + blockIdx.y * kTopParts);
+    f = plane_scale(top);
+    if (blockIdx.x == 0 && threadIdx.x == 0) jobs.tops[blockIdx.y] = top;
   }
   const uint32_t quads = j.pitch / 4, along = along_row(quads), rows = 256 / along;
   for (uint64_t r = (uint64_t)blockIdx.x * rows + threadIdx.x / along; r < j.n; r += (uint64_t)gridDim.x * rows)
@@ -274,34 +276,6 @@ __global__ __launch_bounds__(256) void image_kernel(ImageJobs jobs) {
       if constexpr (two) *(u32x2 *)(o + j.pitch) = u32x2{pack2<FMT>(low_part(x[0]), low_part(x[1])), pack2<FMT>(low_part(x[2]), low_part(x[3]))};
     }
 }
-// The unit the gradient of the logits is rounded in: the largest |grad_losses|, so that the entry of a target, -grad_losses (1 - p), is
-// a whole number of steps where all rows weigh the same (the mean of the losses: without this every such entry is off by the SAME
-// part of 2^-9 in bf16, which no sum averages out).  f16: 2^14 of these units, entries down to 2^-28 of one keep all 11 bits.
-// Where grad_lse outweighs grad_losses the largest of their sum.  One workgroup; 16 bytes a row.
-__global__ __launch_bounds__(1024) void coef_scale_kernel(const float *gl, const float *ge, const int64_t *targets, int64_t ignore, uint32_t n, int power, float *out) {
-  __shared__ float s[2][16];
-  float one = 0.f, both = 0.f;
-  for (uint32_t t = threadIdx.x; t < n; t += 1024) {
-    const float l = targets[t] == ignore ? 0.f : gl[t], b = fabsf(l + (ge ? ge[t] : 0.f)), o = fabsf(l);
-    if (o < INFINITY) one = fmaxf(one, o);
-    if (b < INFINITY) both = fmaxf(both, b);
-  }
-  for (int k = 1; k < 64; k <<= 1) {
-    one = fmaxf(one, __shfl_xor(one, k));
-    both = fmaxf(both, __shfl_xor(both, k));
-  }
-  if ((threadIdx.x & 63) == 0) s[0][threadIdx.x >> 6] = one, s[1][threadIdx.x >> 6] = both;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 16; ++w) one = fmaxf(one, s[0][w]), both = fmaxf(both, s[1][w]);
-    float m = both <= 2.f * one ? one : both;
-    if (!(m >= 1e-36f && m <= 1e36f)) m = 1.f;   // (nothing to scale, or nothing that a factor brings into range)
-    const float unit = m * __uint_as_float((unsigned int)(127 - power) << 23);
-    out[0] = 1.f / unit;
-    out[1] = unit;
-  }
-}
-
 // ---- gradient of the logits ---------------------------------------------------------------------------------------------------------------
 struct GradArgs {
   LossArgs l;
@@ -612,11 +586,13 @@ __global__ __launch_bounds__(FEW ? 256 : 1024) void grad_rows_join_kernel(const 
         for (uint32_t p = lo; p < hi; ++p) x += sums[p * total + i];
       }
       s[w][lane] = x;
+      const uint64_t t = i / pitch, k = i - t * pitch;
+      const bool mine = w == 0 && i < total && k < d;
+      const float extra = mine && rest ? more(t, k) : 0.f;  // (under way while the others add up)
       __syncthreads();
-      if (w == 0 && i < total) {
-        for (int k = 1; k < 16; ++k) x += s[k][lane];
-        const uint64_t t = i / pitch, k = i % pitch;
-        if (k < d) store_from_f32<DT>(out, t * out_stride + k, (rest ? x + more(t, k) : x) * f);
+      if (mine) {
+        for (int o = 1; o < 16; ++o) x += s[o][lane];
+        store_from_f32<DT>(out, t * out_stride + k, (x + extra) * f);
       }
       __syncthreads();
     }
@@ -662,7 +638,7 @@ struct Source {
   bool direct() const { return dt != AS_F32 && d == whole && stride % 8 == 0 && ((uintptr_t)p & 15) == 0; }
   uint32_t pitch() const { return whole; }
   uint32_t planes() const { return dt == AS_F32 ? 2 : 1; }
-  uint64_t image_elems() const { return direct() ? 0 : (uint64_t)rows * pitch() * planes(); }
+  uint64_t image_elems(bool raw) const { return direct() || raw ? 0 : (uint64_t)rows * pitch() * planes(); }
 };
 int image_format(int dt) { return dt == AS_BF16 ? AS_BF16 : AS_F16; }
 
@@ -676,6 +652,7 @@ int product_tile(uint32_t m, uint32_t n) { return n <= 64 ? kSlim : n <= 128 || 
 
 struct Plan {
   uint32_t n, v, d, planes, steps, pitch, parts;
+  int dt;
   int rows_tiles;  // forward for short rows: tiles of 16 rows a wave, 0: the tiled form
   int tile;
   uint32_t n_tiles, v_tiles, per, chunks;
@@ -683,12 +660,15 @@ struct Plan {
   uint32_t piece, pieces, splits;
   int tile_w, tile_x;
   int fused;                 // steps of 32 columns of the form for short rows (table_loss_rows.h), 0: through G in memory
-  uint32_t x_blocks, w_blocks, n_pad;
+  int few;                   // steps of 32 columns a wave of the form for few rows (table_loss_few.h), 0: not taken
+  uint32_t few_groups;       // its workgroups
+  bool raw;                  // ... reads the matrices as they are where they cannot be operands at once (else images are made)
+  uint32_t x_blocks, w_blocks, w_splits, n_pad;
   bool want_x, want_w, want_b;
 };
 Plan make_plan(uint32_t n, uint32_t v, uint32_t d, int dt) {
   Plan p{};
-  p.n = n, p.v = v, p.d = d;
+  p.n = n, p.v = v, p.d = d, p.dt = dt;
   p.planes = dt == AS_F32 ? 2 : 1;
   p.steps = cdiv(d, 64);
   p.pitch = p.steps * 64;
@@ -736,17 +716,38 @@ int fused_steps(uint32_t d, uint32_t planes) { return d <= 64 ? 2 : d <= 128 ? 4
 // 128 values 2 x 3 515 / 439, 3 x 2 490 / 480, 4 x 2 728 / 632 (spills); 256 values 1 x 2 1 273 / 1 262, 2 x 2 1 437 / 1 410 (spills)
 constexpr int fused_rows(int steps, int planes, bool items) { return planes == 2 ? 2 : steps == 8 ? 1 : steps == 2 || items ? 3 : 2; }
 constexpr int fused_waves(int steps, int planes, bool items) { return planes == 2 || steps == 8 ? 2 : steps == 2 || !items ? 3 : 2; }
+// The form for few rows: 16 (forward in 16 bits 64) rows, as many columns as four waves hold.  Waves a SIMD: what its registers leave.
+int few_steps(uint32_t n, uint32_t d, bool forward, int dt) {
+  if (d > 1024 || n > (forward && dt != AS_F32 ? 64u : 16u)) return 0;
+  const int kc = (int)cdiv(d, 128);
+  return kc <= 2 ? kc : kc <= 4 ? 4 : kc <= 6 ? 6 : 8;
+}
+constexpr int few_waves(int steps, bool f32, int tiles) { return f32 ? (steps <= 2 ? 2 : 1) : steps * tiles <= 4 ? 4 : steps * tiles <= 8 ? 2 : steps * tiles <= 16 ? 2 : 1; }
+uint32_t few_groups(int steps, bool f32, int tiles, uint32_t v) { return std::max(1u, std::min((uint32_t)few_waves(steps, f32, tiles) * kChips, cdiv(v, 16))); }
+// An image is read and written once more than the matrix itself; reading the matrix as it is costs each workgroup that walks it the
+// splitting or shifting of its pieces.  Step of 512 f32 rows of 128, 100 000 items: images 295 us, as they are 315; of 777 rows of 200
+// (f16, odd stride), 31 013 items: 171 and 198; one or two blocks of rows: the images would be a third of the time.
+bool raw_pays(const Plan &p) { return p.n <= 128; }
 void plan_backward(Plan &p, bool x, bool w, bool b) {
   p.want_x = x, p.want_w = w, p.want_b = b;
+  p.few = few_steps(p.n, p.d, false, p.dt);
+  if (p.few) {
+    p.few_groups = p.splits = few_groups(p.few, p.planes == 2, 2, p.v);
+    p.n_pad = 64;
+    p.w_splits = 1;
+    return;
+  }
   p.fused = fused_steps(p.d, p.planes);
   if (p.fused) {
     const uint32_t stages = cdiv(p.v, 64), groups = fused_waves(p.fused, p.planes, false) * kChips;
     p.pitch = p.fused * 32;
+    p.raw = raw_pays(p);
     p.x_blocks = cdiv(p.n, 64 * fused_rows(p.fused, p.planes, false));
     p.w_blocks = cdiv(p.v, 64 * fused_rows(p.fused, p.planes, true));
     p.n_pad = up(p.n, 64);
-    // the items in parts, so that the workgroups are there that a compute unit holds
+    // the items in parts, so that the workgroups are there that a compute unit holds; the batch too, where the table is short
     p.splits = std::max(1u, std::min(groups / std::min(p.x_blocks, groups), stages));
+    p.w_splits = std::max(1u, std::min(groups / std::min(p.w_blocks, groups), cdiv(p.n, 256)));
     return;
   }
   const uint32_t bm = kShape[p.tile].bm, bn = kShape[p.tile].bn;
@@ -772,11 +773,19 @@ void plan_backward(Plan &p, bool x, bool w, bool b) {
 
 // waves a SIMD of the forward (1 024 rows x 1 M items of 128: four tiles of rows x 2 waves 293 us, x 3 282, two x 4 316)
 constexpr int sums_waves(int steps, int planes, int tiles) { return steps * planes == 8 || tiles < 4 ? 2 : steps * planes == 4 ? 3 : 4; }
-void plan_forward(Plan &p) {
+void plan_forward(Plan &p, bool direct) {
   p.fused = fused_steps(p.d, p.planes);
+  // (rows that are operands as they lie go by whole stages: a pass at 6.4 TB/s)
+  p.few = direct && p.fused ? 0 : few_steps(p.n, p.d, true, p.dt);
+  if (p.few) {
+    p.fused = 0;
+    p.few_groups = p.parts = few_groups(p.few, p.planes == 2, p.n <= 16 ? 1 : 4, p.v);
+    return;
+  }
   if (p.fused) {
     p.pitch = p.fused * 32;
     p.rows_tiles = p.n <= 64 ? 1 : p.n <= 128 ? 2 : 4;
+    p.raw = raw_pays(p);
     p.x_blocks = cdiv(p.n, 64 * p.rows_tiles);
     // few rows: the pass over the table is all there is, four workgroups a compute unit keep it in flight
     const uint32_t groups = (p.rows_tiles == 1 ? 4 : sums_waves(p.fused, p.planes, p.rows_tiles)) * kChips;
@@ -798,9 +807,9 @@ uint64_t forward_layout(const Plan &p, const Source &x, const Source &t, char *b
   Layout l{base};
   s.part = l.take<float2>((uint64_t)p.parts * p.n);
   s.tops = l.take<unsigned int>(2);
-  s.top_parts = l.take<float>(p.planes == 2 ? 2 * kTopParts : 0);
-  s.x_image = l.take<unsigned short>(x.image_elems());
-  s.t_image = l.take<unsigned short>(t.image_elems());
+  s.top_parts = l.take<float>(p.planes == 2 && !p.few ? 2 * kTopParts : 0);
+  s.x_image = l.take<unsigned short>(x.image_elems(p.few || (p.fused && p.raw)));
+  s.t_image = l.take<unsigned short>(t.image_elems(p.few || (p.fused && p.raw)));
   return l.at;
 }
 struct BackwardScratch {
@@ -809,7 +818,7 @@ struct BackwardScratch {
   unsigned short *x_image, *t_image, *G;
   u32x2 *met;
   uint32_t *met_count;
-  float *sums, *bias_part;
+  float *sums, *w_sums, *bias_part;
   float *lse, *every, *entry, *rest;
   int *target;
 };
@@ -817,17 +826,19 @@ uint64_t backward_layout(const Plan &p, const Source &x, const Source &t, char *
   Layout l{base};
   const uint64_t pl = p.planes;
   s.tops = l.take<unsigned int>(2);
-  s.top_parts = l.take<float>(p.planes == 2 ? 2 * kTopParts : 0);
+  s.top_parts = l.take<float>(p.planes == 2 && !p.few ? 2 * kTopParts : 0);
   s.coef = l.take<float>(2);
-  s.x_image = l.take<unsigned short>(x.image_elems());
-  s.t_image = l.take<unsigned short>(t.image_elems());
+  s.x_image = l.take<unsigned short>(x.image_elems(p.few || (p.fused && p.raw)));
+  s.t_image = l.take<unsigned short>(t.image_elems(p.few || (p.fused && p.raw)));
   s.lse = l.take<float>(p.n_pad);
   s.every = l.take<float>(p.n_pad);
   s.entry = l.take<float>(p.n_pad);
   s.rest = l.take<float>(p.n_pad);
   s.target = l.take<int>(p.n_pad);
-  if (p.fused) {
+  if (p.fused || p.few) {
     s.sums = l.take<float>(p.want_x ? (uint64_t)p.splits * p.n * up(p.d, 8) : 0);
+    s.w_sums = l.take<float>(p.w_splits > 1 ? (uint64_t)p.w_splits * p.v * up(p.d, 8) : 0);
+    s.bias_part = l.take<float>(p.w_splits > 1 ? (uint64_t)p.w_splits * p.v : 0);
     return l.at;
   }
   s.G = l.take<unsigned short>((uint64_t)p.n_pad * p.piece * pl);
@@ -860,78 +871,101 @@ struct Operands {
   const char *x, *t;
   size_t x_ld, t_ld;
 };
-int make_operands(as_ctx *ctx, const Source &x, const Source &t, unsigned int *tops, float *parts, unsigned short *x_image, unsigned short *t_image, Operands *out) {
+// (raw: the kernels take the matrices as they are, f32 needs the magnitudes only)
+int make_operands(as_ctx *ctx, const Source &x, const Source &t, bool raw, unsigned int *tops, float *parts, unsigned short *x_image, unsigned short *t_image,
+                  Operands *out) {
   ImageJobs jobs{};
   jobs.tops = tops, jobs.parts = parts;
   uint32_t count = 0;
   uint64_t most = 1;
   auto add = [&](const Source &s, unsigned short *image, const char **p, size_t *ld) {
-    if (s.direct()) {
-      *p = (const char *)s.p;
-      *ld = s.stride * 2;
-      return;
-    }
     const size_t es = dtype_size(s.dt);
+    if (s.direct() || raw) {
+      *p = (const char *)s.p;
+      *ld = s.stride * es;
+    } else {
+      *p = (const char *)image;
+      *ld = (size_t)s.pitch() * s.planes() * 2;
+    }
+    if (s.direct() || (raw && s.dt != AS_F32)) return;
     jobs.job[count++] = ImageJob{s.p, s.stride, s.rows, s.d, s.pitch(), (s.stride % 4 == 0 && ((uintptr_t)s.p & (4 * es - 1)) == 0) ? 1 : 0, image};
     most = std::max<uint64_t>(most, (uint64_t)s.rows * s.pitch() / 1024);
-    *p = (const char *)image;
-    *ld = (size_t)s.pitch() * s.planes() * 2;
   };
   add(x, x_image, &out->x, &out->x_ld);
   add(t, t_image, &out->t, &out->t_ld);
   if (!count) return AS_OK;
-  if (x.dt == AS_F32) hipLaunchKernelGGL(top_kernel, dim3(kTopParts, 2), dim3(256), 0, ctx->stream, jobs);
-  by_type(x.dt, [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
-    hipLaunchKernelGGL((image_kernel<DT, DT == AS_BF16 ? AS_BF16 : AS_F16>), dim3((unsigned)std::min<uint64_t>(most, 2048), count), dim3(256), 0, ctx->stream, jobs);
-  });
+  if (x.dt == AS_F32) hipLaunchKernelGGL(top_kernel, dim3(kTopParts, 2), dim3(1024), 0, ctx->stream, jobs);
+  if (!raw)
+    by_type(x.dt, [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      hipLaunchKernelGGL((image_kernel<DT, DT == AS_BF16 ? AS_BF16 : AS_F16>), dim3((unsigned)std::min<uint64_t>(most, 2048), count), dim3(256), 0, ctx->stream, jobs);
+    });
   AS_HIP(ctx, hipGetLastError());
   return AS_OK;
 }
-template <int FMT, int P, int KD, bool ITEMS, bool BIAS>
-void launch_rows_grad(as_ctx *ctx, const LossRowsArgs &a) {
-  constexpr int OUT = P == 2 ? AS_F32 : FMT;
-  hipLaunchKernelGGL((loss_rows_grad_kernel<FMT, P, fused_rows(KD, P, ITEMS), KD, ITEMS, BIAS, OUT, fused_waves(KD, P, ITEMS)>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
+template <class F>
+void by_steps(int dt, bool raw, int steps, F &&f) {  // f(type, raw, steps)
+  constexpr std::integral_constant<int, AS_F32> f32{};
+  constexpr std::integral_constant<int, AS_BF16> bf{};
+  constexpr std::integral_constant<int, AS_F16> hf{};
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  auto by = [&](auto type, auto rw) {
+    if (steps == 2) f(type, rw, std::integral_constant<int, 2>{});
+    else if (steps == 4) f(type, rw, std::integral_constant<int, 4>{});
+    else if constexpr (decltype(type)::value != AS_F32) f(type, rw, std::integral_constant<int, 8>{});
+  };
+  if (dt == AS_F32) raw ? by(f32, yes) : by(f32, no);
+  else if (dt == AS_BF16) raw ? by(bf, yes) : by(bf, no);
+  else raw ? by(hf, yes) : by(hf, no);
 }
 template <bool ITEMS>
-void launch_rows_grad(as_ctx *ctx, int dt, int steps, bool bias, const LossRowsArgs &a) {
-  auto go = [&](auto fmt, auto planes, auto kd) {
-    constexpr int FMT = decltype(fmt)::value, P = decltype(planes)::value, KD = decltype(kd)::value;
-    if (bias) launch_rows_grad<FMT, P, KD, ITEMS, true>(ctx, a);
-    else launch_rows_grad<FMT, P, KD, ITEMS, false>(ctx, a);
-  };
-  constexpr std::integral_constant<int, 1> one{};
-  constexpr std::integral_constant<int, 2> two{};
-  constexpr std::integral_constant<int, 4> four{};
-  constexpr std::integral_constant<int, 8> eight{};
-  constexpr std::integral_constant<int, AS_BF16> bf{};
-  constexpr std::integral_constant<int, AS_F16> hf{};
-  if (dt == AS_F32) steps == 2 ? go(hf, two, two) : go(hf, two, four);
-  else if (dt == AS_BF16) steps == 2 ? go(bf, one, two) : steps == 4 ? go(bf, one, four) : go(bf, one, eight);
-  else steps == 2 ? go(hf, one, two) : steps == 4 ? go(hf, one, four) : go(hf, one, eight);
+void launch_rows_grad(as_ctx *ctx, int dt, bool raw, int steps, bool bias, const LossRowsArgs &a) {
+  by_steps(dt, raw, steps, [&](auto type, auto rw, auto kd) {
+    constexpr int DT = decltype(type)::value, KD = decltype(kd)::value, P = DT == AS_F32 ? 2 : 1, RT = fused_rows(KD, P, ITEMS), W = fused_waves(KD, P, ITEMS);
+    constexpr bool RAW = decltype(rw)::value;
+    if (bias) hipLaunchKernelGGL((loss_rows_grad_kernel<DT, RAW, RT, KD, ITEMS, true, W>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((loss_rows_grad_kernel<DT, RAW, RT, KD, ITEMS, false, W>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
+  });
 }
-template <int FMT, int P, int KD, int RT>
-void launch_rows_sums(as_ctx *ctx, bool general, const LossSumsArgs &a) {
-  const dim3 grid(a.r_blocks * a.splits);
-  if (general) hipLaunchKernelGGL((loss_rows_sums_kernel<FMT, P, RT, KD, true, sums_waves(KD, P, RT)>), grid, dim3(256), 0, ctx->stream, a);
-  else hipLaunchKernelGGL((loss_rows_sums_kernel<FMT, P, RT, KD, false, sums_waves(KD, P, RT)>), grid, dim3(256), 0, ctx->stream, a);
+template <class F>
+void by_few_steps(int dt, int steps, F &&f) {  // f(type, steps)
+  by_type(dt, [&](auto type) {
+    if (steps == 1) f(type, std::integral_constant<int, 1>{});
+    else if (steps == 2) f(type, std::integral_constant<int, 2>{});
+    else if (steps == 4) f(type, std::integral_constant<int, 4>{});
+    else if (steps == 6) f(type, std::integral_constant<int, 6>{});
+    else f(type, std::integral_constant<int, 8>{});
+  });
 }
-void launch_rows_sums(as_ctx *ctx, int dt, int steps, int tiles, bool general, const LossSumsArgs &a) {
-  auto go = [&](auto fmt, auto planes, auto kd) {
-    constexpr int FMT = decltype(fmt)::value, P = decltype(planes)::value, KD = decltype(kd)::value;
-    if (tiles == 1) launch_rows_sums<FMT, P, KD, 1>(ctx, general, a);
-    else if (tiles == 2) launch_rows_sums<FMT, P, KD, 2>(ctx, general, a);
-    else launch_rows_sums<FMT, P, KD, 4>(ctx, general, a);
-  };
-  constexpr std::integral_constant<int, 1> one{};
-  constexpr std::integral_constant<int, 2> two{};
-  constexpr std::integral_constant<int, 4> four{};
-  constexpr std::integral_constant<int, 8> eight{};
-  constexpr std::integral_constant<int, AS_BF16> bf{};
-  constexpr std::integral_constant<int, AS_F16> hf{};
-  if (dt == AS_F32) steps == 2 ? go(hf, two, two) : go(hf, two, four);
-  else if (dt == AS_BF16) steps == 2 ? go(bf, one, two) : steps == 4 ? go(bf, one, four) : go(bf, one, eight);
-  else steps == 2 ? go(hf, one, two) : steps == 4 ? go(hf, one, four) : go(hf, one, eight);
+void launch_few_sums(as_ctx *ctx, const Plan &p, bool general, const LossFewArgs &a) {
+  by_few_steps(p.dt, p.few, [&](auto type, auto kc) {
+    constexpr int DT = decltype(type)::value, KC = decltype(kc)::value;
+    constexpr bool F32 = DT == AS_F32;
+    if (p.n <= 16) {
+      if (general) hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 1, true, few_waves(KC, F32, 1)>), dim3(p.few_groups), dim3(256), 0, ctx->stream, a);
+      else hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 1, false, few_waves(KC, F32, 1)>), dim3(p.few_groups), dim3(256), 0, ctx->stream, a);
+    } else if constexpr (!F32) {
+      if (general) hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 4, true, few_waves(KC, F32, 4)>), dim3(p.few_groups), dim3(256), 0, ctx->stream, a);
+      else hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 4, false, few_waves(KC, F32, 4)>), dim3(p.few_groups), dim3(256), 0, ctx->stream, a);
+    }
+  });
+}
+void launch_few_grad(as_ctx *ctx, const Plan &p, const LossFewArgs &a) {
+  by_few_steps(p.dt, p.few, [&](auto type, auto kc) {
+    constexpr int DT = decltype(type)::value, KC = decltype(kc)::value, W = few_waves(KC, DT == AS_F32, 2);
+    if (a.bias) hipLaunchKernelGGL((loss_few_grad_kernel<DT, KC, true, W>), dim3(p.few_groups), dim3(256), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((loss_few_grad_kernel<DT, KC, false, W>), dim3(p.few_groups), dim3(256), 0, ctx->stream, a);
+  });
+}
+template <int RT>
+void launch_rows_sums(as_ctx *ctx, int dt, bool raw, int steps, bool general, const LossSumsArgs &a) {
+  by_steps(dt, raw, steps, [&](auto type, auto rw, auto kd) {
+    constexpr int DT = decltype(type)::value, KD = decltype(kd)::value, W = sums_waves(KD, DT == AS_F32 ? 2 : 1, RT);
+    constexpr bool RAW = decltype(rw)::value;
+    if (general) hipLaunchKernelGGL((loss_rows_sums_kernel<DT, RAW, RT, KD, true, W>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((loss_rows_sums_kernel<DT, RAW, RT, KD, false, W>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
+  });
 }
 void launch_product(as_ctx *ctx, int fmt, int tile, int out_type, const ProductArgs &p) {
   by_tile(tile, [&](auto k) {
@@ -992,8 +1026,10 @@ int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tabl
   AS_TRY(L.bind(ctx, losses, c.n * 4));
   AS_TRY(S.bind(ctx, lse, c.n * 4));
   Plan p = make_plan((uint32_t)c.n, (uint32_t)c.v, (uint32_t)c.d, c.dt);
-  plan_forward(p);
-  const Source xs{X.p, (size_t)c.x_stride, p.n, p.d, c.dt, p.pitch}, ts{W.p, (size_t)c.table_stride, p.v, p.d, c.dt, p.pitch};
+  const int columns = fused_steps(p.d, p.planes) * 32;
+  auto source = [&](const void *m, uint64_t stride, uint32_t rows, uint32_t whole) { return Source{m, (size_t)stride, rows, p.d, c.dt, whole}; };
+  plan_forward(p, columns && source(X.p, c.x_stride, p.n, columns).direct() && source(W.p, c.table_stride, p.v, columns).direct());
+  const Source xs = source(X.p, c.x_stride, p.n, p.pitch), ts = source(W.p, c.table_stride, p.v, p.pitch);
   ForwardScratch s{};
   Scratch scratch;
   AS_TRY(scratch.open(ctx, workspace, workspace_bytes, forward_layout(p, xs, ts, nullptr, s)));
@@ -1001,20 +1037,26 @@ int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tabl
   ProfScope prof(ctx, "cross_entropy");
   LossArgs a{};
   Operands o{};
-  AS_TRY(make_operands(ctx, xs, ts, s.tops, s.top_parts, s.x_image, s.t_image, &o));
+  if (!p.few) AS_TRY(make_operands(ctx, xs, ts, p.fused && p.raw, s.tops, s.top_parts, s.x_image, s.t_image, &o));
   a.rows = o.x, a.rows_ld = o.x_ld, a.table = o.t, a.table_ld = o.t_ld;
   a.table_plane = a.rows_plane = (size_t)p.pitch * 2;
   a.n = p.n, a.v = p.v, a.steps = p.steps, a.planes = p.planes, a.per = p.per, a.v_tiles = p.v_tiles, a.n_tiles = p.n_tiles, a.chunks = p.chunks;
   a.scale = c.scale, a.bias = (const float *)Bi.p;
   if (p.planes == 2) a.rows_top = s.tops, a.table_top = s.tops + 1;
   const bool general = bias || !(c.scale > 0.f);
-  if (p.fused) {
+  if (p.few) {
+    LossFewArgs r{};
+    r.rows = (const char *)X.p, r.rows_ld = c.x_stride * dtype_size(c.dt), r.table = (const char *)W.p, r.table_ld = c.table_stride * dtype_size(c.dt);
+    r.n = p.n, r.v = p.v, r.d = p.d, r.scale = c.scale, r.bias = a.bias, r.part = s.part;
+    launch_few_sums(ctx, p, general, r);
+  } else if (p.fused) {
     LossSumsArgs r{};
-    r.r = a.rows, r.r_ld = a.rows_ld, r.nr = p.n, r.r_top = a.rows_top;
-    r.k = a.table, r.k_ld = a.table_ld, r.nk = p.v, r.k_top = a.table_top;
-    r.r_plane = r.k_plane = (size_t)p.pitch * 2;
+    r.r = a.rows, r.r_ld = a.rows_ld, r.nr = p.n, r.k = a.table, r.k_ld = a.table_ld, r.nk = p.v, r.d = p.d, r.top_parts = s.top_parts;
     r.r_blocks = p.x_blocks, r.splits = p.splits, r.scale = c.scale, r.bias = a.bias, r.part = s.part;
-    launch_rows_sums(ctx, c.dt, p.fused, p.rows_tiles, general, r);
+    const bool raw = p.raw && !(xs.direct() && ts.direct());
+    if (p.rows_tiles == 1) launch_rows_sums<1>(ctx, c.dt, raw, p.fused, general, r);
+    else if (p.rows_tiles == 2) launch_rows_sums<2>(ctx, c.dt, raw, p.fused, general, r);
+    else launch_rows_sums<4>(ctx, c.dt, raw, p.fused, general, r);
   } else {
     by_tile(p.tile, [&](auto k) {
       constexpr int K = decltype(k)::value;
@@ -1086,41 +1128,75 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   GradArgs g{};
   LossArgs &a = g.l;
   Operands o{};
-  AS_TRY(make_operands(ctx, xs, ts, s.tops, s.top_parts, s.x_image, s.t_image, &o));
+  if (!p.few) AS_TRY(make_operands(ctx, xs, ts, p.fused && p.raw, s.tops, s.top_parts, s.x_image, s.t_image, &o));
   const char *table16 = o.t;
   a.rows = o.x, a.rows_ld = o.x_ld, a.table_ld = o.t_ld;
   const unsigned int *x_top = p.planes == 2 ? s.tops : nullptr, *w_top = p.planes == 2 ? s.tops + 1 : nullptr;
-  hipLaunchKernelGGL(coef_scale_kernel, dim3(1), dim3(1024), 0, ctx->stream, (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p, ignore, p.n,
-                     c.dt == AS_BF16 ? 0 : 14, s.coef);
   AS_HIP(ctx, hipGetLastError());
   const float *coef = s.coef;
   const float *rest = p.planes == 1 ? s.rest : nullptr;
+  const LossRowInputs by_row{X.p, W.p, (size_t)c.x_stride, (size_t)c.table_stride, p.d, p.n, p.n_pad, p.v, (const float *)Bi.p, (const float *)Ls.p,
+                             (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p, ignore, c.scale, c.dt == AS_BF16 || (p.few && c.dt == AS_F32) ? 0 : 14, s.coef, s.lse, s.every,
+                             s.entry, s.rest, s.target, p.fused && p.raw ? s.top_parts : nullptr, s.tops};
+  if (p.n > kFewRows)
+    hipLaunchKernelGGL(coef_scale_kernel, dim3(1), dim3(1024), 0, ctx->stream, by_row.gl, by_row.ge, by_row.targets, ignore, p.n, by_row.power, s.coef);
   by_type(c.dt, [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
-    hipLaunchKernelGGL((loss_rows_kernel<DT, DT == AS_BF16 ? AS_BF16 : AS_F16>), dim3(cdiv(p.n_pad, 4)), dim3(256), 0, ctx->stream, X.p, (size_t)c.x_stride, W.p,
-                       (size_t)c.table_stride, p.d, (const float *)Bi.p, c.scale, (const float *)Ls.p, (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p,
-                       ignore, p.n, p.n_pad, p.v, coef, s.lse, s.every, s.entry, s.target, s.rest);
+    constexpr int DT = decltype(dt)::value, FMT = DT == AS_BF16 ? AS_BF16 : AS_F16;
+    if (p.n > kFewRows) hipLaunchKernelGGL((loss_rows_kernel<DT, FMT, false>), dim3(cdiv(p.n_pad, 4)), dim3(256), 0, ctx->stream, by_row);
+    else hipLaunchKernelGGL((loss_rows_kernel<DT, FMT, true>), dim3(cdiv(p.n_pad, 4)), dim3(256), 0, ctx->stream, by_row);
   });
   AS_HIP(ctx, hipGetLastError());
-  if (p.fused) {
+  // dX from its parts, or dW where the batch was split
+  auto join = [&](const float *sums, uint32_t splits, uint32_t n, const unsigned int *top, bool with_rest, void *out, uint64_t stride) {
+    by_type(c.dt, [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      const uint32_t pitch = up(p.d, 8);
+      const uint64_t total = (uint64_t)n * pitch;
+      const float *r = with_rest ? rest : nullptr;
+      if (splits <= 16)
+        hipLaunchKernelGGL((grad_rows_join_kernel<DT, true>), dim3(spread(total, 1024)), dim3(256), 0, ctx->stream, sums, splits, pitch, n, p.d, c.scale, coef, top,
+                           (const int *)s.target, r, W.p, (size_t)c.table_stride, out, (size_t)stride);
+      else
+        hipLaunchKernelGGL((grad_rows_join_kernel<DT, false>), dim3(spread(total, 64)), dim3(1024), 0, ctx->stream, sums, splits, pitch, n, p.d, c.scale, coef, top,
+                           (const int *)s.target, r, W.p, (size_t)c.table_stride, out, (size_t)stride);
+    });
+  };
+  if (p.few) {
+    LossFewArgs r{};
+    r.rows = (const char *)X.p, r.rows_ld = c.x_stride * dtype_size(c.dt), r.table = (const char *)W.p, r.table_ld = c.table_stride * dtype_size(c.dt);
+    r.n = p.n, r.v = p.v, r.d = p.d, r.scale = c.scale, r.bias = (const float *)Bi.p;
+    r.lse = s.lse, r.every = s.every, r.entry = s.entry, r.rest = s.rest, r.target = s.target, r.coef = coef;
+    r.sums = s.sums, r.sums_pitch = up(p.d, 8), r.want_x = p.want_x;
+    r.out = Ow.p, r.out_stride = gw_stride, r.aligned = gw_stride % 8 == 0 && ((uintptr_t)Ow.p & 15) == 0;
+    r.grad_bias = (float *)Ob.p;
+    launch_few_grad(ctx, p, r);
+    AS_HIP(ctx, hipGetLastError());
+  } else if (p.fused) {
+    const bool raw = p.raw && !(xs.direct() && ts.direct());
     LossRowsArgs r{};
     r.d = p.d, r.scale = c.scale, r.bias = (const float *)Bi.p, r.coef = coef;
     r.lse = s.lse, r.every = s.every, r.entry = s.entry, r.rest = s.rest, r.target = s.target;
-    r.r_plane = r.k_plane = (size_t)p.pitch * 2;
+    r.sums_pitch = up(p.d, 8);
     if (p.want_w || p.want_b) {
-      r.r = table16, r.r_ld = a.table_ld, r.nr = p.v, r.r_top = w_top;
-      r.k = a.rows, r.k_ld = a.rows_ld, r.nk = p.n, r.k_top = x_top;
-      r.r_blocks = p.w_blocks, r.splits = 1;
+      r.r = o.t, r.r_ld = o.t_ld, r.nr = p.v, r.r_top = w_top;
+      r.k = o.x, r.k_ld = o.x_ld, r.nk = p.n, r.k_top = x_top;
+      r.r_blocks = p.w_blocks, r.splits = p.w_splits;
+      if (p.w_splits > 1) r.sums = s.w_sums;
       r.out = Ow.p, r.out_stride = gw_stride, r.aligned = gw_stride % 8 == 0 && ((uintptr_t)Ow.p & 15) == 0;
-      r.grad_bias = (float *)Ob.p;
-      launch_rows_grad<true>(ctx, c.dt, p.fused, bias != nullptr, r);
+      r.grad_bias = !p.want_b ? nullptr : p.w_splits > 1 ? s.bias_part : (float *)Ob.p;
+      launch_rows_grad<true>(ctx, c.dt, raw, p.fused, bias != nullptr, r);
+      if (p.w_splits > 1) {
+        if (p.want_w) join(s.w_sums, p.w_splits, p.v, x_top, false, Ow.p, gw_stride);
+        if (p.want_b)
+          hipLaunchKernelGGL(bias_join_kernel, dim3(cdiv(p.v, 256)), dim3(256), 0, ctx->stream, (const float *)s.bias_part, p.w_splits, p.v, p.v, coef, (float *)Ob.p);
+      }
     }
     if (p.want_x) {
-      r.r = a.rows, r.r_ld = a.rows_ld, r.nr = p.n, r.r_top = x_top;
-      r.k = table16, r.k_ld = a.table_ld, r.nk = p.v, r.k_top = w_top;
+      r.r = o.x, r.r_ld = o.x_ld, r.nr = p.n, r.r_top = x_top;
+      r.k = o.t, r.k_ld = o.t_ld, r.nk = p.v, r.k_top = w_top;
       r.r_blocks = p.x_blocks, r.splits = p.splits;
-      r.sums = s.sums, r.sums_pitch = up(p.d, 8);
-      launch_rows_grad<false>(ctx, c.dt, p.fused, bias != nullptr, r);
+      r.sums = s.sums;
+      launch_rows_grad<false>(ctx, c.dt, raw, p.fused, bias != nullptr, r);
     }
     AS_HIP(ctx, hipGetLastError());
   }
@@ -1132,11 +1208,11 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   g.G = s.G, g.g_pitch = p.piece;
   g.bias_part = p.want_b ? s.bias_part : nullptr;
   const int fmt = image_format(c.dt);
-  if (!p.fused && rest && p.want_w) {
+  if (!p.fused && !p.few && rest && p.want_w) {
     const uint32_t groups = cdiv(p.v, 64);
     hipLaunchKernelGGL(met_kernel, dim3(cdiv(groups, 4)), dim3(256), 0, ctx->stream, (const int *)s.target, p.n, groups, s.met, s.met_count);
   }
-  for (uint32_t v0 = 0; !p.fused && v0 < p.v; v0 += p.piece) {
+  for (uint32_t v0 = 0; !p.fused && !p.few && v0 < p.v; v0 += p.piece) {
     const uint32_t items = std::min(p.piece, p.v - v0);
     a.table = table16 + (size_t)v0 * a.table_ld;
     a.v = items, a.v_tiles = cdiv(items, kShape[p.tile].bm), a.chunks = cdiv(a.v_tiles, p.per);
@@ -1184,17 +1260,7 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
     AS_HIP(ctx, hipGetLastError());
   }
   if (p.want_x) {
-    by_type(c.dt, [&](auto dt) {
-      constexpr int DT = decltype(dt)::value;
-      const uint32_t pitch = up(p.d, 8);
-      const uint64_t total = (uint64_t)p.n * pitch;
-      if (p.splits <= 16)
-        hipLaunchKernelGGL((grad_rows_join_kernel<DT, true>), dim3(spread(total, 1024)), dim3(256), 0, ctx->stream, (const float *)s.sums, p.splits, pitch, p.n, p.d,
-                           c.scale, coef, w_top, (const int *)s.target, rest, W.p, (size_t)c.table_stride, Ox.p, (size_t)gx_stride);
-      else
-        hipLaunchKernelGGL((grad_rows_join_kernel<DT, false>), dim3(spread(total, 64)), dim3(1024), 0, ctx->stream, (const float *)s.sums, p.splits, pitch, p.n, p.d,
-                           c.scale, coef, w_top, (const int *)s.target, rest, W.p, (size_t)c.table_stride, Ox.p, (size_t)gx_stride);
-    });
+    join(s.sums, p.splits, p.n, p.few ? nullptr : w_top, true, Ox.p, gx_stride);
     AS_HIP(ctx, hipGetLastError());
   }
   AS_TRY(Ox.finish(ctx));
@@ -1210,16 +1276,22 @@ extern "C" {
 uint64_t as_cross_entropy_workspace(uint64_t n, uint64_t n_items, uint64_t dim, int dtype, int backward) {
   if (n == 0 || n_items == 0 || dim == 0 || n >= (1ull << 31) || n_items >= (1ull << 31) || dim > 65536 || !dtype_is_training(dtype)) return 0;
   Plan p = make_plan((uint32_t)n, (uint32_t)n_items, (uint32_t)dim, dtype);
-  if (backward) plan_backward(p, true, true, true);
-  else plan_forward(p);
   // (a stride of dim + 1: room for the images whether or not the matrices can be taken as they are)
-  const Source xs{nullptr, (size_t)dim + 1, p.n, p.d, dtype, p.pitch}, ts{nullptr, (size_t)dim + 1, p.v, p.d, dtype, p.pitch};
+  auto source = [&](uint64_t rows) { return Source{nullptr, (size_t)dim + 1, (uint32_t)rows, p.d, dtype, p.pitch}; };
   if (backward) {
+    plan_backward(p, true, true, true);
     BackwardScratch s{};
-    return backward_layout(p, xs, ts, nullptr, s);
+    return backward_layout(p, source(n), source(n_items), nullptr, s);
   }
-  ForwardScratch s{};
-  return forward_layout(p, xs, ts, nullptr, s);
+  // whichever form the alignment leads to
+  uint64_t most = 0;
+  for (bool direct : {false, true}) {
+    p = make_plan((uint32_t)n, (uint32_t)n_items, (uint32_t)dim, dtype);
+    plan_forward(p, direct);
+    ForwardScratch s{};
+    most = std::max(most, forward_layout(p, source(n), source(n_items), nullptr, s));
+  }
+  return most;
 }
 
 int as_cross_entropy(as_ctx *ctx, const void *x, uint64_t n, uint64_t x_stride, const void *table, uint64_t n_items, uint64_t table_stride, uint64_t dim,

@@ -72,9 +72,8 @@ __device__ __forceinline__ float low_part(float x) {  // what f16 leaves of x (n
 
 
 struct LossRowsArgs {
-  const char *r, *k;              // the two sides' rows in 16 bits, whole 64 KD / 2 columns (zeros behind d)
+  const char *r, *k;              // the two sides' rows as they are
   size_t r_ld, k_ld;              // bytes
-  size_t r_plane, k_plane;        // bytes to the low plane (f32)
   uint32_t nr, nk, d;
   uint32_t r_blocks, splits;      // blocks of rows r; parts of the k side (sums: one buffer each)
   float scale;
@@ -84,49 +83,116 @@ struct LossRowsArgs {
   const int *target;
   const float *bias;              // by item, or null
   const float *coef;              // {factor, 1 / factor} of g
-  float *sums;                    // r = batch: f32 [split][nr][sums_pitch]
+  float *sums;                    // f32 [split][nr][sums_pitch] (r = items: where the batch is split), or null
   uint32_t sums_pitch;
-  void *out;                      // r = items: rows of out_stride elements
+  void *out;                      // r = items, not split: rows of out_stride elements, or null
   size_t out_stride;
   int aligned;
-  float *grad_bias;               // r = items: sum over k of g, or null
+  float *grad_bias;               // r = items: sum over k of g (split: [split][nr], in units of coef), or null
 };
+
+// The unit the gradient of the logits is rounded in: the largest |grad_losses|, so that the entry of a target, -grad_losses (1 - p), is
+// a whole number of steps where all rows weigh the same (the mean of the losses: without this every such entry is off by the SAME
+// part of 2^-9 in bf16, which no sum averages out).  f16: 2^14 of these units, entries down to 2^-28 of one keep all 11 bits.
+// Where grad_lse outweighs grad_losses the largest of their sum.  Threads of a workgroup together; 16 bytes a row.
+template <int THREADS>
+__device__ __forceinline__ void unit_of_rows(const float *gl, const float *ge, const int64_t *targets, int64_t ignore, uint32_t n, int power, float *factor, float *unit) {
+  __shared__ float s[2][THREADS / 64];
+  float one = 0.f, both = 0.f;
+  for (uint32_t t = threadIdx.x; t < n; t += THREADS) {
+    const float l = targets[t] == ignore ? 0.f : gl[t], b = fabsf(l + (ge ? ge[t] : 0.f)), o = fabsf(l);
+    if (o < INFINITY) one = fmaxf(one, o);
+    if (b < INFINITY) both = fmaxf(both, b);
+  }
+  for (int k = 1; k < 64; k <<= 1) {
+    one = fmaxf(one, __shfl_xor(one, k));
+    both = fmaxf(both, __shfl_xor(both, k));
+  }
+  if ((threadIdx.x & 63) == 0) s[0][threadIdx.x >> 6] = one, s[1][threadIdx.x >> 6] = both;
+  __syncthreads();
+  for (int w = 0; w < THREADS / 64; ++w) one = fmaxf(one, s[0][w]), both = fmaxf(both, s[1][w]);
+  float m = both <= 2.f * one ? one : both;
+  if (!(m >= 1e-36f && m <= 1e36f)) m = 1.f;   // (nothing to scale, or nothing that a factor brings into range)
+  *unit = m * __uint_as_float((unsigned int)(127 - power) << 23);
+  *factor = 1.f / *unit;
+}
+__global__ __launch_bounds__(1024) void coef_scale_kernel(const float *gl, const float *ge, const int64_t *targets, int64_t ignore, uint32_t n, int power, float *out) {
+  float factor, unit;
+  unit_of_rows<1024>(gl, ge, targets, ignore, n, power, &factor, &unit);
+  if (threadIdx.x == 0) out[0] = factor, out[1] = unit;
+}
+
+// f32: the largest finite magnitude of a matrix, a part per workgroup (its bits order as integers; a maximum has no order)
+constexpr uint32_t kTopParts = 256;
+__device__ __forceinline__ unsigned int top_of_parts(const float *parts) {  // 256 threads or more
+  __shared__ float s[4];
+  float m = threadIdx.x < kTopParts ? parts[threadIdx.x] : 0.f;
+  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+  __syncthreads();
+  if (threadIdx.x < kTopParts && (threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+  __syncthreads();
+  return __float_as_uint(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+}
 
 // By row of the batch, a wave each: the coefficient of its probabilities, and its entry at its target.  That entry is most of a row's
 // gradient and often all of its item's, so it comes from a product in f64, the kernels put it in place of their own, and what 16 bits
 // leave of it (`rest`, as much as the rounding of the result) is added in f32: to dX where its parts are joined, to dW behind the
-// product.  coef: {factor, 1 / factor} of g.
-template <int DT, int FMT>
-__global__ __launch_bounds__(256) void loss_rows_kernel(const void *x, size_t x_stride, const void *table, size_t table_stride, uint32_t d, const float *bias,
-                                                        float scale, const float *lse, const float *gl, const float *ge, const int64_t *targets, int64_t ignore,
-                                                        uint32_t n, uint32_t padded, uint32_t v, const float *coef, float *o_lse, float *o_every, float *o_entry,
-                                                        int *o_target, float *o_rest) {
+// product.  coef: {factor, 1 / factor} of g, made here where FEW (up to kFewRows rows, every workgroup for itself).
+constexpr uint32_t kFewRows = 1024;
+struct LossRowInputs {
+  const void *x, *table;
+  size_t x_stride, table_stride;
+  uint32_t d, n, padded, v;
+  const float *bias, *lse, *gl, *ge;
+  const int64_t *targets;
+  int64_t ignore;
+  float scale;
+  int power;
+  float *coef;
+  float *o_lse, *o_every, *o_entry, *o_rest;
+  int *o_target;
+  const float *top_parts;  // f32: parts of the two matrices' largest magnitudes, and where their bits go
+  unsigned int *tops;
+};
+template <int DT, int FMT, bool FEW>
+__global__ __launch_bounds__(256) void loss_rows_kernel(LossRowInputs a) {
   const uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (t >= padded) return;
+  float f, unit;
+  if constexpr (FEW) {
+    unit_of_rows<256>(a.gl, a.ge, a.targets, a.ignore, a.n, a.power, &f, &unit);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.coef[0] = f, a.coef[1] = unit;
+  } else {
+    f = a.coef[0];
+  }
+  if (DT == AS_F32 && blockIdx.x == 0 && a.top_parts) {
+    const unsigned int x_top = top_of_parts(a.top_parts), t_top = top_of_parts(a.top_parts + kTopParts);
+    if (threadIdx.x == 0) a.tops[0] = x_top, a.tops[1] = t_top;
+  }
+  if (t >= a.padded) return;
   float s = INFINITY, every = 0.f, entry = 0.f;   // (behind the last row: probability 0)
   int at = -1;
-  if (t < n && lse[t] != -INFINITY) {  // (-inf: the bias left no item, no gradient)
-    const float f = coef[0];
-    const int64_t y = targets[t];
+  if (t < a.n && a.lse[t] != -INFINITY) {  // (-inf: the bias left no item, no gradient)
+    const int64_t y = a.targets[t];
     float one = 0.f;
-    s = lse[t];
-    if (y != ignore && y >= 0 && y < (int64_t)v) {
+    s = a.lse[t];
+    if (y != a.ignore && y >= 0 && y < (int64_t)a.v) {
       at = (int)y;
-      one = gl[t] * f;
+      one = a.gl[t] * f;
     }
-    every = one + (ge ? ge[t] * f : 0.f);
+    every = one + (a.ge ? a.ge[t] * f : 0.f);
     if (at >= 0) {
       double dot = 0.0;
-      for (uint32_t k = lane; k < d; k += 64)
-        dot += (double)load_as_f32<DT>(x, (size_t)t * x_stride + k) * (double)load_as_f32<DT>(table, (size_t)y * table_stride + k);
+#pragma unroll 4
+      for (uint32_t k = lane; k < a.d; k += 64)
+        dot += (double)load_as_f32<DT>(a.x, (size_t)t * a.x_stride + k) * (double)load_as_f32<DT>(a.table, (size_t)y * a.table_stride + k);
       for (int k = 1; k < 64; k <<= 1) dot += __shfl_xor(dot, k);
-      const double z = (double)scale * dot + (bias ? (double)bias[y] : 0.0) - (double)s;
+      const double z = (double)a.scale * dot + (a.bias ? (double)a.bias[y] : 0.0) - (double)s;
       entry = (float)((double)every * exp(z) - (double)one);
     }
   }
   if (lane == 0) {
-    o_lse[t] = s, o_every[t] = every, o_entry[t] = entry, o_target[t] = at;
-    o_rest[t] = DT == AS_F32 || !__builtin_isfinite(entry) ? 0.f : entry - rounded16<FMT>(entry);
+    a.o_lse[t] = s, a.o_every[t] = every, a.o_entry[t] = entry, a.o_target[t] = at;
+    a.o_rest[t] = DT == AS_F32 || !__builtin_isfinite(entry) ? 0.f : entry - rounded16<FMT>(entry);
   }
 }
 
@@ -135,6 +201,17 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(const void *x, size_t x_
 // the dX of 1 024 rows against a million items; this form: see the kernel).
 typedef short short4v __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ u32x4 lr_row(const char *smem, uint32_t at) { return *(const u32x4 *)(smem + at); }
+// four rows of this lane's column, transposed
+__device__ __forceinline__ u32x2 lr_column4(const char *smem, uint32_t at) {
+  typedef __attribute__((address_space(3))) short4v lds_short4;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(smem + at)));
+}
+// LDS written and read by one wave only: the hardware keeps its operations in order, the compiler is told to
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
 // rows 0 .. 3 and 4 .. 7 (`half` bytes on) of this lane's column, transposed
 __device__ __forceinline__ u32x4 lr_column(const char *smem, uint32_t at, uint32_t half) {
   typedef __attribute__((address_space(3))) short4v lds_short4;
@@ -142,32 +219,119 @@ __device__ __forceinline__ u32x4 lr_column(const char *smem, uint32_t at, uint32
   const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(smem + at + half)));
   return u32x4{x[0], x[1], y[0], y[1]};
 }
+// Eight consecutive values of a row, as the matrix holds them (columns behind the row's d: zeros) and as 16-bit operands.  RAW: rows of
+// any alignment and length (16-byte loads need 4-byte alignment and 16-bit ones less; a piece that sticks out of its row is read 8
+// values before the row's end and shifted); else whole 16-byte pieces, f32 as images of two planes.
+template <int DT, bool RAW>
+struct LrPiece {
+  u32x4 w[DT == AS_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const char *row, uint32_t column, uint32_t d, uint32_t plane) {
+    if constexpr (!RAW) {
+      w[0] = *(const u32x4 *)(row + column * 2);
+      if constexpr (DT == AS_F32) w[1] = *(const u32x4 *)(row + plane + column * 2);
+    } else if constexpr (DT == AS_F32) {
+      const float *p = (const float *)row;
+      if (d < 4) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e >> 2][e & 3] = column + e < d ? __float_as_uint(p[column + e]) : 0u;
+        return;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t c = column + 4 * h, at = c + 4 <= d ? c : d - 4;
+        u32x4 x;
+        __builtin_memcpy(&x, p + at, 16);
+        if (d & 3) {  // (uniform)
+          const uint32_t s = c - at;
+          x = s == 1 ? u32x4{x[1], x[2], x[3], 0u} : s == 2 ? u32x4{x[2], x[3], 0u, 0u} : s == 3 ? u32x4{x[3], 0u, 0u, 0u} : x;
+        }
+        w[h] = c < d ? x : u32x4{0u, 0u, 0u, 0u};
+      }
+    } else {
+      const unsigned short *p = (const unsigned short *)row;
+      if (d < 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[0][e] = (column + 2 * e < d ? (uint32_t)p[column + 2 * e] : 0u) | (column + 2 * e + 1 < d ? (uint32_t)p[column + 2 * e + 1] << 16 : 0u);
+        return;
+      }
+      const uint32_t at = column + 8 <= d ? column : d - 8;
+      u32x4 x;
+      __builtin_memcpy(&x, p + at, 16);
+      if (d & 7) {  // (uniform)
+        const uint32_t s = column < d ? (column - at) * 16 : 0;
+        uint64_t lo = (uint64_t)x[0] | (uint64_t)x[1] << 32, hi = (uint64_t)x[2] | (uint64_t)x[3] << 32;
+        if (s >= 64) lo = hi, hi = 0;
+        const uint32_t r = s & 63;
+        lo = lo >> r | (r ? hi << (64 - r) : 0);
+        hi >>= r;
+        x = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+      }
+      w[0] = column < d ? x : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+  // f32: the high and the low plane of the values times `scale`
+  template <int FMT, int P>
+  __device__ __forceinline__ void planes(float scale, u32x4 (&o)[P]) const {
+    if constexpr (DT == AS_F32 && !RAW) {
+      o[0] = w[0], o[P - 1] = w[1];
+    } else if constexpr (DT == AS_F32) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = __uint_as_float(w[e >> 1][2 * (e & 1)]) * scale, y = __uint_as_float(w[e >> 1][2 * (e & 1) + 1]) * scale;
+        o[0][e] = pack2<FMT>(x, y);
+        if constexpr (P == 2) o[P - 1][e] = pack2<FMT>(low_part(x), low_part(y));
+      }
+    } else {
+      o[0] = w[0];
+    }
+  }
+};
 // A stage of 64 rows of the k side, P planes of 64 KD bytes a row: 16-byte piece c of row r at place c ^ swizzle(r), so that a fragment
 // read (8 rows) and a transposed read (4 rows) spread over the banks
-template <int P, int KD>
+template <int FMT, int P, int KD, int DT, bool RAW>
 struct LrStage {
   static constexpr uint32_t kRow = KD * 64, kPlane = 64 * kRow;
-  u32x4 piece[P][KD];
+  LrPiece<DT, RAW> piece[KD];
   __device__ __forceinline__ static uint32_t swizzle(uint32_t row) {
     const uint32_t key = (row & 3) | ((row >> 1) & 4);
     return KD >= 4 ? key << 1 : key;
   }
-  __device__ __forceinline__ void load(const char *k, size_t ld, size_t plane, uint32_t nk, uint32_t s) {
+  __device__ __forceinline__ void load(const char *k, size_t ld, uint32_t d, uint32_t nk, uint32_t s) {
 #pragma unroll
     for (int t = 0; t < KD; ++t) {
       const uint32_t idx = t * 256 + threadIdx.x, row = idx / (KD * 4), slot = idx % (KD * 4);
-      const char *src = k + (size_t)nt_min(s * 64 + row, nk - 1) * ld + ((slot ^ swizzle(row)) << 4);
-#pragma unroll
-      for (int p = 0; p < P; ++p) piece[p][t] = *(const u32x4 *)(src + p * plane);
+      piece[t].load(k + (size_t)nt_min(s * 64 + row, nk - 1) * ld, (slot ^ swizzle(row)) * 8, d, kRow);
     }
   }
-  __device__ __forceinline__ void store(char *dst) const {
+  __device__ __forceinline__ void store(char *dst, float scale) const {
 #pragma unroll
-    for (int p = 0; p < P; ++p)
+    for (int t = 0; t < KD; ++t) {
+      u32x4 o[P];
+      piece[t].template planes<FMT, P>(scale, o);
 #pragma unroll
-      for (int t = 0; t < KD; ++t) *(u32x4 *)(dst + p * kPlane + (t * 256 + threadIdx.x) * 16) = piece[p][t];
+      for (int p = 0; p < P; ++p) *(u32x4 *)(dst + p * kPlane + (t * 256 + threadIdx.x) * 16) = o[p];
+    }
   }
 };
+// a wave's 16 RT rows as operands, from row r0 (rows behind the last: the last)
+template <int FMT, int P, int RT, int KD, int DT, bool RAW>
+__device__ __forceinline__ void lr_rows(u32x4 (&R)[P][RT][KD], const char *rows, size_t ld, uint32_t r0, uint32_t nr, uint32_t d, float scale) {
+  const uint32_t lane = threadIdx.x & 63, q = lane >> 4, col = lane & 15;
+#pragma unroll
+  for (int j = 0; j < RT; ++j) {
+    const char *row = rows + (size_t)nt_min(r0 + j * 16 + col, nr - 1) * ld;
+#pragma unroll
+    for (int s = 0; s < KD; ++s) {
+      LrPiece<DT, RAW> piece;
+      piece.load(row, s * 32 + q * 8, d, KD * 64);
+      u32x4 o[P];
+      piece.template planes<FMT, P>(scale, o);
+#pragma unroll
+      for (int p = 0; p < P; ++p) R[p][j][s] = o[p];
+    }
+  }
+}
 
 // ---- forward for short rows -----------------------------------------------------------------------------------------------------------------
 // The same walk with only the statistics behind it: rows in registers, items in stages of 64, a running maximum and sum of exponentials
@@ -175,17 +339,18 @@ struct LrStage {
 // exp, add) some 26, so what is saved counts: the maximum that the exponentials are taken against moves only when it is exceeded
 // by 2^20, once per walk in practice, and the rescaling with it.
 struct LossSumsArgs {
-  const char *r, *k;
-  size_t r_ld, k_ld, r_plane, k_plane;
-  uint32_t nr, nk, r_blocks, splits;
+  const char *r, *k;              // the batch and the table as they are
+  size_t r_ld, k_ld;              // bytes
+  uint32_t nr, nk, d, r_blocks, splits;
   float scale;
-  const unsigned int *r_top, *k_top;
+  const float *top_parts;         // f32: of the two matrices' largest magnitudes
   const float *bias;
   float2 *part;  // [split][nr] (maximum, sum of exponentials against it)
 };
-template <int FMT, int P, int RT, int KD, bool GENERAL, int WAVES>
+template <int DT, bool RAW, int RT, int KD, bool GENERAL, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs a) {
-  typedef LrStage<P, KD> Stage;
+  constexpr int FMT = DT == AS_BF16 ? AS_BF16 : AS_F16, P = DT == AS_F32 ? 2 : 1;
+  typedef LrStage<FMT, P, KD, DT, RAW> Stage;
   constexpr uint32_t kRow = Stage::kRow, kPlane = Stage::kPlane, kExtra = GENERAL ? 256 : 0, kStage = P * kPlane + kExtra;
   __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, col = lane & 15;
@@ -194,28 +359,29 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs
   const uint32_t r0 = (rb * 4 + wave) * (16 * RT);
   const uint32_t stages = (a.nk + 63) / 64;
   const uint32_t s_lo = (uint32_t)((uint64_t)stages * split / a.splits), s_hi = (uint32_t)((uint64_t)stages * (split + 1) / a.splits);
-  const float nat = a.scale * (P == 2 ? 1.f / plane_scale(*a.r_top) / plane_scale(*a.k_top) : 1.f);
+  float r_scale = 1.f, k_scale = 1.f;
+  if constexpr (P == 2) {
+    r_scale = plane_scale(top_of_parts(a.top_parts));
+    k_scale = plane_scale(top_of_parts(a.top_parts + kTopParts));
+  }
+  const float nat = a.scale * (P == 2 ? 1.f / r_scale / k_scale : 1.f);
   const float unit = GENERAL ? kLog2e : nat * kLog2e, slack = fminf(20.f / unit, 1e30f);
   Stage stage;
   float extra = 0.f;
   auto load = [&](uint32_t s) {
-    stage.load(a.k, a.k_ld, a.k_plane, a.nk, s);
+    stage.load(a.k, a.k_ld, a.d, a.nk, s);
     if (GENERAL && a.bias && threadIdx.x < 64) extra = a.bias[nt_min(s * 64 + threadIdx.x, a.nk - 1)];
   };
   auto store = [&](int buf) {
-    stage.store(smem + buf * kStage);
+    stage.store(smem + buf * kStage, k_scale);
     if (GENERAL && threadIdx.x < 64) *(float *)(smem + buf * kStage + P * kPlane + threadIdx.x * 4) = extra;
   };
   if (s_lo < s_hi) load(s_lo);
   u32x4 R[P][RT][KD];
+  lr_rows<FMT, P, RT, KD, DT, RAW>(R, a.r, a.r_ld, r0, a.nr, a.d, r_scale);
   float ref[RT], base[RT], sum[RT];
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
-    const uint32_t row = nt_min(r0 + j * 16 + col, a.nr - 1);
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int s = 0; s < KD; ++s) R[p][j][s] = *(const u32x4 *)(a.r + (size_t)row * a.r_ld + p * a.r_plane + s * 64 + q * 16);
     ref[j] = -INFINITY;
     base[j] = sum[j] = 0.f;
   }
@@ -306,11 +472,12 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs
   }
 }
 
-// FMT the operands' type; P planes; RT tiles of 16 rows r a wave; KD steps of 32 columns; ITEMS: the rows r are items (dW), else the
-// batch (dX); OUT: type of dW
-template <int FMT, int P, int RT, int KD, bool ITEMS, bool BIAS, int OUT, int WAVES>
+// DT, RAW: the matrices (LrPiece); RT tiles of 16 rows r a wave; KD steps of 32 columns; ITEMS: the rows r are items (dW), else the
+// batch (dX)
+template <int DT, bool RAW, int RT, int KD, bool ITEMS, bool BIAS, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs a) {
-  typedef LrStage<P, KD> Stage;
+  constexpr int FMT = DT == AS_BF16 ? AS_BF16 : AS_F16, P = DT == AS_F32 ? 2 : 1, OUT = DT;
+  typedef LrStage<FMT, P, KD, DT, RAW> Stage;
   constexpr uint32_t kRow = Stage::kRow, kPlane = Stage::kPlane, kExtra = 1024, kStage = P * kPlane + kExtra;
   constexpr bool FAST = !BIAS && P == 1;  // 16-bit gradients: the exponent in one multiply-add (its constants are rounded: 2e-6 of the probability)
   __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
@@ -320,7 +487,8 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
   const uint32_t r0 = (rb * 4 + wave) * (16 * RT);
   const uint32_t stages = (a.nk + 63) / 64;
   const uint32_t s_lo = (uint32_t)((uint64_t)stages * split / a.splits), s_hi = (uint32_t)((uint64_t)stages * (split + 1) / a.splits);
-  const float nat = a.scale * (P == 2 ? 1.f / plane_scale(*a.r_top) / plane_scale(*a.k_top) : 1.f);
+  const float r_scale = P == 2 ? plane_scale(*a.r_top) : 1.f, k_scale = P == 2 ? plane_scale(*a.k_top) : 1.f;
+  const float nat = P == 2 ? a.scale / r_scale / k_scale : a.scale;
   const float c = FAST ? nat * kLog2e : nat;
   constexpr uint32_t kList = 64;  // (items that more rows meet than that are sums of many entries, whose roundings average out)
   __shared__ u32x2 list[ITEMS && P == 1 ? 4 : 1][kList];
@@ -330,26 +498,23 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
   // by row of the batch: the waves bring one array each; else the items' bias
   const float *by_k = ITEMS ? (wave == 0 ? a.lse : wave == 1 ? a.every : wave == 2 ? a.entry : (const float *)a.target) : a.bias;
   auto load = [&](uint32_t s) {
-    stage.load(a.k, a.k_ld, a.k_plane, a.nk, s);
+    stage.load(a.k, a.k_ld, a.d, a.nk, s);
     if (ITEMS) extra = by_k[s * 64 + lane];
     else if (BIAS && wave == 0) extra = by_k[nt_min(s * 64 + lane, a.nk - 1)];
   };
   auto store = [&](int buf) {
-    stage.store(smem + buf * kStage);
+    stage.store(smem + buf * kStage, k_scale);
     if (ITEMS || (BIAS && wave == 0)) *(float *)(smem + buf * kStage + P * kPlane + threadIdx.x * 4) = extra;
   };
   if (s_lo < s_hi) load(s_lo);
   // this wave's rows
   u32x4 R[P][RT][KD];
+  lr_rows<FMT, P, RT, KD, DT, RAW>(R, a.r, a.r_ld, r0, a.nr, a.d, r_scale);
   float lse[RT], every[RT], entry[RT], rbias[RT], bsum[RT];
   int hit[RT];
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
     const uint32_t row = nt_min(r0 + j * 16 + col, a.nr - 1);
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int s = 0; s < KD; ++s) R[p][j][s] = *(const u32x4 *)(a.r + (size_t)row * a.r_ld + p * a.r_plane + s * 64 + q * 16);
     lse[j] = every[j] = entry[j] = rbias[j] = bsum[j] = 0.f;
     hit[j] = -1;
     if constexpr (ITEMS) {
@@ -499,11 +664,12 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
       const float rest = a.rest[t];
 #pragma unroll
       for (int s = 0; s < KD; ++s) {
-        const u32x4 w = *(const u32x4 *)(a.k + (size_t)t * a.k_ld + s * 64 + q * 16);
+        LrPiece<DT, RAW> piece;
+        piece.load(a.k + (size_t)t * a.k_ld, s * 32 + q * 8, a.d, kRow);
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const unsigned short u = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
+          const unsigned short u = (unsigned short)(piece.w[0][e >> 1] >> (16 * (e & 1)));
           y[e] = FMT == AS_BF16 ? bf16_to_f32(u) : (float)__builtin_bit_cast(_Float16, u);
         }
 #pragma unroll
@@ -516,7 +682,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
       }
     }
   }
-  const float f = ITEMS ? a.scale * a.coef[1] * (P == 2 ? 1.f / plane_scale(*a.k_top) : 1.f) : 1.f;
+  const float f = ITEMS && !a.sums ? a.scale * a.coef[1] / k_scale : 1.f;
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
     const uint32_t row = r0 + j * 16 + col;
@@ -524,7 +690,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
       float b = bsum[j];
       b += __shfl_xor(b, 16);
       b += __shfl_xor(b, 32);
-      if (a.grad_bias && q == 0 && row < a.nr) a.grad_bias[row] = b * a.coef[1];
+      if (a.grad_bias && q == 0 && row < a.nr) a.grad_bias[(size_t)split * a.nr + row] = a.splits > 1 ? b : b * a.coef[1];
     }
     if (row >= a.nr) continue;
 #pragma unroll
@@ -532,7 +698,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
       const uint32_t m = t * 32 + q * 8;
       if (m >= a.d) continue;
       const f32x4 u = out[2 * t][j] * f, v = out[2 * t + 1][j] * f;
-      if constexpr (!ITEMS) {
+      if (!ITEMS || a.sums) {
         f32x4 *o = (f32x4 *)(a.sums + ((size_t)split * a.nr + row) * a.sums_pitch + m);
         o[0] = u, o[1] = v;
       } else if (a.out == nullptr) {
