@@ -161,4 +161,53 @@ __device__ __forceinline__ void store_from_f32(void *p, size_t i, float v) {
   else ((_Float16 *)p)[i] = (_Float16)v;
 }
 
+// Eight consecutive values of a row of any alignment and length as the matrix holds them (16-bit types: w[0]; f32: w[0], w[1]), columns
+// behind the row's d as zeros.  A piece that sticks out of its row is read further left, where it ends with the row, and shifted.
+template <int DT>
+struct Piece8 {
+  u32x4 w[DT == AS_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const char *row, uint32_t column, uint32_t d) {
+    if constexpr (DT == AS_F32) {
+      const float *p = (const float *)row;
+      if (d < 4) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e >> 2][e & 3] = column + e < d ? __float_as_uint(p[column + e]) : 0u;
+        return;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t c = column + 4 * h, at = c + 4 <= d ? c : d - 4;
+        u32x4 x;
+        __builtin_memcpy(&x, p + at, 16);
+        if (d & 3) {  // (uniform)
+          const uint32_t s = c - at;
+          x = s == 1 ? u32x4{x[1], x[2], x[3], 0u} : s == 2 ? u32x4{x[2], x[3], 0u, 0u} : s == 3 ? u32x4{x[3], 0u, 0u, 0u} : x;
+        }
+        w[h] = c < d ? x : u32x4{0u, 0u, 0u, 0u};
+      }
+    } else {
+      const unsigned short *p = (const unsigned short *)row;
+      if (d < 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[0][e] = (column + 2 * e < d ? (uint32_t)p[column + 2 * e] : 0u) | (column + 2 * e + 1 < d ? (uint32_t)p[column + 2 * e + 1] << 16 : 0u);
+        return;
+      }
+      const uint32_t at = column + 8 <= d ? column : d - 8;
+      u32x4 x;
+      __builtin_memcpy(&x, p + at, 16);
+      if (d & 7) {  // (uniform)
+        const uint32_t s = column < d ? (column - at) * 16 : 0;
+        uint64_t lo = (uint64_t)x[0] | (uint64_t)x[1] << 32, hi = (uint64_t)x[2] | (uint64_t)x[3] << 32;
+        if (s >= 64) lo = hi, hi = 0;
+        const uint32_t r = s & 63;
+        lo = lo >> r | (r ? hi << (64 - r) : 0);
+        hi >>= r;
+        x = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+      }
+      w[0] = column < d ? x : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+};
+
 }  // namespace asx
