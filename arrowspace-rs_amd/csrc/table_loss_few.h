@@ -8,6 +8,7 @@
 //   dX (rows x columns, in registers over the whole walk)  A = items transposed (4 of a column a lane), B = g (row, 4 items)
 //   dW (16 items x columns, stored at once)                A = rows transposed (kept),                  B = g turned over in LDS (item, 4 rows)
 // f32 goes as three bf16 planes (24 bits, no common scale to be found first, six products of 2^-24 and more): the matrix pipe has time.
+// Up to 128 columns a wave takes whole items instead, each its own stretch of the table, and nothing meets before the end.
 // Measured: 2 rows, 688 025 items of 678 values at an odd stride (bf16), forward and backward: see the case tables.
 #pragma once
 
@@ -63,7 +64,8 @@ struct LossFewArgs {
   uint32_t n, v, d;
   float scale;
   const float *bias;
-  float2 *part;                   // forward: [workgroup][n]
+  float2 *part;                   // forward: [walker][n]
+  uint32_t slices, row_blocks;    // forward: workgroups a block of rows
   // backward
   const float *lse, *every, *entry, *rest;
   const int *target;
@@ -72,7 +74,6 @@ struct LossFewArgs {
   uint32_t sums_pitch;
   void *out;                      // dW
   size_t out_stride;
-  int aligned;
   float *grad_bias;
   int want_x;
 };
@@ -121,7 +122,7 @@ struct FewSlice {
   }
 };
 template <int DT, int KC, int RT>
-__device__ __forceinline__ void few_rows(const LossFewArgs &a, uint32_t column0, u32x4 (&R)[FewSlice<DT, KC>::P][RT][KC]) {
+__device__ __forceinline__ void few_rows(const LossFewArgs &a, uint32_t n, uint32_t column0, u32x4 (&R)[FewSlice<DT, KC>::P][RT][KC]) {
   constexpr int P = FewSlice<DT, KC>::P, FMT = FewSlice<DT, KC>::FMT;
   const uint32_t lane = threadIdx.x & 63, q = lane >> 4, col = lane & 15;
 #pragma unroll
@@ -129,7 +130,7 @@ __device__ __forceinline__ void few_rows(const LossFewArgs &a, uint32_t column0,
 #pragma unroll
     for (int t = 0; t < KC; ++t) {
       LrPiece<DT, true> piece;
-      piece.load(a.rows + (size_t)nt_min(j * 16 + col, a.n - 1) * a.rows_ld, column0 + t * 32 + q * 8, a.d, 0);
+      piece.load(a.rows + (size_t)nt_min(j * 16 + col, n - 1) * a.rows_ld, column0 + t * 32 + q * 8, a.d, 0);
       u32x4 o[P];
       few_planes<FMT, P, DT>(piece, o);
 #pragma unroll
@@ -137,34 +138,48 @@ __device__ __forceinline__ void few_rows(const LossFewArgs &a, uint32_t column0,
     }
 }
 
-template <int DT, int KC, int RT, bool GENERAL, int WAVES>
+// WK waves share the columns: 4, or 1
+template <int DT, int KC, int RT, bool GENERAL, int WK, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void loss_few_sums_kernel(LossFewArgs a) {
   typedef FewSlice<DT, KC> Slice;
-  constexpr int P = Slice::P;
+  constexpr int P = Slice::P, TS = WK == 1 ? RT : 1;  // TS: row tiles whose statistics a wave keeps (WK 4: wave w those of tile w)
   __shared__ __attribute__((aligned(16))) char smem[4 * Slice::kWave];
-  __shared__ f32x4 meet[2][4][RT][64];
+  __shared__ f32x4 meet[WK == 4 ? 2 : 1][4][RT][64];
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, col = lane & 15;
-  const uint32_t column0 = wave * Slice::CW, stages = (a.v + 15) / 16;
-  const uint32_t s_lo = (uint32_t)((uint64_t)stages * blockIdx.x / gridDim.x), s_hi = (uint32_t)((uint64_t)stages * (blockIdx.x + 1) / gridDim.x);
+  // a die (8 blocks apart) takes the blocks of rows of a stretch of the table one after another: its L2 has the items then
+  const uint32_t turn = blockIdx.x >> 3, block = turn % a.row_blocks, slice_at = turn / a.row_blocks * 8 + (blockIdx.x & 7);
+  if (slice_at >= a.slices) return;
+  a.rows += (size_t)block * 16 * RT * a.rows_ld;
+  const uint32_t row0 = block * 16 * RT, n = a.n - row0;
+  const uint32_t column0 = (WK == 4 ? wave : 0) * Slice::CW, stages = (a.v + 15) / 16;
+  const uint32_t walker = WK == 4 ? slice_at : slice_at * 4 + wave, walkers = a.slices * (4 / WK);
+  const uint32_t s_lo = (uint32_t)((uint64_t)stages * walker / walkers), s_hi = (uint32_t)((uint64_t)stages * (walker + 1) / walkers);
   char *mine = smem + wave * Slice::kWave;
-  Slice slice;
-  if (s_lo < s_hi) slice.load(a, column0, s_lo);
+  Slice even, odd;  // two stages under way
+  if (s_lo < s_hi) even.load(a, column0, s_lo);
+  if (s_lo + 1 < s_hi) odd.load(a, column0, s_lo + 1);
   u32x4 R[P][RT][KC];
-  few_rows<DT, KC, RT>(a, column0, R);
+  few_rows<DT, KC, RT>(a, n, column0, R);
   const float unit = GENERAL ? kLog2e : a.scale * kLog2e, slack = fminf(20.f / unit, 1e30f);
-  // wave w keeps the statistics of row tile w
-  float ref = -INFINITY, base = 0.f, sum = 0.f;
-  for (uint32_t s = s_lo; s < s_hi; ++s) {
+  float ref[TS], base[TS], sum[TS];
+#pragma unroll
+  for (int t = 0; t < TS; ++t) ref[t] = -INFINITY, base[t] = 0.f, sum[t] = 0.f;
+  auto step = [&](uint32_t s, Slice &slice) {
     slice.store(mine);
-    if (s + 1 < s_hi) slice.load(a, column0, s + 1);
+    if (s + 2 < s_hi) slice.load(a, column0, s + 2);
     wave_lds_order();
     f32x4 z[RT];
     Slice::template logits<RT>(mine, R, z);
+    if constexpr (WK == 4) {
 #pragma unroll
-    for (int j = 0; j < RT; ++j) meet[s & 1][wave][j][lane] = z[j];
-    __syncthreads();
-    if (wave < RT) {
-      f32x4 l = meet[s & 1][0][wave][lane] + meet[s & 1][1][wave][lane] + meet[s & 1][2][wave][lane] + meet[s & 1][3][wave][lane];
+      for (int j = 0; j < RT; ++j) meet[s & 1][wave][j][lane] = z[j];
+      __syncthreads();
+      if (wave >= RT) return;
+    }
+#pragma unroll
+    for (int t = 0; t < TS; ++t) {
+      f32x4 l = z[t];
+      if constexpr (WK == 4) l = meet[s & 1][0][wave][lane] + meet[s & 1][1][wave][lane] + meet[s & 1][2][wave][lane] + meet[s & 1][3][wave][lane];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t item = s * 16 + q * 4 + e;
@@ -172,46 +187,56 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_sums_kernel(LossFewArgs a
         if (item >= a.v) l[e] = -INFINITY;
       }
       const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
-      if (__any(top > ref + slack)) {
-        if (top > ref) {
-          sum *= __builtin_amdgcn_exp2f((ref - top) * unit);
-          ref = top;
-          base = GENERAL ? top : -top * unit;
+      if (__any(top > ref[t] + slack)) {
+        if (top > ref[t]) {
+          sum[t] *= __builtin_amdgcn_exp2f((ref[t] - top) * unit);
+          ref[t] = top;
+          base[t] = GENERAL ? top : -top * unit;
         }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(GENERAL ? (l[e] - base) * unit : fmaf(l[e], unit, base));
+      for (int e = 0; e < 4; ++e) sum[t] += __builtin_amdgcn_exp2f(GENERAL ? (l[e] - base[t]) * unit : fmaf(l[e], unit, base[t]));
     }
+  };
+  for (uint32_t s = s_lo; s < s_hi; s += 2) {
+    step(s, even);
+    if (s + 1 < s_hi) step(s + 1, odd);
   }
-  if (wave < RT) {
-    float m = GENERAL ? ref : ref == -INFINITY ? -INFINITY : ref * a.scale;
+  if (WK == 4 && wave >= RT) return;
+#pragma unroll
+  for (int t = 0; t < TS; ++t) {
+    float m = GENERAL ? ref[t] : ref[t] == -INFINITY ? -INFINITY : ref[t] * a.scale;
 #pragma unroll
     for (int x = 16; x < 64; x <<= 1) {
-      const float mo = __shfl_xor(m, x), so = __shfl_xor(sum, x);
+      const float mo = __shfl_xor(m, x), so = __shfl_xor(sum[t], x);
       const float mm = fmaxf(m, mo), b = mm == -INFINITY ? 0.f : mm;
-      sum = sum * __builtin_amdgcn_exp2f((m - b) * kLog2e) + so * __builtin_amdgcn_exp2f((mo - b) * kLog2e);
+      sum[t] = sum[t] * __builtin_amdgcn_exp2f((m - b) * kLog2e) + so * __builtin_amdgcn_exp2f((mo - b) * kLog2e);
       m = mm;
     }
-    const uint32_t row = wave * 16 + col;
-    if (q == 0 && row < a.n) a.part[(size_t)blockIdx.x * a.n + row] = float2{m, sum};
+    const uint32_t row = (WK == 4 ? wave : t) * 16 + col;
+    if (q == 0 && row < n) a.part[(size_t)walker * a.n + row0 + row] = float2{m, sum[t]};
   }
 }
 
-template <int DT, int KC, bool BIAS, int WAVES>
+template <int DT, int KC, bool BIAS, int WK, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void loss_few_grad_kernel(LossFewArgs a) {
   typedef FewSlice<DT, KC> Slice;
   constexpr int P = Slice::P, FMT = Slice::FMT;
   __shared__ __attribute__((aligned(16))) char smem[4 * Slice::kWave];
-  __shared__ f32x4 meet[2][4][64];
+  __shared__ f32x4 meet[WK == 4 ? 2 : 1][4][64];
   __shared__ __attribute__((aligned(16))) char turn[4][P][512];
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, col = lane & 15;
-  const uint32_t column0 = wave * Slice::CW, stages = (a.v + 15) / 16;
-  const uint32_t s_lo = (uint32_t)((uint64_t)stages * blockIdx.x / gridDim.x), s_hi = (uint32_t)((uint64_t)stages * (blockIdx.x + 1) / gridDim.x);
+  const uint32_t column0 = (WK == 4 ? wave : 0) * Slice::CW, stages = (a.v + 15) / 16;
+  const uint32_t walker = WK == 4 ? blockIdx.x : blockIdx.x * 4 + wave, walkers = gridDim.x * (4 / WK);
+  const uint32_t s_lo = (uint32_t)((uint64_t)stages * walker / walkers), s_hi = (uint32_t)((uint64_t)stages * (walker + 1) / walkers);
   char *mine = smem + wave * Slice::kWave;
-  Slice slice;
-  if (s_lo < s_hi) slice.load(a, column0, s_lo);
+  constexpr int AHEAD = KC * P <= 4 ? 2 : 1;  // stages under way
+  Slice ring[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (s_lo + i < s_hi) ring[i].load(a, column0, s_lo + i);
   u32x4 R[P][1][KC];
-  few_rows<DT, KC, 1>(a, column0, R);
+  few_rows<DT, KC, 1>(a, a.n, column0, R);
   // the rows transposed: columns 32 j + 8 (col / 4) + 4 h + col % 4 of rows 4 q .. 4 q + 3 (rows that are not there: zeros)
   u32x2 XT[P][2 * KC];
 #pragma unroll
@@ -235,15 +260,18 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_grad_kernel(LossFewArgs a
 #pragma unroll
   for (int t = 0; t < 2 * KC; ++t) dx[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   const uint32_t trow = q * 4 + ((lane >> 2) & 3);
-  for (uint32_t s = s_lo; s < s_hi; ++s) {
+  auto step = [&](uint32_t s, Slice &slice) {
     slice.store(mine);
-    if (s + 1 < s_hi) slice.load(a, column0, s + 1);
+    if (s + AHEAD < s_hi) slice.load(a, column0, s + AHEAD);
     wave_lds_order();
     f32x4 z[1];
     Slice::template logits<1>(mine, R, z);
-    meet[s & 1][wave][lane] = z[0];
-    __syncthreads();
-    f32x4 g = meet[s & 1][0][lane] + meet[s & 1][1][lane] + meet[s & 1][2][lane] + meet[s & 1][3][lane];
+    f32x4 g = z[0];
+    if constexpr (WK == 4) {
+      meet[s & 1][wave][lane] = g;
+      __syncthreads();
+      g = meet[s & 1][0][lane] + meet[s & 1][1][lane] + meet[s & 1][2][lane] + meet[s & 1][3][lane];
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t item = s * 16 + q * 4 + e;
@@ -254,7 +282,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_grad_kernel(LossFewArgs a
       if (target == item) g[e] = entry;
     }
     if constexpr (BIAS) {
-      if (wave == 0 && a.grad_bias) {
+      if ((WK == 1 || wave == 0) && a.grad_bias) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float b = add16(g[e]);
@@ -313,14 +341,8 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_grad_kernel(LossFewArgs a
         }
         w[0] *= f, w[1] *= f;
         if (item >= a.v || c >= a.d) continue;
-        if (a.aligned && c + 8 <= a.d) {
-          if constexpr (DT == AS_F32) {
-            f32x4 *o = (f32x4 *)((float *)a.out + (size_t)item * a.out_stride + c);
-            o[0] = w[0], o[1] = w[1];
-          } else {
-            *(u32x4 *)((unsigned short *)a.out + (size_t)item * a.out_stride + c) =
-                u32x4{pack2<DT>(w[0][0], w[0][1]), pack2<DT>(w[0][2], w[0][3]), pack2<DT>(w[1][0], w[1][1]), pack2<DT>(w[1][2], w[1][3])};
-          }
+        if (c + 8 <= a.d) {
+          store8<DT>(a.out, (size_t)item * a.out_stride + c, w[0], w[1]);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -328,8 +350,32 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_grad_kernel(LossFewArgs a
         }
       }
     }
+  };
+  for (uint32_t s = s_lo; s < s_hi; s += AHEAD) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (s + i < s_hi) step(s + i, ring[i]);
   }
-  if (a.want_x && col < a.n) {
+  if (!a.want_x) return;
+  if constexpr (WK == 1) {  // the four waves' dX, in their order
+    __syncthreads();
+    f32x4 *other = (f32x4 *)smem;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      if (wave == w) {
+#pragma unroll
+        for (int t = 0; t < 2 * KC; ++t) other[t * 64 + lane] = dx[t];
+      }
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int t = 0; t < 2 * KC; ++t) dx[t] += other[t * 64 + lane];
+      }
+      __syncthreads();
+    }
+    if (wave) return;
+  }
+  if (col < a.n) {
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
       const uint32_t c = column0 + j * 32 + q * 8;

@@ -71,6 +71,18 @@ __device__ __forceinline__ float low_part(float x) {  // what f16 leaves of x (n
 }
 
 
+// eight consecutive values of a row, of any alignment
+template <int DT>
+__device__ __forceinline__ void store8(void *out, size_t at, f32x4 u, f32x4 v) {
+  if constexpr (DT == AS_F32) {
+    __builtin_memcpy((float *)out + at, &u, 16);
+    __builtin_memcpy((float *)out + at + 4, &v, 16);
+  } else {
+    const u32x4 x = {pack2<DT>(u[0], u[1]), pack2<DT>(u[2], u[3]), pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+    __builtin_memcpy((unsigned short *)out + at, &x, 16);
+  }
+}
+
 struct LossRowsArgs {
   const char *r, *k;              // the two sides' rows as they are
   size_t r_ld, k_ld;              // bytes
@@ -87,7 +99,6 @@ struct LossRowsArgs {
   uint32_t sums_pitch;
   void *out;                      // r = items, not split: rows of out_stride elements, or null
   size_t out_stride;
-  int aligned;
   float *grad_bias;               // r = items: sum over k of g (split: [split][nr], in units of coef), or null
 };
 
@@ -668,14 +679,8 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
         o[0] = u, o[1] = v;
       } else if (a.out == nullptr) {
         continue;  // (the bias' gradient alone)
-      } else if (a.aligned && m + 8 <= a.d) {
-        if constexpr (OUT == AS_F32) {
-          f32x4 *o = (f32x4 *)((float *)a.out + (size_t)row * a.out_stride + m);
-          o[0] = u, o[1] = v;
-        } else {
-          *(u32x4 *)((unsigned short *)a.out + (size_t)row * a.out_stride + m) =
-              u32x4{pack2<OUT>(u[0], u[1]), pack2<OUT>(u[2], u[3]), pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
-        }
+      } else if (m + 8 <= a.d) {
+        store8<OUT>(a.out, (size_t)row * a.out_stride + m, u, v);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
