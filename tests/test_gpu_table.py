@@ -551,3 +551,180 @@ def test_train_then_serve():
     q = np.stack((codes & 15, codes >> 4), 2).reshape(v, -1).astype(np.float64)
     w = torch.from_numpy((q - 8) * np.repeat(s, 32, axis=1)).cuda()
     _check4(t, w, hidden[:3].contiguous())
+
+
+# ---- sizes at which another form is taken ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, v, d, pad, offset", [
+    (1, 15, 7, 1, 1), (2, 16, 32, 0, 0), (15, 17, 33, 2, 1), (16, 5003, 64, 0, 0), (3, 1000, 96, 1, 0), (16, 1025, 128, 8, 0), (7, 999, 129, 0, 0),
+    (16, 700, 256, 0, 0), (4, 3001, 300, 5, 2), (16, 333, 384, 0, 0), (9, 800, 400, 8, 0), (16, 1200, 512, 0, 0), (5, 90, 513, 0, 0),
+    (2, 2000, 678, 0, 0), (16, 500, 768, 8, 8), (11, 640, 900, 1, 1), (16, 400, 1024, 0, 0), (16, 300, 1025, 3, 0), (17, 800, 40, 3, 1), (33, 501, 94, 1, 0),
+    (64, 1000, 131, 0, 0), (48, 700, 600, 3, 3), (64, 100, 1024, 8, 0), (65, 1000, 131, 0, 0)])
+def test_cross_entropy_few_rows(n, v, d, pad, offset, dt):
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=n + d, pad=pad, offset=offset, bias=n % 2 == 1, ignored=0.2)
+    _check(x, w, y, b, scale=2.0, ge=torch.linspace(-1e-3, 2e-3, n, device="cuda"))
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, v, d, bias", [(1024, 40, 32, True), (1025, 211, 64, False), (3000, 17, 128, True), (2500, 5, 200, True), (5011, 130, 96, False),
+                                           (1500, 1, 64, True), (1100, 700, 320, True)])
+def test_cross_entropy_more_rows_than_items(n, v, d, bias, dt):
+    """The gradient of a short table is added up over parts of the batch; many rows meet the same item."""
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=n, bias=bias, ignored=0.1)
+    _check(x, w, y, b, scale=2.0)
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, v, d", [(16, 300, 64), (16, 300, 400), (700, 1000, 64), (700, 1000, 320)])
+def test_cross_entropy_all_rows_at_one_item(n, v, d, dt):
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=7, bias=True)
+    y[:] = v - 1
+    _check(x, w, y, b, scale=1.0)
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, d", [(5, 100), (5, 300), (40, 131)])
+def test_cross_entropy_few_rows_masked(n, d, dt):
+    """-inf and the lowest value as masks, every item masked, a row of NaN, a target out of range."""
+    x, w, y, b = _inputs(n, 530, d, TYPES[dt], seed=8, bias=True)
+    y[:] = torch.arange(n, device="cuda") * 13 + 3
+    b[torch.arange(0, 530, 2)] = -float("inf")
+    b[1::4] = torch.finfo(torch.float32).min
+    y |= 1
+    _check(x, w, y, b, scale=2.0)
+    b[:] = -float("inf")
+    losses, lse, grads = _check(x, w, y, b, scale=2.0)
+    assert (losses == 0).all() and all((g == 0).all() for g in grads)
+    x[1] = float("nan")
+    b = torch.zeros(530, device="cuda")
+    y[3] = 530
+    losses, lse = A.cross_entropy(x, w, y, bias=b)
+    keep = torch.tensor([k for k in range(n) if k not in (1, 3)], device="cuda")
+    want = _reference(x[keep], w, y[keep], b, 1.0)
+    _close(losses[keep], *want["losses"], "losses")
+    assert torch.isnan(losses[1]) and torch.isnan(losses[3]) and torch.isnan(lse[1]) and torch.isfinite(lse[3])
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, v, d", [(6, 900, 60), (6, 900, 500), (300, 800, 64), (300, 800, 300)])
+def test_cross_entropy_each_gradient_alone(n, v, d, dt):
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=9, bias=True, ignored=0.1)
+    losses, lse = A.cross_entropy(x, w, y, bias=b)
+    gl = torch.rand(n, device="cuda")
+    every = A.cross_entropy_backward(x, w, y, lse, gl, bias=b)
+    for k in range(3):
+        need = [i == k for i in range(3)]
+        got = A.cross_entropy_backward(x, w, y, lse, gl, bias=b, need_x=need[0], need_table=need[1], need_bias=need[2])
+        assert [g is not None for g in got] == need and torch.equal(got[k], every[k])
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, v, d", [(5, 203, 70), (5, 203, 513), (90, 203, 70), (1500, 33, 70), (90, 203, 300)])
+def test_cross_entropy_strided_gradients(n, v, d, dt):
+    """Gradients into rows of wider matrices of any alignment; what lies between the rows stays."""
+    x, w, y, _ = _inputs(n, v, d, TYPES[dt], seed=10)
+    losses, lse = A.cross_entropy(x, w, y)
+    gl = torch.rand(n, device="cuda")
+    want = A.cross_entropy_backward(x, w, y, lse, gl)
+    kind = getattr(_lib, "AS_" + dt.upper())
+    ctx = A.Context(0)
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    for extra in (1, 3, 8):
+        gx = torch.full((n, d + extra), 5.0, device="cuda", dtype=TYPES[dt])
+        gw = torch.full((v, d + extra), 5.0, device="cuda", dtype=TYPES[dt])
+        at = 1 if extra == 3 else 0
+        rc = ctx.lib.as_cross_entropy_backward(ctx.h, x.data_ptr(), n, d, w.data_ptr(), v, d, d, kind, None, y.data_ptr(), -100, 1.0, lse.data_ptr(),
+                                               gl.data_ptr(), None, gx[:, at:].data_ptr(), d + extra, gw[:, at:].data_ptr(), d + extra, None, None, 0)
+        assert rc == _lib.AS_OK
+        for got, ref in ((gx, want[0]), (gw, want[1])):
+            assert torch.equal(got[:, at:at + d], ref)
+            assert (got[:, :at] == 5).all() and (got[:, at + d:] == 5).all()
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("n, v, d, dt", [(7, 2000, 90, "bf16"), (40, 900, 300, "f32"), (16, 700, 500, "f16"), (2000, 60, 64, "bf16"), (300, 900, 400, "f32")])
+def test_cross_entropy_forms_captured(n, v, d, dt):
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=11, bias=True)
+    gl = torch.full((n,), 1 / n, device="cuda")
+
+    def step():
+        losses, lse = A.cross_entropy(x, w, y, bias=b, scale=2.0)
+        return (losses, lse) + A.cross_entropy_backward(x, w, y, lse, gl, bias=b, scale=2.0)
+
+    _replays(step, (x, w, b))
+
+
+def test_cross_entropy_table_of_more_than_4_gib():
+    """Offsets behind 32 bits in the table and in its gradient: the last items, and the first, against 64 bits."""
+    v, d, n = 10_000_019, 256, 3
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.empty(v, d, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    y = torch.tensor([v - 1, 5, v - 2], device="cuda")
+    x = w[y] * 0.5
+    losses, lse = A.cross_entropy(x, w, y, scale=0.125)
+    z = torch.cat([0.125 * (x.double() @ c.double().t()) for c in w.split(1 << 20)], 1)
+    want = torch.logsumexp(z, 1)
+    hit = z.gather(1, y[:, None])[:, 0]
+    # a product of 256 terms in f32 (|x w| adds up to less than 256), lse, the difference
+    assert (lse.double() - want).abs().max() <= (256 + 8) * E * 0.125 * 256 + 64 * E * 20
+    assert (losses.double() - (want - hit)).abs().max() <= 2 * ((256 + 8) * E * 0.125 * 256 + 64 * E * 20)
+    gl = torch.ones(n, device="cuda")
+    gx, gw, _ = A.cross_entropy_backward(x, w, y, lse, gl, scale=0.125)
+    p = torch.exp(z - want[:, None])
+    p[torch.arange(n), y] -= 1
+    for rows in (slice(v - 40, v), slice(0, 40)):
+        ref = 0.125 * (p[:, rows].t().contiguous() @ x.double())
+        size = 0.125 * (p[:, rows].abs().t().contiguous() @ x.double().abs())
+        # the result's rounding; g's: half a step and exp of two errors of 264 e 32
+        assert ((gw[rows].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2 * 264 * E * 32 + 128 * E * 20) * size + 1e-30).all()
+    ref = 0.125 * sum(p[:, i:i + (1 << 20)] @ w[i:i + (1 << 20)].double() for i in range(0, v, 1 << 20))
+    assert (gx.double() - ref).norm() <= 2.0 ** -7 * ref.norm()
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("m, v, d, group, scales, zeros", [
+    (5, 40, 256, 64, "f32", True), (16, 500, 4000, 128, "f16", True), (16, 3001, 1000, 32, "bf16", False), (8, 100, 20000, 128, "bf16", False),
+    (16, 20000, 2600, 64, "f16", False), (16, 64, 5008, 128, "f32", False), (33, 70, 4500, 64, "bf16", True), (20, 9000, 2700, 128, "f16", False),
+    (64, 40000, 1300, 32, "f32", False), (100, 200, 2500, 64, "bf16", False), (4, 30, 42000, 128, "f32", True), (3, 5, 130, 64, "f16", False)])
+def test_scores4_forms(m, v, d, group, scales, zeros, dt):
+    """Rows in LDS, read as they lie, from an image, and of parts of k."""
+    codes, s, z, w = _plain4(v, d, group, scales, zeros, m + v + d)
+    t = A.Table4.from_codes(codes, s, z, dim=d, group=group)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    for pad, at in ((0, 0), (8, 0), (3, 1)):
+        x = torch.randn(m, d + pad, device="cuda", generator=g).to(TYPES[dt])[:, at:at + d]
+        first = _check4(t, w, x)
+    assert torch.equal(first, t.scores(x))
+    x[m // 2, d - 1] = float("inf")
+    x[0, 0] = float("nan")
+    got = t.scores(x)
+    keep = [k for k in range(1, m) if k != m // 2]
+    if keep:
+        assert torch.equal(got[keep], first[keep])
+    assert torch.isnan(got[0]).all()
+
+
+@pytest.mark.parametrize("m, v, d, dt", [(16, 2000, 3000, "f16"), (16, 900, 6000, "bf16"), (40, 500, 3500, "f32")])
+def test_scores4_forms_captured(m, v, d, dt):
+    codes, s, z, w = _plain4(v, d, 64, "bf16", True, 6)
+    t = A.Table4.from_codes(codes, s, z, dim=d, group=64)
+    x = torch.randn(m, d, device="cuda").to(TYPES[dt])
+    _replays(lambda: (t.scores(x),), (x,))
+
+
+def test_scores4_codes_and_scores_of_more_than_4_gib():
+    """Offsets behind 32 bits in the codes (5.1 GB) and in the scores (2^32 of them)."""
+    v, d = 20_000_003, 512
+    g = torch.Generator(device="cuda").manual_seed(4)
+    codes = torch.randint(0, 256, (v, d // 2), generator=g, dtype=torch.uint8, device="cuda")
+    s = torch.rand(v, d // 128, generator=g, device="cuda").to(torch.float16) + 0.5
+    t = A.Table4.from_codes(codes, s, dim=d, group=128)
+    x = torch.randn(215, d, generator=g, device="cuda").half()
+    got = t.scores(x)
+    at = torch.cat([torch.arange(0, 50), torch.arange(v // 2, v // 2 + 50), torch.arange(v - 50, v)]).cuda()
+    c = codes[at]
+    w = (torch.stack((c & 15, c >> 4), 2).flatten(1).double() - 8) * s[at].double().repeat_interleave(128, 1)
+    want = x.double() @ w.t().contiguous()
+    size = x.double().abs() @ w.abs().t().contiguous()
+    bound = (d + 16) * E * size + 2.0 ** -11 * want.abs() + torch.finfo(torch.float16).tiny
+    _close(got[:, at], want, bound, "scores")
