@@ -745,6 +745,15 @@ class ArrowSpace:
         lam = self.prepare_query_item(item, gl)
         return self.search_lambda_aware(ArrowItem(item, lam), k, alpha)
 
+    def pack4(self, group=64, scale_dtype="bfloat16"):
+        """The items in 4 bits with group scales (Table4), for scores of single queries from half a byte a value.  No counterpart in
+        the reference."""
+        from .table import Table4
+        if _is_torch(self.data):
+            return Table4.pack(self.data, group=group, scale_dtype=scale_dtype)
+        data = self.data.numpy() if isinstance(self.data, DeviceArray) else self.data
+        return Table4.pack(data, group=group, scale_dtype=scale_dtype, ctx=self.ctx)
+
     def __del__(self):
         try:
             self._drop_index()

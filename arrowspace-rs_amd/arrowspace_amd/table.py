@@ -252,7 +252,8 @@ class Table4:
         codes = np.empty((self.n_items, (self.dim + 1) // 2), dtype=np.uint8)
         zeros = np.empty((self.n_items, groups), dtype=np.uint8)
         raw = np.empty((self.n_items, groups), dtype=np.uint16 if self.scale_dtype == "bfloat16" else self.scale_dtype)
-        self.ctx.check(self.ctx.lib.as_table4_export(self.ctx.h, self.h, codes.ctypes.data, raw.ctypes.data, zeros.ctypes.data))
+        c = _thread_context(self.ctx.device)
+        c.check(c.lib.as_table4_export(c.h, self.h, codes.ctypes.data, raw.ctypes.data, zeros.ctypes.data))
         scales = (raw.astype(np.uint32) << 16).view(np.float32) if self.scale_dtype == "bfloat16" else raw
         return codes, scales, zeros
 

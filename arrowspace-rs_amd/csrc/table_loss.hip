@@ -7,14 +7,23 @@
 // Forward: one product (nt_product.h, the table on the m side, so that a lane holds many items of ONE row) whose ending keeps a
 // running maximum and sum of exponentials per lane and row; what leaves the chip is one (maximum, sum) per row and stretch of the
 // table.  A second kernel joins them and takes the target's logit from a product of its own in f64.
-// Backward: in pieces of the table.  Per piece the logits are made again, their gradient G leaves in 16 bits, row-major AND
-// transposed, and two more products of the same kind give the piece's rows of dW and its part of dX (f32, added up over the pieces in
-// a buffer, rounded once at the end).  Nothing is added with atomics: results do not change from run to run.
+// Backward, three forms.  Rows of up to 256 values (f32: 128): the gradient G of the logits stays in registers (table_loss_rows.h).  Up
+// to 16 rows: one pass over the table that writes dW as it goes (table_loss_few.h).  Else in pieces of the table: per piece the logits
+// are made again, G leaves in 16 bits, once, and two more products, which read their operands transposed, give the piece's rows of dW
+// and its part of dX (f32, added up over the pieces in a buffer, rounded once at the end).
+// Nothing is added with atomics: results do not change from run to run.
+// What bounds it: 2 n v d flops forward, 8 more backward, of which 2 are the logits again (through G: 6, written and read once: 2 bytes a
+// logit each).  8 192 rows x 131 072 items of 1 024 (bf16), forward and backward: 8.23 ms = 1 069 TFLOP/s, one library product of this
+// size runs at 1 076; 4 096 x 100 000 of 768 with a bias: 2.83 ms; 1 024 x 1 000 000 of 128: 1.27 ms, 2.01 through G; 777 x 31 013 of 200
+// (f16): 0.16, 0.18 through G; f32, 512 x 100 000 of 128: 0.30, 0.38 through G.
 // Types.  bf16 and f16 go to the matrix pipe as they are.  f32 values go as a sum of two f16 (22 bits, after a power of two that
 // brings the matrix' largest finite value to 2^14 .. 2^15), three products per pair of planes: 2.5 PFLOP/s / 3 against the
 // 0.157 of the f32 instruction, and an error per product of 2^-23 of it, which the f32 sums have anyway.
+// (Few f32 rows: three bf16, table_loss_few.h.)
 // Rounding.  G is rounded to 16 bits in units of the largest coefficient (coef_scale_kernel; f32: two planes, 22 bits): half a
-// step per entry, as the gradients that leave are rounded themselves.  Everything else -- logits, maxima, sums, dX over pieces,
+// step per entry, as the gradients that leave are rounded themselves.  The entries at the targets, nearly the coefficient itself and
+// the same in all rows of an item, come from a product of their own in f64, and what 16 bits leave of them is added in f32: with half a
+// step there, dX of well-trained rows was off by twice the rounding of the result.  Everything else -- logits, maxima, sums, dX over pieces,
 // dbias -- is f32 or wider.
 #include "table_loss_few.h"
 
@@ -410,26 +419,36 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
   }
 }
 
-// The rows of the batch that meet each 64 items of the table, in order, a wave each (64 kept: items that more rows meet are sums of
-// many entries, whose roundings average out).
+// The rows of the batch that meet each 64 items of the table, in order, a workgroup each, its waves an eighth of the batch each (64 kept:
+// items that more rows meet are sums of many entries, whose roundings average out).
 constexpr uint32_t kMet = 64;
-__global__ __launch_bounds__(256) void met_kernel(const int *target, uint32_t n, uint32_t groups, u32x2 *list, uint32_t *count) {
-  const uint32_t group = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (group >= groups) return;
+__global__ __launch_bounds__(512) void met_kernel(const int *target, uint32_t n, u32x2 *list, uint32_t *count) {
+  __shared__ u32x2 part[8][kMet];
+  __shared__ uint32_t part_len[8];
+  const uint32_t group = blockIdx.x, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t each = (n + 511) / 512 * 64, lo = w * each, hi = nt_min(lo + each, n);
   uint32_t len = 0;
-  for (uint32_t t0 = 0; t0 < n && len < kMet; t0 += 512) {
+  for (uint32_t t0 = lo; t0 < hi && len < kMet; t0 += 512) {
     uint32_t v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = t0 + k * 64 + lane < n ? (uint32_t)target[t0 + k * 64 + lane] - group * 64 : ~0u;
+    for (int k = 0; k < 8; ++k) v[k] = t0 + k * 64 + lane < hi ? (uint32_t)target[t0 + k * 64 + lane] - group * 64 : ~0u;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const uint64_t met = __ballot(v[k] < 64);
       const uint32_t place = len + (uint32_t)__popcll(met & ((1ull << lane) - 1));
-      if (v[k] < 64 && place < kMet) list[(size_t)group * kMet + place] = u32x2{t0 + k * 64 + lane, v[k]};
+      if (v[k] < 64 && place < kMet) part[w][place] = u32x2{t0 + k * 64 + lane, v[k]};
       len += (uint32_t)__popcll(met);
     }
   }
-  if (lane == 0) count[group] = len < kMet ? len : kMet;
+  if (lane == 0) part_len[w] = nt_min(len, kMet);
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+  for (uint32_t o = 0; o < 8; ++o) {
+    if (o < w) before += part_len[o];
+    all += part_len[o];
+  }
+  if (lane < part_len[w] && before + lane < kMet) list[(size_t)group * kMet + before + lane] = part[w][lane];
+  if (threadIdx.x == 0) count[group] = nt_min(all, kMet);
 }
 
 // ---- the two gradients: plain products ------------------------------------------------------------------------------------------------------
@@ -464,36 +483,44 @@ __device__ __forceinline__ void add_rest(const ProductArgs &p, const TILE &T, ui
   if (!len) return;
   const u32x2 mine = p.met[(size_t)group * kMet + (T.lane < len ? T.lane : 0)];
   const float mine_rest = p.rest[mine[0]];
+  // Each column of lanes takes the rows that meet its own four items, all columns at once (one row after the other, 300 rows at 300 items
+  // took eight times the product).
+  uint64_t met = 0;
   for (uint32_t k = 0; k < len; ++k) {
-    const uint32_t row = __builtin_amdgcn_readlane(mine[0], k), in = __builtin_amdgcn_readlane(mine[1], k);
-    const float r = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine_rest), k));
-    const uint32_t jj = ((in >> 5) << 1) | ((in >> 2) & 1), c = (((in >> 3) & 3) << 2) | (in & 3);
-    if (col != c) continue;
+    const uint32_t in = __builtin_amdgcn_readlane(mine[1], k);
+    if (((((in >> 3) & 3) << 2) | (in & 3)) == col) met |= 1ull << k;
+  }
+  while (__any(met != 0)) {
+    const int k = met ? __builtin_ctzll(met) : 0;
+    const uint32_t row = __shfl(mine[0], k), in = __shfl(mine[1], k), jj = ((in >> 5) << 1) | ((in >> 2) & 1);
+    const float r = __shfl(mine_rest, k);
+    if (met) {
 #pragma unroll
-    for (int i = 0; i < TILE::TM; i += 2) {
-      const uint32_t m = m0 + wm * (TILE::TM * 16) + i * 16 + q * 8;
-      if (m >= p.m) continue;
-      const u32x4 w = *(const u32x4 *)(p.A + (size_t)row * p.a_ld + m * 2);  // (zeros behind the row's values)
-      float y[8];
+      for (int i = 0; i < TILE::TM; i += 2) {
+        const uint32_t m = m0 + wm * (TILE::TM * 16) + i * 16 + q * 8;
+        if (m >= p.m) continue;
+        const u32x4 w = *(const u32x4 *)(p.A + (size_t)row * p.a_ld + m * 2);  // (zeros behind the row's values)
+        float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const unsigned short u = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
-        y[e] = FMT == AS_BF16 ? bf16_to_f32(u) : (float)__builtin_bit_cast(_Float16, u);
-      }
-#pragma unroll
-      for (uint32_t j = 0; j < TILE::TN; ++j)
-        if (j == jj) {
-          acc[i][j] += f32x4{y[0], y[1], y[2], y[3]} * r;
-          acc[i + 1][j] += f32x4{y[4], y[5], y[6], y[7]} * r;
+        for (int e = 0; e < 8; ++e) {
+          const unsigned short u = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
+          y[e] = FMT == AS_BF16 ? bf16_to_f32(u) : (float)__builtin_bit_cast(_Float16, u);
         }
-      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (uint32_t j = 0; j < TILE::TN; ++j)
+          if (j == jj) {
+            acc[i][j] += f32x4{y[0], y[1], y[2], y[3]} * r;
+            acc[i + 1][j] += f32x4{y[4], y[5], y[6], y[7]} * r;
+          }
+        if (i & 2) __builtin_amdgcn_sched_barrier(0);  // (two pieces at a time: more would spill)
+      }
     }
+    met &= met - 1;
   }
 }
-template <int FMT, class TILE_, int OUT>  // OUT: element type of `out` (dW), or 0 (AS_F64) = into `sums` (dX)
+template <int FMT, class TILE_, int OUT, bool BT>  // OUT: element type of `out`, or 0 (AS_F64) = into `sums`; BT: dW, else dX
 __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
   using TILE = TILE_;
-  constexpr bool BT = OUT != 0;
   __shared__ __attribute__((aligned(1024))) char smem[2 * TILE::kStage];
   TILE T;
   T.init(smem);
@@ -517,8 +544,8 @@ __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
     T.contract(buf, acc);
     buf ^= 1;
   }
-  if constexpr (OUT == FMT)
-    if (p.met) add_rest<FMT>(p, T, m0, n0, acc);
+  if constexpr (BT && OUT != AS_F32)
+    if (p.met && split == 0) add_rest<FMT>(p, T, m0, n0, acc);
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
   const float f = OUT == 0 ? 1.f : p.scale * p.coef[1] * (p.top ? 1.f / plane_scale(*p.top) : 1.f);
 #pragma unroll
@@ -735,7 +762,7 @@ uint32_t few_groups(int steps, uint32_t d, bool f32, int what, uint32_t v) {
   return std::max(1u, std::min((uint32_t)few_waves(steps, f32, what) * kChips, cdiv(v, 16 * (4 / few_share(d)))));
 }
 // An image is read and written once more than the matrix itself; reading the matrix as it is costs each workgroup that walks it the
-// splitting or shifting of its pieces.  Step of 512 f32 rows of 128, 100 000 items: images 295 us, as they are 315; of 777 rows of 200
+// splitting or shifting of its pieces.  A step of 512 f32 rows of 128, 100 000 items: images 295 us, as they are 315; 777 rows of 200
 // (f16, odd stride), 31 013 items: 171 and 198; one or two blocks of rows: the images would be a third of the time.
 bool raw_pays(const Plan &p) { return p.n <= 128; }
 void plan_backward(Plan &p, bool x, bool w, bool b) {
@@ -779,6 +806,9 @@ void plan_backward(Plan &p, bool x, bool w, bool b) {
   const uint64_t tiles = (uint64_t)cdiv(p.d, kShape[p.tile_x].bm) * cdiv(p.n, kShape[p.tile_x].bn);
   // the contraction over the piece is split where the output alone does not fill the chip
   p.splits = plan_splits(tiles, slots_of(p.tile_x), cdiv(p.piece, 256));
+  // so is the batch where the table is short (6 000 rows, 150 items of 800)
+  const uint64_t w_tiles = (uint64_t)cdiv(p.d, kShape[p.tile_w].bm) * cdiv(p.v, kShape[p.tile_w].bn);
+  p.w_splits = p.pieces == 1 && w_tiles * 2 <= slots_of(p.tile_w) ? plan_splits(w_tiles, slots_of(p.tile_w), cdiv(p.n, 512)) : 1;
 }
 
 // waves a SIMD of the forward (1 024 rows x 1 M items of 128: four tiles of rows x 2 waves 293 us, x 3 282, two x 4 316)
@@ -857,6 +887,7 @@ uint64_t backward_layout(const Plan &p, const Source &x, const Source &t, char *
   s.met = l.take<u32x2>(groups * kMet);
   s.met_count = l.take<uint32_t>(groups);
   s.sums = l.take<float>(p.want_x ? (uint64_t)p.splits * p.n * up(p.d, 8) : 0);
+  s.w_sums = l.take<float>(p.want_w && p.w_splits > 1 ? (uint64_t)p.w_splits * p.v * up(p.d, 8) : 0);
   s.bias_part = l.take<float>(p.want_b ? (uint64_t)p.n_tiles * kShape[p.tile].wn * p.piece : 0);
   return l.at;
 }
@@ -991,21 +1022,24 @@ void launch_rows_sums(as_ctx *ctx, int dt, bool raw, int steps, bool general, co
     else hipLaunchKernelGGL((loss_rows_sums_kernel<DT, RAW, RT, KD, false, W>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
   });
 }
-void launch_product(as_ctx *ctx, int fmt, int tile, int out_type, const ProductArgs &p) {
+void launch_product(as_ctx *ctx, int fmt, int tile, bool w, int out_type, const ProductArgs &p) {
   by_tile(tile, [&](auto k) {
     constexpr int K = decltype(k)::value;
     const dim3 grid(p.m_tiles * p.n_tiles * p.splits);
-    auto go = [&](auto f, auto o) {
+    auto go = [&](auto f, auto o, auto bt) {
       constexpr int FMT = decltype(f)::value, OUT = decltype(o)::value;
-      typedef TileOf<FMT, K, true, OUT != 0> TILE;
-      hipLaunchKernelGGL((product_kernel<FMT, TILE, OUT>), grid, dim3(TILE::NT), 0, ctx->stream, p);
+      constexpr bool BT = decltype(bt)::value;
+      typedef TileOf<FMT, K, true, BT> TILE;
+      hipLaunchKernelGGL((product_kernel<FMT, TILE, OUT, BT>), grid, dim3(TILE::NT), 0, ctx->stream, p);
     };
     constexpr std::integral_constant<int, AS_BF16> bf{};
     constexpr std::integral_constant<int, AS_F16> hf{};
     constexpr std::integral_constant<int, AS_F32> f32{};
     constexpr std::integral_constant<int, 0> acc{};
-    if (fmt == AS_BF16) out_type == 0 ? go(bf, acc) : go(bf, bf);
-    else out_type == 0 ? go(hf, acc) : out_type == AS_F32 ? go(hf, f32) : go(hf, hf);
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    if (fmt == AS_BF16) !w ? go(bf, acc, no) : out_type == 0 ? go(bf, acc, yes) : go(bf, bf, yes);
+    else !w ? go(hf, acc, no) : out_type == 0 ? go(hf, acc, yes) : out_type == AS_F32 ? go(hf, f32, yes) : go(hf, hf, yes);
   });
 }
 
@@ -1182,7 +1216,8 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
         hipLaunchKernelGGL((grad_rows_join_kernel<DT, WAYS>), dim3(spread(total, WAYS == 64 ? 64 : WAYS == 4 ? 256 : 1024)), dim3(WAYS == 64 ? 1024 : 256), 0, ctx->stream,
                            sums, splits, pitch, n, p.d, c.scale, coef, top, (const int *)s.target, r, W.p, (size_t)c.table_stride, out, (size_t)stride);
       };
-      // 16 waves a compute unit, or as many ways as parts: 777 x 200 from 64 parts 10 us in 4 ways, 25 in 64; 9 x 64 from 1 024 parts 5.6 us in 64, 12 in 16
+      // 16 waves a compute unit, or as many ways as parts: 777 x 200 from 64 parts 7 us in 4 ways, 25 in 64; 9 x 64 from 1 024 parts 5.6 us
+      // in 64, 12 in 16
       const uint64_t waves = cdiv(total, 256);
       if (splits <= 4 || waves >= 16 * kChips) go(std::integral_constant<int, 1>{});
       else if (splits <= 16 || waves >= kChips) go(std::integral_constant<int, 4>{});
@@ -1238,7 +1273,7 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   const int fmt = image_format(c.dt);
   if (!p.fused && !p.few && rest && p.want_w) {
     const uint32_t groups = cdiv(p.v, 64);
-    hipLaunchKernelGGL(met_kernel, dim3(cdiv(groups, 4)), dim3(256), 0, ctx->stream, (const int *)s.target, p.n, groups, s.met, s.met_count);
+    hipLaunchKernelGGL(met_kernel, dim3(groups), dim3(512), 0, ctx->stream, (const int *)s.target, p.n, s.met, s.met_count);
   }
   for (uint32_t v0 = 0; !p.fused && !p.few && v0 < p.v; v0 += p.piece) {
     const uint32_t items = std::min(p.piece, p.v - v0);
@@ -1271,10 +1306,12 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
     if (p.want_w) {
       w.A = a.rows, w.a_ld = a.rows_ld, w.k_a = p.n;
       w.n = items, w.m_tiles = cdiv(p.d, kShape[p.tile_w].bm), w.n_tiles = cdiv(items, kShape[p.tile_w].bn);
-      w.steps = cdiv(p.n, 64), w.splits = 1, w.top = x_top;
+      w.steps = cdiv(p.n, 64), w.splits = p.w_splits, w.top = x_top;
+      w.sums = s.w_sums, w.sums_pitch = up(p.d, 8), w.first = 1;
       w.out = (char *)Ow.p + (size_t)v0 * gw_stride * dtype_size(c.dt), w.out_stride = gw_stride;
       if (rest) w.met = s.met + (size_t)(v0 / 64) * kMet, w.met_count = s.met_count + v0 / 64, w.rest = rest;
-      launch_product(ctx, fmt, p.tile_w, c.dt, w);
+      launch_product(ctx, fmt, p.tile_w, true, p.w_splits > 1 ? 0 : c.dt, w);
+      if (p.w_splits > 1) join(s.w_sums, p.w_splits, p.v, x_top, false, Ow.p, gw_stride);
     }
     if (p.want_x) {
       w.met = nullptr;
@@ -1282,7 +1319,7 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
       w.n = p.n, w.m_tiles = cdiv(p.d, kShape[p.tile_x].bm), w.n_tiles = cdiv(p.n, kShape[p.tile_x].bn);
       w.steps = cdiv(items, 64), w.splits = p.splits;
       w.sums = s.sums, w.sums_pitch = up(p.d, 8), w.first = v0 == 0;
-      launch_product(ctx, fmt, p.tile_x, 0, w);
+      launch_product(ctx, fmt, p.tile_x, false, 0, w);
     }
     AS_HIP(ctx, hipGetLastError());
   }

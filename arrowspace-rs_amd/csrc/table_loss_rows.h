@@ -7,8 +7,10 @@
 //   logits     A = 16 rows k of the stage, B = the rows r: a lane ends up with 8 consecutive k of ONE row r (nt_product.h's interleaving)
 //   gradient   of those 8 logits in f32, rounded to 16 bits: exactly the operand (row r, 8 consecutive k a lane group) of
 //   output     A = the SAME stage read transposed (ds_read_b64_tr_b16: 4 rows k of a column a lane), B = the gradients.
-// Against the form over G in memory this saves writing and reading 2 x 2 bytes a logit twice, for 2 d flops more a logit: a million
-// items of 128 values and 1 024 rows (bf16), backward 2.8 ms through G, 1.0 ms here.  d is bounded by the registers (d <= 256, f32 128).
+// Against the form over G in memory this saves writing and reading 2 bytes a logit, for 2 d flops more a logit: forward and backward of a
+// million items of 128 values and 1 024 rows (bf16) 2.01 ms through G, 1.27 ms so (sums 282 us, dX 440, dW 490); 512 f32 rows, 100 000
+// items of 128: 383 and 296 us.  What bounds it there: the matrix pipe and the exponentials' and packing's vector work of two waves a SIMD
+// take turns (0.27 TFLOP of logits at 282 us: 950 TFLOP/s).  d is bounded by the registers (d <= 256, f32 128).
 #pragma once
 
 #include "nt_product.h"
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossRowInputs a) {
 
 // Stages go through registers into LDS and not by direct loads: behind a direct load in flight hipcc waits for it in front of every
 // LDS read, and reads written by hand, each batch with its own wait, left the two waves of a SIMD waiting half their time (565 us for
-// the dX of 1 024 rows against a million items; this form: see the kernel).
+// the dX of 1 024 rows against a million items of 128; 440 so).
 typedef short short4v __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ u32x4 lr_row(const char *smem, uint32_t at) { return *(const u32x4 *)(smem + at); }
 // four rows of this lane's column, transposed
@@ -634,9 +636,14 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
   }
   if constexpr (ITEMS && P == 1) {  // what 16 bits left of the entries at the targets
     list_len = nt_min(list_len, kList);
-    for (uint32_t n = 0; n < list_len; ++n) {
-      const uint32_t t = __builtin_amdgcn_readfirstlane(list[wave][n][0]), at = __builtin_amdgcn_readfirstlane(list[wave][n][1]);
-      if (col != (at & 15)) continue;
+    // each column of lanes its own items' rows, all columns at once
+    uint64_t mine = 0;
+    for (uint32_t n = 0; n < list_len; ++n)
+      if ((list[wave][n][1] & 15) == col) mine |= 1ull << n;
+    while (mine) {
+      const int n = __builtin_ctzll(mine);
+      mine &= mine - 1;
+      const uint32_t t = list[wave][n][0], at = list[wave][n][1];
       const float rest = a.rest[t];
 #pragma unroll
       for (int s = 0; s < KD; ++s) {
@@ -654,7 +661,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
             out[2 * s][j] += f32x4{y[0], y[1], y[2], y[3]} * rest;
             out[2 * s + 1][j] += f32x4{y[4], y[5], y[6], y[7]} * rest;
           }
-        __builtin_amdgcn_sched_barrier(0);
+        if (s & 1) __builtin_amdgcn_sched_barrier(0);
       }
     }
   }

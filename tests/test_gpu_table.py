@@ -728,3 +728,27 @@ def test_scores4_codes_and_scores_of_more_than_4_gib():
     size = x.double().abs() @ w.abs().t().contiguous()
     bound = (d + 16) * E * size + 2.0 ** -11 * want.abs() + torch.finfo(torch.float16).tiny
     _close(got[:, at], want, bound, "scores")
+
+
+def test_items_of_an_index_in_4_bits():
+    """ArrowSpace.pack4 of host and of device items: the same codes, and the scores of queries from them."""
+    rows = np.random.default_rng(1).standard_normal((700, 96))
+    host, there = A.ArrowSpace(rows), A.ArrowSpace(torch.from_numpy(rows).cuda())
+    packed = [a.pack4(group=32, scale_dtype="float32") for a in (host, there)]
+    codes, s, zeros = packed[0].to_codes()
+    for a, b in zip((codes, s, zeros), packed[1].to_codes()):
+        assert np.array_equal(a, b)
+    q = np.stack((codes & 15, codes >> 4), 2).reshape(700, -1).astype(np.float64)
+    w = (q - 8) * np.repeat(s, 32, axis=1)
+    assert (np.abs(w - rows) <= np.repeat(s, 32, axis=1) * 0.5000001).all()
+    _check4(packed[1], torch.from_numpy(w).cuda(), torch.from_numpy(rows[:2]).float().cuda())
+    got = packed[0].scores(rows[3].astype(np.float32))
+    assert got.shape == (700,) and got.argmax() == 3
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, v, d", [(6000, 150, 300), (2048, 129, 384), (3001, 3, 500), (1030, 1030, 260), (700, 65, 1000)])
+def test_cross_entropy_long_rows_short_tables(n, v, d, dt):
+    """The batch in parts where the table alone does not fill the chip; many rows at each 64 items."""
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=12, bias=n % 2 == 0)
+    _check(x, w, y, b, scale=2.0)
