@@ -207,10 +207,9 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2 *part, uint
 // ---- what the products are made of ----------------------------------------------------------------------------------------------------
 // A matrix and its image: rows with their length filled to whole steps by zeros, f32 as two planes.
 struct ImageJob {
-  const void *src;
-  size_t stride;
+  const char *src;
+  size_t stride;           // bytes
   uint32_t n, d, pitch;
-  int quads;               // four values at a time can be loaded (aligned rows)
   unsigned short *out;
 };
 struct ImageJobs {
@@ -218,46 +217,39 @@ struct ImageJobs {
   unsigned int *tops;      // f32: [2] bits of the largest finite magnitude, for everyone behind
   float *parts;            // ... [2][kTopParts] of the workgroups that looked for it
 };
-// threads of a workgroup along a row of `quads` groups of four: a power of two
-__device__ __forceinline__ uint32_t along_row(uint32_t quads) { return quads >= 256 ? 256 : quads <= 1 ? 1 : 1u << (32 - __clz(quads - 1)); }
-template <int DT>
-__device__ __forceinline__ f32x4 load_quad(const ImageJob &j, size_t row, uint32_t k) {
-  if constexpr (DT == AS_F32)
-    if (k + 4 <= j.d) {
-      f32x4 x;
-      __builtin_memcpy(&x, (const float *)j.src + row * j.stride + k, 16);  // (16-byte loads need 4-byte alignment)
-      return x;
-    }
-  if (DT != AS_F32 && j.quads && k + 4 <= j.d) {
-    const u32x2 w = *(const u32x2 *)((const unsigned short *)j.src + row * j.stride + k);
-    f32x4 x;
+// A matrix in pieces of eight columns, `across` a row, dealt to all threads of the grid, four at a time under way.  f(piece, row, column)
+template <int DT, int THREADS, class F>
+__device__ __forceinline__ void each_piece(const ImageJob &j, uint32_t across, F &&f) {
+  const uint32_t threads = gridDim.x * THREADS, first = blockIdx.x * THREADS + threadIdx.x;
+  const uint32_t row_step = threads / across, column_step = threads % across;
+  uint32_t row = first / across, column = first % across;
+  while (row < j.n) {
+    Piece8<DT> piece[4];
+    uint32_t r[4], c[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const unsigned short h = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
-      x[e] = DT == AS_BF16 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+    for (int i = 0; i < 4; ++i) {
+      r[i] = row, c[i] = column * 8;
+      if (row < j.n) piece[i].load(j.src + (size_t)row * j.stride, c[i], j.d);
+      row += row_step, column += column_step;
+      if (column >= across) column -= across, ++row;
     }
-    return x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (r[i] < j.n) f(piece[i], r[i], c[i]);
   }
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (k + e < j.d) x[e] = load_as_f32<DT>(j.src, row * j.stride + k + e);
-  return x;
 }
 // f32: the largest finite magnitude, a part per workgroup
 __global__ __launch_bounds__(1024) void top_kernel(ImageJobs jobs) {
   const ImageJob &j = jobs.job[blockIdx.y];
   __shared__ float s[16];
-  const uint32_t quads = (j.d + 3) / 4, along = along_row(quads), rows = 1024 / along;
   float m = 0.f;
-#pragma unroll 2
-  for (uint64_t r = (uint64_t)blockIdx.x * rows + threadIdx.x / along; r < j.n; r += (uint64_t)gridDim.x * rows)
-    for (uint32_t g = threadIdx.x % along; g < quads; g += along) {
-      const f32x4 x = load_quad<AS_F32>(j, r, g * 4);
+  each_piece<AS_F32, 1024>(j, (j.d + 7) / 8, [&](const Piece8<AS_F32> &p, uint32_t, uint32_t) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (fabsf(x[e]) < INFINITY) m = fmaxf(m, fabsf(x[e]));
+    for (int e = 0; e < 8; ++e) {
+      const float y = fabsf(__uint_as_float(p.w[e >> 2][e & 3]));
+      m = y < INFINITY ? fmaxf(m, y) : m;
     }
+  });
   for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
   __syncthreads();
@@ -268,22 +260,28 @@ __global__ __launch_bounds__(1024) void top_kernel(ImageJobs jobs) {
 }
 template <int DT, int FMT>
 __global__ __launch_bounds__(256) void image_kernel(ImageJobs jobs) {
-  constexpr bool two = DT == AS_F32;
   const ImageJob &j = jobs.job[blockIdx.y];
   float f = 1.f;
-  if constexpr (two) {
+  if constexpr (DT == AS_F32) {
     const unsigned int top = top_of_parts(jobs.parts + blockIdx.y * kTopParts);
     f = plane_scale(top);
     if (blockIdx.x == 0 && threadIdx.x == 0) jobs.tops[blockIdx.y] = top;
   }
-  const uint32_t quads = j.pitch / 4, along = along_row(quads), rows = 256 / along;
-  for (uint64_t r = (uint64_t)blockIdx.x * rows + threadIdx.x / along; r < j.n; r += (uint64_t)gridDim.x * rows)
-    for (uint32_t g = threadIdx.x % along; g < quads; g += along) {
-      const f32x4 x = load_quad<DT>(j, r, g * 4) * f;
-      unsigned short *o = j.out + r * j.pitch * (two ? 2 : 1) + g * 4;
-      *(u32x2 *)o = u32x2{pack2<FMT>(x[0], x[1]), pack2<FMT>(x[2], x[3])};
-      if constexpr (two) *(u32x2 *)(o + j.pitch) = u32x2{pack2<FMT>(low_part(x[0]), low_part(x[1])), pack2<FMT>(low_part(x[2]), low_part(x[3]))};
+  each_piece<DT, 256>(j, j.pitch / 8, [&](const Piece8<DT> &p, uint32_t row, uint32_t column) {
+    unsigned short *o = j.out + (size_t)row * j.pitch * (DT == AS_F32 ? 2 : 1) + column;
+    if constexpr (DT == AS_F32) {
+      u32x4 high, low;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = __uint_as_float(p.w[i >> 1][2 * (i & 1)]) * f, y = __uint_as_float(p.w[i >> 1][2 * (i & 1) + 1]) * f;
+        high[i] = pack2<FMT>(x, y), low[i] = pack2<FMT>(low_part(x), low_part(y));
+      }
+      *(u32x4 *)o = high;
+      *(u32x4 *)(o + j.pitch) = low;
+    } else {
+      *(u32x4 *)o = p.w[0];
     }
+  });
 }
 // ---- gradient of the logits ---------------------------------------------------------------------------------------------------------------
 struct GradArgs {
@@ -754,9 +752,9 @@ int few_steps(uint32_t n, uint32_t d, bool forward) {
   return kc <= 4 ? kc : kc <= 6 ? 6 : 8;
 }
 int few_share(uint32_t d) { return d <= 128 ? 1 : 4; }
-enum { kFewOne, kFewFour, kFewGrad };  // forward with one or four tiles of 16 rows, backward
+enum { kFewOne, kFewTwo, kFewFour, kFewGrad };  // forward with one, two or four tiles of 16 rows, backward
 constexpr int few_waves(int steps, bool f32, int what) {
-  return f32 ? (steps <= (what == kFewOne ? 4 : 2) ? 2 : 1) : what == kFewOne ? (steps <= 4 ? 4 : steps <= 6 ? 3 : 2) : what == kFewFour ? (steps <= 1 ? 4 : steps <= 6 ? 2 : 1) : steps <= 2 ? 4 : 2;
+  return f32 ? (steps <= (what == kFewOne ? 4 : 2) ? 2 : 1) : what == kFewOne ? (steps <= 4 ? 4 : steps <= 6 ? 3 : 2) : what == kFewTwo ? (steps <= 2 ? 4 : steps <= 4 ? 3 : 2) : what == kFewFour ? (steps <= 1 ? 4 : steps <= 6 ? 2 : 1) : steps <= 2 ? 4 : 2;
 }
 uint32_t few_groups(int steps, uint32_t d, bool f32, int what, uint32_t v) {
   return std::max(1u, std::min((uint32_t)few_waves(steps, f32, what) * kChips, cdiv(v, 16 * (4 / few_share(d)))));
@@ -819,7 +817,7 @@ void plan_forward(Plan &p, bool direct) {
   p.few = direct && p.fused ? 0 : few_steps(p.n, p.d, true);
   if (p.few) {
     p.fused = 0;
-    p.few_groups = few_groups(p.few, p.d, p.planes == 2, p.n <= 16 || p.planes == 2 ? kFewOne : kFewFour, p.v);
+    p.few_groups = few_groups(p.few, p.d, p.planes == 2, p.n <= 16 || p.planes == 2 ? kFewOne : p.n <= 32 ? kFewTwo : kFewFour, p.v);
     p.parts = p.few_groups * (4 / few_share(p.d));
     return;
   }
@@ -930,8 +928,8 @@ int make_operands(as_ctx *ctx, const Source &x, const Source &t, bool raw, unsig
       *ld = (size_t)s.pitch() * s.planes() * 2;
     }
     if (s.direct() || (raw && s.dt != AS_F32)) return;
-    jobs.job[count++] = ImageJob{s.p, s.stride, s.rows, s.d, s.pitch(), (s.stride % 4 == 0 && ((uintptr_t)s.p & (4 * es - 1)) == 0) ? 1 : 0, image};
-    most = std::max<uint64_t>(most, (uint64_t)s.rows * s.pitch() / 1024);
+    jobs.job[count++] = ImageJob{(const char *)s.p, s.stride * es, s.rows, s.d, s.pitch(), image};
+    most = std::max<uint64_t>(most, (uint64_t)s.rows * s.pitch() / 4096);
   };
   add(x, x_image, &out->x, &out->x_ld);
   add(t, t_image, &out->t, &out->t_ld);
@@ -1001,8 +999,13 @@ void launch_few_sums(as_ctx *ctx, const Plan &p, bool general, LossFewArgs a) {
     } else if constexpr (!F32) {
       a.row_blocks = 1;
       const dim3 grid(up(p.few_groups, 8));
-      if (general) hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 4, true, WK, few_waves(KC, F32, kFewFour)>), grid, dim3(256), 0, ctx->stream, a);
-      else hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 4, false, WK, few_waves(KC, F32, kFewFour)>), grid, dim3(256), 0, ctx->stream, a);
+      if (p.n <= 32) {
+        if (general) hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 2, true, WK, few_waves(KC, F32, kFewTwo)>), grid, dim3(256), 0, ctx->stream, a);
+        else hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 2, false, WK, few_waves(KC, F32, kFewTwo)>), grid, dim3(256), 0, ctx->stream, a);
+      } else {
+        if (general) hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 4, true, WK, few_waves(KC, F32, kFewFour)>), grid, dim3(256), 0, ctx->stream, a);
+        else hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 4, false, WK, few_waves(KC, F32, kFewFour)>), grid, dim3(256), 0, ctx->stream, a);
+      }
     }
   });
 }

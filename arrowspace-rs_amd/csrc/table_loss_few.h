@@ -82,13 +82,24 @@ struct LossFewArgs {
 };
 
 // KC steps of 32 columns a wave (d <= 128 KC); RT tiles of 16 rows
-template <int DT, int KC>
+template <int DT, int KC, bool BIAS>
 struct FewSlice {
   static constexpr int FMT = DT == AS_F16 ? AS_F16 : AS_BF16, P = DT == AS_F32 ? 3 : 1;
   static constexpr uint32_t CW = 32 * KC, kRow = CW * 2 + 16, kPlane = 16 * kRow, kWave = P * kPlane;  // (16 bytes between rows: eight rows of a read in different banks)
   LrPiece<DT, true> piece[KC];
+  f32x4 bias;  // of this lane's four items
   __device__ __forceinline__ void load(const LossFewArgs &a, uint32_t column0, uint32_t stage) {
     const uint32_t lane = threadIdx.x & 63;
+    bias = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (BIAS && a.bias) {
+      const uint32_t item = stage * 16 + (lane >> 4) * 4;
+      if (stage * 16 + 16 <= a.v) {
+        __builtin_memcpy(&bias, a.bias + item, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bias[e] = a.bias[nt_min(item + e, a.v - 1)];
+      }
+    }
 #pragma unroll
     for (int t = 0; t < KC; ++t) {
       const uint32_t idx = t * 64 + lane, row = idx / (4 * KC), slot = idx % (4 * KC);
@@ -125,8 +136,8 @@ struct FewSlice {
   }
 };
 template <int DT, int KC, int RT>
-__device__ __forceinline__ void few_rows(const LossFewArgs &a, uint32_t n, uint32_t column0, u32x4 (&R)[FewSlice<DT, KC>::P][RT][KC]) {
-  constexpr int P = FewSlice<DT, KC>::P, FMT = FewSlice<DT, KC>::FMT;
+__device__ __forceinline__ void few_rows(const LossFewArgs &a, uint32_t n, uint32_t column0, u32x4 (&R)[FewSlice<DT, KC, false>::P][RT][KC]) {
+  constexpr int P = FewSlice<DT, KC, false>::P, FMT = FewSlice<DT, KC, false>::FMT;
   const uint32_t lane = threadIdx.x & 63, q = lane >> 4, col = lane & 15;
 #pragma unroll
   for (int j = 0; j < RT; ++j)
@@ -144,7 +155,7 @@ __device__ __forceinline__ void few_rows(const LossFewArgs &a, uint32_t n, uint3
 // WK waves share the columns: 4, or 1
 template <int DT, int KC, int RT, bool GENERAL, int WK, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void loss_few_sums_kernel(LossFewArgs a) {
-  typedef FewSlice<DT, KC> Slice;
+  typedef FewSlice<DT, KC, GENERAL> Slice;
   constexpr int P = Slice::P, TS = WK == 1 ? RT : 1;  // TS: row tiles whose statistics a wave keeps (WK 4: wave w those of tile w)
   __shared__ __attribute__((aligned(16))) char smem[4 * Slice::kWave];
   __shared__ f32x4 meet[WK == 4 ? 2 : 1][4][RT][64];
@@ -169,6 +180,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_sums_kernel(LossFewArgs a
   for (int t = 0; t < TS; ++t) ref[t] = -INFINITY, base[t] = 0.f, sum[t] = 0.f;
   auto step = [&](uint32_t s, Slice &slice) {
     slice.store(mine);
+    const f32x4 bias = slice.bias;
     if (s + 2 < s_hi) slice.load(a, column0, s + 2);
     wave_lds_order();
     f32x4 z[RT];
@@ -186,7 +198,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_sums_kernel(LossFewArgs a
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t item = s * 16 + q * 4 + e;
-        if (GENERAL) l[e] = fmaf(l[e], a.scale, a.bias && item < a.v ? a.bias[item] : 0.f);
+        if (GENERAL) l[e] = fmaf(l[e], a.scale, bias[e]);
         if (item >= a.v) l[e] = -INFINITY;
       }
       const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
@@ -223,7 +235,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_sums_kernel(LossFewArgs a
 
 template <int DT, int KC, bool BIAS, int WK, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void loss_few_grad_kernel(LossFewArgs a) {
-  typedef FewSlice<DT, KC> Slice;
+  typedef FewSlice<DT, KC, BIAS> Slice;
   constexpr int P = Slice::P, FMT = Slice::FMT;
   __shared__ __attribute__((aligned(16))) char smem[4 * Slice::kWave];
   __shared__ f32x4 meet[WK == 4 ? 2 : 1][4][64];
@@ -265,6 +277,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_grad_kernel(LossFewArgs a
   const uint32_t trow = q * 4 + ((lane >> 2) & 3);
   auto step = [&](uint32_t s, Slice &slice) {
     slice.store(mine);
+    const f32x4 bias = slice.bias;
     if (s + AHEAD < s_hi) slice.load(a, column0, s + AHEAD);
     wave_lds_order();
     f32x4 z[1];
@@ -278,9 +291,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_grad_kernel(LossFewArgs a
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t item = s * 16 + q * 4 + e;
-      float b = 0.f;
-      if constexpr (BIAS) b = item < a.v ? a.bias[item] : 0.f;
-      const float l = BIAS ? fmaf(g[e], a.scale, b) - lse : fmaf(g[e], a.scale, -lse);
+      const float l = BIAS ? fmaf(g[e], a.scale, bias[e]) - lse : fmaf(g[e], a.scale, -lse);
       g[e] = item < a.v ? every * __builtin_amdgcn_exp2f(l * kLog2e) : 0.f;
       if (target == item) g[e] = entry;
     }
