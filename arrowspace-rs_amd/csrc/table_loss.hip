@@ -13,9 +13,9 @@
 // and its part of dX (f32, added up over the pieces in a buffer, rounded once at the end).
 // Nothing is added with atomics: results do not change from run to run.
 // What bounds it: 2 n v d flops forward, 8 more backward, of which 2 are the logits again (through G: 6, written and read once: 2 bytes a
-// logit each).  8 192 rows x 131 072 items of 1 024 (bf16), forward and backward: 8.23 ms = 1 069 TFLOP/s, one library product of this
-// size runs at 1 076; 4 096 x 100 000 of 768 with a bias: 2.83 ms; 1 024 x 1 000 000 of 128: 1.27 ms, 2.01 through G; 777 x 31 013 of 200
-// (f16): 0.16, 0.18 through G; f32, 512 x 100 000 of 128: 0.30, 0.38 through G.
+// logit each).  8 192 rows x 131 072 items of 1 024 (bf16), forward and backward: 8.04 ms = 1 094 TFLOP/s, one library product of this
+// size runs at 1 076; 4 096 x 100 000 of 768 with a bias: 2.67 ms; 1 024 x 1 000 000 of 128: 1.27 ms, 2.01 through G; 777 x 31 013 of 200
+// (f16): 0.14, 0.18 through G; f32, 512 x 100 000 of 128: 0.29, 0.38 through G.
 // Types.  bf16 and f16 go to the matrix pipe as they are.  f32 values go as a sum of two f16 (22 bits, after a power of two that
 // brings the matrix' largest finite value to 2^14 .. 2^15), three products per pair of planes: 2.5 PFLOP/s / 3 against the
 // 0.157 of the f32 instruction, and an error per product of 2^-23 of it, which the f32 sums have anyway.
