@@ -791,7 +791,7 @@ void plan_backward(Plan &p, bool x, bool w, bool b) {
   const uint64_t per_item = (uint64_t)p.n_pad * 2 * p.planes;
   const uint32_t round = std::max(1u, (uint32_t)kChips / cdiv(p.d, 256)) * 256;
   uint64_t piece = std::max<uint64_t>((320ull << 20) / per_item / round, 1) * round;
-  if (piece * per_item > (512ull << 20)) piece = std::max<uint64_t>((256ull << 20) / per_item / 1024 * 1024, 1024);
+  if (piece * per_item > (512ull << 20)) piece = std::max<uint64_t>((256ull << 20) / per_item / 256 * 256, 256);
   piece = std::min<uint64_t>(piece, up(p.v, bm));
   p.piece = (uint32_t)up(piece, bm);
   p.pieces = cdiv(p.v, p.piece);

@@ -112,10 +112,20 @@ template <int THREADS>
 __device__ __forceinline__ void unit_of_rows(const float *gl, const float *ge, const int64_t *targets, int64_t ignore, uint32_t n, int power, float *factor, float *unit) {
   __shared__ float s[2][THREADS / 64];
   float one = 0.f, both = 0.f;
-  for (uint32_t t = threadIdx.x; t < n; t += THREADS) {
-    const float l = targets[t] == ignore ? 0.f : gl[t], b = fabsf(l + (ge ? ge[t] : 0.f)), o = fabsf(l);
-    if (o < INFINITY) one = fmaxf(one, o);
-    if (b < INFINITY) both = fmaxf(both, b);
+  for (uint32_t t0 = threadIdx.x; t0 < n; t0 += 4 * THREADS) {
+    float l[4], e[4];
+    int64_t y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t t = t0 + k * THREADS, at = t < n ? t : threadIdx.x;
+      y[k] = targets[at], l[k] = gl[at], e[k] = ge ? ge[at] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float x = y[k] == ignore ? 0.f : l[k], b = fabsf(x + e[k]), o = fabsf(x);
+      if (o < INFINITY) one = fmaxf(one, o);
+      if (b < INFINITY) both = fmaxf(both, b);
+    }
   }
   for (int k = 1; k < 64; k <<= 1) {
     one = fmaxf(one, __shfl_xor(one, k));

@@ -752,3 +752,17 @@ def test_cross_entropy_long_rows_short_tables(n, v, d, dt):
     """The batch in parts where the table alone does not fill the chip; many rows at each 64 items."""
     x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=12, bias=n % 2 == 0)
     _check(x, w, y, b, scale=2.0)
+
+
+@pytest.mark.parametrize("n, v, d, dt", [(150_001, 300, 40, "bf16"), (150_001, 260, 270, "f16"), (70_001, 33, 300, "f32"), (5, 40, 5000, "bf16"),
+                                         (70, 130, 20000, "f32"), (3, 17, 65536, "f16")])
+def test_cross_entropy_many_rows_and_long_rows(n, v, d, dt):
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=13, bias=True, ignored=0.1)
+    _check(x, w, y, b, scale=1.0)
+
+
+def test_scores4_no_rows_and_many():
+    codes, s, z, w = _plain4(60, 90, 32, "f32", True, 14)
+    t = A.Table4.from_codes(codes, s, z, dim=90, group=32)
+    assert t.scores(torch.empty(0, 90, device="cuda")).shape == (0, 60)
+    _check4(t, w, torch.randn(1000, 90, device="cuda").bfloat16())
