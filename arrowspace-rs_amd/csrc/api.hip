@@ -518,7 +518,11 @@ void as_ctx_destroy(as_ctx *ctx) {
   prof_resolve(ctx);
   handle_cache_stream(ctx->device, ctx->stream, false);
   if (ctx->own_stream) (void)hipStreamDestroy(ctx->stream);
-  for (hipStream_t s : ctx->capture_left) (void)hipStreamSynchronize(s);
+  for (hipStream_t s : ctx->capture_left) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &st) == hipSuccess && st == hipStreamCaptureStatusNone) (void)hipStreamSynchronize(s);
+    (void)hipGetLastError();
+  }
   for (hipStream_t s : ctx->parked_streams) {
     (void)hipStreamSynchronize(s);
     (void)hipStreamDestroy(s);
@@ -550,9 +554,16 @@ int as_ctx_set_stream(as_ctx *ctx, void *hip_stream) {
     handle_cache_stream(ctx->device, ctx->stream, true);
     return AS_OK;
   }
-  (void)hipStreamSynchronize(ctx->stream);
-  for (hipStream_t s : ctx->capture_left) (void)hipStreamSynchronize(s);   // (streams left for a capture, not waited for then)
-  ctx->capture_left.clear();
+  // (streams left for a capture, not waited for then; one that is being captured cannot be waited for now either)
+  if (std::find(ctx->capture_left.begin(), ctx->capture_left.end(), ctx->stream) == ctx->capture_left.end()) ctx->capture_left.push_back(ctx->stream);
+  std::vector<hipStream_t> still;
+  for (hipStream_t s : ctx->capture_left) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &st) != hipSuccess) (void)hipGetLastError();
+    if (st != hipStreamCaptureStatusNone) still.push_back(s);
+    else (void)hipStreamSynchronize(s);
+  }
+  ctx->capture_left.swap(still);
   for (hipStream_t s : ctx->parked_streams) {
     (void)hipStreamSynchronize(s);
     (void)hipStreamDestroy(s);

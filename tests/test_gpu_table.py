@@ -766,3 +766,32 @@ def test_scores4_no_rows_and_many():
     t = A.Table4.from_codes(codes, s, z, dim=90, group=32)
     assert t.scores(torch.empty(0, 90, device="cuda")).shape == (0, 60)
     _check4(t, w, torch.randn(1000, 90, device="cuda").bfloat16())
+
+
+def test_leaving_a_stream_while_it_is_captured():
+    """A context moved to another stream in the middle of a capture: the capture goes on, and the graph's results are the eager ones."""
+    x, w, y, _ = _inputs(40, 900, 64, torch.bfloat16, seed=15)
+    want = A.cross_entropy(x, w, y)
+    ctx = A.Context(0)
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+    out, lse = torch.empty(40, device="cuda"), torch.empty(40, device="cuda")
+    ws = torch.empty(ctx.lib.as_cross_entropy_workspace(40, 900, 64, _lib.AS_BF16, 0), dtype=torch.uint8, device="cuda")
+    call = (x.data_ptr(), 40, 64, w.data_ptr(), 900, 64, 64, _lib.AS_BF16, None, y.data_ptr(), -100, 1.0, out.data_ptr(), lse.data_ptr(), ws.data_ptr(),
+            ws.numel())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        graph.capture_begin(capture_error_mode="relaxed")
+        ctx.set_stream(stream.cuda_stream)
+        first = ctx.lib.as_cross_entropy(ctx.h, *call)
+        ctx.set_stream(other.cuda_stream)
+        ctx.set_stream(stream.cuda_stream)
+        second = ctx.lib.as_cross_entropy(ctx.h, *call)
+        graph.capture_end()
+    assert (first, second) == (_lib.AS_OK, _lib.AS_OK)
+    for _ in range(3):
+        out.zero_(), lse.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    ctx.set_stream(other.cuda_stream)
