@@ -743,10 +743,10 @@ int fused_steps(uint32_t d, uint32_t planes) { return d <= 64 ? 2 : d <= 128 ? 4
 // 128 values 2 x 3 515 / 439, 3 x 2 490 / 480, 4 x 2 728 / 632 (spills); 256 values 1 x 2 1 273 / 1 262, 2 x 2 1 437 / 1 410 (spills)
 constexpr int fused_rows(int steps, int planes, bool items) { return planes == 2 ? 2 : steps == 8 ? 1 : steps == 2 || items ? 3 : 2; }
 constexpr int fused_waves(int steps, int planes, bool items) { return planes == 2 || steps == 8 ? 2 : steps == 2 || !items ? 3 : 2; }
-// The form for few rows: 16 (forward 64) rows, as many columns as four waves hold; up to 128 columns (four steps) a wave takes whole
-// items.  Waves a SIMD: what its registers leave.
-int few_steps(uint32_t n, uint32_t d, bool forward) {
-  if (d > 1024 || n > (forward ? 64u : 16u)) return 0;
+// The form for few rows: its steps of 32 columns a wave, as many columns as four waves hold; up to 128 columns (four steps) a wave takes
+// whole items.  Waves a SIMD: what its registers leave.
+int few_steps(uint32_t d) {
+  if (d > 1024) return 0;
   if (d <= 128) return d <= 32 ? 1 : d <= 64 ? 2 : 4;
   const int kc = (int)cdiv(d, 128);
   return kc <= 4 ? kc : kc <= 6 ? 6 : 8;
@@ -765,7 +765,7 @@ uint32_t few_groups(int steps, uint32_t d, bool f32, int what, uint32_t v) {
 bool raw_pays(const Plan &p) { return p.n <= 128; }
 void plan_backward(Plan &p, bool x, bool w, bool b) {
   p.want_x = x, p.want_w = w, p.want_b = b;
-  p.few = few_steps(p.n, p.d, false);
+  p.few = p.n <= 16 ? few_steps(p.d) : 0;
   if (p.few) {
     p.few_groups = p.splits = few_groups(p.few, p.d, p.planes == 2, kFewGrad, p.v);
     p.n_pad = 64;
@@ -811,10 +811,20 @@ void plan_backward(Plan &p, bool x, bool w, bool b) {
 
 // waves a SIMD of the forward (1 024 rows x 1 M items of 128: four tiles of rows x 2 waves 293 us, x 3 282, two x 4 316)
 constexpr int sums_waves(int steps, int planes, int tiles) { return steps * planes == 8 || tiles < 4 ? 2 : steps * planes == 4 ? 3 : 4; }
-void plan_forward(Plan &p, bool direct) {
+// Forward, up to 64 rows: a table that is an operand as it lies streams through the other forms at 5 to 6 TB/s (4 to 64 rows, 512 187 items
+// of 640 (f16): 124 us, in the form for few rows 190 to 281; small tables are quicker without the tiles: 20 rows, 10 000 of 768 16 and
+// 19 us).  What would need an image does not: 56 bf16 rows, 500 000 of 700 at an odd stride, 297 and 432 us; 16 rows of 200 47 and 75
+// (60 rows 84 and 81); 16 f32 rows, 500 000 of 128 62 and 105 (42 rows 95 and 90).  16-bit rows of up to 128 are shifted as quickly by
+// the short rows' form (16 rows of 100, 50 us, here 57).
+bool few_pays(const Plan &p, bool table_direct) {
+  if (p.n > 64) return false;
+  if (p.planes == 2) return p.n <= 32 || p.d > 128;
+  if (table_direct) return !p.fused && (uint64_t)p.v * p.d < (16ull << 20);
+  return p.d > 128 && (p.n <= 32 || p.d > 256);
+}
+void plan_forward(Plan &p, bool table_direct) {
   p.fused = fused_steps(p.d, p.planes);
-  // (rows that are operands as they lie go by whole stages: a pass at 6.4 TB/s)
-  p.few = direct && p.fused ? 0 : few_steps(p.n, p.d, true);
+  p.few = few_pays(p, table_direct) ? few_steps(p.d) : 0;
   if (p.few) {
     p.fused = 0;
     p.few_groups = few_groups(p.few, p.d, p.planes == 2, p.n <= 16 || p.planes == 2 ? kFewOne : p.n <= 32 ? kFewTwo : kFewFour, p.v);
@@ -991,21 +1001,25 @@ void launch_few_sums(as_ctx *ctx, const Plan &p, bool general, LossFewArgs a) {
     constexpr int DT = decltype(type)::value, KC = decltype(kc)::value, WK = decltype(share)::value;
     constexpr bool F32 = DT == AS_F32;
     a.slices = p.few_groups;
-    if (p.n <= 16 || F32) {  // (f32: 16 rows at a time, their planes leave no room for more)
+    if constexpr (F32) {  // (16 rows at a time, their planes leave no room for more)
       a.row_blocks = cdiv(p.n, 16);
       const dim3 grid(up(p.few_groups, 8) * a.row_blocks);
       if (general) hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 1, true, WK, few_waves(KC, F32, kFewOne)>), grid, dim3(256), 0, ctx->stream, a);
       else hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 1, false, WK, few_waves(KC, F32, kFewOne)>), grid, dim3(256), 0, ctx->stream, a);
-    } else if constexpr (!F32) {
+    } else if constexpr (WK == 4) {  // (few_pays: 16-bit rows of up to 128 columns, and 33 to 64 of up to 256, go another way)
+      auto go = [&](auto tiles, auto gen) {
+        constexpr int RT = decltype(tiles)::value;
+        hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, RT, decltype(gen)::value, WK, few_waves(KC, F32, RT == 1 ? kFewOne : RT == 2 ? kFewTwo : kFewFour)>),
+                           dim3(up(p.few_groups, 8)), dim3(256), 0, ctx->stream, a);
+      };
+      auto by_rows = [&](auto gen) {
+        if (p.n <= 16) go(std::integral_constant<int, 1>{}, gen);
+        else if (p.n <= 32) go(std::integral_constant<int, 2>{}, gen);
+        else if constexpr (KC > 2) go(std::integral_constant<int, 4>{}, gen);
+      };
       a.row_blocks = 1;
-      const dim3 grid(up(p.few_groups, 8));
-      if (p.n <= 32) {
-        if (general) hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 2, true, WK, few_waves(KC, F32, kFewTwo)>), grid, dim3(256), 0, ctx->stream, a);
-        else hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 2, false, WK, few_waves(KC, F32, kFewTwo)>), grid, dim3(256), 0, ctx->stream, a);
-      } else {
-        if (general) hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 4, true, WK, few_waves(KC, F32, kFewFour)>), grid, dim3(256), 0, ctx->stream, a);
-        else hipLaunchKernelGGL((loss_few_sums_kernel<DT, KC, 4, false, WK, few_waves(KC, F32, kFewFour)>), grid, dim3(256), 0, ctx->stream, a);
-      }
+      if (general) by_rows(std::true_type{});
+      else by_rows(std::false_type{});
     }
   });
 }
@@ -1088,9 +1102,8 @@ int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tabl
   AS_TRY(S.bind(ctx, lse, c.n * 4));
   Plan p = make_plan((uint32_t)c.n, (uint32_t)c.v, (uint32_t)c.d, c.dt);
   const int columns = fused_steps(p.d, p.planes) * 32;
-  auto source = [&](const void *m, uint64_t stride, uint32_t rows, uint32_t whole) { return Source{m, (size_t)stride, rows, p.d, c.dt, whole}; };
-  plan_forward(p, columns && source(X.p, c.x_stride, p.n, columns).direct() && source(W.p, c.table_stride, p.v, columns).direct());
-  const Source xs = source(X.p, c.x_stride, p.n, p.pitch), ts = source(W.p, c.table_stride, p.v, p.pitch);
+  plan_forward(p, Source{W.p, (size_t)c.table_stride, p.v, p.d, c.dt, columns ? columns : p.pitch}.direct());
+  const Source xs{X.p, (size_t)c.x_stride, p.n, p.d, c.dt, p.pitch}, ts{W.p, (size_t)c.table_stride, p.v, p.d, c.dt, p.pitch};
   ForwardScratch s{};
   Scratch scratch;
   AS_TRY(scratch.open(ctx, workspace, workspace_bytes, forward_layout(p, xs, ts, nullptr, s)));

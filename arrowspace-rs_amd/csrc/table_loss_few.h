@@ -11,8 +11,9 @@
 // Up to 128 columns a wave takes whole items instead, each its own stretch of the table, and nothing meets before the end.
 // Rows of any alignment go in and out in 16-byte pieces: element by element the stores of 8 rows' dW (538 194 items of 337, f16) took
 // 532 us, so 274.
-// Measured, forward and backward: 8 rows, 500 000 items of 384 (bf16, 384 MB read, then read and written): 99 and 235 us = 3.9 and
-// 3.3 TB/s; 2 rows, 688 025 of 678 at an odd stride: 266 and 641 (through images and G 2 744 in all); 9 rows, 496 726 of 64: backward 27.
+// Measured: backward of 8 rows, 500 000 items of 384 (bf16, 384 MB read and written) 235 us = 3.3 TB/s, through G 389; of 9 rows, 496 726
+// of 64 27 and 63; of 8 f32 rows, 300 000 of 384 353 and 817.  Forward (few_pays in table_loss.hip: where the table would need an image)
+// of 2 rows, 688 025 of 678 at an odd stride 266, backward 641, through images and G 2 744 in all.
 #pragma once
 
 #include "table_loss_rows.h"
