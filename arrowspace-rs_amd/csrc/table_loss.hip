@@ -1164,6 +1164,8 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   if (gb && !bias) return fail(ctx, AS_ERR_ARG, "a gradient of the bias without a bias");
   if ((gx && gx_stride < c.d) || (gw && gw_stride < c.d)) return fail(ctx, AS_ERR_ARG, "a row stride below the number of columns");
   if (!gx && !gw && !gb) return AS_OK;
+  if ((gx && (gx == x || gx == table || gx == gw)) || (gw && (gw == x || gw == table)))
+    return fail(ctx, AS_ERR_ARG, "gradients must not share memory with the inputs or each other");
   if (c.n && (!x || !table || !targets || !lse || !gl)) return fail(ctx, AS_ERR_ARG, "null argument");
   AS_TRY(check_targets(ctx, targets, c.n, c.v, ignore));
   BytesIn X, W, Bi, Y, Ls, Gl, Ge;

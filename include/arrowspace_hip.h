@@ -502,8 +502,8 @@ int as_range_search(as_ctx *ctx, const as_index *index, double lambda_q, double 
  *     scratch.  A call on a stream that is being captured into a graph must bring one (AS_ERR_UNSUPPORTED otherwise): the graph
  *     keeps its address, so two graphs that may run at once need two.  Host memory and as_table4_import / _pack / _export are
  *     refused during a capture.
- *   - Every pointer is host memory or memory of the context's device (AS_ERR_ARG for another device's).  The caller's current
- *     device is left as it was.  Results are the same from run to run: nothing is summed with atomics.
+ *   - Every pointer is host memory or memory of the context's device (AS_ERR_ARG for another device's).  Outputs share no memory
+ *     with inputs, the workspace or each other.  The caller's current device is left as it was.  Results are the same from run to run: nothing is summed with atomics.
  *
  * Softmax cross entropy of n rows against n_items items, without keeping the n x n_items logits:
  *   l_tv = scale <x_t, w_v> + bias_v     lse_t = log sum_v exp(l_tv)     losses_t = lse_t - l_{t, targets_t}

@@ -795,3 +795,16 @@ def test_leaving_a_stream_while_it_is_captured():
         torch.cuda.synchronize()
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
     ctx.set_stream(other.cuda_stream)
+
+
+def test_gradients_in_place_of_the_inputs_are_refused():
+    x, w, y, _ = _inputs(8, 100, 64, torch.bfloat16, seed=16)
+    losses, lse = A.cross_entropy(x, w, y)
+    gl = torch.ones(8, device="cuda")
+    ctx = A.Context(0)
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    gx, gw = torch.empty_like(x), torch.empty_like(w)
+    for a, b in ((x, gw), (w, gw), (gx, w), (gx, x), (gw, gw)):
+        rc = ctx.lib.as_cross_entropy_backward(ctx.h, x.data_ptr(), 8, 64, w.data_ptr(), 100, 64, 64, _lib.AS_BF16, None, y.data_ptr(), -100, 1.0,
+                                               lse.data_ptr(), gl.data_ptr(), None, a.data_ptr(), 64, b.data_ptr(), 64, None, None, 0)
+        assert rc == _lib.AS_ERR_ARG
