@@ -17,6 +17,7 @@
 // of a group are summed in f32 by the matrix pipe, groups in f32 after their scale.
 // Layout (made once, by the handle): tiles of 16 items x 128 k, 1 KB: lane l of a wave holds item l & 15 and, of each 32 k, the 8
 // from 8 (l >> 4): its operand of four instructions in one 16-byte load.  Scales of a tile: item by item its 4 / 2 / 1 groups.
+#include "table4_address.h"
 #include "table_common.h"
 
 using namespace asx;
@@ -335,15 +336,14 @@ struct RowOperands {};
 template <int PLANES>
 struct RowOperands<PLANES, kInMemory> {
   u32x4 x[PLANES][4];
-  __device__ __forceinline__ void load(const ScoresArgs &a, size_t at, uint32_t in_row, uint32_t kt) {  // in_row: bytes from the row's start at step 0
+  __device__ __forceinline__ void load(const ScoresArgs &a, size_t row_at, uint32_t q, uint32_t kt) {
 #pragma unroll
     for (int p = 0; p < PLANES; ++p)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t k = kt * a.per_tile + j * a.per_step;
-        const bool there = in_row + k < a.k_bytes;
-        const u32x4 y = *(const u32x4 *)(a.operand + p * a.plane + at + (there ? k : 0u));
-        x[p][j] = there ? y : u32x4{0u, 0u, 0u, 0u};
+        const u32x4 y = *(const u32x4 *)(a.operand + p * a.plane + row_piece_at(row_at, q * a.lane_q, q * 16, k, a.k_bytes));
+        x[p][j] = row_piece_there(q * 16, k, a.k_bytes) ? y : u32x4{0u, 0u, 0u, 0u};
       }
   }
 };
@@ -368,12 +368,12 @@ __global__ __launch_bounds__(64 * kWaves, 2 * resident_groups(MB, PG)) void scor
   const uint32_t k_lo = (uint32_t)((uint64_t)a.k_tiles * sub / a.split), k_hi = (uint32_t)((uint64_t)a.k_tiles * (sub + 1) / a.split);
   const uint32_t first = blockIdx.x * teams + wave / a.split;
   const uint32_t rounds = (a.units + stride - 1) / stride;
-  const size_t of_lane = at_most(FEW ? col >> 2 : col, a.m - 1) * a.lane_row + q * a.lane_q, in_row = q * 16;
+  const size_t row_at = at_most(FEW ? col >> 2 : col, a.m - 1) * a.lane_row;
   Step ring[AHEAD + 1];
   uint32_t ahead_unit = first, ahead_kt = k_lo;  // what is asked for next (behind the last unit: that one again)
   auto ask = [&](Step &s) {
     s.tiles.load(a, at_most(ahead_unit, a.units - 1), ahead_kt);
-    if constexpr (FROM == kInMemory) s.rows.load(a, of_lane, in_row, ahead_kt);
+    if constexpr (FROM == kInMemory) s.rows.load(a, row_at, q, ahead_kt);
     if (++ahead_kt == k_hi) ahead_kt = k_lo, ahead_unit += stride;
   };
 #pragma unroll
