@@ -1,9 +1,11 @@
 """Operators over a table of rows (what an index holds), over the C ABI: softmax cross entropy against all its items with the
 gradient, and products with a table held in 4 bits.  They have no counterpart in the reference.
 
-Matrices are torch tensors (on a GPU: used in place, on torch's current stream of that GPU, nothing waited for, capturable into a
-graph) or numpy arrays (staged; results come back as numpy arrays, complete).  Rows may be rows of a wider tensor; the values of a
-row must be adjacent.
+Matrices are torch tensors (on a GPU: used in place, on torch's current stream of that GPU, capturable into a graph) or numpy arrays
+(staged; results come back as numpy arrays, complete).  Results lie where the first argument does; the others may be host memory or on
+one GPU, and as soon as one of them is, the call runs on torch's current stream there.  The host waits for the GPU only where host memory
+is copied, and where a thread goes on to another stream than its last call's: for that call's stream.  Rows may be rows of a wider
+tensor; the values of a row must be adjacent.
 """
 import ctypes as C
 import threading
@@ -46,13 +48,15 @@ def _thread_context(device):
 
 
 class _Call:
-    """Where a call's data live, and its context with the right stream."""
+    """Where a call's data live, and its context with the right stream: torch's current one of the GPU that ANY of the arguments is on
+    (that is where the others are written too, whether the first one is host memory or not).  Outputs lie beside the first."""
     __slots__ = ("device", "cuda", "ctx", "torch")
 
-    def __init__(self, first, ctx):
+    def __init__(self, first, ctx, *others):
         if isinstance(first, DeviceArray):
             raise TypeError("a DeviceArray is not taken here: torch tensors or numpy arrays")
         self.device, self.cuda, self.torch = None, False, False
+        index = None
         if is_tensor(first):
             if _torch is None:
                 _need_torch()
@@ -60,7 +64,15 @@ class _Call:
             self.device = first.device
             self.cuda = first.is_cuda
         if self.cuda:
-            index = self.device.index
+            index = self.device.index   # (a tensor of another device than this one's is refused by the library)
+        else:
+            for a in others:
+                if a is not None and is_tensor(a) and a.is_cuda:
+                    if _torch is None:
+                        _need_torch()
+                    index = a.device.index
+                    break
+        if index is not None:
             if ctx is None:
                 ctx = _thread_context(index)
             elif ctx.device != index:
@@ -135,7 +147,7 @@ def _vector(a, n, dtype, what):
     return a.data_ptr(), a
 
 
-def _loss_args(x, table, bias, targets, ctx):
+def _loss_args(x, table, bias, targets, ctx, *others):
     first = x
     x, n, d, xs, xp = _matrix(x, "x")
     table, v, dw, ts, tp = _matrix(table, "table")
@@ -148,7 +160,7 @@ def _loss_args(x, table, bias, targets, ctx):
     yp, targets = _vector(targets, n, "int64", "targets")
     if yp is None:
         raise ArrowSpaceError(_lib.AS_ERR_ARG, "null argument")
-    call = _Call(first, ctx)
+    call = _Call(first, ctx, table, bias, targets, *others)
     return call, (xp, n, xs, tp, v, ts, d, kind, bp, yp), (x, table, bias, targets)
 
 
@@ -178,7 +190,7 @@ def cross_entropy_backward(x, table, targets, lse, grad_losses, bias=None, scale
     ep, grad_lse = _vector(grad_lse, rows, "float32", "grad_lse")
     if lp is None or gp is None:
         raise ArrowSpaceError(_lib.AS_ERR_ARG, "null argument")
-    call, (xp, n, xs, tp, v, ts, d, kind, bp, yp), alive = _loss_args(x, table, bias, targets, ctx)
+    call, (xp, n, xs, tp, v, ts, d, kind, bp, yp), alive = _loss_args(x, table, bias, targets, ctx, lse, grad_losses, grad_lse)
     none = (None, None)
     gx, gxp = call.empty((n, d), _NAMES[kind]) if need_x else none
     gw, gwp = call.empty((v, d), _NAMES[kind]) if need_table else none
@@ -241,7 +253,7 @@ class Table4:
         if n > 1 and (step != half or sstep != groups or (zeros is not None and zstep != groups)):
             raise ArrowSpaceError(_lib.AS_ERR_ARG, "codes, scales and zeros must be dense")
         scale_kind = _scale_kind(_name(scales))
-        call = _Call(first, ctx)
+        call = _Call(first, ctx, scales, zeros)
         h = C.c_void_p()
         call.ctx.check(call.ctx.lib.as_table4_import(call.ctx.h, cp, sp, zp, n, dim, int(group), scale_kind, C.byref(h)))
         return cls(call.ctx, h)

@@ -1,0 +1,87 @@
+"""Which stream a call of the operators over a table runs on, without a GPU: tensors that say they are on one, a library that notes calls."""
+import numpy as np
+import pytest
+
+import arrowspace_amd as A
+from arrowspace_amd import _lib
+from arrowspace_amd import table as T
+
+torch = pytest.importorskip("torch")
+
+
+class _OnGpu(torch.Tensor):
+    is_cuda = True
+    device = torch.device("cuda", 0)
+
+
+def _gpu(a):
+    return torch.Tensor._make_subclass(_OnGpu, torch.as_tensor(a))
+
+
+class _Library:
+    def __init__(self, calls):
+        self.calls = calls
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append(name)
+            if name.endswith("_workspace") or name in ("as_table4_items", "as_table4_dim", "as_table4_group"):
+                return 0
+            return _lib.AS_F32 if name == "as_table4_scale_dtype" else _lib.AS_OK
+        return call
+
+
+class _Ctx:
+    device = 0
+    h = None
+
+    def __init__(self):
+        self.calls = []
+        self.lib = _Library(self.calls)
+
+    def set_stream(self, s):
+        self.calls.append(("stream", s))
+
+    def check(self, rc):
+        assert rc == 0
+
+
+@pytest.fixture
+def ctx(monkeypatch):
+    T._need_torch()
+    monkeypatch.setattr(T, "_raw_stream", lambda index: 4096 + index)
+    return _Ctx()
+
+
+def _arguments():
+    return {"x": np.zeros((3, 8), np.float32), "table": np.zeros((5, 8), np.float32), "targets": np.zeros(3, np.int64),
+            "bias": np.zeros(5, np.float32), "lse": np.zeros(3, np.float32), "grad_losses": np.zeros(3, np.float32), "grad_lse": np.zeros(3, np.float32)}
+
+
+@pytest.mark.parametrize("host", ["numpy", "tensor"])
+@pytest.mark.parametrize("there", ["table", "targets", "bias", "lse", "grad_losses", "grad_lse"])
+def test_a_call_with_one_argument_on_a_gpu_runs_on_its_current_stream(ctx, there, host):
+    a = _arguments()
+    if host == "tensor":
+        a = {k: torch.from_numpy(v) for k, v in a.items()}
+    a[there] = _gpu(a[there])
+    if there in ("table", "targets", "bias"):
+        A.cross_entropy(ctx=ctx, **{k: a[k] for k in ("x", "table", "targets", "bias")})
+        assert ctx.calls.index(("stream", 4096)) < ctx.calls.index("as_cross_entropy")
+        ctx.calls.clear()
+        del ctx._stream
+    A.cross_entropy_backward(ctx=ctx, **a)
+    assert ctx.calls.index(("stream", 4096)) < ctx.calls.index("as_cross_entropy_backward")
+
+
+@pytest.mark.parametrize("there", ["scales", "zeros"])
+def test_codes_of_the_host_with_scales_on_a_gpu(ctx, there):
+    a = {"codes": np.zeros((5, 32), np.uint8), "scales": np.zeros((5, 1), np.float32), "zeros": np.zeros((5, 1), np.uint8)}
+    a[there] = _gpu(a[there])
+    A.Table4.from_codes(ctx=ctx, **a)
+    assert ctx.calls.index(("stream", 4096)) < ctx.calls.index("as_table4_import")
+
+
+def test_host_memory_alone_moves_no_stream(ctx):
+    A.cross_entropy_backward(ctx=ctx, **_arguments())
+    assert ctx.calls == ["as_cross_entropy_backward"] or ctx.calls == ["as_cross_entropy_workspace", "as_cross_entropy_backward"]
