@@ -53,8 +53,6 @@ class _Call:
     __slots__ = ("device", "cuda", "ctx", "torch")
 
     def __init__(self, first, ctx, *others):
-        if isinstance(first, DeviceArray):
-            raise TypeError("a DeviceArray is not taken here: torch tensors or numpy arrays")
         self.device, self.cuda, self.torch = None, False, False
         index = None
         if is_tensor(first):
@@ -106,8 +104,14 @@ def _name(a):
     return name if name is not None else str(a.dtype).replace("torch.", "")
 
 
+def _known(a, what):
+    if isinstance(a, DeviceArray):
+        raise TypeError("%s is a DeviceArray, which is not taken here: torch tensors or numpy arrays" % what)
+
+
 def _matrix(a, what):
     """(array, rows, columns, row stride in elements, address) of a matrix whose rows' values are adjacent."""
+    _known(a, what)
     if not is_tensor(a):
         a = np.asarray(a)
         if a.ndim != 2:
@@ -131,6 +135,7 @@ def _vector(a, n, dtype, what):
     """Address of a dense vector of n elements, and the array that has to stay alive."""
     if a is None:
         return None, None
+    _known(a, what)
     if not is_tensor(a):
         a = np.asarray(a)
         if a.dtype != np.dtype(dtype):
@@ -271,6 +276,7 @@ class Table4:
 
     def scores(self, x, ctx=None):
         """x @ W.T for one row or a few (float32, bfloat16 or float16), in x's type."""
+        _known(x, "x")
         first = x
         single = len(x.shape) == 1
         if single:

@@ -85,3 +85,14 @@ def test_codes_of_the_host_with_scales_on_a_gpu(ctx, there):
 def test_host_memory_alone_moves_no_stream(ctx):
     A.cross_entropy_backward(ctx=ctx, **_arguments())
     assert ctx.calls == ["as_cross_entropy_backward"] or ctx.calls == ["as_cross_entropy_workspace", "as_cross_entropy_backward"]
+
+
+def test_device_arrays_are_refused_wherever_they_stand(ctx):
+    buffer = A.api.DeviceArray.__new__(A.api.DeviceArray)
+    buffer.shape, buffer.dtype, buffer._h = (5, 8), np.dtype(np.float32), None
+    for name in ("x", "table", "targets", "bias"):
+        a = {k: v for k, v in _arguments().items() if k in ("x", "table", "targets", "bias")}
+        a[name] = buffer
+        with pytest.raises(TypeError):
+            A.cross_entropy(ctx=ctx, **a)
+    assert ctx.calls == []
