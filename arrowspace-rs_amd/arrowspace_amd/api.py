@@ -139,6 +139,7 @@ class Context:
 
     def set_stream(self, stream):
         self.check(self.lib.as_ctx_set_stream(self.h, C.c_void_p(stream)))
+        self._stream = stream or 0   # (what the calls that adopt torch's current stream compare with; 0: the default stream)
 
     def synchronize(self):
         self.check(self.lib.as_ctx_synchronize(self.h))
@@ -207,7 +208,6 @@ def _adopt_torch_stream(ctx):
     st = torch.cuda.current_stream().cuda_stream
     if getattr(ctx, "_stream", "own") != st:
         ctx.set_stream(st)
-        ctx._stream = st
 
 
 def _is_torch(x):

@@ -78,7 +78,6 @@ class _Call:
             st = _raw_stream(index)
             if getattr(ctx, "_stream", "own") != st:
                 ctx.set_stream(st)
-                ctx._stream = st
         elif ctx is None:
             ctx = _thread_context(0)
         self.ctx = ctx

@@ -31,19 +31,17 @@ class _Library:
         return call
 
 
-class _Ctx:
-    device = 0
-    h = None
-
+class _Ctx(A.Context):
     def __init__(self):
-        self.calls = []
+        self.device, self.h, self.calls = 0, None, []
         self.lib = _Library(self.calls)
 
     def set_stream(self, s):
         self.calls.append(("stream", s))
+        super().set_stream(s)
 
-    def check(self, rc):
-        assert rc == 0
+    def __del__(self):
+        pass
 
 
 @pytest.fixture
@@ -68,8 +66,7 @@ def test_a_call_with_one_argument_on_a_gpu_runs_on_its_current_stream(ctx, there
     if there in ("table", "targets", "bias"):
         A.cross_entropy(ctx=ctx, **{k: a[k] for k in ("x", "table", "targets", "bias")})
         assert ctx.calls.index(("stream", 4096)) < ctx.calls.index("as_cross_entropy")
-        ctx.calls.clear()
-        del ctx._stream
+        ctx = _Ctx()
     A.cross_entropy_backward(ctx=ctx, **a)
     assert ctx.calls.index(("stream", 4096)) < ctx.calls.index("as_cross_entropy_backward")
 
@@ -96,3 +93,16 @@ def test_device_arrays_are_refused_wherever_they_stand(ctx):
         with pytest.raises(TypeError):
             A.cross_entropy(ctx=ctx, **a)
     assert ctx.calls == []
+
+
+def test_a_context_that_its_owner_moved_comes_back_to_the_current_stream(ctx):
+    a = _arguments()
+    a["table"] = _gpu(a["table"])
+    for k in range(3):
+        A.cross_entropy_backward(ctx=ctx, **a)
+        if k == 0:
+            ctx.set_stream(8192)
+            ctx.calls.clear()
+    # (moved back once, and not again while it is there)
+    assert [c for c in ctx.calls if isinstance(c, tuple)] == [("stream", 4096)]
+    assert ctx.calls[0] == ("stream", 4096)
