@@ -95,6 +95,7 @@ struct HandleCache {
   std::multimap<std::pair<int, size_t>, void *> idle;                // blocks given back, by (device, bytes)
   std::deque<std::pair<void *, std::pair<int, size_t>>> idle_order;  // ... oldest first, for eviction
   size_t idle_bytes = 0;
+  std::map<int, int> unsettled;  // by device: contexts with work on a stream that they left beside a capture (as_ctx_set_stream): no stamp covers it
   // time this process spent in the allocator on behalf of handles (microseconds, counts): "handle_cache_*" statistics
   std::atomic<uint64_t> us_malloc{0}, us_free{0}, us_wait{0}, n_malloc{0}, n_free{0}, n_hit{0};
   size_t cap = [] {
@@ -221,7 +222,7 @@ hipError_t handle_free(void *p) {
       if (c.cap > 0 && key.second <= c.cap) {
         // stamp: an event on every registered stream of the block's device (recorded under the lock: a handful of microseconds)
         std::vector<hipEvent_t> evs;
-        bool ok = true;
+        bool ok = c.unsettled[key.first] == 0;
         hipStream_t last = (hipStream_t)-1;
         for (auto sit = c.streams.lower_bound({key.first, (hipStream_t)0}); ok && sit != c.streams.end() && sit->first == key.first; ++sit) {
           if (sit->second == last) continue;  // (a stream several contexts share)
@@ -281,6 +282,13 @@ void handle_cache_stream(int device, hipStream_t s, bool add) {
   }
 }
 
+static void handle_cache_unsettled(int device, int by) {
+  if (!by) return;
+  HandleCache &c = handle_cache();
+  std::lock_guard<std::mutex> g(c.mu);
+  c.unsettled[device] += by;
+}
+
 void handle_cache_release() {
   HandleCache &c = handle_cache();
   std::vector<void *> drop;
@@ -322,6 +330,52 @@ void host_copy_parallel(void *dst, const void *src, size_t bytes) {
   std::unique_lock<std::mutex> lk(p->m);
   p->cv_done.wait(lk, [&] { return p->pending == 0; });
 }
+// What as_ctx_set_stream left unwaited-for beside a capture has been waited for (or the context's stream will have): its blocks are free.
+static void left_is_settled(as_ctx *ctx) {
+  for (auto &b : ctx->set_aside) ctx->free_blocks.emplace(b.first, b.second);
+  ctx->set_aside.clear();
+  handle_cache_unsettled(ctx->device, -ctx->unsettled);
+  ctx->unsettled = 0;
+}
+// ... by the host (no capture beside)
+static void wait_for_left(as_ctx *ctx) {
+  for (hipEvent_t ev : ctx->left_events) {
+    (void)hipEventSynchronize(ev);
+    (void)hipEventDestroy(ev);
+  }
+  ctx->left_events.clear();
+  if (ctx->left_default) (void)hipStreamSynchronize(nullptr);
+  ctx->left_default = false;
+  for (hipStream_t s : ctx->parked_streams) {
+    (void)hipStreamSynchronize(s);
+    (void)hipStreamDestroy(s);
+  }
+  ctx->parked_streams.clear();
+  left_is_settled(ctx);
+}
+// ... by the context's stream, in front of the first call behind the capture
+void ctx_enter(as_ctx *ctx) {
+  if (!ctx->clean && ctx->left_events.empty() && !ctx->left_default) return;
+  if (stream_is_capturing(ctx->stream)) return;
+  ctx->clean = false;
+  if (ctx->left_default) {
+    hipEvent_t ev = nullptr;
+    if (hipEventCreateWithFlags(&ev, hipEventDisableTiming) != hipSuccess) return (void)hipGetLastError();
+    if (hipEventRecord(ev, nullptr) != hipSuccess) {
+      (void)hipEventDestroy(ev);
+      return (void)hipGetLastError();
+    }
+    ctx->left_events.push_back(ev);
+    ctx->left_default = false;
+  }
+  while (!ctx->left_events.empty()) {
+    if (hipStreamWaitEvent(ctx->stream, ctx->left_events.back(), 0) != hipSuccess) return (void)hipGetLastError();
+    (void)hipEventDestroy(ctx->left_events.back());
+    ctx->left_events.pop_back();
+  }
+  if (ctx->unsettled) left_is_settled(ctx);
+}
+
 int ctx_side_stream(as_ctx *ctx) {
   if (ctx->side && ctx->side_word) return AS_OK;
   if (!ctx->side) AS_HIP(ctx, hipStreamCreateWithFlags(&ctx->side, hipStreamNonBlocking));
@@ -427,10 +481,15 @@ __global__ void range_scatter_kernel(const double *__restrict__ lambdas, uint64_
   }
 }
 
-int check_ctx(as_ctx *ctx) {
+int select_device(as_ctx *ctx) {
   if (!ctx) return AS_ERR_ARG;
   if (hipSetDevice(ctx->device) != hipSuccess) return fail(ctx, AS_ERR_HIP, "hipSetDevice failed");
   ctx->err.clear();
+  return AS_OK;
+}
+int check_ctx(as_ctx *ctx) {
+  AS_TRY(select_device(ctx));
+  ctx_enter(ctx);
   return AS_OK;
 }
 
@@ -518,15 +577,9 @@ void as_ctx_destroy(as_ctx *ctx) {
   prof_resolve(ctx);
   handle_cache_stream(ctx->device, ctx->stream, false);
   if (ctx->own_stream) (void)hipStreamDestroy(ctx->stream);
-  for (hipStream_t s : ctx->capture_left) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(s, &st) == hipSuccess && st == hipStreamCaptureStatusNone) (void)hipStreamSynchronize(s);
-    (void)hipGetLastError();
-  }
-  for (hipStream_t s : ctx->parked_streams) {
-    (void)hipStreamSynchronize(s);
-    (void)hipStreamDestroy(s);
-  }
+  wait_for_left(ctx);
+  for (auto &b : ctx->kept_out) (void)hipFree(b.second);
+  handle_cache_unsettled(ctx->device, -ctx->kept_unsettled);
   if (ctx->pinned) (void)hipHostFree(ctx->pinned);
   join_session_close(ctx);
   if (ctx->join_order) (void)hipFree(ctx->join_order);
@@ -539,41 +592,52 @@ void as_ctx_destroy(as_ctx *ctx) {
 const char *as_last_error(const as_ctx *ctx) { return ctx ? ctx->err.c_str() : "null context"; }
 
 int as_ctx_set_stream(as_ctx *ctx, void *hip_stream) {
-  AS_TRY(check_ctx(ctx));
-  hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing((hipStream_t)hip_stream, &capturing) != hipSuccess) (void)hipGetLastError();
-  if (capturing != hipStreamCaptureStatusNone) {
-    // Nothing may be waited for or destroyed beside a capture.  Calls on a capturing stream bring their own workspace, so none of
-    // the context's scratch passes from the old stream's work to the new one's here; its next owner is on a stream that the switch
-    // back synchronises with.
-    if (ctx->own_stream) ctx->parked_streams.push_back(ctx->stream);
-    else if (std::find(ctx->capture_left.begin(), ctx->capture_left.end(), ctx->stream) == ctx->capture_left.end()) ctx->capture_left.push_back(ctx->stream);
-    ctx->own_stream = false;
-    handle_cache_stream(ctx->device, ctx->stream, false);
-    ctx->stream = (hipStream_t)hip_stream;
-    handle_cache_stream(ctx->device, ctx->stream, true);
-    return AS_OK;
-  }
-  // (streams left for a capture, not waited for then; one that is being captured cannot be waited for now either)
-  if (std::find(ctx->capture_left.begin(), ctx->capture_left.end(), ctx->stream) == ctx->capture_left.end()) ctx->capture_left.push_back(ctx->stream);
-  std::vector<hipStream_t> still;
-  for (hipStream_t s : ctx->capture_left) {
+  AS_TRY(select_device(ctx));
+  const hipStream_t to = (hipStream_t)hip_stream;  // NULL = HIP's default (null) stream
+  auto captured = [](hipStream_t s) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(s, &st) != hipSuccess) (void)hipGetLastError();
-    if (st != hipStreamCaptureStatusNone) still.push_back(s);
-    else (void)hipStreamSynchronize(s);
+    return st != hipStreamCaptureStatusNone;
+  };
+  const bool into = captured(to), out_of = !ctx->own_stream && captured(ctx->stream);
+  if (into || out_of) {
+    if (to == ctx->stream) return AS_OK;
+    // Beside a capture nothing may be waited for or destroyed.  What this context has queued on the stream it leaves (calls on a stream
+    // under capture bring their own workspace and do not count) may still run, so until a later call's stream has waited for it (ctx_enter)
+    // its workspace blocks are set aside, and a handle's memory is given to a next owner behind a wait for the device.  A stream left in the
+    // middle of its own capture cannot be marked: its blocks stay out of use until the context goes.
+    if (ctx->own_stream) {
+      ctx->parked_streams.push_back(ctx->stream);  // (calls there have returned when their work was done)
+    } else if (!ctx->clean) {
+      bool marked = !out_of;
+      if (marked && ctx->stream == nullptr) {
+        ctx->left_default = true;
+      } else if (marked) {
+        hipEvent_t ev = nullptr;
+        marked = hipEventCreateWithFlags(&ev, hipEventDisableTiming) == hipSuccess;
+        if (marked && hipEventRecord(ev, ctx->stream) != hipSuccess) {
+          (void)hipEventDestroy(ev);
+          marked = false;
+        }
+        if (marked) ctx->left_events.push_back(ev);
+        else (void)hipGetLastError();
+      }
+      auto &blocks = marked ? ctx->set_aside : ctx->kept_out;
+      blocks.insert(blocks.end(), ctx->free_blocks.begin(), ctx->free_blocks.end());
+      ctx->free_blocks.clear();
+      int &count = marked ? ctx->unsettled : ctx->kept_unsettled;
+      if (!count) handle_cache_unsettled(ctx->device, count = 1);
+    }
+  } else {
+    (void)hipStreamSynchronize(ctx->stream);
+    wait_for_left(ctx);
+    prof_resolve(ctx);
   }
-  ctx->capture_left.swap(still);
-  for (hipStream_t s : ctx->parked_streams) {
-    (void)hipStreamSynchronize(s);
-    (void)hipStreamDestroy(s);
-  }
-  ctx->parked_streams.clear();
-  prof_resolve(ctx);
   handle_cache_stream(ctx->device, ctx->stream, false);
-  if (ctx->own_stream) (void)hipStreamDestroy(ctx->stream);
+  if (ctx->own_stream && !into) (void)hipStreamDestroy(ctx->stream);
   ctx->own_stream = false;
-  ctx->stream = (hipStream_t)hip_stream;  // NULL = HIP's default (null) stream
+  ctx->stream = to;
+  ctx->clean = true;
   handle_cache_stream(ctx->device, ctx->stream, true);
   return AS_OK;
 }

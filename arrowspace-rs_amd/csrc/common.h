@@ -74,7 +74,15 @@ struct as_ctx {
   hipEvent_t side_start = nullptr, side_done = nullptr;
   int *side_word = nullptr;               // pinned: what the side stream reads back
   bool own_stream = false;
-  std::vector<hipStream_t> parked_streams, capture_left;  // as_ctx_set_stream beside a capture: the context's own stream until it may be destroyed; streams not yet waited for
+  // as_ctx_set_stream beside a capture, where nothing may be waited for (api.hip): the context's own stream until it may be destroyed; what
+  // its work on a stream it left has to be waited for by; the workspace blocks that this work may still use; those of a stream left in the
+  // middle of its own capture, which is never known to be done
+  std::vector<hipStream_t> parked_streams;
+  std::vector<hipEvent_t> left_events;
+  bool left_default = false;              // ... the default stream: no event can be recorded on it beside a capture
+  std::vector<std::pair<size_t, void *>> set_aside, kept_out;
+  int unsettled = 0, kept_unsettled = 0;  // how often this context counts in the handle cache's `unsettled`
+  bool clean = false;                     // nothing of this context has been queued on its stream, outside a capture, since it came there
   std::string err;
   void *pinned = nullptr;  // staging buffer for host <-> device transfers
   std::multimap<size_t, void *> free_blocks;  // workspace cache (capacity -> block)
@@ -449,7 +457,18 @@ inline hipError_t copy_d2h(as_ctx *ctx, void *dst, const void *src, size_t bytes
 // was dropped: mixed with the blocking hipMalloc/hipFree of the long-lived handles it produced
 // intermittent stale reads on this stack.)
 void handle_cache_release();  // (below: the cache of handle memory) every idle block back to the device
+// Every call that queues work: behind a switch of streams beside a capture, the stream first waits for what the context left behind (api.hip).
+void ctx_enter(as_ctx *ctx);
+inline bool stream_is_capturing(hipStream_t s) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(s, &st) != hipSuccess) {
+    (void)hipGetLastError();
+    return true;  // (the default stream beside a capture: nothing may be allocated or waited for either)
+  }
+  return st != hipStreamCaptureStatusNone;
+}
 inline int ws_alloc(as_ctx *ctx, size_t bytes, void **out, size_t *cap) {
+  ctx_enter(ctx);
   if (bytes == 0) bytes = 1;
   bytes = (bytes + 255) & ~(size_t)255;
   auto it = ctx->free_blocks.lower_bound(bytes);

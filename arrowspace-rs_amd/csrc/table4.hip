@@ -662,6 +662,7 @@ uint64_t scores_layout(const as_table4 *t, uint32_t m, int dt, char *base, Score
 int check_shape(as_ctx *ctx, uint64_t v, uint64_t d, uint64_t group, int scale_dt) {
   if (!ctx) return AS_ERR_ARG;
   if (hipSetDevice(ctx->device) != hipSuccess) return fail(ctx, AS_ERR_HIP, "hipSetDevice failed");
+  ctx_enter(ctx);
   if (v == 0 || d == 0) return fail(ctx, AS_ERR_SHAPE, "the table needs at least one row and one column");
   if (v >= (1ull << 31) || d > (1u << 20)) return fail(ctx, AS_ERR_UNSUPPORTED, "at most 2^31 - 1 items and 2^20 columns");
   if (group != 32 && group != 64 && group != 128) return fail(ctx, AS_ERR_UNSUPPORTED, "groups of 32, 64 or 128 columns");
@@ -843,6 +844,7 @@ int as_table4_export(as_ctx *ctx, const as_table4 *t, uint8_t *codes, void *scal
     if (!t || !codes || !scales) return fail(ctx, AS_ERR_ARG, "null argument");
     if (t->device != ctx->device) return fail(ctx, AS_ERR_ARG, "a table of another device than the context's");
     if (hipSetDevice(ctx->device) != hipSuccess) return fail(ctx, AS_ERR_HIP, "hipSetDevice failed");
+    ctx_enter(ctx);
     const uint64_t groups = cdiv(t->d, t->group), row_bytes = (t->d + 1) / 2;
     BytesOut C, S, Z;
     AS_TRY(C.bind(ctx, codes, t->v * row_bytes));
@@ -885,6 +887,7 @@ int as_table4_scores(as_ctx *ctx, const as_table4 *t, const void *x, uint64_t m,
     if (!t) return fail(ctx, AS_ERR_ARG, "null argument");
     if (t->device != ctx->device) return fail(ctx, AS_ERR_ARG, "a table of another device than the context's");
     if (hipSetDevice(ctx->device) != hipSuccess) return fail(ctx, AS_ERR_HIP, "hipSetDevice failed");
+    ctx_enter(ctx);
     if (!dtype_is_training(dtype)) return fail(ctx, AS_ERR_ARG, "dtype must be AS_F32, AS_BF16 or AS_F16");
     if (m == 0) return AS_OK;
     if (!x || !out) return fail(ctx, AS_ERR_ARG, "null argument");

@@ -40,15 +40,6 @@ inline int pointer_home(as_ctx *ctx, const void *p) {
   return a.device == ctx->device ? 1 : -1;
 }
 
-inline bool stream_is_capturing(hipStream_t s) {
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(s, &st) != hipSuccess) {
-    (void)hipGetLastError();
-    return true;  // (the default stream beside a capture: nothing may be allocated or waited for either)
-  }
-  return st != hipStreamCaptureStatusNone;
-}
-
 // Scratch of one call: the caller's workspace (what a captured graph needs: its addresses stay the graph's own), else blocks of
 // the context's cache, which are in use until the call's work on the stream is done and so never part of a graph.
 struct Scratch {

@@ -1068,6 +1068,7 @@ struct LossCall {
 int check_loss(as_ctx *ctx, const LossCall &c) {
   if (!ctx) return AS_ERR_ARG;
   if (hipSetDevice(ctx->device) != hipSuccess) return fail(ctx, AS_ERR_HIP, "hipSetDevice failed");
+  ctx_enter(ctx);
   if (!dtype_is_training(c.dt)) return fail(ctx, AS_ERR_ARG, "dtype must be AS_F32, AS_BF16 or AS_F16");
   if (c.v == 0 || c.d == 0) return fail(ctx, AS_ERR_SHAPE, "the table needs at least one row and one column");
   if (c.n >= (1ull << 31) || c.v >= (1ull << 31) || c.d > 65536) return fail(ctx, AS_ERR_UNSUPPORTED, "at most 2^31 - 1 rows and items and 65536 columns");

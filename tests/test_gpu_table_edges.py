@@ -3,6 +3,7 @@ References in 64 bits; the bounds are those of test_gpu_table.py, whose docstrin
 import pytest
 
 import arrowspace_amd as A
+from arrowspace_amd import _lib
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -63,3 +64,76 @@ def test_codes_in_host_memory_and_scales_that_are_being_written():
         _busy_write(late, s)
         t = A.Table4.from_codes(codes.cpu(), late, dim=128, group=64)
     _check4(t, w, torch.randn(3, 128, device="cuda"))
+
+
+def _backward(ctx, x, w, y, lse, gl, out, workspace=None):
+    n, d = x.shape
+    v = w.shape[0]
+    rc = ctx.lib.as_cross_entropy_backward(ctx.h, x.data_ptr(), n, d, w.data_ptr(), v, d, d, _lib.AS_BF16, None, y.data_ptr(), -100, 1.0, lse.data_ptr(),
+                                           gl.data_ptr(), None, out[0].data_ptr(), d, out[1].data_ptr(), d, None,
+                                           None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel())
+    assert rc == _lib.AS_OK
+
+
+@pytest.mark.parametrize("first", ["stream", "default"])
+def test_scratch_of_a_stream_that_was_left_beside_a_capture(first):
+    """Work on one stream with the context's own scratch; a capture on another; work there with the context's scratch, without a switch
+    of streams between: each gets what it gets alone."""
+    sets = [_inputs(300, 20000, 320, torch.bfloat16, seed=s)[:3] for s in (33, 34, 35)]
+    gl = torch.full((300,), 1 / 300, device="cuda")
+    lse = [A.cross_entropy(*s)[1] for s in sets]
+    want = [A.cross_entropy_backward(*s, l, gl)[:2] for s, l in zip(sets, lse)]
+    out = [[torch.zeros_like(t) for t in w] for w in want]
+    ctx = A.Context(0)
+    one, two = torch.cuda.Stream() if first == "stream" else torch.cuda.default_stream(), torch.cuda.Stream()
+    ws = torch.empty(ctx.lib.as_cross_entropy_workspace(300, 20000, 320, _lib.AS_BF16, 1), dtype=torch.uint8, device="cuda")
+    late = torch.zeros_like(sets[0][0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(one):
+        ctx.set_stream(one.cuda_stream)
+        _busy_write(late, sets[0][0])
+        _backward(ctx, late, *sets[0][1:], lse[0], gl, out[0])
+    with torch.cuda.stream(two):
+        graph.capture_begin()
+        ctx.set_stream(two.cuda_stream)
+        _backward(ctx, *sets[1], lse[1], gl, out[1], ws)
+        graph.capture_end()
+        _backward(ctx, *sets[2], lse[2], gl, out[2])
+        graph.replay()
+    torch.cuda.synchronize()
+    for got, w in zip(out, want):
+        assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])
+    ctx.set_stream(one.cuda_stream)
+    _backward(ctx, *sets[1], lse[1], gl, out[0])
+    torch.cuda.synchronize()
+    assert torch.equal(out[0][0], want[1][0]) and torch.equal(out[0][1], want[1][1])
+
+
+def test_a_table_freed_while_a_stream_left_beside_a_capture_reads_it():
+    v, d = 200_000, 256
+    codes, s, _, _ = _plain4(v, d, 64, "f16", False, 36)
+    other = codes.flip(0).contiguous()
+    x = torch.randn(3, d, device="cuda")
+    ctx = A.Context(0)
+    t = A.Table4.from_codes(codes, s, dim=d, group=64)
+    keep = A.Table4.from_codes(other, s, dim=d, group=64)
+    want = t.scores(x)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    late = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(one):
+        _busy_write(late, x)
+        got = t.scores(late, ctx=ctx)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(two):
+        graph.capture_begin()
+        out = keep.scores(x, ctx=ctx)
+        graph.capture_end()
+    del t
+    fresh = [A.Table4.from_codes(other, s, dim=d, group=64) for _ in range(2)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, keep.scores(x)) and torch.equal(out, fresh[0].scores(x)) and torch.equal(out, fresh[1].scores(x))
