@@ -32,7 +32,7 @@ struct NtOperand {
   size_t ld;          // bytes from row to row of the matrix
   uint32_t last;      // rows behind this one read it instead (their results are dropped); transposed: 16-byte pieces of a row
   uint32_t last_k;    // transposed: rows behind this one read it instead (the other operand has zeros there)
-  size_t plane;       // bytes from the high to the low plane (two planes: f32 values as a sum of two f16)
+  size_t plane;       // bytes from plane to plane (f32: three bf16, table_loss_rows.h)
 };
 
 template <int FMT>  // AS_BF16 / AS_F16
@@ -144,11 +144,10 @@ struct NtTile {
     fa = AT ? column_address<BM>(ra) : (ra + r) * 128 + piece;
     fb = BM * 128 + (BT ? column_address<BN>(rb) : (rb + r) * 128 + piece);
   }
-  // Step s of `steps` a plane; with two planes high x high, high x low, low x high -- the product of the two low planes is 2^-24 of the
-  // whole and left out.
+  // Step s of `steps` a pair of planes; three planes: the pairs (A, B) 00, 01, 10, 11, 02, 20.
   template <bool T, uint32_t W, uint32_t PIECES>
-  __device__ __forceinline__ void fetch_side(char *dst, const NtOperand &o, uint32_t k, bool low) const {
-    const char *src = o.p + (low ? o.plane : 0) + (T ? 0 : (size_t)k * 128);
+  __device__ __forceinline__ void fetch_side(char *dst, const NtOperand &o, uint32_t k, uint32_t plane) const {
+    const char *src = o.p + plane * o.plane + (T ? 0 : (size_t)k * 128);
 #pragma unroll
     for (uint32_t p = 0; p < PIECES; ++p) {
       const char *from;
@@ -164,9 +163,9 @@ struct NtTile {
   }
   __device__ __forceinline__ void fetch(int buf, const NtOperand &A, const NtOperand &B, uint32_t s, uint32_t steps) const {
     char *dst = smem + buf * kStage;
-    const uint32_t third = s < steps ? 0 : s < 2 * steps ? 1 : 2, k = s - third * steps;
-    fetch_side<AT, BM, PA>(dst, A, k, third == 2);
-    fetch_side<BT, BN, PB>(dst + BM * 128, B, k, third == 1);
+    const uint32_t pair = s < steps ? 0 : s / steps, k = s - pair * steps;
+    fetch_side<AT, BM, PA>(dst, A, k, 0x850u >> (2 * pair) & 3);
+    fetch_side<BT, BN, PB>(dst + BM * 128, B, k, 0x244u >> (2 * pair) & 3);
   }
   __device__ __forceinline__ void zero(f32x4 (&acc)[TM][TN]) const {
 #pragma unroll

@@ -15,13 +15,13 @@
 // What bounds it: 2 n v d flops forward, 8 more backward, of which 2 are the logits again (through G: 6, written and read once: 2 bytes a
 // logit each).  8 192 rows x 131 072 items of 1 024 (bf16), forward and backward: 8.04 ms = 1 094 TFLOP/s, one library product of this
 // size runs at 1 076; 4 096 x 100 000 of 768 with a bias: 2.67 ms; 1 024 x 1 000 000 of 128: 1.27 ms, 2.01 through G; 777 x 31 013 of 200
-// (f16): 0.14, 0.18 through G; f32, 512 x 100 000 of 128: 0.29, 0.38 through G.
-// Types.  bf16 and f16 go to the matrix pipe as they are.  f32 values go as a sum of two f16 (22 bits, after a power of two that
-// brings the matrix' largest finite value to 2^14 .. 2^15), three products per pair of planes: 2.5 PFLOP/s / 3 against the
-// 0.157 of the f32 instruction, and an error per product of 2^-23 of it, which the f32 sums have anyway.
-// (Few f32 rows: three bf16, table_loss_few.h.)
-// Rounding.  G is rounded to 16 bits in units of the largest coefficient (coef_scale_kernel; f32: two planes, 22 bits): half a
-// step per entry, as the gradients that leave are rounded themselves.  The entries at the targets, nearly the coefficient itself and
+// (f16): 0.14, 0.18 through G; f32, 512 x 100 000 of 128: 0.47, 0.55 through G.
+// Types.  bf16 and f16 go to the matrix pipe as they are.  f32 values go as a sum of three bf16 (table_loss_rows.h): 24 bits, of values
+// below 2^-108 what a step of 2^-133 leaves, and no scale that one large value would set for everyone.  Six products a pair of values: 2.5
+// PFLOP/s / 6 against the 0.157 of the f32 instruction.  (Two f16 under a power of two a matrix need three: the same step 0.31.  But a value
+// keeps 22 bits only down to 2^-17 of the matrix' largest, 14 at 2^-24: a row of garbage in the padding left the others none.)
+// Rounding.  16-bit matrices: G is rounded to their type, in units of the largest coefficient (coef_scale_kernel): half a step per entry, as
+// the gradients that leave are rounded themselves (f32: three planes, as the values).  The entries at the targets, nearly the coefficient itself and
 // the same in all rows of an item, come from a product of their own in f64, and what 16 bits leave of them is added in f32: with half a
 // step there, dX of well-trained rows was off by twice the rounding of the result.  Everything else -- logits, maxima, sums, dX over pieces,
 // dbias -- is f32 or wider.
@@ -37,20 +37,14 @@ struct LossArgs {
   // operands of the product: A the table side (m), B the rows (n)
   const char *table, *rows;
   size_t table_ld, rows_ld;       // bytes
-  size_t table_plane, rows_plane; // bytes to the low plane
+  size_t table_plane, rows_plane; // bytes from plane to plane
   uint32_t n, v;                  // rows of B and of A
-  uint32_t steps, planes;         // steps of 64 along k per plane; 1, or 2 (three passes)
+  uint32_t steps, all;            // steps of 64 along k, and with every pair of planes
   uint32_t per;                   // tiles of A a workgroup walks
   uint32_t v_tiles, n_tiles, chunks;
   float scale;
   const float *bias;
-  const unsigned int *rows_top, *table_top;  // two planes: bits of the largest finite magnitude of each matrix, else null
 };
-
-__device__ __forceinline__ float product_scale(const LossArgs &a) {
-  if (a.rows_top == nullptr) return 1.f;
-  return 1.f / plane_scale(*a.rows_top) / plane_scale(*a.table_top);
-}
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------------
 // GENERAL: with a bias, or a scale that is not positive (the maximum is then taken of the scaled logits); else of the raw products.
@@ -65,14 +59,14 @@ __global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2
   grid_order(work, a.n_tiles, a.chunks, &nt, &chunk);
   const uint32_t n0 = nt * TILE::BN, vt_end = nt_min((chunk + 1) * a.per, a.v_tiles);
   uint32_t vt = chunk * a.per;
-  const float nat = a.scale * product_scale(a), unit = GENERAL ? kLog2e : nat * kLog2e;  // exponentials of (x - maximum) * unit to the base 2
+  const float unit = GENERAL ? kLog2e : a.scale * kLog2e;  // exponentials of (x - maximum) * unit to the base 2
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
   NtOperand B{a.rows + (size_t)n0 * a.rows_ld, a.rows_ld, nt_min(TILE::BN, a.n - n0) - 1, 0, a.rows_plane};
   auto side = [&](uint32_t tile) {
     const uint32_t r0 = tile * TILE::BM;
     return NtOperand{a.table + (size_t)r0 * a.table_ld, a.table_ld, nt_min(TILE::BM, a.v - r0) - 1, 0, a.table_plane};
   };
-  const uint32_t all = a.planes == 2 ? 3 * a.steps : a.steps;
+  const uint32_t all = a.all;
   float top[TILE::TN], sum[TILE::TN];
 #pragma unroll
   for (int j = 0; j < TILE::TN; ++j) top[j] = -INFINITY, sum[j] = 0.f;
@@ -104,7 +98,7 @@ __global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2
           const uint32_t r = row0 + (i >> 1) * 32 + (i & 1) * 4 + e;
           const float b = a.bias && r <= last ? a.bias[(size_t)vt * TILE::BM + r] : 0.f;
 #pragma unroll
-          for (int j = 0; j < TILE::TN; ++j) acc[i][j][e] = r > last ? -INFINITY : fmaf(acc[i][j][e], nat, b);
+          for (int j = 0; j < TILE::TN; ++j) acc[i][j][e] = r > last ? -INFINITY : fmaf(acc[i][j][e], a.scale, b);
         }
     } else if (last + 1 < TILE::BM) {
 #pragma unroll
@@ -142,7 +136,7 @@ __global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2
   // the four lane groups of a row
 #pragma unroll
   for (int j = 0; j < TILE::TN; ++j) {
-    float m = GENERAL ? top[j] : top[j] == -INFINITY ? -INFINITY : top[j] * nat, s = sum[j];
+    float m = GENERAL ? top[j] : top[j] == -INFINITY ? -INFINITY : top[j] * a.scale, s = sum[j];
 #pragma unroll
     for (int x = 16; x < 64; x <<= 1) {
       const float mo = __shfl_xor(m, x), so = __shfl_xor(s, x);
@@ -205,7 +199,7 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2 *part, uint
 }
 
 // ---- what the products are made of ----------------------------------------------------------------------------------------------------
-// A matrix and its image: rows with their length filled to whole steps by zeros, f32 as two planes.
+// A matrix and its image: rows with their length filled to whole steps by zeros, f32 as three planes.
 struct ImageJob {
   const char *src;
   size_t stride;           // bytes
@@ -214,8 +208,6 @@ struct ImageJob {
 };
 struct ImageJobs {
   ImageJob job[2];
-  unsigned int *tops;      // f32: [2] bits of the largest finite magnitude, for everyone behind
-  float *parts;            // ... [2][kTopParts] of the workgroups that looked for it
 };
 // A matrix in pieces of eight columns, `across` a row, dealt to all threads of the grid, four at a time under way.  f(piece, row, column)
 template <int DT, int THREADS, class F>
@@ -224,12 +216,12 @@ __device__ __forceinline__ void each_piece(const ImageJob &j, uint32_t across, F
   const uint32_t row_step = threads / across, column_step = threads % across;
   uint32_t row = first / across, column = first % across;
   while (row < j.n) {
-    Piece8<DT> piece[4];
+    LrPiece<DT, true> piece[4];
     uint32_t r[4], c[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       r[i] = row, c[i] = column * 8;
-      if (row < j.n) piece[i].load(j.src + (size_t)row * j.stride, c[i], j.d);
+      if (row < j.n) piece[i].load(j.src + (size_t)row * j.stride, c[i], j.d, 0);
       row += row_step, column += column_step;
       if (column >= across) column -= across, ++row;
     }
@@ -238,49 +230,16 @@ __device__ __forceinline__ void each_piece(const ImageJob &j, uint32_t across, F
       if (r[i] < j.n) f(piece[i], r[i], c[i]);
   }
 }
-// f32: the largest finite magnitude, a part per workgroup
-__global__ __launch_bounds__(1024) void top_kernel(ImageJobs jobs) {
-  const ImageJob &j = jobs.job[blockIdx.y];
-  __shared__ float s[16];
-  float m = 0.f;
-  each_piece<AS_F32, 1024>(j, (j.d + 7) / 8, [&](const Piece8<AS_F32> &p, uint32_t, uint32_t) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float y = fabsf(__uint_as_float(p.w[e >> 2][e & 3]));
-      m = y < INFINITY ? fmaxf(m, y) : m;
-    }
-  });
-  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 16; ++w) m = fmaxf(m, s[w]);
-    jobs.parts[blockIdx.y * kTopParts + blockIdx.x] = m;
-  }
-}
-template <int DT, int FMT>
+template <int DT>
 __global__ __launch_bounds__(256) void image_kernel(ImageJobs jobs) {
+  constexpr int P = planes_of(DT);
   const ImageJob &j = jobs.job[blockIdx.y];
-  float f = 1.f;
-  if constexpr (DT == AS_F32) {
-    const unsigned int top = top_of_parts(jobs.parts + blockIdx.y * kTopParts);
-    f = plane_scale(top);
-    if (blockIdx.x == 0 && threadIdx.x == 0) jobs.tops[blockIdx.y] = top;
-  }
-  each_piece<DT, 256>(j, j.pitch / 8, [&](const Piece8<DT> &p, uint32_t row, uint32_t column) {
-    unsigned short *o = j.out + (size_t)row * j.pitch * (DT == AS_F32 ? 2 : 1) + column;
-    if constexpr (DT == AS_F32) {
-      u32x4 high, low;
+  each_piece<DT, 256>(j, j.pitch / 8, [&](const LrPiece<DT, true> &piece, uint32_t row, uint32_t column) {
+    unsigned short *o = j.out + (size_t)row * j.pitch * P + column;
+    u32x4 w[P];
+    piece.template planes<format_of(DT), P>(w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = __uint_as_float(p.w[i >> 1][2 * (i & 1)]) * f, y = __uint_as_float(p.w[i >> 1][2 * (i & 1) + 1]) * f;
-        high[i] = pack2<FMT>(x, y), low[i] = pack2<FMT>(low_part(x), low_part(y));
-      }
-      *(u32x4 *)o = high;
-      *(u32x4 *)(o + j.pitch) = low;
-    } else {
-      *(u32x4 *)o = p.w[0];
-    }
+    for (int p = 0; p < P; ++p) *(u32x4 *)(o + p * j.pitch) = w[p];
   });
 }
 // ---- gradient of the logits ---------------------------------------------------------------------------------------------------------------
@@ -295,7 +254,7 @@ struct GradArgs {
   float *bias_part;                // (n_tiles WN) x g_pitch sums over the tile's rows, or null
 };
 
-template <int FMT, class TILE_, bool TWO, bool BIAS>
+template <int FMT, class TILE_, int P, bool BIAS>
 __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
   using TILE = TILE_;
   __shared__ __attribute__((aligned(1024))) char smem[2 * TILE::kStage];
@@ -307,7 +266,6 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
   grid_order(work, a.n_tiles, a.chunks, &nt, &chunk);
   const uint32_t n0 = nt * TILE::BN, vt_end = nt_min((chunk + 1) * a.per, a.v_tiles);
   uint32_t vt = chunk * a.per;
-  const float c = a.scale * product_scale(a);
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
   NtOperand B{a.rows + (size_t)n0 * a.rows_ld, a.rows_ld, nt_min(TILE::BN, a.n - n0) - 1, 0, a.rows_plane};
   auto side = [&](uint32_t tile) {
@@ -328,7 +286,7 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
     const uint32_t at = (uint32_t)g.target[t] - g.v_begin;
     hit[j] = at < a.v ? (int32_t)at : -1;
   }
-  const uint32_t all = a.planes == 2 ? 3 * a.steps : a.steps;
+  const uint32_t all = a.all;
   f32x4 acc[TILE::TM][TILE::TN];
   NtOperand A = side(vt);
   T.fetch(0, A, B, 0, a.steps);
@@ -358,7 +316,7 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
         if constexpr (BIAS) b = r > last ? -INFINITY : a.bias[at0 + r];
 #pragma unroll
         for (int j = 0; j < TILE::TN; ++j) {
-          const float z = BIAS ? fmaf(acc[i][j][e], c, b) - lse[j] : fmaf(acc[i][j][e], c, -lse[j]);
+          const float z = BIAS ? fmaf(acc[i][j][e], a.scale, b) - lse[j] : fmaf(acc[i][j][e], a.scale, -lse[j]);
           acc[i][j][e] = every[j] * __builtin_amdgcn_exp2f(z * kLog2e);
         }
       }
@@ -401,24 +359,29 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
       }
     }
     // eight consecutive items a lane (rows behind the last: zeros, the product over the batch reads them)
-    const size_t gp = (size_t)g.g_pitch * (TWO ? 2 : 1);
+    const size_t gp = (size_t)g.g_pitch * P;
 #pragma unroll
     for (int j = 0; j < TILE::TN; ++j) {
       unsigned short *o = g.G + (size_t)row[j] * gp + at0 + row0;
 #pragma unroll
       for (int i = 0; i < TILE::TM; i += 2) {
-        const f32x4 u = acc[i][j], v = acc[i + 1][j];
-        *(u32x4 *)(o + i * 16) = u32x4{pack2<FMT>(u[0], u[1]), pack2<FMT>(u[2], u[3]), pack2<FMT>(v[0], v[1]), pack2<FMT>(v[2], v[3])};
-        if constexpr (TWO)
-          *(u32x4 *)(o + g.g_pitch + i * 16) = u32x4{pack2<FMT>(low_part(u[0]), low_part(u[1])), pack2<FMT>(low_part(u[2]), low_part(u[3])),
-                                                     pack2<FMT>(low_part(v[0]), low_part(v[1])), pack2<FMT>(low_part(v[2]), low_part(v[3]))};
+        u32x4 w[P];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          uint32_t pair[P];
+          pack_planes<FMT, P>(acc[i + (h >> 1)][j][2 * (h & 1)], acc[i + (h >> 1)][j][2 * (h & 1) + 1], pair);
+#pragma unroll
+          for (int p = 0; p < P; ++p) w[p][h] = pair[p];
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) *(u32x4 *)(o + (size_t)p * g.g_pitch + i * 16) = w[p];
       }
     }
   }
 }
 
 // The rows of the batch that meet each 64 items of the table, in order, a workgroup each, its waves an eighth of the batch each (64 kept:
-// items that more rows meet are sums of many entries, whose roundings average out).
+// the entries of further rows stay rounded, as all other entries of G are).
 constexpr uint32_t kMet = 64;
 __global__ __launch_bounds__(512) void met_kernel(const int *target, uint32_t n, u32x2 *list, uint32_t *count) {
   __shared__ u32x2 part[8][kMet];
@@ -458,10 +421,9 @@ struct ProductArgs {
   uint32_t a_cols, b_cols;          // 16-byte pieces of a row that may be read (transposed)
   uint32_t k_a, k_b;                // rows that may be read (transposed)
   uint32_t m, n, m_tiles, n_tiles;
-  uint32_t steps, planes, splits;   // steps of 64 of the whole contraction; a split takes an even share of them
+  uint32_t steps, pairs, splits;    // steps of 64 of the whole contraction, a split takes an even share of them; pairs of planes
   float scale;
   const float *coef;                // 1 / factor of G at [1]
-  const unsigned int *top;          // largest magnitude of the other operand's matrix (two planes), or null
   void *out;                        // n x m rows of `out_stride` elements
   size_t out_stride;
   float *sums;                      // instead: f32 [split][n][sums_pitch], added to unless `first`
@@ -528,7 +490,7 @@ __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
   grid_order(work - split * p.m_tiles * p.n_tiles, p.n_tiles, p.m_tiles, &nt, &mt);
   const uint32_t m0 = mt * TILE::BM, n0 = nt * TILE::BN;
   const uint32_t k0 = (uint32_t)((uint64_t)p.steps * split / p.splits), k1 = (uint32_t)((uint64_t)p.steps * (split + 1) / p.splits);
-  const uint32_t steps = k1 - k0, all = p.planes == 2 ? 3 * steps : steps;
+  const uint32_t steps = k1 - k0, all = p.pairs * steps;
   const NtOperand A{p.A + (size_t)k0 * 64 * p.a_ld + m0 * 2, p.a_ld, p.a_cols - 1 - m0 / 8, p.k_a - 1 - k0 * 64, p.a_plane};
   const NtOperand B = BT ? NtOperand{p.B + (size_t)k0 * 64 * p.b_ld + n0 * 2, p.b_ld, p.b_cols - 1 - n0 / 8, p.k_b - 1 - k0 * 64, p.b_plane}
                          : NtOperand{p.B + (size_t)n0 * p.b_ld + (size_t)k0 * 128, p.b_ld, nt_min(TILE::BN, p.n - n0) - 1, 0, p.b_plane};
@@ -545,7 +507,7 @@ __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
   if constexpr (BT && OUT != AS_F32)
     if (p.met && split == 0) add_rest<FMT>(p, T, m0, n0, acc);
   const uint32_t wm = T.wave / TILE::WN, wn = T.wave % TILE::WN, q = T.lane >> 4, col = T.lane & 15;
-  const float f = OUT == 0 ? 1.f : p.scale * p.coef[1] * (p.top ? 1.f / plane_scale(*p.top) : 1.f);
+  const float f = OUT == 0 ? 1.f : p.scale * p.coef[1];
 #pragma unroll
   for (int j = 0; j < TILE::TN; ++j) {
     const uint32_t n = n0 + wn * (TILE::TN * 16) + (j >> 1) * 32 + (col >> 2) * 8 + (j & 1) * 4 + (col & 3);
@@ -575,13 +537,13 @@ __global__ __launch_bounds__(TILE_::NT) void product_kernel(ProductArgs p) {
 // waves): a few rows have a thousand parts, one thread's chain of them would be the whole time; many rows have lanes enough.
 template <int DT, int WAYS>
 __global__ __launch_bounds__(WAYS == 64 ? 1024 : 256) void grad_rows_join_kernel(const float *sums, uint32_t splits, uint32_t pitch, uint32_t n, uint32_t d, float scale,
-                                                                                 const float *coef, const unsigned int *top, const int *target, const float *rest,
+                                                                                 const float *coef, const int *target, const float *rest,
                                                                                  const void *table, size_t table_stride, void *out, size_t out_stride) {
   constexpr uint32_t WAVES = WAYS == 64 ? 16 : 4, LANES = WAYS == 64 ? 16 : 64, EACH = WAYS == 1 ? 1024 : LANES * 4;  // EACH: columns a workgroup
   __shared__ f32x4 s[WAVES][LANES];
   const uint32_t lane = threadIdx.x & (LANES - 1), w = threadIdx.x >> 6, sub = WAYS == 1 ? 0 : threadIdx.x / LANES;
   const uint32_t lo = splits * sub / WAYS, hi = splits * (sub + 1) / WAYS;
-  const float f = scale * coef[1] * (top ? 1.f / plane_scale(*top) : 1.f);
+  const float f = scale * coef[1];
   const uint64_t total = (uint64_t)n * pitch;
   for (uint64_t i0 = (uint64_t)blockIdx.x * EACH; i0 < total; i0 += (uint64_t)gridDim.x * EACH) {
     const uint64_t i = i0 + (WAYS == 1 ? w * 256 : 0) + lane * 4, t = i / pitch, k = i - t * pitch;
@@ -655,7 +617,7 @@ constexpr TileShape kShape[3] = {{256, 64, 4, 1}, {128, 128, 2, 2}, {256, 256, 2
 
 uint32_t up(uint64_t a, uint32_t b) { return (uint32_t)((a + b - 1) / b * b); }
 
-// How a matrix reaches the products: as it is, or as an image (whole steps of 64, 16-byte rows; f32 always: two planes).
+// How a matrix reaches the products: as it is, or as an image (whole steps of 64, 16-byte rows; f32 always: its planes).
 struct Source {
   const void *p;
   size_t stride;
@@ -664,10 +626,9 @@ struct Source {
   uint32_t whole;  // columns of an image
   bool direct() const { return dt != AS_F32 && d == whole && stride % 8 == 0 && ((uintptr_t)p & 15) == 0; }
   uint32_t pitch() const { return whole; }
-  uint32_t planes() const { return dt == AS_F32 ? 2 : 1; }
+  uint32_t planes() const { return planes_of(dt); }
   uint64_t image_elems(bool raw) const { return direct() || raw ? 0 : (uint64_t)rows * pitch() * planes(); }
 };
-int image_format(int dt) { return dt == AS_BF16 ? AS_BF16 : AS_F16; }
 
 // Which tile.  Rounds of workgroups times what one takes: the large one has the chip's 256 units to itself, two square ones share a
 // unit, each a quarter of the work at 0.8 of the rate (8192 x 16384 x 1024: 259 and 330 us).
@@ -696,7 +657,7 @@ struct Plan {
 Plan make_plan(uint32_t n, uint32_t v, uint32_t d, int dt) {
   Plan p{};
   p.n = n, p.v = v, p.d = d, p.dt = dt;
-  p.planes = dt == AS_F32 ? 2 : 1;
+  p.planes = planes_of(dt);
   p.steps = cdiv(d, 64);
   p.pitch = p.steps * 64;
   p.tile = product_tile(v, n);
@@ -740,9 +701,11 @@ uint32_t plan_splits(uint64_t tiles, uint32_t slots, uint32_t most) {
 // the form for short rows: its steps of 32 columns, and tiles of 16 rows a wave holds (what 256 registers take)
 int fused_steps(uint32_t d, uint32_t planes) { return d <= 64 ? 2 : d <= 128 ? 4 : d <= 256 && planes == 1 ? 8 : 0; }
 // ... and waves a SIMD.  1 024 rows x 1 M items, bf16, us (dW / dX): 64 values 2 tiles x 4 waves 270 / -, 3 x 3 257 / -, 4 x 2 283 / 264;
-// 128 values 2 x 3 515 / 439, 3 x 2 490 / 480, 4 x 2 728 / 632 (spills); 256 values 1 x 2 1 273 / 1 262, 2 x 2 1 437 / 1 410 (spills)
-constexpr int fused_rows(int steps, int planes, bool items) { return planes == 2 ? 2 : steps == 8 ? 1 : steps == 2 || items ? 3 : 2; }
-constexpr int fused_waves(int steps, int planes, bool items) { return planes == 2 || steps == 8 ? 2 : steps == 2 || !items ? 3 : 2; }
+// 128 values 2 x 3 515 / 439, 3 x 2 490 / 480, 4 x 2 728 / 632 (spills); 256 values 1 x 2 1 273 / 1 262, 2 x 2 1 437 / 1 410 (spills).
+// f32 (stages of three planes: one workgroup a unit at 128 values), 512 rows x 100 000 items: 64 values 2 x 3 79 / 62, 4 x 2 81 / 81; 128 values
+// 1 x 1 244 / 191, 2 x 1 218 / 147, 4 x 1 181 / 138
+constexpr int fused_rows(int steps, int planes, bool items) { return planes > 1 ? steps : steps == 8 ? 1 : steps == 2 || items ? 3 : 2; }
+constexpr int fused_waves(int steps, int planes, bool items) { return planes > 1 ? (steps == 2 ? 3 : 1) : steps == 8 ? 2 : steps == 2 || !items ? 3 : 2; }
 // The form for few rows: its steps of 32 columns a wave, as many columns as four waves hold; up to 128 columns (four steps) a wave takes
 // whole items.  Waves a SIMD: what its registers leave.
 int few_steps(uint32_t d) {
@@ -760,14 +723,14 @@ uint32_t few_groups(int steps, uint32_t d, bool f32, int what, uint32_t v) {
   return std::max(1u, std::min((uint32_t)few_waves(steps, f32, what) * kChips, cdiv(v, 16 * (4 / few_share(d)))));
 }
 // An image is read and written once more than the matrix itself; reading the matrix as it is costs each workgroup that walks it the
-// splitting or shifting of its pieces.  A step of 512 f32 rows of 128, 100 000 items: images 295 us, as they are 315; 777 rows of 200
+// splitting or shifting of its pieces.  A step of 512 f32 rows of 128, 100 000 items: images 490 us, as they are 515; 777 rows of 200
 // (f16, odd stride), 31 013 items: 171 and 198; one or two blocks of rows: the images would be a third of the time.
 bool raw_pays(const Plan &p) { return p.n <= 128; }
 void plan_backward(Plan &p, bool x, bool w, bool b) {
   p.want_x = x, p.want_w = w, p.want_b = b;
   p.few = p.n <= 16 ? few_steps(p.d) : 0;
   if (p.few) {
-    p.few_groups = p.splits = few_groups(p.few, p.d, p.planes == 2, kFewGrad, p.v);
+    p.few_groups = p.splits = few_groups(p.few, p.d, p.planes > 1, kFewGrad, p.v);
     p.n_pad = 64;
     p.w_splits = 1;
     return;
@@ -810,15 +773,16 @@ void plan_backward(Plan &p, bool x, bool w, bool b) {
 }
 
 // waves a SIMD of the forward (1 024 rows x 1 M items of 128: four tiles of rows x 2 waves 293 us, x 3 282, two x 4 316)
-constexpr int sums_waves(int steps, int planes, int tiles) { return steps * planes == 8 || tiles < 4 ? 2 : steps * planes == 4 ? 3 : 4; }
+constexpr int sums_waves(int steps, int planes, int tiles) { return planes > 1 ? (steps == 2 ? 2 : 1) : steps == 8 || tiles < 4 ? 2 : steps == 4 ? 3 : 4; }
 // Forward, up to 64 rows: a table that is an operand as it lies streams through the other forms at 5 to 6 TB/s (4 to 64 rows, 512 187 items
 // of 640 (f16): 124 us, in the form for few rows 190 to 281; small tables are quicker without the tiles: 20 rows, 10 000 of 768 16 and
 // 19 us).  What would need an image does not: 56 bf16 rows, 500 000 of 700 at an odd stride, 297 and 432 us; 16 rows of 200 47 and 75
-// (60 rows 84 and 81); 16 f32 rows, 500 000 of 128 62 and 105 (42 rows 95 and 90).  16-bit rows of up to 128 are shifted as quickly by
+// (60 rows 84 and 81); 24 f32 rows, 500 000 of 128 98 and 135
+// (of 64: 51 and 48).  16-bit rows of up to 128 are shifted as quickly by
 // the short rows' form (16 rows of 100, 50 us, here 57).
 bool few_pays(const Plan &p, bool table_direct) {
   if (p.n > 64) return false;
-  if (p.planes == 2) return p.n <= 32 || p.d > 128;  // (718 298 items of 384: 16 rows 306 us, 48 539, by images 908)
+  if (p.planes > 1) return p.n <= 32 || p.d > 128;  // (718 298 items of 384: 24 rows 500 us, 48 535, by images 1 020; only long rows of small tables lose: 48 x 100 000 of 768 402 and 311)
   if (table_direct) return !p.fused && (uint64_t)p.v * p.d < (16ull << 20);
   return p.d > 128 && (p.n <= 32 || p.d > 256);
 }
@@ -827,7 +791,7 @@ void plan_forward(Plan &p, bool table_direct) {
   p.few = few_pays(p, table_direct) ? few_steps(p.d) : 0;
   if (p.few) {
     p.fused = 0;
-    p.few_groups = few_groups(p.few, p.d, p.planes == 2, p.n <= 16 || p.planes == 2 ? kFewOne : p.n <= 32 ? kFewTwo : kFewFour, p.v);
+    p.few_groups = few_groups(p.few, p.d, p.planes > 1, p.n <= 16 || p.planes > 1 ? kFewOne : p.n <= 32 ? kFewTwo : kFewFour, p.v);
     p.parts = p.few_groups * (4 / few_share(p.d));
     return;
   }
@@ -848,22 +812,17 @@ void plan_forward(Plan &p, bool table_direct) {
 
 struct ForwardScratch {
   float2 *part;
-  unsigned int *tops;
-  float *top_parts;
   unsigned short *x_image, *t_image;
 };
 uint64_t forward_layout(const Plan &p, const Source &x, const Source &t, char *base, ForwardScratch &s) {
   Layout l{base};
   s.part = l.take<float2>((uint64_t)p.parts * p.n);
-  s.tops = l.take<unsigned int>(2);
-  s.top_parts = l.take<float>(p.planes == 2 && !p.few ? 2 * kTopParts : 0);
   s.x_image = l.take<unsigned short>(x.image_elems(p.few || (p.fused && p.raw)));
   s.t_image = l.take<unsigned short>(t.image_elems(p.few || (p.fused && p.raw)));
   return l.at;
 }
 struct BackwardScratch {
-  unsigned int *tops;
-  float *top_parts, *coef;
+  float *coef;
   unsigned short *x_image, *t_image, *G;
   u32x2 *met;
   uint32_t *met_count;
@@ -874,8 +833,6 @@ struct BackwardScratch {
 uint64_t backward_layout(const Plan &p, const Source &x, const Source &t, char *base, BackwardScratch &s) {
   Layout l{base};
   const uint64_t pl = p.planes;
-  s.tops = l.take<unsigned int>(2);
-  s.top_parts = l.take<float>(p.planes == 2 && !p.few ? 2 * kTopParts : 0);
   s.coef = l.take<float>(2);
   s.x_image = l.take<unsigned short>(x.image_elems(p.few || (p.fused && p.raw)));
   s.t_image = l.take<unsigned short>(t.image_elems(p.few || (p.fused && p.raw)));
@@ -916,16 +873,14 @@ void by_type(int dt, F &&f) {
 }
 unsigned spread(uint64_t items, uint64_t per_block) { return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((items + per_block - 1) / per_block, 16384)); }
 
-// The two matrices as the products read them: each as it is, or its image; f32 with the largest magnitudes first.
+// The two matrices as the products read them: each as it is, or its image.
 struct Operands {
   const char *x, *t;
   size_t x_ld, t_ld;
 };
-// (raw: the kernels take the matrices as they are, f32 needs the magnitudes only)
-int make_operands(as_ctx *ctx, const Source &x, const Source &t, bool raw, unsigned int *tops, float *parts, unsigned short *x_image, unsigned short *t_image,
-                  Operands *out) {
+// (raw: the kernels take the matrices as they are)
+int make_operands(as_ctx *ctx, const Source &x, const Source &t, bool raw, unsigned short *x_image, unsigned short *t_image, Operands *out) {
   ImageJobs jobs{};
-  jobs.tops = tops, jobs.parts = parts;
   uint32_t count = 0;
   uint64_t most = 1;
   auto add = [&](const Source &s, unsigned short *image, const char **p, size_t *ld) {
@@ -937,19 +892,16 @@ int make_operands(as_ctx *ctx, const Source &x, const Source &t, bool raw, unsig
       *p = (const char *)image;
       *ld = (size_t)s.pitch() * s.planes() * 2;
     }
-    if (s.direct() || (raw && s.dt != AS_F32)) return;
+    if (s.direct() || raw) return;
     jobs.job[count++] = ImageJob{(const char *)s.p, s.stride * es, s.rows, s.d, s.pitch(), image};
     most = std::max<uint64_t>(most, (uint64_t)s.rows * s.pitch() / 4096);
   };
   add(x, x_image, &out->x, &out->x_ld);
   add(t, t_image, &out->t, &out->t_ld);
   if (!count) return AS_OK;
-  if (x.dt == AS_F32) hipLaunchKernelGGL(top_kernel, dim3(kTopParts, 2), dim3(1024), 0, ctx->stream, jobs);
-  if (!raw)
-    by_type(x.dt, [&](auto dt) {
-      constexpr int DT = decltype(dt)::value;
-      hipLaunchKernelGGL((image_kernel<DT, DT == AS_BF16 ? AS_BF16 : AS_F16>), dim3((unsigned)std::min<uint64_t>(most, 2048), count), dim3(256), 0, ctx->stream, jobs);
-    });
+  by_type(x.dt, [&](auto dt) {
+    hipLaunchKernelGGL((image_kernel<decltype(dt)::value>), dim3((unsigned)std::min<uint64_t>(most, 2048), count), dim3(256), 0, ctx->stream, jobs);
+  });
   AS_HIP(ctx, hipGetLastError());
   return AS_OK;
 }
@@ -972,7 +924,7 @@ void by_steps(int dt, bool raw, int steps, F &&f) {  // f(type, raw, steps)
 template <bool ITEMS>
 void launch_rows_grad(as_ctx *ctx, int dt, bool raw, int steps, bool bias, const LossRowsArgs &a) {
   by_steps(dt, raw, steps, [&](auto type, auto rw, auto kd) {
-    constexpr int DT = decltype(type)::value, KD = decltype(kd)::value, P = DT == AS_F32 ? 2 : 1, RT = fused_rows(KD, P, ITEMS), W = fused_waves(KD, P, ITEMS);
+    constexpr int DT = decltype(type)::value, KD = decltype(kd)::value, P = planes_of(DT), RT = fused_rows(KD, P, ITEMS), W = fused_waves(KD, P, ITEMS);
     constexpr bool RAW = decltype(rw)::value;
     if (bias) hipLaunchKernelGGL((loss_rows_grad_kernel<DT, RAW, RT, KD, ITEMS, true, W>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
     else hipLaunchKernelGGL((loss_rows_grad_kernel<DT, RAW, RT, KD, ITEMS, false, W>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
@@ -1033,7 +985,7 @@ void launch_few_grad(as_ctx *ctx, const Plan &p, const LossFewArgs &a) {
 template <int RT>
 void launch_rows_sums(as_ctx *ctx, int dt, bool raw, int steps, bool general, const LossSumsArgs &a) {
   by_steps(dt, raw, steps, [&](auto type, auto rw, auto kd) {
-    constexpr int DT = decltype(type)::value, KD = decltype(kd)::value, W = sums_waves(KD, DT == AS_F32 ? 2 : 1, RT);
+    constexpr int DT = decltype(type)::value, KD = decltype(kd)::value, W = sums_waves(KD, planes_of(DT), RT);
     constexpr bool RAW = decltype(rw)::value;
     if (general) hipLaunchKernelGGL((loss_rows_sums_kernel<DT, RAW, RT, KD, true, W>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
     else hipLaunchKernelGGL((loss_rows_sums_kernel<DT, RAW, RT, KD, false, W>), dim3(a.r_blocks * a.splits), dim3(256), 0, ctx->stream, a);
@@ -1055,8 +1007,8 @@ void launch_product(as_ctx *ctx, int fmt, int tile, bool w, int out_type, const 
     constexpr std::integral_constant<int, 0> acc{};
     constexpr std::true_type yes{};
     constexpr std::false_type no{};
-    if (fmt == AS_BF16) !w ? go(bf, acc, no) : out_type == 0 ? go(bf, acc, yes) : go(bf, bf, yes);
-    else !w ? go(hf, acc, no) : out_type == 0 ? go(hf, acc, yes) : out_type == AS_F32 ? go(hf, f32, yes) : go(hf, hf, yes);
+    if (fmt == AS_BF16) !w ? go(bf, acc, no) : out_type == 0 ? go(bf, acc, yes) : out_type == AS_F32 ? go(bf, f32, yes) : go(bf, bf, yes);
+    else !w ? go(hf, acc, no) : out_type == 0 ? go(hf, acc, yes) : go(hf, hf, yes);
   });
 }
 
@@ -1112,12 +1064,11 @@ int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tabl
   ProfScope prof(ctx, "cross_entropy");
   LossArgs a{};
   Operands o{};
-  if (!p.few) AS_TRY(make_operands(ctx, xs, ts, p.fused && p.raw, s.tops, s.top_parts, s.x_image, s.t_image, &o));
+  if (!p.few) AS_TRY(make_operands(ctx, xs, ts, p.fused && p.raw, s.x_image, s.t_image, &o));
   a.rows = o.x, a.rows_ld = o.x_ld, a.table = o.t, a.table_ld = o.t_ld;
   a.table_plane = a.rows_plane = (size_t)p.pitch * 2;
-  a.n = p.n, a.v = p.v, a.steps = p.steps, a.planes = p.planes, a.per = p.per, a.v_tiles = p.v_tiles, a.n_tiles = p.n_tiles, a.chunks = p.chunks;
+  a.n = p.n, a.v = p.v, a.steps = p.steps, a.all = p.steps * pairs_of(p.planes), a.per = p.per, a.v_tiles = p.v_tiles, a.n_tiles = p.n_tiles, a.chunks = p.chunks;
   a.scale = c.scale, a.bias = (const float *)Bi.p;
-  if (p.planes == 2) a.rows_top = s.tops, a.table_top = s.tops + 1;
   const bool general = bias || !(c.scale > 0.f);
   if (p.few) {
     LossFewArgs r{};
@@ -1126,7 +1077,7 @@ int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tabl
     launch_few_sums(ctx, p, general, r);
   } else if (p.fused) {
     LossSumsArgs r{};
-    r.r = a.rows, r.r_ld = a.rows_ld, r.nr = p.n, r.k = a.table, r.k_ld = a.table_ld, r.nk = p.v, r.d = p.d, r.top_parts = s.top_parts;
+    r.r = a.rows, r.r_ld = a.rows_ld, r.nr = p.n, r.k = a.table, r.k_ld = a.table_ld, r.nk = p.v, r.d = p.d;
     r.r_blocks = p.x_blocks, r.splits = p.splits, r.scale = c.scale, r.bias = a.bias, r.part = s.part;
     const bool raw = p.raw && !(xs.direct() && ts.direct());
     if (p.rows_tiles == 1) launch_rows_sums<1>(ctx, c.dt, raw, p.fused, general, r);
@@ -1142,7 +1093,7 @@ int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tabl
       };
       constexpr std::integral_constant<int, AS_BF16> bf{};
       constexpr std::integral_constant<int, AS_F16> hf{};
-      if (c.dt == AS_BF16) general ? go(bf, std::true_type{}) : go(bf, std::false_type{});
+      if (format_of(c.dt) == AS_BF16) general ? go(bf, std::true_type{}) : go(bf, std::false_type{});
       else general ? go(hf, std::true_type{}) : go(hf, std::false_type{});
     });
   }
@@ -1205,26 +1156,25 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
   GradArgs g{};
   LossArgs &a = g.l;
   Operands o{};
-  if (!p.few) AS_TRY(make_operands(ctx, xs, ts, p.fused && p.raw, s.tops, s.top_parts, s.x_image, s.t_image, &o));
+  if (!p.few) AS_TRY(make_operands(ctx, xs, ts, p.fused && p.raw, s.x_image, s.t_image, &o));
   const char *table16 = o.t;
   a.rows = o.x, a.rows_ld = o.x_ld, a.table_ld = o.t_ld;
-  const unsigned int *x_top = p.planes == 2 ? s.tops : nullptr, *w_top = p.planes == 2 ? s.tops + 1 : nullptr;
   AS_HIP(ctx, hipGetLastError());
   const float *coef = s.coef;
   const float *rest = p.planes == 1 ? s.rest : nullptr;
   const LossRowInputs by_row{X.p, W.p, (size_t)c.x_stride, (size_t)c.table_stride, p.d, p.n, p.n_pad, p.v, (const float *)Bi.p, (const float *)Ls.p,
-                             (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p, ignore, c.scale, c.dt == AS_BF16 || (p.few && c.dt == AS_F32) ? 0 : 14, s.coef, s.lse, s.every,
-                             s.entry, s.rest, s.target, p.fused && p.raw ? s.top_parts : nullptr, s.tops};
+                             (const float *)Gl.p, (const float *)Ge.p, (const int64_t *)Y.p, ignore, c.scale, c.dt == AS_F16 ? 14 : 0, s.coef, s.lse, s.every,
+                             s.entry, s.rest, s.target};
   if (p.n > kFewRows)
     hipLaunchKernelGGL(coef_scale_kernel, dim3(1), dim3(1024), 0, ctx->stream, by_row.gl, by_row.ge, by_row.targets, ignore, p.n, by_row.power, s.coef);
   by_type(c.dt, [&](auto dt) {
-    constexpr int DT = decltype(dt)::value, FMT = DT == AS_BF16 ? AS_BF16 : AS_F16;
+    constexpr int DT = decltype(dt)::value, FMT = format_of(DT);
     if (p.n > kFewRows) hipLaunchKernelGGL((loss_rows_kernel<DT, FMT, false>), dim3(cdiv(p.n_pad, 4)), dim3(256), 0, ctx->stream, by_row);
     else hipLaunchKernelGGL((loss_rows_kernel<DT, FMT, true>), dim3(cdiv(p.n_pad, 4)), dim3(256), 0, ctx->stream, by_row);
   });
   AS_HIP(ctx, hipGetLastError());
   // dX from its parts, or dW where the batch was split
-  auto join = [&](const float *sums, uint32_t splits, uint32_t n, const unsigned int *top, bool with_rest, void *out, uint64_t stride) {
+  auto join = [&](const float *sums, uint32_t splits, uint32_t n, bool with_rest, void *out, uint64_t stride) {
     by_type(c.dt, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
       const uint32_t pitch = up(p.d, 8);
@@ -1233,7 +1183,7 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
       auto go = [&](auto ways) {
         constexpr int WAYS = decltype(ways)::value;
         hipLaunchKernelGGL((grad_rows_join_kernel<DT, WAYS>), dim3(spread(total, WAYS == 64 ? 64 : WAYS == 4 ? 256 : 1024)), dim3(WAYS == 64 ? 1024 : 256), 0, ctx->stream,
-                           sums, splits, pitch, n, p.d, c.scale, coef, top, (const int *)s.target, r, W.p, (size_t)c.table_stride, out, (size_t)stride);
+                           sums, splits, pitch, n, p.d, c.scale, coef, (const int *)s.target, r, W.p, (size_t)c.table_stride, out, (size_t)stride);
       };
       // 16 waves a compute unit, or as many ways as parts: 777 x 200 from 64 parts 7 us in 4 ways, 25 in 64; 9 x 64 from 1 024 parts 5.6 us
       // in 64, 12 in 16
@@ -1260,22 +1210,22 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
     r.lse = s.lse, r.every = s.every, r.entry = s.entry, r.rest = s.rest, r.target = s.target;
     r.sums_pitch = up(p.d, 8);
     if (p.want_w || p.want_b) {
-      r.r = o.t, r.r_ld = o.t_ld, r.nr = p.v, r.r_top = w_top;
-      r.k = o.x, r.k_ld = o.x_ld, r.nk = p.n, r.k_top = x_top;
+      r.r = o.t, r.r_ld = o.t_ld, r.nr = p.v;
+      r.k = o.x, r.k_ld = o.x_ld, r.nk = p.n;
       r.r_blocks = p.w_blocks, r.splits = p.w_splits;
       if (p.w_splits > 1) r.sums = s.w_sums;
       r.out = Ow.p, r.out_stride = gw_stride;
       r.grad_bias = !p.want_b ? nullptr : p.w_splits > 1 ? s.bias_part : (float *)Ob.p;
       launch_rows_grad<true>(ctx, c.dt, raw, p.fused, bias != nullptr, r);
       if (p.w_splits > 1) {
-        if (p.want_w) join(s.w_sums, p.w_splits, p.v, x_top, false, Ow.p, gw_stride);
+        if (p.want_w) join(s.w_sums, p.w_splits, p.v, false, Ow.p, gw_stride);
         if (p.want_b)
           hipLaunchKernelGGL(bias_join_kernel, dim3(cdiv(p.v, 256)), dim3(256), 0, ctx->stream, (const float *)s.bias_part, p.w_splits, p.v, p.v, coef, (float *)Ob.p);
       }
     }
     if (p.want_x) {
-      r.r = o.x, r.r_ld = o.x_ld, r.nr = p.n, r.r_top = x_top;
-      r.k = o.t, r.k_ld = o.t_ld, r.nk = p.v, r.k_top = w_top;
+      r.r = o.x, r.r_ld = o.x_ld, r.nr = p.n;
+      r.k = o.t, r.k_ld = o.t_ld, r.nk = p.v;
       r.r_blocks = p.x_blocks, r.splits = p.splits;
       r.sums = s.sums;
       launch_rows_grad<false>(ctx, c.dt, raw, p.fused, bias != nullptr, r);
@@ -1283,13 +1233,12 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
     AS_HIP(ctx, hipGetLastError());
   }
   a.table_plane = a.rows_plane = (size_t)p.pitch * 2;
-  a.n = p.n, a.steps = p.steps, a.planes = p.planes, a.n_tiles = p.n_tiles, a.per = p.per;
+  a.n = p.n, a.steps = p.steps, a.all = p.steps * pairs_of(p.planes), a.n_tiles = p.n_tiles, a.per = p.per;
   a.scale = c.scale;
-  a.rows_top = x_top, a.table_top = w_top;
   g.lse = s.lse, g.every = s.every, g.entry = s.entry, g.target = s.target, g.coef = coef;
   g.G = s.G, g.g_pitch = p.piece;
   g.bias_part = p.want_b ? s.bias_part : nullptr;
-  const int fmt = image_format(c.dt);
+  const int fmt = format_of(c.dt);
   if (!p.fused && !p.few && rest && p.want_w) {
     const uint32_t groups = cdiv(p.v, 64);
     hipLaunchKernelGGL(met_kernel, dim3(groups), dim3(512), 0, ctx->stream, (const int *)s.target, p.n, s.met, s.met_count);
@@ -1302,35 +1251,37 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
     g.v_begin = v0;
     by_tile(p.tile, [&](auto k) {
       constexpr int K = decltype(k)::value;
-      auto go = [&](auto f, auto two, auto with_bias) {
+      auto go = [&](auto f, auto planes, auto with_bias) {
         constexpr int FMT = decltype(f)::value;
-        hipLaunchKernelGGL((loss_grad_kernel<FMT, TileOf<FMT, K>, decltype(two)::value, decltype(with_bias)::value>), dim3(a.n_tiles * a.chunks),
+        hipLaunchKernelGGL((loss_grad_kernel<FMT, TileOf<FMT, K>, decltype(planes)::value, decltype(with_bias)::value>), dim3(a.n_tiles * a.chunks),
                            dim3(TileOf<FMT, K>::NT), 0, ctx->stream, g);
       };
       constexpr std::integral_constant<int, AS_BF16> bf{};
       constexpr std::integral_constant<int, AS_F16> hf{};
       constexpr std::true_type yes{};
       constexpr std::false_type no{};
-      if (c.dt == AS_BF16) bias ? go(bf, no, yes) : go(bf, no, no);
-      else if (c.dt == AS_F16) bias ? go(hf, no, yes) : go(hf, no, no);
-      else bias ? go(hf, yes, yes) : go(hf, yes, no);
+      constexpr std::integral_constant<int, 1> one{};
+      constexpr std::integral_constant<int, kF32Planes> three{};
+      if (c.dt == AS_BF16) bias ? go(bf, one, yes) : go(bf, one, no);
+      else if (c.dt == AS_F16) bias ? go(hf, one, yes) : go(hf, one, no);
+      else bias ? go(bf, three, yes) : go(bf, three, no);
     });
     if (p.want_b)
       hipLaunchKernelGGL(bias_join_kernel, dim3(cdiv(items, 256)), dim3(256), 0, ctx->stream, (const float *)s.bias_part, p.n_tiles * kShape[p.tile].wn, p.piece, items,
                          coef, (float *)Ob.p + v0);
     ProductArgs w{};
     w.B = (const char *)s.G, w.b_ld = (size_t)p.piece * p.planes * 2, w.b_plane = (size_t)p.piece * 2, w.b_cols = p.piece / 8, w.k_b = p.n_pad;
-    w.m = p.d, w.a_plane = (size_t)p.pitch * 2, w.a_cols = p.pitch / 8, w.planes = p.planes;
+    w.m = p.d, w.a_plane = (size_t)p.pitch * 2, w.a_cols = p.pitch / 8, w.pairs = pairs_of(p.planes);
     w.scale = c.scale, w.coef = coef;
     if (p.want_w) {
       w.A = a.rows, w.a_ld = a.rows_ld, w.k_a = p.n;
       w.n = items, w.m_tiles = cdiv(p.d, kShape[p.tile_w].bm), w.n_tiles = cdiv(items, kShape[p.tile_w].bn);
-      w.steps = cdiv(p.n, 64), w.splits = p.w_splits, w.top = x_top;
+      w.steps = cdiv(p.n, 64), w.splits = p.w_splits;
       w.sums = s.w_sums, w.sums_pitch = up(p.d, 8), w.first = 1;
       w.out = (char *)Ow.p + (size_t)v0 * gw_stride * dtype_size(c.dt), w.out_stride = gw_stride;
       if (rest) w.met = s.met + (size_t)(v0 / 64) * kMet, w.met_count = s.met_count + v0 / 64, w.rest = rest;
       launch_product(ctx, fmt, p.tile_w, true, p.w_splits > 1 ? 0 : c.dt, w);
-      if (p.w_splits > 1) join(s.w_sums, p.w_splits, p.v, x_top, false, Ow.p, gw_stride);
+      if (p.w_splits > 1) join(s.w_sums, p.w_splits, p.v, false, Ow.p, gw_stride);
     }
     if (p.want_x) {
       w.met = nullptr;
@@ -1343,7 +1294,7 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
     AS_HIP(ctx, hipGetLastError());
   }
   if (p.want_x) {
-    join(s.sums, p.splits, p.n, p.few ? nullptr : w_top, true, Ox.p, gx_stride);
+    join(s.sums, p.splits, p.n, true, Ox.p, gx_stride);
     AS_HIP(ctx, hipGetLastError());
   }
   AS_TRY(Ox.finish(ctx));

@@ -7,12 +7,12 @@
 // four partial logits meet in LDS (one barrier a stage).  Backward each wave then knows g and makes its columns of both gradients:
 //   dX (rows x columns, in registers over the whole walk)  A = items transposed (4 of a column a lane), B = g (row, 4 items)
 //   dW (16 items x columns, stored at once)                A = rows transposed (kept),                  B = g turned over in LDS (item, 4 rows)
-// f32 goes as three bf16 planes (24 bits, no common scale to be found first, six products of 2^-24 and more): the matrix pipe has time.
+// f32 goes as three bf16 planes, split on the way into the LDS: the matrix pipe has time.
 // Up to 128 columns a wave takes whole items instead, each its own stretch of the table, and nothing meets before the end.
 // Rows of any alignment go in and out in 16-byte pieces: element by element the stores of 8 rows' dW (538 194 items of 337, f16) took
 // 532 us, so 274.
 // Measured: backward of 8 rows, 500 000 items of 384 (bf16, 384 MB read and written) 235 us = 3.3 TB/s, through G 389; of 9 rows, 496 726
-// of 64 27 and 63; of 8 f32 rows, 300 000 of 384 353 and 817.  Forward (few_pays in table_loss.hip: where the table would need an image)
+// of 64 27 and 63; of 8 f32 rows, 300 000 of 384 351 and 1 167.  Forward (few_pays in table_loss.hip: where the table would need an image)
 // of 2 rows, 688 025 of 678 at an odd stride 266, backward 641, through images and G 2 744 in all.
 #pragma once
 
@@ -27,41 +27,6 @@ __device__ __forceinline__ f32x4 few_mfma16(u32x2 a, u32x2 b, f32x4 c) {  // 16 
   if constexpr (FMT == AS_BF16) return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4v, a), __builtin_bit_cast(short4v, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4, a), __builtin_bit_cast(half4, b), c, 0, 0, 0);
 }
-// P planes of a value: 1 in its own type, 3 as bf16 (an infinity or NaN in the first alone)
-template <int P>
-__device__ __forceinline__ void few_split(float x, float (&o)[P]) {
-  o[0] = x;
-  if constexpr (P == 3) {
-    const float hi = (float)(__bf16)x;
-    const float r = __builtin_isfinite(hi) ? x - hi : 0.f;
-    o[1] = r;
-    o[2] = r - (float)(__bf16)r;
-  }
-}
-template <int FMT, int P>
-__device__ __forceinline__ void few_pack(float x, float y, uint32_t (&o)[P]) {
-  float a[P], b[P];
-  few_split<P>(x, a);
-  few_split<P>(y, b);
-#pragma unroll
-  for (int p = 0; p < P; ++p) o[p] = pack2<FMT>(a[p], b[p]);
-}
-// eight values of a piece as planes
-template <int FMT, int P, int DT>
-__device__ __forceinline__ void few_planes(const LrPiece<DT, true> &piece, u32x4 (&o)[P]) {
-  if constexpr (P == 1) {
-    o[0] = piece.w[0];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      uint32_t w[P];
-      few_pack<FMT, P>(__uint_as_float(piece.w[e >> 1][2 * (e & 1)]), __uint_as_float(piece.w[e >> 1][2 * (e & 1) + 1]), w);
-#pragma unroll
-      for (int p = 0; p < P; ++p) o[p][e] = w[p];
-    }
-  }
-}
-
 struct LossFewArgs {
   const char *rows, *table;
   size_t rows_ld, table_ld;       // bytes
@@ -85,7 +50,7 @@ struct LossFewArgs {
 // KC steps of 32 columns a wave (d <= 128 KC); RT tiles of 16 rows
 template <int DT, int KC, bool BIAS>
 struct FewSlice {
-  static constexpr int FMT = DT == AS_F16 ? AS_F16 : AS_BF16, P = DT == AS_F32 ? 3 : 1;
+  static constexpr int FMT = format_of(DT), P = planes_of(DT);
   static constexpr uint32_t CW = 32 * KC, kRow = CW * 2 + 16, kPlane = 16 * kRow, kWave = P * kPlane;  // (16 bytes between rows: eight rows of a read in different banks)
   LrPiece<DT, true> piece[KC];
   f32x4 bias;  // of this lane's four items
@@ -113,7 +78,7 @@ struct FewSlice {
     for (int t = 0; t < KC; ++t) {
       const uint32_t idx = t * 64 + lane, row = idx / (4 * KC), slot = idx % (4 * KC);
       u32x4 o[P];
-      few_planes<FMT, P, DT>(piece[t], o);
+      piece[t].template planes<FMT, P>(o);
 #pragma unroll
       for (int p = 0; p < P; ++p) *(u32x4 *)(dst + p * kPlane + row * kRow + slot * 16) = o[p];
     }
@@ -147,7 +112,7 @@ __device__ __forceinline__ void few_rows(const LossFewArgs &a, uint32_t n, uint3
       LrPiece<DT, true> piece;
       piece.load(a.rows + (size_t)nt_min(j * 16 + col, n - 1) * a.rows_ld, column0 + t * 32 + q * 8, a.d, 0);
       u32x4 o[P];
-      few_planes<FMT, P, DT>(piece, o);
+      piece.template planes<FMT, P>(o);
 #pragma unroll
       for (int p = 0; p < P; ++p) R[p][j][t] = o[p];
     }
@@ -264,7 +229,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_grad_kernel(LossFewArgs a
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t w[P];
-      few_pack<FMT, P>(x[2 * h], x[2 * h + 1], w);
+      pack_planes<FMT, P>(x[2 * h], x[2 * h + 1], w);
 #pragma unroll
       for (int p = 0; p < P; ++p) XT[p][t][h] = w[p];
     }
@@ -309,7 +274,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_grad_kernel(LossFewArgs a
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t w[P];
-      few_pack<FMT, P>(g[2 * h], g[2 * h + 1], w);
+      pack_planes<FMT, P>(g[2 * h], g[2 * h + 1], w);
 #pragma unroll
       for (int p = 0; p < P; ++p) G[p][h] = w[p];
     }

@@ -8,8 +8,8 @@
 //   gradient   of those 8 logits in f32, rounded to 16 bits: exactly the operand (row r, 8 consecutive k a lane group) of
 //   output     A = the SAME stage read transposed (ds_read_b64_tr_b16: 4 rows k of a column a lane), B = the gradients.
 // Against the form over G in memory this saves writing and reading 2 bytes a logit, for 2 d flops more a logit: forward and backward of a
-// million items of 128 values and 1 024 rows (bf16) 2.01 ms through G, 1.27 ms so (sums 282 us, dX 440, dW 490); 512 f32 rows, 100 000
-// items of 128: 383 and 296 us.  What bounds it there: the matrix pipe and the exponentials' and packing's vector work of two waves a SIMD
+// million items of 128 values and 1 024 rows (bf16) 2.01 ms through G, 1.27 ms so (sums 282 us, dX 440, dW 490); the gradients of 512 f32 rows,
+// 100 000 items of 128: 453 and 374 us.  What bounds it there: the matrix pipe and the exponentials' and packing's vector work of two waves a SIMD
 // take turns (0.27 TFLOP of logits at 282 us: 950 TFLOP/s).  d is bounded by the registers (d <= 256, f32 128).
 #pragma once
 
@@ -18,13 +18,6 @@
 namespace asx {
 
 constexpr float kLog2e = 1.44269504088896340736f;
-// the power of two a matrix with this largest magnitude is multiplied by (0 or not a number: 1)
-__device__ __forceinline__ float plane_scale(unsigned int top_bits) {
-  const int e = (int)(top_bits >> 23);
-  if (e == 0 || e >= 255) return 1.f;
-  const int s = min(max(14 - (e - 127), -100), 100);
-  return __uint_as_float((unsigned int)(127 + s) << 23);
-}
 // Workgroups are dealt to the 8 dies in turn; consecutive pieces of work should share a die's cache, so die d takes the d-th eighth.
 __device__ __forceinline__ uint32_t die_order(uint32_t b, uint32_t total) {
   const uint32_t die = b & 7, at = b >> 3, each = total >> 3, rest = total & 7;
@@ -67,11 +60,32 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     return __builtin_bit_cast(uint32_t, p);
   }
 }
-__device__ __forceinline__ float low_part(float x) {  // what f16 leaves of x (nothing of an infinity)
-  const float hi = (float)(_Float16)x;
-  return __builtin_isfinite(hi) ? x - hi : 0.f;
+// What the matrix pipe is fed, by the type of the matrices: their own 16-bit type, or f32 as the sum of three bf16 (24 bits, the exponents
+// of f32: no scale that an outlier would set for everyone).  Of the nine products of two such sums the six of 2^-18 and more are made: planes
+// (p, o) with p + o <= 2; what is left out is 2^-26 of a product.
+constexpr int kF32Planes = 3;
+constexpr int format_of(int dt) { return dt == AS_F16 ? AS_F16 : AS_BF16; }
+constexpr int planes_of(int dt) { return dt == AS_F32 ? kF32Planes : 1; }
+constexpr uint32_t pairs_of(uint32_t planes) { return planes == 1 ? 1 : 6; }
+// P planes of a value (an infinity or NaN in the first alone)
+template <int P>
+__device__ __forceinline__ void split_planes(float x, float (&o)[P]) {
+  o[0] = x;
+  if constexpr (P == 3) {
+    const float hi = (float)(__bf16)x;
+    const float r = __builtin_isfinite(hi) ? x - hi : 0.f;
+    o[1] = r;
+    o[2] = r - (float)(__bf16)r;
+  }
 }
-
+template <int FMT, int P>
+__device__ __forceinline__ void pack_planes(float x, float y, uint32_t (&o)[P]) {
+  float a[P], b[P];
+  split_planes<P>(x, a);
+  split_planes<P>(y, b);
+#pragma unroll
+  for (int p = 0; p < P; ++p) o[p] = pack2<FMT>(a[p], b[p]);
+}
 
 // eight consecutive values of a row, of any alignment
 template <int DT>
@@ -91,7 +105,6 @@ struct LossRowsArgs {
   uint32_t nr, nk, d;
   uint32_t r_blocks, splits;      // blocks of rows r; parts of the k side (sums: one buffer each)
   float scale;
-  const unsigned int *r_top, *k_top;  // f32: bits of the largest magnitude of the two matrices
   // by row of the batch, filled to whole 64s (probability 0, no target)
   const float *lse, *every, *entry, *rest;
   const int *target;
@@ -145,18 +158,6 @@ __global__ __launch_bounds__(1024) void coef_scale_kernel(const float *gl, const
   if (threadIdx.x == 0) out[0] = factor, out[1] = unit;
 }
 
-// f32: the largest finite magnitude of a matrix, a part per workgroup (its bits order as integers; a maximum has no order)
-constexpr uint32_t kTopParts = 256;
-__device__ __forceinline__ unsigned int top_of_parts(const float *parts) {  // 256 threads or more
-  __shared__ float s[4];
-  float m = threadIdx.x < kTopParts ? parts[threadIdx.x] : 0.f;
-  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
-  __syncthreads();
-  if (threadIdx.x < kTopParts && (threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
-  __syncthreads();
-  return __float_as_uint(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-}
-
 // By row of the batch, a wave each: the coefficient of its probabilities, and its entry at its target.  That entry is most of a row's
 // gradient and often all of its item's, so it comes from a product in f64, the kernels put it in place of their own, and what 16 bits
 // leave of it (`rest`, as much as the rounding of the result) is added in f32: to dX where its parts are joined, to dW behind the
@@ -174,8 +175,6 @@ struct LossRowInputs {
   float *coef;
   float *o_lse, *o_every, *o_entry, *o_rest;
   int *o_target;
-  const float *top_parts;  // f32: parts of the two matrices' largest magnitudes, and where their bits go
-  unsigned int *tops;
 };
 template <int DT, int FMT, bool FEW>
 __global__ __launch_bounds__(256) void loss_rows_kernel(LossRowInputs a) {
@@ -186,10 +185,6 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossRowInputs a) {
     if (blockIdx.x == 0 && threadIdx.x == 0) a.coef[0] = f, a.coef[1] = unit;
   } else {
     f = a.coef[0];
-  }
-  if (DT == AS_F32 && blockIdx.x == 0 && a.top_parts) {
-    const unsigned int x_top = top_of_parts(a.top_parts), t_top = top_of_parts(a.top_parts + kTopParts);
-    if (threadIdx.x == 0) a.tops[0] = x_top, a.tops[1] = t_top;
   }
   if (t >= a.padded) return;
   float s = INFINITY, every = 0.f, entry = 0.f;   // (behind the last row: probability 0)
@@ -243,14 +238,14 @@ __device__ __forceinline__ u32x4 lr_column(const char *smem, uint32_t at, uint32
   return u32x4{x[0], x[1], y[0], y[1]};
 }
 // Eight consecutive values of a row, as the matrix holds them (columns behind the row's d: zeros) and as 16-bit operands.  RAW: rows of
-// any alignment and length; else whole 16-byte pieces, f32 as images of two planes.
+// any alignment and length; else whole 16-byte pieces, f32 as images of its planes (`plane` bytes apart).
 template <int DT, bool RAW>
 struct LrPiece {
-  u32x4 w[DT == AS_F32 ? 2 : 1];
+  u32x4 w[DT != AS_F32 ? 1 : RAW ? 2 : kF32Planes];
   __device__ __forceinline__ void load(const char *row, uint32_t column, uint32_t d, uint32_t plane) {
     if constexpr (!RAW) {
-      w[0] = *(const u32x4 *)(row + column * 2);
-      if constexpr (DT == AS_F32) w[1] = *(const u32x4 *)(row + plane + column * 2);
+#pragma unroll
+      for (int p = 0; p < planes_of(DT); ++p) w[p] = *(const u32x4 *)(row + p * plane + column * 2);
     } else {
       Piece8<DT> raw;
       raw.load(row, column, d);
@@ -258,20 +253,21 @@ struct LrPiece {
       if constexpr (DT == AS_F32) w[1] = raw.w[1];
     }
   }
-  // f32: the high and the low plane of the values times `scale`
   template <int FMT, int P>
-  __device__ __forceinline__ void planes(float scale, u32x4 (&o)[P]) const {
-    if constexpr (DT == AS_F32 && !RAW) {
-      o[0] = w[0], o[P - 1] = w[1];
-    } else if constexpr (DT == AS_F32) {
+  __device__ __forceinline__ void planes(u32x4 (&o)[P]) const {
+    if constexpr (P == 1) {
+      o[0] = w[0];
+    } else if constexpr (!RAW) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) o[p] = w[p];
+    } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x = __uint_as_float(w[e >> 1][2 * (e & 1)]) * scale, y = __uint_as_float(w[e >> 1][2 * (e & 1) + 1]) * scale;
-        o[0][e] = pack2<FMT>(x, y);
-        if constexpr (P == 2) o[P - 1][e] = pack2<FMT>(low_part(x), low_part(y));
+        uint32_t pair[P];
+        pack_planes<FMT, P>(__uint_as_float(w[e >> 1][2 * (e & 1)]), __uint_as_float(w[e >> 1][2 * (e & 1) + 1]), pair);
+#pragma unroll
+        for (int p = 0; p < P; ++p) o[p][e] = pair[p];
       }
-    } else {
-      o[0] = w[0];
     }
   }
 };
@@ -292,11 +288,11 @@ struct LrStage {
       piece[t].load(k + (size_t)nt_min(s * 64 + row, nk - 1) * ld, (slot ^ swizzle(row)) * 8, d, kRow);
     }
   }
-  __device__ __forceinline__ void store(char *dst, float scale) const {
+  __device__ __forceinline__ void store(char *dst) const {
 #pragma unroll
     for (int t = 0; t < KD; ++t) {
       u32x4 o[P];
-      piece[t].template planes<FMT, P>(scale, o);
+      piece[t].template planes<FMT, P>(o);
 #pragma unroll
       for (int p = 0; p < P; ++p) *(u32x4 *)(dst + p * kPlane + (t * 256 + threadIdx.x) * 16) = o[p];
     }
@@ -304,7 +300,7 @@ struct LrStage {
 };
 // a wave's 16 RT rows as operands, from row r0 (rows behind the last: the last)
 template <int FMT, int P, int RT, int KD, int DT, bool RAW>
-__device__ __forceinline__ void lr_rows(u32x4 (&R)[P][RT][KD], const char *rows, size_t ld, uint32_t r0, uint32_t nr, uint32_t d, float scale) {
+__device__ __forceinline__ void lr_rows(u32x4 (&R)[P][RT][KD], const char *rows, size_t ld, uint32_t r0, uint32_t nr, uint32_t d) {
   const uint32_t lane = threadIdx.x & 63, q = lane >> 4, col = lane & 15;
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
@@ -314,7 +310,7 @@ __device__ __forceinline__ void lr_rows(u32x4 (&R)[P][RT][KD], const char *rows,
       LrPiece<DT, RAW> piece;
       piece.load(row, s * 32 + q * 8, d, KD * 64);
       u32x4 o[P];
-      piece.template planes<FMT, P>(scale, o);
+      piece.template planes<FMT, P>(o);
 #pragma unroll
       for (int p = 0; p < P; ++p) R[p][j][s] = o[p];
     }
@@ -331,13 +327,12 @@ struct LossSumsArgs {
   size_t r_ld, k_ld;              // bytes
   uint32_t nr, nk, d, r_blocks, splits;
   float scale;
-  const float *top_parts;         // f32: of the two matrices' largest magnitudes
   const float *bias;
   float2 *part;  // [split][nr] (maximum, sum of exponentials against it)
 };
 template <int DT, bool RAW, int RT, int KD, bool GENERAL, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs a) {
-  constexpr int FMT = DT == AS_BF16 ? AS_BF16 : AS_F16, P = DT == AS_F32 ? 2 : 1;
+  constexpr int FMT = format_of(DT), P = planes_of(DT);
   typedef LrStage<FMT, P, KD, DT, RAW> Stage;
   constexpr uint32_t kRow = Stage::kRow, kPlane = Stage::kPlane, kExtra = GENERAL ? 256 : 0, kStage = P * kPlane + kExtra;
   __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
@@ -347,13 +342,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs
   const uint32_t r0 = (rb * 4 + wave) * (16 * RT);
   const uint32_t stages = (a.nk + 63) / 64;
   const uint32_t s_lo = (uint32_t)((uint64_t)stages * split / a.splits), s_hi = (uint32_t)((uint64_t)stages * (split + 1) / a.splits);
-  float r_scale = 1.f, k_scale = 1.f;
-  if constexpr (P == 2) {
-    r_scale = plane_scale(top_of_parts(a.top_parts));
-    k_scale = plane_scale(top_of_parts(a.top_parts + kTopParts));
-  }
-  const float nat = a.scale * (P == 2 ? 1.f / r_scale / k_scale : 1.f);
-  const float unit = GENERAL ? kLog2e : nat * kLog2e, slack = fminf(20.f / unit, 1e30f);
+  const float unit = GENERAL ? kLog2e : a.scale * kLog2e, slack = fminf(20.f / unit, 1e30f);
   Stage stage;
   float extra = 0.f;
   auto load = [&](uint32_t s) {
@@ -361,12 +350,12 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs
     if (GENERAL && a.bias && threadIdx.x < 64) extra = a.bias[nt_min(s * 64 + threadIdx.x, a.nk - 1)];
   };
   auto store = [&](int buf) {
-    stage.store(smem + buf * kStage, k_scale);
+    stage.store(smem + buf * kStage);
     if (GENERAL && threadIdx.x < 64) *(float *)(smem + buf * kStage + P * kPlane + threadIdx.x * 4) = extra;
   };
   if (s_lo < s_hi) load(s_lo);
   u32x4 R[P][RT][KD];
-  lr_rows<FMT, P, RT, KD, DT, RAW>(R, a.r, a.r_ld, r0, a.nr, a.d, r_scale);
+  lr_rows<FMT, P, RT, KD, DT, RAW>(R, a.r, a.r_ld, r0, a.nr, a.d);
   float ref[RT], base[RT], sum[RT];
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
@@ -391,22 +380,21 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs
         for (int j = 0; j < RT; ++j) z[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         const uint32_t at = h * 32 * kRow + fa + i * 4 * kRow;
 #pragma unroll
-        for (int p = 0; p < P; ++p)
+        for (int p = P - 1; p >= 0; --p)
 #pragma unroll
           for (int t = 0; t < KD; ++t) {
             const u32x4 A = lr_row(here_in, p * kPlane + (at ^ (t << 6)));
 #pragma unroll
-            for (int j = 0; j < RT; ++j) {
-              z[i][j] = nt_mfma<FMT>(A, R[0][j][t], z[i][j]);
-              if (P == 2 && p == 0) z[i][j] = nt_mfma<FMT>(A, R[P - 1][j][t], z[i][j]);
-            }
+            for (int o = P - 1 - p; o >= 0; --o)
+#pragma unroll
+              for (int j = 0; j < RT; ++j) z[i][j] = nt_mfma<FMT>(A, R[o][j][t], z[i][j]);
           }
         if constexpr (GENERAL) {
           const f32x4 kb = *(const f32x4 *)(here_in + P * kPlane + h * 128 + q * 32 + i * 16);
 #pragma unroll
           for (int j = 0; j < RT; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) z[i][j][e] = fmaf(z[i][j][e], nat, kb[e]);
+            for (int e = 0; e < 4; ++e) z[i][j][e] = fmaf(z[i][j][e], a.scale, kb[e]);
         }
         if (k0 + 32 > a.nk) {  // items behind the last
 #pragma unroll
@@ -447,7 +435,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs
   if (!here) return;
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
-    float m = GENERAL ? ref[j] : ref[j] == -INFINITY ? -INFINITY : ref[j] * nat, s = sum[j];
+    float m = GENERAL ? ref[j] : ref[j] == -INFINITY ? -INFINITY : ref[j] * a.scale, s = sum[j];
 #pragma unroll
     for (int x = 16; x < 64; x <<= 1) {
       const float mo = __shfl_xor(m, x), so = __shfl_xor(s, x);
@@ -464,7 +452,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs
 // batch (dX)
 template <int DT, bool RAW, int RT, int KD, bool ITEMS, bool BIAS, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs a) {
-  constexpr int FMT = DT == AS_BF16 ? AS_BF16 : AS_F16, P = DT == AS_F32 ? 2 : 1, OUT = DT;
+  constexpr int FMT = format_of(DT), P = planes_of(DT), OUT = DT;
   typedef LrStage<FMT, P, KD, DT, RAW> Stage;
   constexpr uint32_t kRow = Stage::kRow, kPlane = Stage::kPlane, kExtra = 1024, kStage = P * kPlane + kExtra;
   constexpr bool FAST = !BIAS && P == 1;  // 16-bit gradients: the exponent in one multiply-add (its constants are rounded: 2e-6 of the probability)
@@ -475,10 +463,8 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
   const uint32_t r0 = (rb * 4 + wave) * (16 * RT);
   const uint32_t stages = (a.nk + 63) / 64;
   const uint32_t s_lo = (uint32_t)((uint64_t)stages * split / a.splits), s_hi = (uint32_t)((uint64_t)stages * (split + 1) / a.splits);
-  const float r_scale = P == 2 ? plane_scale(*a.r_top) : 1.f, k_scale = P == 2 ? plane_scale(*a.k_top) : 1.f;
-  const float nat = P == 2 ? a.scale / r_scale / k_scale : a.scale;
-  const float c = FAST ? nat * kLog2e : nat;
-  constexpr uint32_t kList = 64;  // (items that more rows meet than that are sums of many entries, whose roundings average out)
+  const float c = FAST ? a.scale * kLog2e : a.scale;
+  constexpr uint32_t kList = 64;  // (the entries of further rows stay rounded, as all others are)
   __shared__ u32x2 list[ITEMS && P == 1 ? 4 : 1][kList];
   uint32_t list_len = 0;
   Stage stage;
@@ -491,13 +477,13 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
     else if (BIAS && wave == 0) extra = by_k[nt_min(s * 64 + lane, a.nk - 1)];
   };
   auto store = [&](int buf) {
-    stage.store(smem + buf * kStage, k_scale);
+    stage.store(smem + buf * kStage);
     if (ITEMS || (BIAS && wave == 0)) *(float *)(smem + buf * kStage + P * kPlane + threadIdx.x * 4) = extra;
   };
   if (s_lo < s_hi) load(s_lo);
   // this wave's rows
   u32x4 R[P][RT][KD];
-  lr_rows<FMT, P, RT, KD, DT, RAW>(R, a.r, a.r_ld, r0, a.nr, a.d, r_scale);
+  lr_rows<FMT, P, RT, KD, DT, RAW>(R, a.r, a.r_ld, r0, a.nr, a.d);
   float lse[RT], every[RT], entry[RT], rbias[RT], bsum[RT];
   int hit[RT];
 #pragma unroll
@@ -541,15 +527,14 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
         __builtin_amdgcn_s_setprio(1);
         const uint32_t at = h * 32 * kRow + fa + i * 4 * kRow;
 #pragma unroll
-        for (int p = 0; p < P; ++p)
+        for (int p = P - 1; p >= 0; --p)
 #pragma unroll
           for (int t = 0; t < KD; ++t) {
             const u32x4 A = lr_row(here_in, p * kPlane + (at ^ (t << 6)));
 #pragma unroll
-            for (int j = 0; j < RT; ++j) {
-              z[j] = nt_mfma<FMT>(A, R[0][j][t], z[j]);
-              if (P == 2 && p == 0) z[j] = nt_mfma<FMT>(A, R[P - 1][j][t], z[j]);
-            }
+            for (int o = P - 1 - p; o >= 0; --o)
+#pragma unroll
+              for (int j = 0; j < RT; ++j) z[j] = nt_mfma<FMT>(A, R[o][j][t], z[j]);
           }
         __builtin_amdgcn_s_setprio(0);
         // the gradients of four logits a row
@@ -612,11 +597,12 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
           if constexpr (ITEMS && BIAS) bsum[j] += (z[j][0] + z[j][1]) + (z[j][2] + z[j][3]);
-          G[0][j][2 * i] = pack2<FMT>(z[j][0], z[j][1]);
-          G[0][j][2 * i + 1] = pack2<FMT>(z[j][2], z[j][3]);
-          if constexpr (P == 2) {
-            G[1][j][2 * i] = pack2<FMT>(low_part(z[j][0]), low_part(z[j][1]));
-            G[1][j][2 * i + 1] = pack2<FMT>(low_part(z[j][2]), low_part(z[j][3]));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t pair[P];
+            pack_planes<FMT, P>(z[j][2 * h], z[j][2 * h + 1], pair);
+#pragma unroll
+            for (int p = 0; p < P; ++p) G[p][j][2 * i + h] = pair[p];
           }
         }
       }
@@ -625,20 +611,17 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
 #pragma unroll
       for (int t = 0; t < KD; ++t)
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
+        for (int p = P - 1; p >= 0; --p) {
           // columns 4 h .. 4 h + 3 of each eight: two tiles
           const u32x4 y0 = lr_column(here_in, p * kPlane + (at ^ (t << 6)), 4 * kRow), y1 = lr_column(here_in, p * kPlane + (at ^ (t << 6)) + 8, 4 * kRow);
 #pragma unroll
-          for (int j = 0; j < RT; ++j) {
-            const u32x4 g0 = u32x4{G[0][j][0], G[0][j][1], G[0][j][2], G[0][j][3]};
-            out[2 * t][j] = nt_mfma<FMT>(y0, g0, out[2 * t][j]);
-            out[2 * t + 1][j] = nt_mfma<FMT>(y1, g0, out[2 * t + 1][j]);
-            if (P == 2 && p == 0) {
-              const u32x4 g1 = u32x4{G[P - 1][j][0], G[P - 1][j][1], G[P - 1][j][2], G[P - 1][j][3]};
-              out[2 * t][j] = nt_mfma<FMT>(y0, g1, out[2 * t][j]);
-              out[2 * t + 1][j] = nt_mfma<FMT>(y1, g1, out[2 * t + 1][j]);
+          for (int o = P - 1 - p; o >= 0; --o)
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+              const u32x4 g = u32x4{G[o][j][0], G[o][j][1], G[o][j][2], G[o][j][3]};
+              out[2 * t][j] = nt_mfma<FMT>(y0, g, out[2 * t][j]);
+              out[2 * t + 1][j] = nt_mfma<FMT>(y1, g, out[2 * t + 1][j]);
             }
-          }
         }
     }
     __builtin_amdgcn_s_setprio(0);
@@ -675,7 +658,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
       }
     }
   }
-  const float f = ITEMS && !a.sums ? a.scale * a.coef[1] / k_scale : 1.f;
+  const float f = ITEMS && !a.sums ? a.scale * a.coef[1] : 1.f;
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
     const uint32_t row = r0 + j * 16 + col;

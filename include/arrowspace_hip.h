@@ -510,7 +510,7 @@ int as_range_search(as_ctx *ctx, const as_index *index, double lambda_q, double 
  * bias[n_items] f32 or NULL; -inf takes an item out.  losses_t is 0 where targets_t == ignore_index (lse_t is still written) and
  * where the bias leaves no item (lse_t = -inf).  A target outside the table that is not ignore_index: AS_ERR_ARG when the targets
  * are host memory, a loss of NaN when they are device memory; its row has no gradient through the loss.  n = 0 is allowed.
- * Products are summed in 32 bits (f32 inputs: as a sum of two f16 each, 22 bits, products of 2^-23). */
+ * Products are summed in 32 bits (f32 inputs: as a sum of three bf16 each, 24 bits; of values below 2^-108 what steps of 2^-133 leave). */
 uint64_t as_cross_entropy_workspace(uint64_t n, uint64_t n_items, uint64_t dim, int dtype, int backward);
 int as_cross_entropy(as_ctx *ctx, const void *x, uint64_t n, uint64_t x_stride, const void *table, uint64_t n_items,
                      uint64_t table_stride, uint64_t dim, int dtype, const float *bias, const int64_t *targets, int64_t ignore_index,
@@ -519,7 +519,9 @@ int as_cross_entropy(as_ctx *ctx, const void *x, uint64_t n, uint64_t x_stride, 
  *   g_tv = (grad_losses_t + grad_lse_t) exp(l_tv - lse_t) - grad_losses_t [v = targets_t]   (grad_losses_t as 0 on ignored rows)
  *   grad_x = scale g table      grad_table = scale g^T x      grad_bias_v = sum_t g_tv
  * grad_x and grad_table have the inputs' type, grad_bias is f32; each may be NULL (not computed).  The logits are made again in
- * pieces of the table; g is rounded to 16 bits between the products (f32 inputs: to 22), sums are 32 bits wide. */
+ * pieces of the table.  Between the products g is rounded to the inputs' type, half a step an entry (f32 inputs: it keeps 24 bits); what
+ * that leaves of the entries at the targets is added in 32 bits (to grad_table for 64 of the rows that meet each 64 items).  f16: g is held
+ * in units of 2^-14 of the largest coefficient, entries below 2^-28 of that lose bits.  Sums are 32 bits wide. */
 int as_cross_entropy_backward(as_ctx *ctx, const void *x, uint64_t n, uint64_t x_stride, const void *table, uint64_t n_items,
                               uint64_t table_stride, uint64_t dim, int dtype, const float *bias, const int64_t *targets,
                               int64_t ignore_index, double scale, const float *lse, const float *grad_losses, const float *grad_lse,

@@ -8,7 +8,7 @@ from arrowspace_amd import _lib
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from .test_gpu_table import _check4, _inputs, _plain4  # noqa: E402
+from .test_gpu_table import E, _check, _check4, _close, _inputs, _plain4, _reference  # noqa: E402
 
 
 @pytest.mark.parametrize("zeros", [False, True])
@@ -137,3 +137,76 @@ def test_a_table_freed_while_a_stream_left_beside_a_capture_reads_it():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, keep.scores(x)) and torch.equal(out, fresh[0].scores(x)) and torch.equal(out, fresh[1].scores(x))
+
+
+# rows, items, columns by the form that f32 takes: short rows as they lie and from images, tiles through G, a few rows
+F32_FORMS = [(70, 3000, 64), (300, 3000, 128), (300, 2000, 200), (12, 900, 200), (24, 900, 40)]
+
+
+@pytest.mark.parametrize("n, v, d", F32_FORMS)
+@pytest.mark.parametrize("scale", [1.0, 1e30])
+def test_f32_tiny_values(n, v, d, scale):
+    """Matrices whose products are far below the smallest normal number: all items the same, unless the scale brings them back."""
+    x, w, y, _ = _inputs(n, v, d, torch.float32, seed=41)
+    _check(x * 1e-20, w * 1e-20, y, None, scale=scale)
+
+
+@pytest.mark.parametrize("n, v, d", F32_FORMS)
+@pytest.mark.parametrize("power", [120, -120])
+def test_f32_large_and_tiny_values_together(n, v, d, power):
+    """Values at both ends of the range.  Their planes are bf16, whose smallest step is 2^-133, so values near 2^-120 are held to 2^-134 and not
+    to 24 bits: a logit is off by another scale * 2^-134 * (the sums of |x| and |w|), a probability by e to twice that, a product with such
+    values by 2^-134 of the other factor's sum."""
+    x, w, y, b = _inputs(n, v, d, torch.float32, seed=42, bias=power < 0)
+    x, w = x * 2.0 ** power, w * 2.0 ** -power
+    gl = torch.full((n,), 1 / n, device="cuda")
+    losses, lse = A.cross_entropy(x, w, y, bias=b, scale=4.0)
+    grads = A.cross_entropy_backward(x, w, y, lse, gl, bias=b, scale=4.0)
+    want = _reference(x, w, y, b, 4.0, gl)
+    X, W, step = x.double().abs(), w.double().abs(), 2.0 ** -134
+    off = 4.0 * step * (X.sum(1).max() + W.sum(1).max())
+    z = 4.0 * (x.double() @ w.double().t().contiguous()) + (0 if b is None else b.double())
+    p = torch.exp(z - torch.logsumexp(z, 1)[:, None]) / n
+    dg = p * torch.expm1(2 * off)
+    p[torch.arange(n, device="cuda"), y] += 1 / n
+    _close(lse, want["lse"][0], want["lse"][1] + off, "lse")
+    _close(losses, want["losses"][0], want["losses"][1] + 2 * off, "losses")
+    _close(grads[0], want["grad_x"][0], want["grad_x"][1] + 4.0 * (dg @ W + step * p.sum(1, keepdim=True)), "grad_x")
+    _close(grads[1], want["grad_table"][0], want["grad_table"][1] + 4.0 * (dg.t().contiguous() @ X + step * p.sum(0)[:, None]), "grad_table")
+
+
+@pytest.mark.parametrize("n, v, d", F32_FORMS)
+def test_f32_rows_far_apart(n, v, d):
+    """One row 2^24 times as large as the others, and one item: the others keep the bits that they have alone."""
+    x, w, y, _ = _inputs(n, v, d, torch.float32, seed=43)
+    x, w = x.clone(), w.clone()
+    x[n // 2] *= 2.0 ** 24
+    w[v // 2] = 0
+    w[v // 2, 0] = 2.0 ** 24
+    x[torch.arange(n, device="cuda") != n // 2, 0] = -1.0    # (its logits: -2^26, its probability 0)
+    x[n // 2, 0] = 0
+    y = torch.where(y == v // 2, y - 1, y)
+    losses, lse = A.cross_entropy(x, w, y)
+    want = _reference(x, w, y, None, 1.0)
+    _close(lse, *want["lse"], "lse")
+    _close(losses, *want["losses"], "losses")
+
+
+@pytest.mark.parametrize("n, v, d", F32_FORMS)
+def test_f32_gradients_of_improbable_items(n, v, d):
+    """Items of probabilities down to 1e-12: their gradients keep f32's bits."""
+    x, w, y, b = _inputs(n, v, d, torch.float32, seed=45, bias=True)
+    b[100:500] = -torch.linspace(0, 27, 400, device="cuda")
+    y = torch.where((y >= 100) & (y < 500), y % 100, y)
+    gl = torch.full((n,), 1 / n, device="cuda")
+    _, lse = A.cross_entropy(x, w, y, bias=b)
+    _, gw, gb = A.cross_entropy_backward(x, w, y, lse, gl, bias=b)
+    X, W = x.double(), w.double()
+    z = X @ W.t().contiguous() + b.double()
+    p = torch.exp(z - torch.logsumexp(z, 1)[:, None])[:, 100:500] / n
+    size = X.abs() @ W.abs().t().contiguous() + b.double().abs()
+    # relative: exp of a logit and of a normaliser that are each (d + 8) e of their terms off, the exponent's own rounding, e a sum of n
+    off = 2 * (d + 8) * E * size.max() + 8 * E * (z.abs().max() + 30) + (n + 64) * E + 2.0 ** -21
+    want, terms = p.t().contiguous() @ X, p.t().contiguous() @ X.abs()
+    _close(gw[100:500], want, off * terms, "grad_table")
+    _close(gb[100:500], p.sum(0), off * p.sum(0), "grad_bias")
