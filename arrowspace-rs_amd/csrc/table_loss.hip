@@ -67,9 +67,9 @@ __global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2
     return NtOperand{a.table + (size_t)r0 * a.table_ld, a.table_ld, nt_min(TILE::BM, a.v - r0) - 1, 0, a.table_plane};
   };
   const uint32_t all = a.all;
-  float top[TILE::TN], sum[TILE::TN];
+  float top[TILE::TN], sum[TILE::TN], shift[TILE::TN];
 #pragma unroll
-  for (int j = 0; j < TILE::TN; ++j) top[j] = -INFINITY, sum[j] = 0.f;
+  for (int j = 0; j < TILE::TN; ++j) top[j] = -INFINITY, sum[j] = shift[j] = 0.f;
   f32x4 acc[TILE::TM][TILE::TN];
   NtOperand A = side(vt);
   T.fetch(0, A, B, 0, a.steps);
@@ -119,9 +119,10 @@ __global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2
 #pragma unroll
         for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[i][j][e]);
       // (with a bias the difference first: a bias of the type's lowest value times log2 e would be infinite)
-      const float base = m == -INFINITY ? 0.f : m, shift = -base * unit;
-      auto power = [&](float x) { return __builtin_amdgcn_exp2f(GENERAL ? (x - base) * unit : fmaf(x, unit, shift)); };
-      float s0 = sum[j] * power(top[j]), s1 = 0.f;
+      const float base = m == -INFINITY ? 0.f : m, to = GENERAL ? 0.f : base_of(base, unit);
+      auto power = [&](float x) { return __builtin_amdgcn_exp2f(GENERAL ? (x - base) * unit : fmaf(x, unit, to)); };
+      float s0 = sum[j] * (GENERAL ? power(top[j]) : rebased(top[j], shift[j], to)), s1 = 0.f;
+      shift[j] = to;
 #pragma unroll
       for (int i = 0; i < TILE::TM; ++i) {
         s0 += power(acc[i][j][0]);
@@ -136,7 +137,11 @@ __global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2
   // the four lane groups of a row
 #pragma unroll
   for (int j = 0; j < TILE::TN; ++j) {
-    float m = GENERAL ? top[j] : top[j] == -INFINITY ? -INFINITY : top[j] * a.scale, s = sum[j];
+    float m = top[j], s = sum[j];
+    if (!GENERAL && m != -INFINITY) {
+      m *= a.scale;
+      s = sum_against(top[j], unit, shift[j], a.scale, m, s);
+    }
 #pragma unroll
     for (int x = 16; x < 64; x <<= 1) {
       const float mo = __shfl_xor(m, x), so = __shfl_xor(s, x);

@@ -170,9 +170,9 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_sums_kernel(LossFewArgs a
       const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
       if (__any(top > ref[t] + slack)) {
         if (top > ref[t]) {
-          sum[t] *= __builtin_amdgcn_exp2f((ref[t] - top) * unit);
-          ref[t] = top;
-          base[t] = GENERAL ? top : -top * unit;
+          const float to = GENERAL ? top : base_of(top, unit);
+          sum[t] *= GENERAL ? __builtin_amdgcn_exp2f((ref[t] - top) * unit) : rebased(ref[t], base[t], to);
+          ref[t] = top, base[t] = to;
         }
       }
 #pragma unroll
@@ -186,7 +186,11 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_sums_kernel(LossFewArgs a
   if (WK == 4 && wave >= RT) return;
 #pragma unroll
   for (int t = 0; t < TS; ++t) {
-    float m = GENERAL ? ref[t] : ref[t] == -INFINITY ? -INFINITY : ref[t] * a.scale;
+    float m = ref[t];
+    if (!GENERAL && m != -INFINITY) {
+      m *= a.scale;
+      sum[t] = sum_against(ref[t], unit, base[t], a.scale, m, sum[t]);
+    }
 #pragma unroll
     for (int x = 16; x < 64; x <<= 1) {
       const float mo = __shfl_xor(m, x), so = __shfl_xor(sum[t], x);

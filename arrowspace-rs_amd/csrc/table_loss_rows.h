@@ -330,6 +330,20 @@ struct LossSumsArgs {
   const float *bias;
   float2 *part;  // [split][nr] (maximum, sum of exponentials against it)
 };
+// Without a bias the exponent of a product x is fma(x, unit, base) with base = -(the largest) unit, rounded down: no term overflows, all of
+// them carry 2^off, where off = fma(largest, unit, base) <= 0 is that rounding.  Logits behind 2^29 lie further apart than exp2 has range for
+// there, so that the largest is all of the sum.
+__device__ __forceinline__ float base_of(float largest, float unit) {
+  const float base = -largest * unit;
+  return fmaf(largest, unit, base) > 0.f ? base - fabsf(base) * 0x1p-23f : base;
+}
+// ... the sum against m = largest scale (rounded as well: what that leaves belongs to the sum, while it has range for it)
+__device__ __forceinline__ float sum_against(float largest, float unit, float base, float scale, float m, float sum) {
+  const float off = fmaf(largest, unit, base), rest = fmaf(largest, scale, -m) * kLog2e;
+  return off < -64.f ? 1.f : sum * __builtin_amdgcn_exp2f((fabsf(rest) > 32.f ? 0.f : rest) - off);
+}
+// ... and what it is multiplied by when the base moves (nothing yet: 0)
+__device__ __forceinline__ float rebased(float before, float base, float now) { return before == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(now - base); }
 template <int DT, bool RAW, int RT, int KD, bool GENERAL, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs a) {
   constexpr int FMT = format_of(DT), P = planes_of(DT);
@@ -415,10 +429,9 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs
 #pragma unroll
         for (int j = 0; j < RT; ++j)
           if (top[j] > ref[j]) {
-            const float was = ref[j];
-            ref[j] = top[j];
-            sum[j] *= __builtin_amdgcn_exp2f((was - top[j]) * unit);  // (nothing yet: -inf, 0)
-            base[j] = GENERAL ? top[j] : -top[j] * unit;
+            const float to = GENERAL ? top[j] : base_of(top[j], unit);
+            sum[j] *= GENERAL ? __builtin_amdgcn_exp2f((ref[j] - top[j]) * unit) : rebased(ref[j], base[j], to);  // (nothing yet: 0)
+            ref[j] = top[j], base[j] = to;
           }
       }
 #pragma unroll
@@ -435,7 +448,11 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_sums_kernel(LossSumsArgs
   if (!here) return;
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
-    float m = GENERAL ? ref[j] : ref[j] == -INFINITY ? -INFINITY : ref[j] * a.scale, s = sum[j];
+    float m = ref[j], s = sum[j];
+    if (!GENERAL && m != -INFINITY) {
+      m *= a.scale;
+      s = sum_against(ref[j], unit, base[j], a.scale, m, s);
+    }
 #pragma unroll
     for (int x = 16; x < 64; x <<= 1) {
       const float mo = __shfl_xor(m, x), so = __shfl_xor(s, x);

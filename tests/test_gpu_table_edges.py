@@ -8,7 +8,7 @@ from arrowspace_amd import _lib
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from .test_gpu_table import E, _check, _check4, _close, _inputs, _plain4, _reference  # noqa: E402
+from .test_gpu_table import E, TYPES, _check, _check4, _close, _inputs, _plain4, _reference  # noqa: E402
 
 
 @pytest.mark.parametrize("zeros", [False, True])
@@ -190,6 +190,24 @@ def test_f32_rows_far_apart(n, v, d):
     want = _reference(x, w, y, None, 1.0)
     _close(lse, *want["lse"], "lse")
     _close(losses, *want["losses"], "losses")
+
+
+# ... and those that 16-bit types take besides: rows of 256, few rows
+FORMS = F32_FORMS + [(200, 2000, 256), (24, 900, 256)]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("n, v, d", FORMS)
+@pytest.mark.parametrize("power, scale", [(13, 1.0), (24, 1.0), (24, 30.0), (40, 1.0), (60, 30.0)])
+def test_logits_beyond_the_exponents_range(n, v, d, dt, power, scale):
+    """Logits of 2^13 to 2^60: the normaliser is the largest logit to f32's bits, whatever its rounding is as an exponent."""
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=48, bias=True)
+    x = x * 2.0 ** power
+    for bias in (None, b):
+        losses, lse = A.cross_entropy(x, w, y, bias=bias, scale=scale)
+        want = _reference(x, w, y, bias, scale)
+        _close(lse, *want["lse"], "lse")
+        _close(losses, *want["losses"], "losses")
 
 
 @pytest.mark.parametrize("n, v, d", F32_FORMS)
