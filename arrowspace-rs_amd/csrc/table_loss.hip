@@ -322,7 +322,7 @@ __global__ __launch_bounds__(TILE_::NT) void loss_grad_kernel(GradArgs g) {
 #pragma unroll
         for (int j = 0; j < TILE::TN; ++j) {
           const float z = BIAS ? fmaf(acc[i][j][e], a.scale, b) - lse[j] : fmaf(acc[i][j][e], a.scale, -lse[j]);
-          acc[i][j][e] = every[j] * __builtin_amdgcn_exp2f(z * kLog2e);
+          acc[i][j][e] = every[j] * probability(z * kLog2e);
         }
       }
     if (last + 1 < TILE::BM) {

@@ -262,7 +262,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_few_grad_kernel(LossFewArgs a
     for (int e = 0; e < 4; ++e) {
       const uint32_t item = s * 16 + q * 4 + e;
       const float l = BIAS ? fmaf(g[e], a.scale, bias[e]) - lse : fmaf(g[e], a.scale, -lse);
-      g[e] = item < a.v ? every * __builtin_amdgcn_exp2f(l * kLog2e) : 0.f;
+      g[e] = item < a.v ? every * probability(l * kLog2e) : 0.f;
       if (target == item) g[e] = entry;
     }
     if constexpr (BIAS) {

@@ -99,6 +99,10 @@ __device__ __forceinline__ void store8(void *out, size_t at, f32x4 u, f32x4 v) {
   }
 }
 
+// e^(logit - lse) from the exponent to the base 2: at most 1 -- of logits in the millions the lse and the logits of another kernel's order
+// of sums are whole units apart.  (The bound is a modifier of the instruction.)
+__device__ __forceinline__ float probability(float x) { return __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(x), 0.f, 1.f); }
+
 struct LossRowsArgs {
   const char *r, *k;              // the two sides' rows as they are
   size_t r_ld, k_ld;              // bytes
@@ -198,14 +202,16 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossRowInputs a) {
       one = a.gl[t] * f;
     }
     every = one + (a.ge ? a.ge[t] * f : 0.f);
+    if (every == 0.f) s = INFINITY;                          // (nothing but the entry: probability 0, whatever a padded row holds)
+    else if (!(s < INFINITY)) every = __builtin_nanf("");    // (no normaliser, no gradient: probability() gives no NaN)
     if (at >= 0) {
       double dot = 0.0;
 #pragma unroll 4
       for (uint32_t k = lane; k < a.d; k += 64)
         dot += (double)load_as_f32<DT>(a.x, (size_t)t * a.x_stride + k) * (double)load_as_f32<DT>(a.table, (size_t)y * a.table_stride + k);
       for (int k = 1; k < 64; k <<= 1) dot += __shfl_xor(dot, k);
-      const double z = (double)a.scale * dot + (a.bias ? (double)a.bias[y] : 0.0) - (double)s;
-      entry = (float)((double)every * exp(z) - (double)one);
+      const double z = (double)a.scale * dot + (a.bias ? (double)a.bias[y] : 0.0) - (double)a.lse[t];
+      entry = (float)((double)every * (z > 0.0 ? 1.0 : exp(z)) - (double)one);
     }
   }
   if (lane == 0) {
@@ -573,7 +579,7 @@ __global__ __launch_bounds__(256, WAVES) void loss_rows_grad_kernel(LossRowsArgs
             if constexpr (FAST) x = fmaf(z[j][e], c, ITEMS ? -l * kLog2e : -l);
             else if constexpr (BIAS) x = (fmaf(z[j][e], c, ITEMS ? rbias[j] : kb[e]) - l) * kLog2e;
             else x = fmaf(z[j][e], c, -l) * kLog2e;
-            g[e] = w * __builtin_amdgcn_exp2f(x);
+            g[e] = w * probability(x);
           }
           z[j] = g;
         }

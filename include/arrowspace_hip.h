@@ -518,7 +518,9 @@ int as_cross_entropy(as_ctx *ctx, const void *x, uint64_t n, uint64_t x_stride, 
 /* Its gradient, from grad_losses[n] = dL/dlosses and grad_lse[n] = dL/dlse (or NULL: 0), with lse as the forward call wrote it:
  *   g_tv = (grad_losses_t + grad_lse_t) exp(l_tv - lse_t) - grad_losses_t [v = targets_t]   (grad_losses_t as 0 on ignored rows)
  *   grad_x = scale g table      grad_table = scale g^T x      grad_bias_v = sum_t g_tv
- * grad_x and grad_table have the inputs' type, grad_bias is f32; each may be NULL (not computed).  The logits are made again in
+ * grad_x and grad_table have the inputs' type, grad_bias is f32; each may be NULL (not computed).  exp(...) is held to at most 1.
+ * A row whose coefficients are 0 (an ignored row of a padded batch) has no part in grad_x and grad_bias whatever it holds, and none in
+ * grad_table if it is finite; a row without a finite lse gives NaN.  The logits are made again in
  * pieces of the table.  Between the products g is rounded to the inputs' type, half a step an entry (f32 inputs: it keeps 24 bits); what
  * that leaves of the entries at the targets is added in 32 bits (to grad_table for 64 of the rows that meet each 64 items).  f16: g is held
  * in units of 2^-14 of the largest coefficient, entries below 2^-28 of that lose bits.  Sums are 32 bits wide. */

@@ -186,14 +186,37 @@ def test_f32_rows_far_apart(n, v, d):
     x[torch.arange(n, device="cuda") != n // 2, 0] = -1.0    # (its logits: -2^26, its probability 0)
     x[n // 2, 0] = 0
     y = torch.where(y == v // 2, y - 1, y)
-    losses, lse = A.cross_entropy(x, w, y)
-    want = _reference(x, w, y, None, 1.0)
-    _close(lse, *want["lse"], "lse")
-    _close(losses, *want["losses"], "losses")
+    _check(x, w, y, None)
 
 
 # ... and those that 16-bit types take besides: rows of 256, few rows
 FORMS = F32_FORMS + [(200, 2000, 256), (24, 900, 256)]
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, v, d", FORMS)
+def test_garbage_in_ignored_rows_and_masked_items(n, v, d, dt):
+    """Finite garbage where the batch is padded and where the bias takes an item out: everyone else gets what zeros there give."""
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=44, bias=True)
+    y = torch.where(y == 7, 8, y)
+    y[3] = -100
+    b[7] = -float("inf")
+    gl = torch.full((n,), 1 / n, device="cuda")
+    results = []
+    for garbage in (0.0, 3e4 if dt == "f16" else 1e18):
+        x, w = x.clone(), w.clone()
+        x[3], w[7] = garbage, garbage
+        losses, lse = A.cross_entropy(x, w, y, bias=b)
+        results.append((losses, lse) + A.cross_entropy_backward(x, w, y, lse, gl, bias=b))
+    want = _reference(torch.cat((x[:3], 0 * x[3:4], x[4:])), torch.cat((w[:7], 0 * w[7:8], w[8:])), y, b, 1.0, gl)
+    rows = torch.arange(n, device="cuda") != 3
+    for r in results:
+        for got, what in zip(r, ("losses", "lse", "grad_x", "grad_table", "grad_bias")):
+            exact, bound = want[what]
+            if what in ("losses", "lse", "grad_x"):
+                got, exact, bound = got[rows], exact[rows], bound[rows]
+            _close(got, exact, bound, what)
+        assert not r[2][3].any() and not r[3][7].any() and r[4][7] == 0
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
@@ -208,6 +231,38 @@ def test_logits_beyond_the_exponents_range(n, v, d, dt, power, scale):
         want = _reference(x, w, y, bias, scale)
         _close(lse, *want["lse"], "lse")
         _close(losses, *want["losses"], "losses")
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, v, d", FORMS)
+def test_logits_of_millions(n, v, d, dt):
+    """Probabilities are at most 1 where a logit's rounding is whole units: the gradient of a row with such logits is bounded by its coefficient."""
+    x, w, y, _ = _inputs(n, v, d, TYPES[dt], seed=46)
+    x = x.clone()
+    x[: n // 2] *= 2.0 ** 12 if dt == "f16" else 2.0 ** 24
+    gl = torch.full((n,), 1 / n, device="cuda")
+    losses, lse = A.cross_entropy(x, w, y, scale=30.0)
+    gx, gw, _ = A.cross_entropy_backward(x, w, y, lse, gl, scale=30.0)
+    assert torch.isfinite(losses).all() and torch.isfinite(lse).all()
+    # every |g| adds up to at most (1 + the number of items at the maximum, few) times the coefficient a row: 8 of them
+    assert (gx.double().abs() <= 8 * 30 / n * w.double().abs().max()).all()
+    assert (gw.double().abs() <= 8 * 30 / n * x.double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("n, v, d", FORMS)
+def test_a_row_of_nan_has_no_gradient_and_an_ignored_one_no_part_in_the_others(n, v, d):
+    x, w, y, b = _inputs(n, v, d, torch.bfloat16, seed=47, bias=True)
+    x = x.clone()
+    x[2] = float("nan")
+    gl = torch.full((n,), 1 / n, device="cuda")
+    _, lse = A.cross_entropy(x, w, y, bias=b)
+    gx, gw, gb = A.cross_entropy_backward(x, w, y, lse, gl, bias=b)
+    assert torch.isnan(gx[2]).all() and torch.isnan(gb).all()
+    rows = torch.arange(n, device="cuda") != 2
+    assert torch.isfinite(gx[rows]).all()
+    y[2] = -100
+    gx, gw, gb = A.cross_entropy_backward(x, w, y, lse, gl, bias=b)
+    assert not gx[2].any() and torch.isfinite(gx).all() and torch.isfinite(gb).all()
 
 
 @pytest.mark.parametrize("n, v, d", F32_FORMS)
