@@ -152,7 +152,7 @@ __device__ __forceinline__ void unit_of_rows(const float *gl, const float *ge, c
   __syncthreads();
   for (int w = 0; w < THREADS / 64; ++w) one = fmaxf(one, s[0][w]), both = fmaxf(both, s[1][w]);
   float m = both <= 2.f * one ? one : both;
-  if (!(m >= 1e-36f && m <= 1e36f)) m = 1.f;   // (nothing to scale, or nothing that a factor brings into range)
+  m = m > 0.f ? fmaxf(m, 0x1p-100f) : 1.f;  // (its inverse is finite behind the power too; f16 has its bits left for 2^-100 and less)
   *unit = m * __uint_as_float((unsigned int)(127 - power) << 23);
   *factor = 1.f / *unit;
 }

@@ -283,3 +283,20 @@ def test_f32_gradients_of_improbable_items(n, v, d):
     want, terms = p.t().contiguous() @ X, p.t().contiguous() @ X.abs()
     _close(gw[100:500], want, off * terms, "grad_table")
     _close(gb[100:500], p.sum(0), off * p.sum(0), "grad_bias")
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, v, d", FORMS)
+@pytest.mark.parametrize("size, scale", [(1e-37, 1.0), (1e-35, 1.0), (5e-35, 1.0), (2e36, 1e-36), (1e38, 1e-38)])
+def test_gradients_of_tiny_and_huge_coefficients(n, v, d, dt, size, scale):
+    """Whatever the losses are weighted with, no unit of the logits' gradient under- or overflows."""
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=49, bias=True)
+    gl = torch.linspace(0.5, 1.5, n, device="cuda") * size
+    _, lse = A.cross_entropy(x, w, y, bias=b, scale=scale)
+    grads = A.cross_entropy_backward(x, w, y, lse, gl, bias=b, scale=scale)
+    want = _reference(x, w, y, b, scale, gl)
+    for got, what in zip(grads, ("grad_x", "grad_table", "grad_bias")):
+        exact, bound = want[what]
+        # (three rows of 1.2e38 at one item are 3.6e38, more than the type's largest value: infinite)
+        exact = torch.where(exact.abs() > torch.finfo(got.dtype).max, exact.sign() * float("inf"), exact)
+        _close(got, exact, bound, what)
