@@ -171,12 +171,8 @@ struct ScoresArgs {
   float *part;
 };
 
-// the power of two that brings a largest magnitude to 2^14 .. 2^15 (1 for zero)
-__device__ __forceinline__ float row_scale(unsigned int top) {
-  const int e = (int)(top >> 23);
-  if (e == 0 || e >= 255) return 1.f;
-  return __uint_as_float((unsigned int)(127 + min(max(14 - (e - 127), -100), 100)) << 23);
-}
+// the power of two that brings a largest finite magnitude to 2^14 .. 2^15 (those below 2^-112: as far as 2^126 goes, 2^0 and more)
+__device__ __forceinline__ float row_scale(unsigned int top) { return __uint_as_float((unsigned int)(127 + min(141 - (int)(top >> 23), 126)) << 23); }
 __device__ __forceinline__ uint32_t f16_pair(float a, float b) {
   typedef _Float16 half2v __attribute__((ext_vector_type(2)));
   const half2v p = {(_Float16)a, (_Float16)b};

@@ -547,7 +547,9 @@ uint64_t as_table4_dim(const as_table4 *t);
 uint64_t as_table4_group(const as_table4 *t);
 int as_table4_scale_dtype(const as_table4 *t);
 /* out_mv = sum_k x_mk W_vk for m rows (made for a few: 64 are one pass over the codes); out has the rows' type (AS_F32, AS_BF16 or
- * AS_F16), rounded once.  The handle is only read: any number of contexts may use it at once. */
+ * AS_F16), rounded once.  Products are summed in 32 bits; a row goes in as f16 (f32: a sum of two) under a power of two of its own: f32
+ * values keep 22 bits down to 2^-17 of their row's largest, bf16 values all bits down to 2^-28 of it, smaller ones what 2^-39 of it leaves.
+ * The handle is only read: any number of contexts may use it at once. */
 uint64_t as_table4_workspace(const as_table4 *t, uint64_t m, int dtype);
 int as_table4_scores(as_ctx *ctx, const as_table4 *t, const void *x, uint64_t m, uint64_t x_stride, int dtype, void *out,
                      uint64_t out_stride, void *workspace, uint64_t workspace_bytes);

@@ -300,3 +300,25 @@ def test_gradients_of_tiny_and_huge_coefficients(n, v, d, dt, size, scale):
         # (three rows of 1.2e38 at one item are 3.6e38, more than the type's largest value: infinite)
         exact = torch.where(exact.abs() > torch.finfo(got.dtype).max, exact.sign() * float("inf"), exact)
         _close(got, exact, bound, what)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("m, v, d", [(3, 300, 200), (16, 300, 200), (16, 100, 6000), (40, 300, 200), (40, 100, 6000)])
+@pytest.mark.parametrize("power", [110, 116, 122, -90, -105, -118])
+def test_scores4_of_rows_at_both_ends_of_the_range(m, v, d, dt, power):
+    """A row's values up to 2^124 and down to 2^-120, every other row of ordinary size.  (Scales of 1 / 64: the scores stay below 2^128.)"""
+    codes, s, z, _ = _plain4(v, d, 32, "f32", True, m + d)
+    s = s / 64
+    t = A.Table4.from_codes(codes, s, z, dim=d, group=32)
+    q = torch.stack((codes & 15, codes >> 4), 2).flatten(1)[:, :d].double()
+    w = (q - z.double().repeat_interleave(32, 1)[:, :d]) * s.double().repeat_interleave(32, 1)[:, :d]
+    g = torch.Generator(device="cuda").manual_seed(50)
+    x = torch.rand(m, d, device="cuda", generator=g) * 2 - 1
+    x[::2] *= 2.0 ** power
+    x = x.to(TYPES[dt])
+    got, X = t.scores(x), x.double()
+    want, size = X @ w.t().contiguous(), X.abs() @ w.abs().t().contiguous()
+    # the bound of _check4 without its smallest normal number for the small rows: these stay normal here
+    bound = ((d + 16) * E + 2.0 ** -22) * size + torch.finfo(x.dtype).eps / 2 * want.abs() + 2.0 ** -134
+    exact = torch.where(want.abs() > torch.finfo(x.dtype).max, want.sign() * float("inf"), want)
+    _close(got, exact, bound, "scores")
