@@ -5,7 +5,8 @@ Matrices are torch tensors (on a GPU: used in place, on torch's current stream o
 (staged; results come back as numpy arrays, complete).  Results lie where the first argument does; the others may be host memory or on
 one GPU, and as soon as one of them is, the call runs on torch's current stream there.  The host waits for the GPU only where host memory
 is copied, and where a thread goes on to another stream than its last call's: for that call's stream.  Rows may be rows of a wider
-tensor; the values of a row must be adjacent.
+tensor; the values of a row must be adjacent.  Tensors that require gradients get them: cross_entropy is differentiable (once), and a
+backward pass through the scores of a Table4, which have no gradient, raises.
 """
 import ctypes as C
 import threading
@@ -22,6 +23,7 @@ _local = threading.local()
 _torch = None          # the module, once a tensor has been seen
 _raw_stream = None     # device index -> address of torch's current stream there
 _kinds = {}            # torch dtype -> name
+_Loss = _Scores = None  # torch.autograd.Functions
 
 
 def _need_torch():
@@ -31,6 +33,63 @@ def _need_torch():
     for name in ("float64", "float32", "bfloat16", "float16", "int64", "uint8"):
         _kinds[getattr(torch, name)] = name
     _torch = torch
+    _differentiable()
+
+
+def _differentiable():
+    """The operators as torch.autograd.Functions (made once torch is there)."""
+    global _Loss, _Scores
+    once = _torch.autograd.function.once_differentiable
+
+    class Loss(_torch.autograd.Function):
+        @staticmethod
+        def forward(node, x, table, bias, targets, scale, ignore_index, ctx):
+            losses, lse = _cross_entropy(x, table, targets, bias, scale, ignore_index, ctx)
+            kept = [x, table, bias, targets, lse]
+            # (host arrays beside tensors: on the node itself)
+            node.save_for_backward(*[a if a is None or isinstance(a, _torch.Tensor) else None for a in kept])
+            node.host = [None if a is None or isinstance(a, _torch.Tensor) else a for a in kept]
+            node.scale, node.ignore_index = scale, ignore_index
+            node.set_materialize_grads(False)
+            return losses, lse
+
+        @staticmethod
+        @once
+        def backward(node, grad_losses, grad_lse):
+            none = (None,) * 7
+            if grad_losses is None and grad_lse is None:
+                return none
+            x, table, bias, targets, lse = [h if t is None else t for t, h in zip(node.saved_tensors, node.host)]
+            if grad_losses is None:
+                grad_losses = _torch.zeros_like(lse)
+            need = node.needs_input_grad
+            # (on the thread that runs this, with a context of its own: the forward call's is its caller's)
+            grads = cross_entropy_backward(x, table, targets, lse, grad_losses, bias=bias, scale=node.scale, ignore_index=node.ignore_index,
+                                           grad_lse=grad_lse, need_x=need[0], need_table=need[1], need_bias=need[2])
+            return tuple(g if g is None else g.to(a.device) for g, a in zip(grads, (x, table, bias))) + none[3:]
+
+    class Scores(_torch.autograd.Function):
+        @staticmethod
+        def forward(node, x, table, ctx):
+            return table._scores(x, ctx)
+
+        @staticmethod
+        def backward(node, grad):
+            raise ArrowSpaceError(_lib.AS_ERR_UNSUPPORTED, "the scores of a table in 4 bits have no gradient")
+
+    _Loss, _Scores = Loss, Scores
+
+
+def _recorded(first, *others):
+    """Whether torch records a call with these arguments for a backward pass."""
+    if not is_tensor(first):
+        return False
+    for a in (first,) + others:
+        if getattr(a, "requires_grad", False):
+            if _torch is None:
+                _need_torch()
+            return _torch.is_grad_enabled()
+    return False
 
 
 def _thread_context(device):
@@ -171,7 +230,16 @@ def _loss_args(x, table, bias, targets, ctx, *others):
 def cross_entropy(x, table, targets, bias=None, scale=1.0, ignore_index=-100, ctx=None):
     """Softmax cross entropy of every row of x (n x d) against all rows of the table (v x d), the n x v logits never kept:
     (losses, lse), both float32 of n.  logits = scale * x @ table.T + bias; losses are 0 where targets == ignore_index and where the
-    bias (-inf) leaves no item.  The mean over the counted rows is losses.sum() / count."""
+    bias (-inf) leaves no item.  The mean over the counted rows is losses.sum() / count.  Tensors: x, table and bias have gradients,
+    through both results; scale is a number."""
+    if _recorded(x, table, bias, scale):
+        if is_tensor(scale):
+            raise TypeError("scale is a number: it has no gradient here")
+        return _Loss.apply(x, table, bias, targets, scale, ignore_index, ctx)
+    return _cross_entropy(x, table, targets, bias, scale, ignore_index, ctx)
+
+
+def _cross_entropy(x, table, targets, bias, scale, ignore_index, ctx):
     call, (xp, n, xs, tp, v, ts, d, kind, bp, yp), alive = _loss_args(x, table, bias, targets, ctx)
     (losses, op), (lse, lp) = call.empty((n,), "float32"), call.empty((n,), "float32")
     c = call.ctx
@@ -274,7 +342,10 @@ class Table4:
         return codes, scales, zeros
 
     def scores(self, x, ctx=None):
-        """x @ W.T for one row or a few (float32, bfloat16 or float16), in x's type."""
+        """x @ W.T for one row or a few (float32, bfloat16 or float16), in x's type.  They have no gradient: a backward pass raises."""
+        return _Scores.apply(x, self, ctx) if _recorded(x) else self._scores(x, ctx)
+
+    def _scores(self, x, ctx):
         _known(x, "x")
         first = x
         single = len(x.shape) == 1

@@ -8,7 +8,7 @@ from arrowspace_amd import _lib
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from .test_gpu_table import E, TYPES, _check, _check4, _close, _inputs, _plain4, _reference  # noqa: E402
+from .test_gpu_table import E, TYPES, _check, _check4, _close, _inputs, _plain4, _reference, _replays  # noqa: E402
 
 
 @pytest.mark.parametrize("zeros", [False, True])
@@ -322,3 +322,51 @@ def test_scores4_of_rows_at_both_ends_of_the_range(m, v, d, dt, power):
     bound = ((d + 16) * E + 2.0 ** -22) * size + torch.finfo(x.dtype).eps / 2 * want.abs() + 2.0 ** -134
     exact = torch.where(want.abs() > torch.finfo(x.dtype).max, want.sign() * float("inf"), want)
     _close(got, exact, bound, "scores")
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, v, d", [(12, 300, 40), (130, 900, 96), (130, 900, 300)])
+def test_cross_entropy_in_a_graph_of_torch(n, v, d, dt):
+    """Beside another term of a loss, through both results, on another stream: the gradients are those of the backward call."""
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=51, pad=3, offset=1, bias=True, ignored=0.2)
+    leaves = [t.detach().clone().requires_grad_() for t in (x, w, b)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        losses, lse = A.cross_entropy(leaves[0], leaves[1], y, bias=leaves[2], scale=2.0)
+        total = losses.sum() / n + 1e-3 * (lse ** 2).mean() + leaves[1].float().pow(2).sum()
+        total.backward()
+        ge = 2e-3 * lse.detach() / n
+        want = A.cross_entropy_backward(x, w, y, lse.detach(), torch.full((n,), 1 / n, device="cuda"), bias=b, scale=2.0, grad_lse=ge)
+        want = [want[0], (want[1].double() + 2 * w.double()), want[2]]
+    torch.cuda.synchronize()
+    half = torch.finfo(TYPES[dt]).eps / 2
+    for leaf, g, u in zip(leaves, want, (half, half, 2.0 ** -24)):
+        # torch's own rounding of 1 / n and of the mean's gradient: a few f32 roundings of coefficients; the sum of two terms of the table's
+        assert ((leaf.grad.double() - g.double()).abs() <= 3 * u * g.double().abs() + 2.0 ** -20 * g.double().abs().max() + 2 * u * g.double().abs().max()).all()
+    with pytest.raises(RuntimeError):
+        again = torch.autograd.grad(A.cross_entropy(leaves[0], leaves[1], y)[0].sum(), leaves[0], create_graph=True)[0]
+        again.sum().backward()
+
+
+def test_cross_entropy_in_a_graph_of_torch_captured():
+    x, w, y, b = _inputs(100, 1500, 96, torch.bfloat16, seed=52, bias=True)
+    x, w, b = x.contiguous().requires_grad_(), w.contiguous().requires_grad_(), b.requires_grad_()
+    data = [t.detach() for t in (x, w, b)]
+
+    def step():
+        losses, lse = A.cross_entropy(x, w, y, bias=b, scale=2.0)
+        return (losses.detach(), lse.detach()) + torch.autograd.grad(losses.mean() + lse.mean() * 1e-3, (x, w, b))
+
+    _replays(step, data)
+
+
+def test_scores4_have_no_gradient_and_say_so():
+    codes, s, z, w = _plain4(90, 64, 32, "f32", False, 53)
+    t = A.Table4.from_codes(codes, s, dim=64, group=32)
+    x = torch.randn(3, 64, device="cuda", requires_grad=True)
+    scores = t.scores(x)
+    assert torch.equal(scores.detach(), t.scores(x.detach()))
+    with pytest.raises(A.ArrowSpaceError) as e:
+        scores.sum().backward()
+    assert e.value.status == _lib.AS_ERR_UNSUPPORTED

@@ -106,3 +106,33 @@ def test_a_context_that_its_owner_moved_comes_back_to_the_current_stream(ctx):
     # (moved back once, and not again while it is there)
     assert [c for c in ctx.calls if isinstance(c, tuple)] == [("stream", 4096)]
     assert ctx.calls[0] == ("stream", 4096)
+
+
+def test_tensors_that_require_gradients_get_them(ctx, monkeypatch):
+    """The graph reaches the library's backward, with the gradients that are asked for; a table's scores say that they have none."""
+    monkeypatch.setattr(T, "_thread_context", lambda device: ctx)
+    x, w, b, y = torch.randn(3, 8), torch.randn(5, 8), torch.zeros(5), torch.zeros(3, dtype=torch.int64)
+    for a in (x, w, b):
+        a.requires_grad_(True)
+        for through in (lambda r: r[0].sum(), lambda r: r[1].sum(), lambda r: r[0].sum() + (r[1] ** 2).sum()):
+            ctx.calls.clear()
+            result = A.cross_entropy(x, w, y, bias=b, ctx=ctx)
+            through(result).backward()
+            assert ctx.calls[-1] == "as_cross_entropy_backward" and a.grad.shape == a.shape
+            a.grad = None
+    with torch.no_grad():
+        assert not any(t.requires_grad for t in A.cross_entropy(x, w, y, bias=b, ctx=ctx))
+    assert not any(t.requires_grad for t in A.cross_entropy(x.detach(), w.detach(), y, ctx=ctx))
+    assert all(g is not None for g in A.cross_entropy_backward(x, w, y, torch.zeros(3), torch.zeros(3), bias=b, ctx=ctx))
+    with pytest.raises(TypeError):
+        A.cross_entropy(x, w, y, scale=torch.tensor(2.0, requires_grad=True), ctx=ctx)
+    # targets in host memory beside tensors
+    torch.autograd.backward(A.cross_entropy(x, w, y.numpy(), ctx=ctx)[0].sum())
+    assert x.grad is not None
+    table = A.Table4(ctx, None)
+    table.n_items, table.dim = 5, 8
+    scores = table.scores(x)
+    assert not table.scores(x.detach()).requires_grad and not table.scores(x.detach().numpy()).shape[0] == 0
+    with pytest.raises(A.ArrowSpaceError) as e:
+        scores.sum().backward()
+    assert e.value.status == _lib.AS_ERR_UNSUPPORTED
