@@ -370,3 +370,23 @@ def test_scores4_have_no_gradient_and_say_so():
     with pytest.raises(A.ArrowSpaceError) as e:
         scores.sum().backward()
     assert e.value.status == _lib.AS_ERR_UNSUPPORTED
+
+
+# Long rows whose logits' gradient lies in memory in pieces of the table, with the sizes at which each tile is taken for each product.  The pieces
+# follow from n padded to the tile and 2 bytes a logit (f32: 6).
+@pytest.mark.parametrize("n, v, d, dt, bias", [
+    (8100, 50003, 600, "bf16", True),      # 256 x 256 everywhere; pieces of 16896, 16896, 16211
+    (8100, 50003, 600, "bf16", False),
+    (8100, 50003, 600, "f16", True),
+    (3000, 35003, 700, "f32", True),       # 256 x 256 everywhere; pieces of 17664 and 17339
+    (3000, 35003, 700, "f32", False),
+    (40, 2_700_011, 264, "bf16", True),    # 256 x 64 (the table's gradient 128 x 128); two pieces of 1.35 M
+    (100, 1_400_003, 264, "f16", True),    # 128 x 128 everywhere; two pieces of 0.7 M
+])
+def test_cross_entropy_large_tiles_and_several_pieces(n, v, d, dt, bias):
+    x, w, y, b = _inputs(n, v, d, TYPES[dt], seed=54, bias=bias, ignored=0.1)
+    y[: n // 4] = v - 1 - torch.arange(n // 4, device="cuda") // 7       # several rows at items of the last piece, up to 64 and more of a group
+    y[n // 4: n // 2] = (torch.arange(n // 2 - n // 4, device="cuda") * 7919) % v
+    y[n // 2] = 0
+    ge = torch.full((n,), 1e-3 / n, device="cuda") if bias else None
+    _check(x, w, y, b, scale=2.0, ge=ge)
