@@ -154,52 +154,56 @@ __global__ __launch_bounds__(TILE_::NT) void loss_sums_kernel(LossArgs a, float2
   }
 }
 
+// Workgroups of the kernels that take four rows of the batch each: a launch holds less than 2^32 threads, 2^26 rows of a wave.
+unsigned row_groups(uint64_t rows) { return (unsigned)std::min<uint64_t>((rows + 3) / 4, 1u << 20); }
+
 // A wave a row: the stretches' (maximum, sum) joined, the target's logit from the inputs themselves.  f64 behind the sums: the loss is a
 // difference of two near numbers where the model is right.
 template <int DT>
 __global__ __launch_bounds__(256) void loss_join_kernel(const float2 *part, uint32_t parts, const void *x, size_t x_stride, const void *table,
                                                         size_t table_stride, const float *bias, const int64_t *targets, uint32_t n, uint32_t v,
                                                         uint32_t d, float scale, int64_t ignore, float *losses, float *lse_out) {
-  const uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (t >= n) return;
-  float top = -INFINITY;
-  double s = 0.0;
-  for (uint32_t p0 = 0; p0 < parts; p0 += 1024) {
-    float2 o[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const uint32_t p = p0 + k * 64 + lane;
-      o[k] = p < parts ? part[(size_t)p * n + t] : float2{-INFINITY, 0.f};
+  const uint32_t lane = threadIdx.x & 63;
+  for (uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6); t < n; t += gridDim.x * 4) {
+    float top = -INFINITY;
+    double s = 0.0;
+    for (uint32_t p0 = 0; p0 < parts; p0 += 1024) {
+      float2 o[16];
+  #pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const uint32_t p = p0 + k * 64 + lane;
+        o[k] = p < parts ? part[(size_t)p * n + t] : float2{-INFINITY, 0.f};
+      }
+      float m = top;
+  #pragma unroll
+      for (int k = 0; k < 16; ++k) m = fmaxf(m, o[k].x);
+      const float base = m == -INFINITY ? 0.f : m;
+      float here = 0.f;
+  #pragma unroll
+      for (int k = 0; k < 16; ++k) here += o[k].y * __builtin_amdgcn_exp2f((o[k].x - base) * kLog2e);
+      s = s * (double)__builtin_amdgcn_exp2f((top - base) * kLog2e) + (double)here;
+      top = m;
     }
-    float m = top;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) m = fmaxf(m, o[k].x);
-    const float base = m == -INFINITY ? 0.f : m;
-    float here = 0.f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) here += o[k].y * __builtin_amdgcn_exp2f((o[k].x - base) * kLog2e);
-    s = s * (double)__builtin_amdgcn_exp2f((top - base) * kLog2e) + (double)here;
-    top = m;
-  }
-  const float m = top;
-  for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
-  const float base = top == -INFINITY ? 0.f : top;
-  s *= (double)__builtin_amdgcn_exp2f((m - base) * kLog2e);
-  for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
-  const int64_t y = targets[t];
-  const bool ignored = y == ignore, inside = y >= 0 && y < (int64_t)v;
-  double dot = 0.0;
-  if (!ignored && inside) {
-    const size_t xr = (size_t)t * x_stride, wr = (size_t)y * table_stride;
-    for (uint32_t k = lane; k < d; k += 64) dot += (double)load_as_f32<DT>(x, xr + k) * (double)load_as_f32<DT>(table, wr + k);
-    for (int k = 1; k < 64; k <<= 1) dot += __shfl_xor(dot, k);
-  }
-  if (lane == 0) {
-    // (no item left by the bias: the maximum and every term are -inf, s = 0)
-    const double lse = s == 0.0 ? -INFINITY : (double)base + log(s);
-    const double logit = (double)scale * dot + (inside && bias ? (double)bias[y] : 0.0);
-    lse_out[t] = (float)lse;
-    losses[t] = ignored || s == 0.0 ? 0.f : !inside ? NAN : (float)(lse - logit);
+    const float m = top;
+    for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+    const float base = top == -INFINITY ? 0.f : top;
+    s *= (double)__builtin_amdgcn_exp2f((m - base) * kLog2e);
+    for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+    const int64_t y = targets[t];
+    const bool ignored = y == ignore, inside = y >= 0 && y < (int64_t)v;
+    double dot = 0.0;
+    if (!ignored && inside) {
+      const size_t xr = (size_t)t * x_stride, wr = (size_t)y * table_stride;
+      for (uint32_t k = lane; k < d; k += 64) dot += (double)load_as_f32<DT>(x, xr + k) * (double)load_as_f32<DT>(table, wr + k);
+      for (int k = 1; k < 64; k <<= 1) dot += __shfl_xor(dot, k);
+    }
+    if (lane == 0) {
+      // (no item left by the bias: the maximum and every term are -inf, s = 0)
+      const double lse = s == 0.0 ? -INFINITY : (double)base + log(s);
+      const double logit = (double)scale * dot + (inside && bias ? (double)bias[y] : 0.0);
+      lse_out[t] = (float)lse;
+      losses[t] = ignored || s == 0.0 ? 0.f : !inside ? NAN : (float)(lse - logit);
+    }
   }
 }
 
@@ -1104,7 +1108,7 @@ int forward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tabl
   }
   AS_HIP(ctx, hipGetLastError());
   by_type(c.dt, [&](auto dt) {
-    hipLaunchKernelGGL((loss_join_kernel<decltype(dt)::value>), dim3(cdiv(c.n, 4)), dim3(256), 0, ctx->stream, (const float2 *)s.part,
+    hipLaunchKernelGGL((loss_join_kernel<decltype(dt)::value>), dim3(row_groups(c.n)), dim3(256), 0, ctx->stream, (const float2 *)s.part,
                        p.parts, X.p, (size_t)c.x_stride, W.p, (size_t)c.table_stride, (const float *)Bi.p, (const int64_t *)Y.p, p.n, p.v, p.d,
                        c.scale, ignore, (float *)L.p, (float *)S.p);
   });
@@ -1174,8 +1178,8 @@ int backward_call(as_ctx *ctx, const LossCall &c, const void *x, const void *tab
     hipLaunchKernelGGL(coef_scale_kernel, dim3(1), dim3(1024), 0, ctx->stream, by_row.gl, by_row.ge, by_row.targets, ignore, p.n, by_row.power, s.coef);
   by_type(c.dt, [&](auto dt) {
     constexpr int DT = decltype(dt)::value, FMT = format_of(DT);
-    if (p.n > kFewRows) hipLaunchKernelGGL((loss_rows_kernel<DT, FMT, false>), dim3(cdiv(p.n_pad, 4)), dim3(256), 0, ctx->stream, by_row);
-    else hipLaunchKernelGGL((loss_rows_kernel<DT, FMT, true>), dim3(cdiv(p.n_pad, 4)), dim3(256), 0, ctx->stream, by_row);
+    if (p.n > kFewRows) hipLaunchKernelGGL((loss_rows_kernel<DT, FMT, false>), dim3(row_groups(p.n_pad)), dim3(256), 0, ctx->stream, by_row);
+    else hipLaunchKernelGGL((loss_rows_kernel<DT, FMT, true>), dim3(row_groups(p.n_pad)), dim3(256), 0, ctx->stream, by_row);
   });
   AS_HIP(ctx, hipGetLastError());
   // dX from its parts, or dW where the batch was split

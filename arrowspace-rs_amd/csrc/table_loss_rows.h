@@ -182,7 +182,7 @@ struct LossRowInputs {
 };
 template <int DT, int FMT, bool FEW>
 __global__ __launch_bounds__(256) void loss_rows_kernel(LossRowInputs a) {
-  const uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t lane = threadIdx.x & 63;
   float f, unit;
   if constexpr (FEW) {
     unit_of_rows<256>(a.gl, a.ge, a.targets, a.ignore, a.n, a.power, &f, &unit);
@@ -190,33 +190,34 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossRowInputs a) {
   } else {
     f = a.coef[0];
   }
-  if (t >= a.padded) return;
-  float s = INFINITY, every = 0.f, entry = 0.f;   // (behind the last row: probability 0)
-  int at = -1;
-  if (t < a.n && a.lse[t] != -INFINITY) {  // (-inf: the bias left no item, no gradient)
-    const int64_t y = a.targets[t];
-    float one = 0.f;
-    s = a.lse[t];
-    if (y != a.ignore && y >= 0 && y < (int64_t)a.v) {
-      at = (int)y;
-      one = a.gl[t] * f;
+  for (uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6); t < a.padded; t += gridDim.x * 4) {
+    float s = INFINITY, every = 0.f, entry = 0.f;   // (behind the last row: probability 0)
+    int at = -1;
+    if (t < a.n && a.lse[t] != -INFINITY) {  // (-inf: the bias left no item, no gradient)
+      const int64_t y = a.targets[t];
+      float one = 0.f;
+      s = a.lse[t];
+      if (y != a.ignore && y >= 0 && y < (int64_t)a.v) {
+        at = (int)y;
+        one = a.gl[t] * f;
+      }
+      every = one + (a.ge ? a.ge[t] * f : 0.f);
+      if (every == 0.f) s = INFINITY;                          // (nothing but the entry: probability 0, whatever a padded row holds)
+      else if (!(s < INFINITY)) every = __builtin_nanf("");    // (no normaliser, no gradient: probability() gives no NaN)
+      if (at >= 0) {
+        double dot = 0.0;
+  #pragma unroll 4
+        for (uint32_t k = lane; k < a.d; k += 64)
+          dot += (double)load_as_f32<DT>(a.x, (size_t)t * a.x_stride + k) * (double)load_as_f32<DT>(a.table, (size_t)y * a.table_stride + k);
+        for (int k = 1; k < 64; k <<= 1) dot += __shfl_xor(dot, k);
+        const double z = (double)a.scale * dot + (a.bias ? (double)a.bias[y] : 0.0) - (double)a.lse[t];
+        entry = (float)((double)every * (z > 0.0 ? 1.0 : exp(z)) - (double)one);
+      }
     }
-    every = one + (a.ge ? a.ge[t] * f : 0.f);
-    if (every == 0.f) s = INFINITY;                          // (nothing but the entry: probability 0, whatever a padded row holds)
-    else if (!(s < INFINITY)) every = __builtin_nanf("");    // (no normaliser, no gradient: probability() gives no NaN)
-    if (at >= 0) {
-      double dot = 0.0;
-#pragma unroll 4
-      for (uint32_t k = lane; k < a.d; k += 64)
-        dot += (double)load_as_f32<DT>(a.x, (size_t)t * a.x_stride + k) * (double)load_as_f32<DT>(a.table, (size_t)y * a.table_stride + k);
-      for (int k = 1; k < 64; k <<= 1) dot += __shfl_xor(dot, k);
-      const double z = (double)a.scale * dot + (a.bias ? (double)a.bias[y] : 0.0) - (double)a.lse[t];
-      entry = (float)((double)every * (z > 0.0 ? 1.0 : exp(z)) - (double)one);
+    if (lane == 0) {
+      a.o_lse[t] = s, a.o_every[t] = every, a.o_entry[t] = entry, a.o_target[t] = at;
+      a.o_rest[t] = DT == AS_F32 || !__builtin_isfinite(entry) ? 0.f : entry - rounded16<FMT>(entry);
     }
-  }
-  if (lane == 0) {
-    a.o_lse[t] = s, a.o_every[t] = every, a.o_entry[t] = entry, a.o_target[t] = at;
-    a.o_rest[t] = DT == AS_F32 || !__builtin_isfinite(entry) ? 0.f : entry - rounded16<FMT>(entry);
   }
 }
 

@@ -390,3 +390,26 @@ def test_cross_entropy_large_tiles_and_several_pieces(n, v, d, dt, bias):
     y[n // 2] = 0
     ge = torch.full((n,), 1e-3 / n, device="cuda") if bias else None
     _check(x, w, y, b, scale=2.0, ge=ge)
+
+
+def test_cross_entropy_of_more_than_2_to_the_26_rows():
+    n, v = (1 << 26) + 5, 3
+    g = torch.Generator(device="cuda").manual_seed(55)
+    x = torch.randn(n, 1, device="cuda", generator=g).bfloat16()
+    w = torch.tensor([[-1.5], [0.5], [2.0]], device="cuda").bfloat16()
+    y = torch.randint(0, v, (n,), device="cuda", generator=g)
+    y[-1] = 2
+    losses, lse = A.cross_entropy(x, w, y)
+    z = x.double() * w.double()[:, 0]
+    exact = torch.logsumexp(z, 1)
+    off = 16 * E * (z.abs().amax() + 2)
+    assert (lse.double() - exact).abs().max() <= off
+    assert (losses.double() - (exact - z.gather(1, y[:, None])[:, 0])).abs().max() <= 2 * off
+    gl = torch.ones(n, device="cuda")
+    gx, gw, _ = A.cross_entropy_backward(x, w, y, lse, gl)
+    p = torch.exp(z - exact[:, None])
+    p.scatter_add_(1, y[:, None], -torch.ones_like(z[:, :1]))
+    # three products with g of 2^-8 each, the result's rounding
+    assert ((gx.double() - p @ w.double()).abs()[:, 0] <= 2.0 ** -8 * ((p.abs() @ w.double().abs())[:, 0] + 4)).all()
+    # sums of n / 768 and then of 768 parts in f32; g's roundings to nearest have no direction
+    assert ((gw.double() - p.t().contiguous() @ x.double()).abs() <= 2.0 ** -6 * (p.t().contiguous() @ x.double()).abs() + 1e-3 * (p.abs().t().contiguous() @ x.double().abs())).all()
