@@ -67,15 +67,17 @@ constexpr int kF32Planes = 3;
 constexpr int format_of(int dt) { return dt == AS_F16 ? AS_F16 : AS_BF16; }
 constexpr int planes_of(int dt) { return dt == AS_F32 ? kF32Planes : 1; }
 constexpr uint32_t pairs_of(uint32_t planes) { return planes == 1 ? 1 : 6; }
-// P planes of a value (an infinity or NaN in the first alone)
+// P planes of a value.  Three: the first is the nearest finite bf16 (values next to the largest would round to infinity), so an infinity
+// or NaN goes on into the second, where the third stops it.
 template <int P>
 __device__ __forceinline__ void split_planes(float x, float (&o)[P]) {
   o[0] = x;
   if constexpr (P == 3) {
-    const float hi = (float)(__bf16)x;
-    const float r = __builtin_isfinite(hi) ? x - hi : 0.f;
+    constexpr float largest = 0x1.fep127f;
+    o[0] = __builtin_amdgcn_fmed3f(x, -largest, largest);
+    const float r = x - (float)(__bf16)o[0];
     o[1] = r;
-    o[2] = r - (float)(__bf16)r;
+    o[2] = __builtin_isfinite(r) ? r - (float)(__bf16)r : 0.f;
   }
 }
 template <int FMT, int P>

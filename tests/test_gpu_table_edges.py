@@ -413,3 +413,43 @@ def test_cross_entropy_of_more_than_2_to_the_26_rows():
     assert ((gx.double() - p @ w.double()).abs()[:, 0] <= 2.0 ** -8 * ((p.abs() @ w.double().abs())[:, 0] + 4)).all()
     # sums of n / 768 and then of 768 parts in f32; g's roundings to nearest have no direction
     assert ((gw.double() - p.t().contiguous() @ x.double()).abs() <= 2.0 ** -6 * (p.t().contiguous() @ x.double()).abs() + 1e-3 * (p.abs().t().contiguous() @ x.double().abs())).all()
+
+
+@pytest.mark.parametrize("n, v, d", FORMS)
+def test_f32_largest_values_in_ignored_rows(n, v, d):
+    """A padded row of the type's largest value, which no bf16 rounds to: it has no part in anyone's gradient."""
+    x, w, y, b = _inputs(n, v, d, torch.float32, seed=56, bias=True)
+    y[3] = -100
+    gl = torch.full((n,), 1 / n, device="cuda")
+    want = _reference(torch.cat((x[:3], 0 * x[3:4], x[4:])), w, y, b, 1.0, gl)
+    for value in (torch.finfo(torch.float32).max, torch.finfo(torch.float32).min):
+        x = x.clone()
+        x[3] = value
+        _, lse = A.cross_entropy(x, w, y, bias=b)
+        got = A.cross_entropy_backward(x, w, y, lse, gl, bias=b)
+        # (held to the bounds, not to the bits that zeros there give: the maximum a row's sum is taken against moves with its neighbours')
+        for g, what in zip(got, ("grad_x", "grad_table", "grad_bias")):
+            _close(g, *want[what], what)
+        assert not got[0][3].any()
+
+
+@pytest.mark.parametrize("n, v, d", F32_FORMS)
+def test_f32_the_largest_value(n, v, d):
+    """Rows and items that hold it, and logits of ordinary size."""
+    top = torch.finfo(torch.float32).max
+    x, w, y, _ = _inputs(n, v, d, torch.float32, seed=57)
+    x, w = x.clone(), w.clone()
+    x[1, 0], w[:, 0] = top, 2.0 ** -126 * torch.arange(v, device="cuda").remainder(64)
+    w[2, 1], x[:, 1] = -top, 2.0 ** -127
+    x[1, 1] = 0
+    _check(x, w, y, None, scale=1.0)
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("n, v, d", FORMS)
+@pytest.mark.parametrize("scale", [1e-36, 1e-40, 1e-45])
+def test_scales_next_to_zero(n, v, d, dt, scale):
+    x, w, y, _ = _inputs(n, v, d, TYPES[dt], seed=58)
+    losses, lse = A.cross_entropy(x, w, y, scale=scale)
+    exact = torch.tensor(float(v), dtype=torch.float64, device="cuda").log()
+    assert ((lse.double() - exact).abs() <= 64 * E * exact).all() and ((losses.double() - exact).abs() <= 64 * E * exact).all()
