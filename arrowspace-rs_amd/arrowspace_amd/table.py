@@ -22,7 +22,7 @@ _NAMES = {AS_F64: "float64", AS_F32: "float32", AS_BF16: "bfloat16", AS_F16: "fl
 _local = threading.local()
 _torch = None          # the module, once a tensor has been seen
 _raw_stream = None     # device index -> address of torch's current stream there
-_kinds = {}            # torch dtype -> name
+_kinds, _types = {}, {}  # torch dtype -> name and back
 _Loss = _Scores = None  # torch.autograd.Functions
 
 
@@ -31,7 +31,8 @@ def _need_torch():
     import torch
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
     for name in ("float64", "float32", "bfloat16", "float16", "int64", "uint8"):
-        _kinds[getattr(torch, name)] = name
+        _types[name] = getattr(torch, name)
+        _kinds[_types[name]] = name
     _torch = torch
     _differentiable()
 
@@ -80,16 +81,15 @@ def _differentiable():
     _Loss, _Scores = Loss, Scores
 
 
-def _recorded(first, *others):
-    """Whether torch records a call with these arguments for a backward pass."""
-    if not is_tensor(first):
-        return False
-    for a in (first,) + others:
-        if getattr(a, "requires_grad", False):
-            if _torch is None:
-                _need_torch()
-            return _torch.is_grad_enabled()
-    return False
+def _recording():
+    """Whether torch records calls for a backward pass."""
+    if _torch is None:
+        _need_torch()
+    return _torch.is_grad_enabled()
+
+
+def _requires_grad(a):
+    return getattr(a, "requires_grad", False)
 
 
 def _thread_context(device):
@@ -111,7 +111,7 @@ class _Call:
     (that is where the others are written too, whether the first one is host memory or not).  Outputs lie beside the first."""
     __slots__ = ("device", "cuda", "ctx", "torch")
 
-    def __init__(self, first, ctx, *others):
+    def __init__(self, first, ctx, others=()):
         self.device, self.cuda, self.torch = None, False, False
         index = None
         if is_tensor(first):
@@ -144,7 +144,7 @@ class _Call:
     def empty(self, shape, dtype):
         """(array, address) of an output beside the call's inputs; dtype a name."""
         if self.torch:
-            a = _torch.empty(shape, dtype=getattr(_torch, dtype), device=self.device)
+            a = _torch.empty(shape, dtype=_types[dtype], device=self.device)
             return a, a.data_ptr()
         a = np.empty(shape, dtype=dtype)
         return a, a.ctypes.data
@@ -169,13 +169,13 @@ def _known(a, what):
 
 def _matrix(a, what):
     """(array, rows, columns, row stride in elements, address) of a matrix whose rows' values are adjacent."""
-    _known(a, what)
     if not is_tensor(a):
         a = np.asarray(a)
         if a.ndim != 2:
             raise ArrowSpaceError(_lib.AS_ERR_SHAPE, "%s must be a matrix, got %d dimensions" % (what, a.ndim))
         a = np.ascontiguousarray(a)
         return a, a.shape[0], a.shape[1], a.shape[1], a.ctypes.data
+    _known(a, what)
     if a.dim() != 2:
         raise ArrowSpaceError(_lib.AS_ERR_SHAPE, "%s must be a matrix, got %d dimensions" % (what, a.dim()))
     n, d = a.shape
@@ -193,7 +193,6 @@ def _vector(a, n, dtype, what):
     """Address of a dense vector of n elements, and the array that has to stay alive."""
     if a is None:
         return None, None
-    _known(a, what)
     if not is_tensor(a):
         a = np.asarray(a)
         if a.dtype != np.dtype(dtype):
@@ -202,6 +201,7 @@ def _vector(a, n, dtype, what):
         if a.shape != (n,):
             raise ArrowSpaceError(_lib.AS_ERR_SHAPE, "%s must have %d elements, has shape %s" % (what, n, a.shape))
         return a.ctypes.data, a
+    _known(a, what)
     if _name(a) != dtype:
         raise TypeError("%s must be %s, got %s" % (what, dtype, a.dtype))
     if tuple(a.shape) != (n,):
@@ -223,7 +223,7 @@ def _loss_args(x, table, bias, targets, ctx, *others):
     yp, targets = _vector(targets, n, "int64", "targets")
     if yp is None:
         raise ArrowSpaceError(_lib.AS_ERR_ARG, "null argument")
-    call = _Call(first, ctx, table, bias, targets, *others)
+    call = _Call(first, ctx, (table, bias, targets) + others)
     return call, (xp, n, xs, tp, v, ts, d, kind, bp, yp), (x, table, bias, targets)
 
 
@@ -232,7 +232,11 @@ def cross_entropy(x, table, targets, bias=None, scale=1.0, ignore_index=-100, ct
     (losses, lse), both float32 of n.  logits = scale * x @ table.T + bias; losses are 0 where targets == ignore_index and where the
     bias (-inf) leaves no item.  The mean over the counted rows is losses.sum() / count.  Tensors: x, table and bias have gradients,
     through both results; scale is a number."""
-    if _recorded(x, table, bias, scale):
+    try:
+        graph = x.requires_grad or table.requires_grad or (bias is not None and bias.requires_grad) or (type(scale) is not float and _requires_grad(scale))
+    except AttributeError:   # (host arrays)
+        graph = any(map(_requires_grad, (x, table, bias, scale)))
+    if graph and is_tensor(x) and _recording():
         if is_tensor(scale):
             raise TypeError("scale is a number: it has no gradient here")
         return _Loss.apply(x, table, bias, targets, scale, ignore_index, ctx)
@@ -325,7 +329,7 @@ class Table4:
         if n > 1 and (step != half or sstep != groups or (zeros is not None and zstep != groups)):
             raise ArrowSpaceError(_lib.AS_ERR_ARG, "codes, scales and zeros must be dense")
         scale_kind = _scale_kind(_name(scales))
-        call = _Call(first, ctx, scales, zeros)
+        call = _Call(first, ctx, (scales, zeros))
         h = C.c_void_p()
         call.ctx.check(call.ctx.lib.as_table4_import(call.ctx.h, cp, sp, zp, n, dim, int(group), scale_kind, C.byref(h)))
         return cls(call.ctx, h)
@@ -343,13 +347,13 @@ class Table4:
 
     def scores(self, x, ctx=None):
         """x @ W.T for one row or a few (float32, bfloat16 or float16), in x's type.  They have no gradient: a backward pass raises."""
-        return _Scores.apply(x, self, ctx) if _recorded(x) else self._scores(x, ctx)
+        return _Scores.apply(x, self, ctx) if _requires_grad(x) and _recording() else self._scores(x, ctx)
 
     def _scores(self, x, ctx):
-        _known(x, "x")
         first = x
         single = len(x.shape) == 1
         if single:
+            _known(x, "x")
             x = x.reshape(1, -1)
         x, m, d, step, p = _matrix(x, "x")
         if d != self.dim:
