@@ -89,7 +89,8 @@ const char *as_status_message(int status); /* the reference's panic text for a s
 /* Run on an existing HIP stream (e.g. PyTorch's current stream; NULL = HIP's default stream).
  * Until this is called the context uses a private stream and every call is synchronous with
  * the host.  Afterwards calls whose outputs are device buffers are stream-ordered (no host
- * sync); host outputs are always complete on return. */
+ * sync); host outputs are always complete on return.  The switch waits for the stream it leaves; beside a graph's capture (either stream is
+ * being captured) it waits for nothing, and the first call behind the capture makes its stream wait instead. */
 int as_ctx_set_stream(as_ctx *ctx, void *hip_stream);
 int as_ctx_synchronize(as_ctx *ctx);
 /* Options.  None of them changes a result -- only which stage produces it; defaults in parentheses.  The 35 below are the supported
