@@ -604,7 +604,8 @@ struct ProfScope {
   bool active;
   const char *outer = nullptr;
   std::chrono::steady_clock::time_point host_t0;  // (with the profile on: the HOST's time inside the stage too, stat "host_us_in_<stage>")
-  ProfScope(as_ctx *c, const char *name) : ctx(c), active(c->prof_on) {
+  // (an event recorded in a capture has no time, and asking for it is an error that the next call would find)
+  ProfScope(as_ctx *c, const char *name) : ctx(c), active(c->prof_on && !stream_is_capturing(c->stream)) {
     if (!active) return;
     host_t0 = std::chrono::steady_clock::now();
     ev.name = name;
