@@ -169,17 +169,17 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2 *part, uint
     double s = 0.0;
     for (uint32_t p0 = 0; p0 < parts; p0 += 1024) {
       float2 o[16];
-  #pragma unroll
+#pragma unroll
       for (int k = 0; k < 16; ++k) {
         const uint32_t p = p0 + k * 64 + lane;
         o[k] = p < parts ? part[(size_t)p * n + t] : float2{-INFINITY, 0.f};
       }
       float m = top;
-  #pragma unroll
+#pragma unroll
       for (int k = 0; k < 16; ++k) m = fmaxf(m, o[k].x);
       const float base = m == -INFINITY ? 0.f : m;
       float here = 0.f;
-  #pragma unroll
+#pragma unroll
       for (int k = 0; k < 16; ++k) here += o[k].y * __builtin_amdgcn_exp2f((o[k].x - base) * kLog2e);
       s = s * (double)__builtin_amdgcn_exp2f((top - base) * kLog2e) + (double)here;
       top = m;
@@ -198,11 +198,11 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2 *part, uint
       for (int k = 1; k < 64; k <<= 1) dot += __shfl_xor(dot, k);
     }
     if (lane == 0) {
-      // (no item left by the bias: the maximum and every term are -inf, s = 0)
-      const double lse = s == 0.0 ? -INFINITY : (double)base + log(s);
+      // (no item left by the bias: the maximum and every term are -inf, s = 0; without a bias these are products that overflowed)
+      const double lse = s == 0.0 ? (bias ? -INFINITY : NAN) : (double)base + log(s);
       const double logit = (double)scale * dot + (inside && bias ? (double)bias[y] : 0.0);
       lse_out[t] = (float)lse;
-      losses[t] = ignored || s == 0.0 ? 0.f : !inside ? NAN : (float)(lse - logit);
+      losses[t] = ignored || (s == 0.0 && bias) ? 0.f : !inside ? NAN : (float)(lse - logit);
     }
   }
 }

@@ -208,7 +208,7 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossRowInputs a) {
       else if (!(s < INFINITY)) every = __builtin_nanf("");    // (no normaliser, no gradient: probability() gives no NaN)
       if (at >= 0) {
         double dot = 0.0;
-  #pragma unroll 4
+#pragma unroll 4
         for (uint32_t k = lane; k < a.d; k += 64)
           dot += (double)load_as_f32<DT>(a.x, (size_t)t * a.x_stride + k) * (double)load_as_f32<DT>(a.table, (size_t)y * a.table_stride + k);
         for (int k = 1; k < 64; k <<= 1) dot += __shfl_xor(dot, k);

@@ -473,3 +473,21 @@ def test_a_captured_call_with_the_profile_on():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     ms, launches = ctx.profile_get("cross_entropy")
     assert launches == 3 and ms > 0
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("n, v, d", FORMS)
+def test_products_that_overflow_to_minus_infinity(n, v, d, dt):
+    """A row whose products are all -infinity in f32 has no loss of 0: without a bias nothing takes items out."""
+    x = torch.randn(n, d, device="cuda").to(TYPES[dt])
+    w = -torch.ones(v, d, device="cuda").to(TYPES[dt])
+    x[1] = 1e30
+    w[:, 0] = -1e30
+    x[torch.arange(n, device="cuda") != 1, 0] = 0
+    y = torch.randint(0, v, (n,), device="cuda")
+    losses, lse = A.cross_entropy(x, w, y)
+    rows = torch.arange(n, device="cuda") != 1
+    assert torch.isnan(losses[1]) and torch.isnan(lse[1]) and torch.isfinite(losses[rows]).all()
+    y[1] = -100
+    losses, lse = A.cross_entropy(x, w, y)
+    assert losses[1] == 0 and torch.isfinite(losses).all()
